@@ -143,6 +143,11 @@ _SIGS = {
     "df_layernorm_quantize_delayed": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _vp, _vp, _c_f, _vp, _c_int,
                                                _c_int, _vp, _vp, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_sz,
                                                _vp]),
+    "df_layernorm_forward": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _c_f,
+                                      _vp, _c_int, _vp, _vp, _vp]),
+    "df_layernorm_backward_workspace_bytes": (_c_sz, [_c_int, _c_int]),
+    "df_layernorm_backward": (_c_int, [_c_int, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_f, _vp,
+                                       _c_int, _vp, _c_int, _vp, _vp, _vp, _c_sz, _vp]),
     "df_grad_norm_workspace_bytes": (_c_sz, [_c_int, _vp]),
     "df_grad_norm_f32": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _c_sz, _vp]),
     "df_clip_grad_norm_f32": (_c_int, [_vp, _vp, _c_int, _c_f, _vp, _vp, _c_sz, _vp]),
@@ -664,3 +669,113 @@ def layernorm(x, gamma=None, beta=None, eps=1e-5, fmt: Fmt | None = None, want_y
              float(eps), _ptr(y), ldy, int(fmt), _ptr(scale), _ptr(delayed.scale), _ptr(delayed.history),
              delayed.history.numel(), _ptr(q), ldq, _ptr(qt), ldqt, _ptr(ws), ws.numel(), _stream())
     return y, q, qt, scale
+
+
+# ----------------------------------------------------------------------------
+# LayerNorm for training: the forward with its statistics, and the backward
+# ----------------------------------------------------------------------------
+class _on:
+    """Context: the device of ``t`` is the current one, so that the call goes
+    to that device's current stream."""
+
+    def __init__(self, t):
+        self.device = t.device
+
+    def __enter__(self):
+        torch = _torch()
+        self.before = torch.cuda.current_device()
+        if self.device.index != self.before:
+            torch.cuda.set_device(self.device)
+
+    def __exit__(self, *exc):
+        if self.device.index != self.before:
+            _torch().cuda.set_device(self.before)
+
+
+def _check_gpu(fn: str, **tensors):
+    """Every given tensor is on one and the same GPU."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{fn}: {name} is on {t.device}, not on a GPU")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{fn}: {name} is on {t.device}, others on {dev}")
+        dev = t.device
+
+
+def _check_like(fn: str, name: str, t, shape, dtype):
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise ValueError(f"{fn}: {name} is {tuple(t.shape)} {t.dtype}, not {tuple(shape)} {dtype}")
+
+
+def _rows(fn: str, name: str, t, shape, dtype) -> int:
+    """The leading dimension of a [rows, cols] operand whose rows are
+    contiguous and do not overlap."""
+    _check_like(fn, name, t, shape, dtype)
+    rows, cols = shape
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+        raise ValueError(f"{fn}: {name} with strides {tuple(t.stride())} has no contiguous rows of its own")
+    return max(t.stride(0), cols) if rows > 1 else cols
+
+
+def _row_vector(fn: str, name: str, t, n: int, dtype):
+    if t is not None:
+        _check_like(fn, name, t, (n,), dtype)
+        if n > 1 and t.stride(0) != 1:
+            raise ValueError(f"{fn}: {name} is not contiguous")
+
+
+def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, residual=None):
+    """LayerNorm over the last dim of a 2-D fp32/bf16/f16 tensor for training
+    (df_layernorm_forward): returns (y, s, mean, rstd), where s = x + residual
+    is what the norm saw (x itself without a residual) and mean and rstd are
+    its rows' fp32 statistics: what :func:`layernorm_backward` takes."""
+    fn, torch = "layernorm_forward", _torch()
+    if x.dim() != 2:
+        raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
+    _check_gpu(fn, x=x, gamma=gamma, beta=beta, residual=residual)
+    rows, cols = x.shape
+    dt, ldx = int(_in_dtype(x)), _rows(fn, "x", x, x.shape, x.dtype)
+    ldr = 0 if residual is None else _rows(fn, "residual", residual, x.shape, x.dtype)
+    _row_vector(fn, "gamma", gamma, cols, x.dtype)
+    _row_vector(fn, "beta", beta, cols, x.dtype)
+    with _on(x):
+        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+        s = x if residual is None else torch.empty_like(y)
+        mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+        call("df_layernorm_forward", dt, _ptr(x), rows, cols, ldx, _ptr(residual), ldr,
+             None if residual is None else _ptr(s), cols, _ptr(gamma), _ptr(beta), float(eps), _ptr(y), cols,
+             _ptr(mean), _ptr(rstd), _stream())
+    return y, s, mean, rstd
+
+
+def layernorm_backward(dy, x, gamma=None, mean=None, rstd=None, eps=1e-5, dresidual=None, sums=True):
+    """The gradients of :func:`layernorm_forward` (df_layernorm_backward), x
+    being what the norm saw: returns (dx, dgamma, dbeta), the last two in fp32
+    (None with ``sums=False``).  Without mean and rstd they are taken from x
+    at eps again.  ``dresidual`` (the gradient that reaches the residual
+    stream past the norm) is added to dx."""
+    fn, torch = "layernorm_backward", _torch()
+    if x.dim() != 2:
+        raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
+    _check_gpu(fn, dy=dy, x=x, gamma=gamma, mean=mean, rstd=rstd, dresidual=dresidual)
+    rows, cols = x.shape
+    dt, ldx, lddy = int(_in_dtype(x)), _rows(fn, "x", x, x.shape, x.dtype), _rows(fn, "dy", dy, x.shape, x.dtype)
+    lddr = 0 if dresidual is None else _rows(fn, "dresidual", dresidual, x.shape, x.dtype)
+    _row_vector(fn, "gamma", gamma, cols, x.dtype)
+    _row_vector(fn, "mean", mean, rows, torch.float32)
+    _row_vector(fn, "rstd", rstd, rows, torch.float32)
+    with _on(x):
+        dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+        dg = torch.empty(cols, dtype=torch.float32, device=x.device) if sums else None
+        db = torch.empty_like(dg) if sums else None
+        # not a cached one: a captured graph keeps the workspace it was given
+        ws = torch.empty(int(lib().df_layernorm_backward_workspace_bytes(rows, cols)), dtype=torch.uint8,
+                         device=x.device)
+        call("df_layernorm_backward", dt, _ptr(dy), lddy, _ptr(x), ldx, rows, cols, _ptr(gamma), _ptr(mean),
+             _ptr(rstd), float(eps), _ptr(dresidual), lddr, _ptr(dx), cols, _ptr(dg), _ptr(db), _ptr(ws),
+             ws.numel(), _stream())
+    return dx, dg, db

@@ -281,6 +281,42 @@ int df_layernorm_quantize_delayed(int dtype, const void* x, int rows, int cols, 
                                   int ldq, uint8_t* qt, int ldqt, void* ws, size_t ws_bytes,
                                   void* stream);
 
+/* ---- LayerNorm for training (forward with the residual add in front of it
+ * and its row statistics: layer_norm_forward_kernel,
+ * dnn/layers/layer_norm_layer.cu:26-63; the backward is new: the reference's
+ * copies the incoming gradient, .cu:82-90) ----
+ * dtype fp32, f16 or bf16, every matrix [rows, cols] with its own leading
+ * dimension (>= cols), pointers aligned to their elements; sums and statistics
+ * in binary32.
+ *  df_layernorm_forward : s = x + residual rounded to the dtype (s = x when
+ *                         residual is NULL), stored to `sum` when non-NULL;
+ *                         mean, var and rstd of s as above;
+ *                         y = fma((s - mean) * rstd, gamma, beta), rounded
+ *                         once.  mean and rstd (fp32 [rows]) may be NULL.
+ *                         sum may be x or residual, y may be x or residual;
+ *                         sum and y differ.
+ *  df_layernorm_backward: with xh = (x - mean) * rstd and g = dy * gamma,
+ *                         dx = rstd * (g - mean(g) - xh * mean(g * xh))
+ *                         + dresidual (NULL: none; the gradient that reaches
+ *                         the residual stream past the norm), rounded once;
+ *                         dgamma[c] = sum_r dy * xh, dbeta[c] = sum_r dy in
+ *                         fp32 [cols], overwritten (both NULL: not wanted).
+ *                         x is the forward's s.  mean and rstd NULL: taken
+ *                         from x at eps again (after df_layernorm_quantize,
+ *                         which keeps none).  dx may be dy, x or dresidual.
+ *                         No rows: dgamma and dbeta are zeroed.  ws:
+ *                         df_layernorm_backward_workspace_bytes(rows, cols)
+ *                         bytes, 16-byte aligned.  The column sums add rows in
+ *                         a fixed order: deterministic. */
+int df_layernorm_forward(int dtype, const void* x, int rows, int cols, int ldx, const void* residual,
+                         int ldr, void* sum, int lds, const void* gamma, const void* beta, float eps,
+                         void* y, int ldy, float* mean, float* rstd, void* stream);
+size_t df_layernorm_backward_workspace_bytes(int rows, int cols);
+int df_layernorm_backward(int dtype, const void* dy, int lddy, const void* x, int ldx, int rows,
+                          int cols, const void* gamma, const float* mean, const float* rstd, float eps,
+                          const void* dresidual, int lddr, void* dx, int lddx, float* dgamma,
+                          float* dbeta, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- fp8 GEMM, "NT": C[m,n] = (sum_k A[m,k] * B[n,k]) * sa * sb + bias[n]
  *   A [M, lda] fp8 (fmt_a), B [N, ldb] fp8 (fmt_b), both row-major with the
  *   reduction dimension contiguous; lda, ldb multiples of 16 and >= K;
