@@ -155,6 +155,10 @@ _SIGS = {
                                     _c_int, _vp, _c_f, _vp]),
     "df_adam_update_absmax_f32": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_int, _c_f, _c_f, _c_f, _c_f, _c_f,
                                            _c_int, _vp, _c_f, _vp, _vp]),
+    "df_grad_norm": (_c_int, [_c_int, _vp, _vp, _c_int, _vp, _vp, _c_sz, _vp]),
+    "df_adamw_scale_count": (_c_i64, [_c_i64]),
+    "df_adamw_update": (_c_int, [_c_int, _vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _c_f, _c_f,
+                                 _c_f, _c_f, _vp, _c_int, _vp, _vp, _vp, _c_f, _vp, _vp]),
 }
 
 _lib = None
@@ -568,9 +572,12 @@ def _sizes(tensors):
 def grad_norm(grads, clip: float | None = None):
     """Global L2 norm of fp32 device tensors as a 1-element device tensor;
     with ``clip`` the tensors are scaled in place by clip / norm when
-    norm > clip (utils::clip_grad_norm)."""
+    norm > clip (utils::clip_grad_norm).  bf16 and float16 tensors (one type
+    for all) are measured too, without ``clip``."""
     torch = _torch()
     dev = grads[0].device
+    if grads[0].dtype in (torch.bfloat16, torch.float16):
+        return _grad_norm16(grads, clip)
     sizes = _sizes(grads)
     nbytes = lib().df_grad_norm_workspace_bytes(len(grads), sizes)
     ws = _scratch(dev, nbytes, "grad_norm")
@@ -779,3 +786,114 @@ def layernorm_backward(dy, x, gamma=None, mean=None, rstd=None, eps=1e-5, dresid
              _ptr(rstd), float(eps), _ptr(dresidual), lddr, _ptr(dx), cols, _ptr(dg), _ptr(db), _ptr(ws),
              ws.numel(), _stream())
     return dx, dg, db
+
+
+# ----------------------------------------------------------------------------
+# AdamW over lists of tensors, states in 32 or in 8 bits
+# ----------------------------------------------------------------------------
+def _list_of(fn: str, what: str, tensors, like, dtype, sizes=None):
+    """Checks a list of contiguous GPU tensors of one dtype, one per entry of ``like`` and of its size (or sizes[i])."""
+    if len(tensors) != len(like):
+        raise ValueError(f"{fn}: {len(tensors)} {what} for {len(like)} parameters")
+    dev = like[0].device if like else None
+    for i, t in enumerate(tensors):
+        n = like[i].numel() if sizes is None else sizes[i]
+        if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.device != dev or not t.is_cuda:
+            raise ValueError(f"{fn}: {what}[{i}] ({tuple(t.shape)} {t.dtype} on {t.device}) is not a contiguous {dtype} "
+                             f"tensor of {n} values on {dev}" + ("" if t.is_cuda else ", a GPU"))
+
+
+def _grad_norm16(grads, clip):
+    fn, torch = "grad_norm", _torch()
+    if clip is not None:
+        raise TypeError(f"{fn}: {grads[0].dtype} gradients are not clipped in place (give adamw_update the norm)")
+    _list_of(fn, "grads", grads, grads, grads[0].dtype)
+    sizes = _sizes(grads)
+    with _on(grads[0]):
+        ws = torch.empty(int(lib().df_grad_norm_workspace_bytes(len(grads), sizes)), dtype=torch.uint8,
+                         device=grads[0].device)
+        norm = torch.empty(1, dtype=torch.float32, device=grads[0].device)
+        call("df_grad_norm", int(_in_dtype(grads[0])), _ptrs(grads), sizes, len(grads), _ptr(norm), _ptr(ws), ws.numel(),
+             _stream())
+    return norm
+
+
+def adamw_state(params, bits: int = 32):
+    """(ms, vs, m_scales, v_scales) for :func:`adamw_update` before the first
+    step: fp32 zeros and no scales (None), or with ``bits=8`` e4m3 zeros and
+    an fp32 scale per 256 values."""
+    torch = _torch()
+    if bits == 32:
+        return [torch.zeros_like(p) for p in params], [torch.zeros_like(p) for p in params], None, None
+    if bits != 8:
+        raise ValueError(f"adamw_state: states in {bits} bits (8 or 32)")
+    codes = lambda p: torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+    ones = lambda p: torch.ones(-(-p.numel() // 256), dtype=torch.float32, device=p.device)
+    return ([codes(p) for p in params], [codes(p) for p in params], [ones(p) for p in params],
+            [ones(p) for p in params])
+
+
+def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
+                 m_scales=None, v_scales=None, copies=None, clip_norm=None, max_norm=0.0, absmax=None):
+    """One AdamW step (df_adamw_update) over contiguous fp32 parameters, in
+    place on params, the states (fp32, or float8_e4m3fn with m_scales and
+    v_scales: see :func:`adamw_state`) and ``copies`` (bf16 or float16, the
+    updated parameters).  Gradients are fp32, bf16 or float16, one type for
+    all.  ``weight_decay`` is one number or one per tensor; ``timestep`` an int
+    or an int32 device tensor and ``lr`` a number or an fp32 device tensor,
+    read when the kernel runs (a captured step follows them on replay).
+    ``clip_norm`` (a device norm from :func:`grad_norm`) applies max_norm /
+    norm to the gradients; ``absmax`` (fp32 of len(params)) receives max |p|
+    of each updated tensor."""
+    fn, torch = "adamw_update", _torch()
+    n = len(params)
+    if n == 0:
+        return
+    eight = m_scales is not None
+    if eight != (v_scales is not None):
+        raise ValueError(f"{fn}: m_scales and v_scales go together")
+    gt = _in_dtype(grads[0]) if grads else DType.FLOAT32
+    state = torch.float8_e4m3fn if eight else torch.float32
+    _list_of(fn, "params", params, params, torch.float32)
+    _list_of(fn, "grads", grads, params, grads[0].dtype if grads else None)
+    _list_of(fn, "ms", ms, params, state)
+    _list_of(fn, "vs", vs, params, state)
+    written = [params, ms, vs]
+    if eight:
+        blocks = [-(-p.numel() // 256) for p in params]
+        _list_of(fn, "m_scales", m_scales, params, torch.float32, blocks)
+        _list_of(fn, "v_scales", v_scales, params, torch.float32, blocks)
+        written += [m_scales, v_scales]
+    ct = DType.FLOAT32
+    if copies is not None:
+        ct = _in_dtype(copies[0]) if copies else ct
+        if ct == DType.FLOAT32:
+            raise TypeError(f"{fn}: copies are bf16 or float16")
+        _list_of(fn, "copies", copies, params, copies[0].dtype)
+        written.append(copies)
+    arrays = [_ptrs(ts) for ts in written]
+    at = [a for arr, ts in zip(arrays, written) for a, t in zip(arr, ts) if t.numel()]
+    if len(set(at)) != len(at):
+        raise ValueError(f"{fn}: a tensor that the step writes is listed twice")
+    if isinstance(weight_decay, (int, float)):
+        wd = (_c_f * n)(*[weight_decay] * n)
+    else:
+        if len(weight_decay) != n:
+            raise ValueError(f"{fn}: {len(weight_decay)} weight decays for {n} parameters")
+        wd = (_c_f * n)(*weight_decay)
+    scalars = {}
+    for name, v, dt in (("timestep", timestep, torch.int32), ("lr", lr, torch.float32), ("clip_norm", clip_norm, torch.float32)):
+        if isinstance(v, torch.Tensor):
+            if v.numel() != 1 or v.dtype != dt or v.device != params[0].device:
+                raise ValueError(f"{fn}: {name} is not one {dt} on {params[0].device}")
+            scalars[name] = v.data_ptr()
+    if absmax is not None and (absmax.dtype != torch.float32 or absmax.numel() < n or not absmax.is_contiguous()
+                               or absmax.device != params[0].device):
+        raise ValueError(f"{fn}: absmax is not {n} contiguous fp32 values on {params[0].device}")
+    p, m, v = arrays[:3]
+    sm, sv = arrays[3:5] if eight else (None, None)
+    with _on(params[0]):
+        call("df_adamw_update", n, _sizes(params), p, int(gt), _ptrs(grads), int(DType.FP8E4M3 if eight else DType.FLOAT32), m, v, sm,
+             sv, int(ct), arrays[-1] if copies is not None else None, 0.0 if "lr" in scalars else float(lr), float(beta1),
+             float(beta2), float(eps), wd, 0 if "timestep" in scalars else int(timestep), scalars.get("lr"),
+             scalars.get("timestep"), scalars.get("clip_norm"), float(max_norm), _ptr(absmax), _stream())

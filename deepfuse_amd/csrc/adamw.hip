@@ -1,0 +1,437 @@
+// adamw.hip -- the AdamW update (decoupled weight decay) over lists of tensors,
+// its states in binary32 or in 8 bits (gfx950).
+//
+// Per element, every operation rounded to binary32 as written (no fused
+// multiply-adds; IEEE division and square root):
+//   g = grad * f                       f: the clip factor (1 when not clipping)
+//   m = b1*m + (1-b1)*g;  v = b2*v + ((1-b2)*g)*g
+//   p = p*(1 - lr*wd) - (lr*(m / (1-b1^t))) / (sqrt(v / (1-b2^t)) + eps)
+//
+// 8-bit states: 256 consecutive values of a tensor share a binary32 scale.
+// m is kept as e4m3 codes of m / scale, scale = max|m| / 448 over the block's
+// finite values; v as codes of sqrt(v), which the update needs anyway: e4m3
+// spans 2^-9 to 448, so the square root covers 2^35 of v in one block.  A v
+// above 0 never goes to code 0: the next step would divide its m by eps alone.
+// The update itself uses the binary32 m and v; only what is kept is rounded
+// (to 4 significant bits: off by at most 2^-4 of the value, or 2^-10 of the
+// scale).
+//
+// Bound by HBM: 24 bytes and the gradient per element with binary32 states,
+// 12.1 and the gradient with 8-bit ones.  A wave takes 256 values at a time,
+// four consecutive ones per lane, which is also the block of a scale: 16-byte
+// accesses of p (m, v), 4-byte ones of codes, and the block's maxima fold
+// across the wave's lanes (DPP) without leaving registers.
+//
+// Extends the reference's optimizer set, whose Adam couples the decay
+// (dnn/optimizers/adam_optimizer.cu:24-30); no counterpart of the rest.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "df_common.hpp"
+
+// Rounding of every operation as written: no fused multiply-adds.
+#pragma clang fp contract(off)
+
+namespace dfk {
+
+namespace {
+
+constexpr int kWThreads = 256;
+constexpr int kUnit = 256;                              // values of a wave at a time, and of a scale
+constexpr int kUnits = 4;                               // units whose loads are in flight together
+constexpr int kRounds = 2;
+constexpr int kWaveSpan = kUnit * kUnits * kRounds;     // values of a wave
+constexpr int kSpan = kWaveSpan * (kWThreads / 64);     // values of a block
+constexpr int kWList = 40;                              // tensors of a launch (their table is in the arguments)
+
+struct WTensor {
+    float* p;
+    const void* g;
+    void* m;
+    void* v;
+    float* ms;
+    float* vs;
+    uint16_t* copy;
+    int64_t n;
+};
+struct WList {
+    WTensor t[kWList];
+    float wd[kWList];
+    int first[kWList + 1];  // first block of each tensor; first[count] = blocks
+    int idx[kWList];        // position in the caller's list
+    int count;
+};
+struct WHyper {
+    float lr, b1, b2, omb1, omb2, eps, max_norm;
+    float bc1, bc2;         // 1 - beta^t, unless step is given
+    const float* lr_dev;
+    const int* step;
+    const float* norm;
+    uint32_t* absmax;
+};
+
+// 1 - beta^t: beta^t by squaring in binary64, rounded once to binary32; the
+// same operations on host and device, so both forms of the step agree
+__host__ __device__ inline float bias_corr(float beta, int t) {
+    double r = 1.0, b = beta;
+    for (int k = t < 1 ? 1 : t; k > 0; k >>= 1) {
+        if (k & 1) r = r * b;
+        b = b * b;
+    }
+    return 1.0f - (float)r;
+}
+
+// 16, 8 or 4 bytes at element alignment
+typedef f32x4 f32x4_el __attribute__((aligned(4)));
+typedef u32x2 u32x2_el __attribute__((aligned(2)));
+typedef uint32_t u32_el __attribute__((aligned(1)));
+
+// maximum over the wave (VALU only): rows of 16 lanes, then across them
+__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
+#define DF_DPP_MAX(CTRL) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true))
+    DF_DPP_MAX(0x111);  // row_shr:1
+    DF_DPP_MAX(0x112);  // row_shr:2
+    DF_DPP_MAX(0x114);  // row_shr:4
+    DF_DPP_MAX(0x118);  // row_shr:8: lane 15 of a row has the row's
+    DF_DPP_MAX(0x142);  // row_bcast:15
+    DF_DPP_MAX(0x143);  // row_bcast:31: lane 63 has the wave's
+#undef DF_DPP_MAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+template <typename G> __device__ __forceinline__ float grad_one(const G* p);
+template <> __device__ __forceinline__ float grad_one<float>(const float* p) { return *p; }
+template <> __device__ __forceinline__ float grad_one<uint16_t>(const uint16_t* p) { return bf16_to_f32(*p); }
+template <> __device__ __forceinline__ float grad_one<f16_t>(const f16_t* p) {
+    return (float)__builtin_bit_cast(_Float16, p->bits);
+}
+
+// four gradients as loaded, and widened
+template <typename G> struct Grad4 {
+    u32x2 w;
+    __device__ __forceinline__ void load(const G* p) { w = *reinterpret_cast<const u32x2_el*>(p); }
+    __device__ __forceinline__ void widen(float* g) const {
+        if constexpr (std::is_same<G, uint16_t>::value) {
+            g[0] = __uint_as_float(w.x << 16); g[1] = __uint_as_float(w.x & 0xFFFF0000u);
+            g[2] = __uint_as_float(w.y << 16); g[3] = __uint_as_float(w.y & 0xFFFF0000u);
+        } else {
+            g[0] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w.x & 0xFFFFu));
+            g[1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w.x >> 16));
+            g[2] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w.y & 0xFFFFu));
+            g[3] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w.y >> 16));
+        }
+    }
+};
+template <> struct Grad4<float> {
+    f32x4 w;
+    __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const f32x4_el*>(p); }
+    __device__ __forceinline__ void widen(float* g) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = w[e];
+    }
+};
+
+__device__ __forceinline__ void decode4(uint32_t w, float s, float* v) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    v[0] = a.x * s; v[1] = a.y * s; v[2] = b.x * s; v[3] = b.y * s;
+}
+
+// the scale of a block whose largest finite magnitude is the pattern `am`
+__device__ __forceinline__ float block_scale(uint32_t am) {
+    const float a = __uint_as_float(am);
+    return am ? __builtin_fmaxf(a / 448.0f, 0x1p-126f) : 1.0f;
+}
+
+template <int COPY> __device__ __forceinline__ uint32_t copy_bits(float v) {
+    return COPY == DF_DTYPE_HALF ? f32_to_f16_rne(v) : f32_to_bf16_rne(v);
+}
+
+// COPY: DF_DTYPE_BFLOAT16 or DF_DTYPE_HALF: the updated parameters are also
+// written in that type; -1: not.
+template <typename G, bool S8, int COPY>
+__global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const WHyper h) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int lo = 0, hi = L.count - 1;  // the tensor that owns this block: the last with first <= blockIdx.x
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (L.first[mid] <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
+    }
+    const WTensor t = L.t[lo];
+    const G* gp = static_cast<const G*>(t.g);
+    float f = 1.0f;
+    if (h.norm) {
+        const float nv = h.norm[0];
+        if (nv > h.max_norm) f = h.max_norm / nv;
+    }
+    const float lr = h.lr_dev ? h.lr_dev[0] : h.lr;
+    float bc1 = h.bc1, bc2 = h.bc2;
+    if (h.step) {
+        bc1 = bias_corr(h.b1, h.step[0]);
+        bc2 = bias_corr(h.b2, h.step[0]);
+    }
+    const float keep = 1.0f - lr * L.wd[lo];
+    uint32_t am = 0;
+
+    auto update = [&](float* p, const float* g, float* m, float* v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float ge = g[e] * f;
+            m[e] = h.b1 * m[e] + h.omb1 * ge;
+            v[e] = h.b2 * v[e] + h.omb2 * ge * ge;
+            p[e] = p[e] * keep - lr * (m[e] / bc1) / (__builtin_sqrtf(v[e] / bc2) + h.eps);
+            if (h.absmax) am = fold_f32(am, __float_as_uint(p[e]));
+        }
+    };
+    // codes and scale of a unit's values; ROOT: of their square roots, above 0 from code 1 up
+    auto encode = [&](const float* x, auto root, float& s) __attribute__((always_inline)) -> uint32_t {
+        constexpr bool ROOT = decltype(root)::value;
+        float y[4];
+        uint32_t a = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            y[e] = ROOT ? __builtin_sqrtf(x[e]) : x[e];
+            a = fold_f32(a, __float_as_uint(y[e]));
+        }
+        s = block_scale(wave_umax(a));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool some = ROOT && y[e] > 0.0f;
+            y[e] = y[e] / s;
+            if (some) y[e] = __builtin_fmaxf(y[e], 0x1p-9f);
+        }
+        return encode2_hw<E4M3>(y[0], y[1]) | (encode2_hw<E4M3>(y[2], y[3]) << 16);
+    };
+
+    const int64_t base = (int64_t)((int)blockIdx.x - L.first[lo]) * kSpan + (int64_t)wave * kWaveSpan;
+    for (int round = 0; round < kRounds; ++round) {
+        const int64_t u0 = base + (int64_t)round * kUnits * kUnit;
+        if (u0 >= t.n) break;
+        if (u0 + kUnits * kUnit <= t.n) {
+            f32x4 rp[kUnits], rm[S8 ? 1 : kUnits], rv[S8 ? 1 : kUnits];
+            uint32_t cm[S8 ? kUnits : 1], cv[S8 ? kUnits : 1];
+            float sm[S8 ? kUnits : 1], sv[S8 ? kUnits : 1];
+            Grad4<G> rg[kUnits];
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                const int64_t i = u0 + u * kUnit + lane * 4;
+                rg[u].load(gp + i);
+                rp[u] = *reinterpret_cast<const f32x4_el*>(t.p + i);
+                if constexpr (S8) {
+                    cm[u] = *reinterpret_cast<const u32_el*>(static_cast<const uint8_t*>(t.m) + i);
+                    cv[u] = *reinterpret_cast<const u32_el*>(static_cast<const uint8_t*>(t.v) + i);
+                    sm[u] = t.ms[(u0 >> 8) + u];
+                    sv[u] = t.vs[(u0 >> 8) + u];
+                } else {
+                    rm[u] = *reinterpret_cast<const f32x4_el*>(static_cast<const float*>(t.m) + i);
+                    rv[u] = *reinterpret_cast<const f32x4_el*>(static_cast<const float*>(t.v) + i);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                const int64_t i = u0 + u * kUnit + lane * 4;
+                float p[4], g[4], m[4], v[4];
+                rg[u].widen(g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = rp[u][e];
+                if constexpr (S8) {
+                    decode4(cm[u], sm[u], m);
+                    decode4(cv[u], sv[u], v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] *= v[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        m[e] = rm[u][e];
+                        v[e] = rv[u][e];
+                    }
+                }
+                update(p, g, m, v);
+                *reinterpret_cast<f32x4_el*>(t.p + i) = f32x4{p[0], p[1], p[2], p[3]};
+                if constexpr (COPY >= 0)
+                    *reinterpret_cast<u32x2_el*>(t.copy + i) =
+                        u32x2{copy_bits<COPY>(p[0]) | (copy_bits<COPY>(p[1]) << 16),
+                              copy_bits<COPY>(p[2]) | (copy_bits<COPY>(p[3]) << 16)};
+                if constexpr (S8) {
+                    float s0, s1;
+                    const uint32_t c0 = encode(m, std::false_type{}, s0), c1 = encode(v, std::true_type{}, s1);
+                    *reinterpret_cast<u32_el*>(static_cast<uint8_t*>(t.m) + i) = c0;
+                    *reinterpret_cast<u32_el*>(static_cast<uint8_t*>(t.v) + i) = c1;
+                    if (lane == 0) {
+                        t.ms[(u0 >> 8) + u] = s0;
+                        t.vs[(u0 >> 8) + u] = s1;
+                    }
+                } else {
+                    *reinterpret_cast<f32x4_el*>(static_cast<float*>(t.m) + i) = f32x4{m[0], m[1], m[2], m[3]};
+                    *reinterpret_cast<f32x4_el*>(static_cast<float*>(t.v) + i) = f32x4{v[0], v[1], v[2], v[3]};
+                }
+            }
+            continue;
+        }
+        // the tensor's end: value by value; what lies past it counts as 0
+        for (int64_t ub = u0; ub < t.n && ub < u0 + kUnits * kUnit; ub += kUnit) {
+            float p[4], g[4], m[4], v[4];
+            float s0 = 0.0f, s1 = 0.0f;
+            if constexpr (S8) {
+                s0 = t.ms[ub >> 8];
+                s1 = t.vs[ub >> 8];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t i = ub + lane * 4 + e;
+                const bool in = i < t.n;
+                p[e] = in ? t.p[i] : 0.0f;
+                g[e] = in ? grad_one<G>(gp + i) : 0.0f;
+                if constexpr (S8) {
+                    float d[4];
+                    decode4(in ? static_cast<const uint8_t*>(t.m)[i] : 0u, s0, d);
+                    m[e] = in ? d[0] : 0.0f;
+                    decode4(in ? static_cast<const uint8_t*>(t.v)[i] : 0u, s1, d);
+                    v[e] = in ? d[0] * d[0] : 0.0f;
+                } else {
+                    m[e] = in ? static_cast<const float*>(t.m)[i] : 0.0f;
+                    v[e] = in ? static_cast<const float*>(t.v)[i] : 0.0f;
+                }
+            }
+            const uint32_t before = am;
+            update(p, g, m, v);
+            uint32_t c0 = 0, c1 = 0;
+            if constexpr (S8) {
+                // past the end g, m and v are 0 (f and the hyperparameters are
+                // finite or every value is lost anyway): they add nothing
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (ub + lane * 4 + e >= t.n) m[e] = v[e] = 0.0f;
+                c0 = encode(m, std::false_type{}, s0);
+                c1 = encode(v, std::true_type{}, s1);
+                if (lane == 0) {
+                    t.ms[ub >> 8] = s0;
+                    t.vs[ub >> 8] = s1;
+                }
+            }
+            am = before;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t i = ub + lane * 4 + e;
+                if (i >= t.n) continue;
+                t.p[i] = p[e];
+                if (h.absmax) am = fold_f32(am, __float_as_uint(p[e]));
+                if constexpr (COPY >= 0) t.copy[i] = (uint16_t)copy_bits<COPY>(p[e]);
+                if constexpr (S8) {
+                    static_cast<uint8_t*>(t.m)[i] = (uint8_t)(c0 >> (8 * e));
+                    static_cast<uint8_t*>(t.v)[i] = (uint8_t)(c1 >> (8 * e));
+                } else {
+                    static_cast<float*>(t.m)[i] = m[e];
+                    static_cast<float*>(t.v)[i] = v[e];
+                }
+            }
+        }
+    }
+    if (h.absmax) {
+        // patterns of non-negative values order like unsigned integers: the
+        // atomic maximum is exact in any order
+        am = wave_umax(am);
+        if (lane == 0 && am) atomicMax(h.absmax + L.idx[lo], am);
+    }
+}
+
+template <typename G, bool S8>
+void launch_copy(int copy_dtype, int blocks, const WList& L, const WHyper& h, hipStream_t st) {
+    if (copy_dtype == DF_DTYPE_BFLOAT16) adamw_kernel<G, S8, DF_DTYPE_BFLOAT16><<<blocks, kWThreads, 0, st>>>(L, h);
+    else if (copy_dtype == DF_DTYPE_HALF) adamw_kernel<G, S8, DF_DTYPE_HALF><<<blocks, kWThreads, 0, st>>>(L, h);
+    else adamw_kernel<G, S8, -1><<<blocks, kWThreads, 0, st>>>(L, h);
+}
+
+template <typename G> void launch_state(bool s8, int copy_dtype, int blocks, const WList& L, const WHyper& h,
+                                        hipStream_t st) {
+    if (s8) launch_copy<G, true>(copy_dtype, blocks, L, h, st);
+    else launch_copy<G, false>(copy_dtype, blocks, L, h, st);
+}
+
+}  // namespace
+
+}  // namespace dfk
+
+using namespace dfk;
+
+extern "C" int64_t df_adamw_scale_count(int64_t n) { return n <= 0 ? 0 : (n + kUnit - 1) / kUnit; }
+
+extern "C" int df_adamw_update(int count, const int64_t* sizes, float* const* params, int grad_dtype,
+                               const void* const* grads, int state_dtype, void* const* m, void* const* v,
+                               float* const* m_scale, float* const* v_scale, int copy_dtype, void* const* copies,
+                               float lr, float beta1, float beta2, float eps, const float* weight_decay, int timestep,
+                               const float* lr_dev, const int* timestep_dev, const float* clip_norm_dev,
+                               float max_norm, float* absmax_dev, void* stream) {
+    clear_error();
+    const char* fn = "df_adamw_update";
+    DF_CHECK(count >= 0, DF_ERR_INVALID, "%s: count = %d is negative", fn, count);
+    DF_CHECK(grad_dtype == DF_DTYPE_FLOAT32 || grad_dtype == DF_DTYPE_BFLOAT16 || grad_dtype == DF_DTYPE_HALF,
+             DF_ERR_UNSUPPORTED, "%s: gradient dtype %d not supported", fn, grad_dtype);
+    DF_CHECK(state_dtype == DF_DTYPE_FLOAT32 || state_dtype == DF_DTYPE_FP8E4M3, DF_ERR_UNSUPPORTED,
+             "%s: state dtype %d not supported", fn, state_dtype);
+    DF_CHECK(!copies || copy_dtype == DF_DTYPE_BFLOAT16 || copy_dtype == DF_DTYPE_HALF, DF_ERR_UNSUPPORTED,
+             "%s: copy dtype %d not supported", fn, copy_dtype);
+    const bool s8 = state_dtype == DF_DTYPE_FP8E4M3;
+    DF_CHECK(count == 0 || (sizes && params && grads && m && v), DF_ERR_INVALID, "%s: an array is NULL", fn);
+    DF_CHECK(count == 0 || !s8 || (m_scale && v_scale), DF_ERR_INVALID, "%s: 8-bit states without scales", fn);
+    DF_CHECK(timestep_dev || timestep >= 1, DF_ERR_INVALID, "%s: timestep = %d (the first step is 1)", fn, timestep);
+    DF_CHECK(aligned4(lr_dev) && aligned4(timestep_dev) && aligned4(clip_norm_dev) && aligned4(absmax_dev),
+             DF_ERR_ALIGN, "%s: a device scalar is not 4-byte aligned", fn);
+    const unsigned gmask = grad_dtype == DF_DTYPE_FLOAT32 ? 3u : 1u;
+    int64_t total = 0;
+    for (int i = 0; i < count; ++i) {
+        DF_CHECK(sizes[i] >= 0, DF_ERR_INVALID, "%s: sizes[%d] = %lld is negative", fn, i, (long long)sizes[i]);
+        if (sizes[i] == 0) continue;
+        total += (sizes[i] + kSpan - 1) / kSpan;
+        DF_CHECK(total < (1ll << 31), DF_ERR_INVALID, "%s: too many elements", fn);
+        DF_CHECK(params[i] && grads[i] && m[i] && v[i] && (!s8 || (m_scale[i] && v_scale[i])) && (!copies || copies[i]),
+                 DF_ERR_INVALID, "%s: a pointer of tensor %d is NULL", fn, i);
+        DF_CHECK(aligned4(params[i]) && ((uintptr_t)grads[i] & gmask) == 0 &&
+                     (s8 ? aligned4(m_scale[i]) && aligned4(v_scale[i]) : aligned4(m[i]) && aligned4(v[i])) &&
+                     (!copies || ((uintptr_t)copies[i] & 1u) == 0),
+                 DF_ERR_ALIGN, "%s: a pointer of tensor %d is not aligned to its elements", fn, i);
+    }
+    WHyper h;
+    h.lr = lr;
+    h.b1 = beta1;
+    h.b2 = beta2;
+    h.omb1 = 1.0f - beta1;
+    h.omb2 = 1.0f - beta2;
+    h.eps = eps;
+    h.max_norm = max_norm;
+    h.bc1 = bias_corr(beta1, timestep);
+    h.bc2 = bias_corr(beta2, timestep);
+    h.lr_dev = lr_dev;
+    h.step = timestep_dev;
+    h.norm = clip_norm_dev;
+    h.absmax = reinterpret_cast<uint32_t*>(absmax_dev);
+    hipStream_t st = as_stream(stream);
+    if (total == 0 && (!absmax_dev || count == 0)) return DF_OK;
+    if (absmax_dev) {
+        const uint32_t zero = 0;
+        if (int rc = df_fill(absmax_dev, count, 4, &zero, stream)) return rc;  // empty tensors stay at 0
+    }
+    for (int i = 0; i < count;) {
+        WList L{};
+        int blocks = 0, c = 0;
+        for (; i < count && c < kWList; ++i) {
+            if (sizes[i] == 0) continue;
+            L.t[c] = WTensor{params[i], grads[i], m[i], v[i], s8 ? m_scale[i] : nullptr, s8 ? v_scale[i] : nullptr,
+                             copies ? static_cast<uint16_t*>(copies[i]) : nullptr, sizes[i]};
+            L.wd[c] = weight_decay ? weight_decay[i] : 0.0f;
+            L.first[c] = blocks;
+            L.idx[c] = i;
+            blocks += (int)((sizes[i] + kSpan - 1) / kSpan);
+            ++c;
+        }
+        if (c == 0) break;
+        L.first[c] = blocks;
+        L.count = c;
+        const int cd = copies ? copy_dtype : -1;
+        if (grad_dtype == DF_DTYPE_FLOAT32) launch_state<float>(s8, cd, blocks, L, h, st);
+        else if (grad_dtype == DF_DTYPE_HALF) launch_state<f16_t>(s8, cd, blocks, L, h, st);
+        else launch_state<uint16_t>(s8, cd, blocks, L, h, st);
+    }
+    return launch_status(fn);
+}

@@ -123,6 +123,43 @@ __global__ __launch_bounds__(kOThreads) void sumsq_kernel(const NormList L, doub
     if (threadIdx.x == 0) partial[part0 + b] = acc;
 }
 
+// The same for 2-byte gradients (their squares are exact in binary32), eight
+// values per 16-byte load; any element alignment.
+typedef u32x4 u32x4_el __attribute__((aligned(2)));
+template <typename T> static __device__ __forceinline__ float widen16(uint32_t h);
+template <> __device__ __forceinline__ float widen16<uint16_t>(uint32_t h) { return bf16_to_f32(h); }
+template <> __device__ __forceinline__ float widen16<f16_t>(uint32_t h) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+template <typename T>
+__global__ __launch_bounds__(kOThreads) void sumsq16_kernel(const NormList L, double* __restrict__ partial,
+                                                            int part0) {
+    const int b = blockIdx.x;
+    const int t = owner(L.first, L.count, b);
+    const uint16_t* x = reinterpret_cast<const uint16_t*>(L.ptr[t]);
+    const int64_t n = L.n[t];
+    double acc = 0.0;
+    for (int sub = 0; sub < kNormSub; ++sub) {
+        const int64_t base = (int64_t)(b - L.first[t]) * kNormChunk + sub * kChunk;
+        if (base + kChunk <= n) {
+            constexpr int kLoads = kVec / 2;
+            const u32x4_el* xv = reinterpret_cast<const u32x4_el*>(x + base);
+            u32x4 r[kLoads];
+#pragma unroll
+            for (int k = 0; k < kLoads; ++k) r[k] = xv[k * kOThreads + threadIdx.x];
+#pragma unroll
+            for (int k = 0; k < kLoads; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc += sq(widen16<T>(r[k][i] & 0xFFFFu)) + sq(widen16<T>(r[k][i] >> 16));
+        } else {
+            for (int64_t i = base + threadIdx.x; i < n; i += kOThreads) acc += sq(widen16<T>(x[i]));
+            break;
+        }
+    }
+    acc = block_sum_f64(acc);
+    if (threadIdx.x == 0) partial[part0 + b] = acc;
+}
+
 // Stage 2: fixed-order fold of every partial; norm = RN32(sqrt(sum)).
 // A GPT-2 XL sized list leaves ~180K partials: each thread keeps kFold
 // independent loads in flight (a single dependent chain per thread made this
@@ -291,7 +328,7 @@ static int check_list(const char* fn, const void* const* ptrs, const int64_t* si
 
 // Launches sumsq_kernel over the list in groups of kNormList tensors; the
 // partials of all groups land back to back in `partial`.
-static int launch_sumsq(const float* const* grads, const int64_t* sizes, int count, double* partial,
+static int launch_sumsq(int dtype, const void* const* grads, const int64_t* sizes, int count, double* partial,
                  hipStream_t st, int* nparts) {
     int parts = 0;
     for (int i0 = 0; i0 < count;) {
@@ -300,7 +337,7 @@ static int launch_sumsq(const float* const* grads, const int64_t* sizes, int cou
         int c = 0;
         for (; i0 < count && c < kNormList; ++i0) {
             if (sizes[i0] == 0) continue;
-            L.ptr[c] = const_cast<float*>(grads[i0]);
+            L.ptr[c] = static_cast<float*>(const_cast<void*>(grads[i0]));
             L.n[c] = sizes[i0];
             L.first[c] = blocks;
             blocks += (int)norm_chunks(sizes[i0]);
@@ -309,7 +346,9 @@ static int launch_sumsq(const float* const* grads, const int64_t* sizes, int cou
         if (c == 0) break;
         L.first[c] = blocks;
         L.count = c;
-        sumsq_kernel<<<blocks, kOThreads, 0, st>>>(L, partial, parts);
+        if (dtype == DF_DTYPE_FLOAT32) sumsq_kernel<<<blocks, kOThreads, 0, st>>>(L, partial, parts);
+        else if (dtype == DF_DTYPE_HALF) sumsq16_kernel<f16_t><<<blocks, kOThreads, 0, st>>>(L, partial, parts);
+        else sumsq16_kernel<uint16_t><<<blocks, kOThreads, 0, st>>>(L, partial, parts);
         parts += blocks;
     }
     *nparts = parts;
@@ -327,14 +366,24 @@ extern "C" size_t df_grad_norm_workspace_bytes(int count, const int64_t* sizes) 
     return (size_t)(b > 0 ? b : 1) * sizeof(double);
 }
 
-static int grad_norm_impl(const char* fn, const float* const* grads, const int64_t* sizes, int count,
+static int grad_norm_impl(const char* fn, int dtype, const void* const* grads, const int64_t* sizes, int count,
                           float* norm_dev, void* ws, size_t ws_bytes, void* stream) {
     DF_CHECK(count >= 0, DF_ERR_INVALID, "%s: count = %d is negative", fn, count);
     DF_CHECK(count == 0 || (grads && sizes), DF_ERR_INVALID, "%s: grads or sizes is NULL", fn);
     DF_CHECK(norm_dev && ws, DF_ERR_INVALID, "%s: norm_dev or ws is NULL", fn);
     DF_CHECK(aligned4(norm_dev), DF_ERR_ALIGN, "%s: norm_dev is not 4-byte aligned", fn);
     DF_CHECK(((uintptr_t)ws & 7u) == 0, DF_ERR_ALIGN, "%s: ws is not 8-byte aligned", fn);
-    if (int rc = check_list(fn, reinterpret_cast<const void* const*>(grads), sizes, count, "grads")) return rc;
+    if (dtype == DF_DTYPE_FLOAT32) {
+        if (int rc = check_list(fn, grads, sizes, count, "grads")) return rc;
+    } else {
+        for (int i = 0; i < count; ++i) {
+            DF_CHECK(sizes[i] >= 0, DF_ERR_INVALID, "%s: grads size[%d] = %lld is negative", fn, i,
+                     (long long)sizes[i]);
+            DF_CHECK(sizes[i] == 0 || grads[i], DF_ERR_INVALID, "%s: grads[%d] is NULL", fn, i);
+            DF_CHECK(sizes[i] == 0 || ((uintptr_t)grads[i] & 1u) == 0, DF_ERR_ALIGN,
+                     "%s: grads[%d] is not 2-byte aligned", fn, i);
+        }
+    }
     const size_t need = df_grad_norm_workspace_bytes(count, sizes);
     DF_CHECK(ws_bytes >= need, DF_ERR_WORKSPACE, "%s: workspace %zu B < %zu B", fn, ws_bytes, need);
     DF_CHECK(total_blocks(sizes, count) < (1ll << 31), DF_ERR_INVALID, "%s: %lld blocks exceed the grid limit", fn,
@@ -342,7 +391,7 @@ static int grad_norm_impl(const char* fn, const float* const* grads, const int64
     hipStream_t st = as_stream(stream);
     double* partial = static_cast<double*>(ws);
     int nparts = 0;
-    if (int rc = launch_sumsq(grads, sizes, count, partial, st, &nparts)) return rc;
+    if (int rc = launch_sumsq(dtype, grads, sizes, count, partial, st, &nparts)) return rc;
     // nparts == 0 (no elements): the finalize pass writes norm 0
     norm_finalize_kernel<<<1, kOThreads, 0, st>>>(partial, nparts, norm_dev);
     return launch_status("norm_finalize_kernel");
@@ -351,15 +400,24 @@ static int grad_norm_impl(const char* fn, const float* const* grads, const int64
 extern "C" int df_grad_norm_f32(const float* const* grads, const int64_t* sizes, int count, float* norm_dev,
                                 void* ws, size_t ws_bytes, void* stream) {
     clear_error();
-    return grad_norm_impl("df_grad_norm_f32", grads, sizes, count, norm_dev, ws, ws_bytes, stream);
+    return grad_norm_impl("df_grad_norm_f32", DF_DTYPE_FLOAT32, reinterpret_cast<const void* const*>(grads), sizes,
+                          count, norm_dev, ws, ws_bytes, stream);
+}
+
+extern "C" int df_grad_norm(int dtype, const void* const* grads, const int64_t* sizes, int count, float* norm_dev,
+                            void* ws, size_t ws_bytes, void* stream) {
+    clear_error();
+    DF_CHECK(dtype == DF_DTYPE_FLOAT32 || dtype == DF_DTYPE_BFLOAT16 || dtype == DF_DTYPE_HALF, DF_ERR_UNSUPPORTED,
+             "df_grad_norm: dtype %d not supported", dtype);
+    return grad_norm_impl("df_grad_norm", dtype, grads, sizes, count, norm_dev, ws, ws_bytes, stream);
 }
 
 extern "C" int df_clip_grad_norm_f32(float* const* grads, const int64_t* sizes, int count, float max_norm,
                                      float* norm_dev, void* ws, size_t ws_bytes, void* stream) {
     clear_error();
     const char* fn = "df_clip_grad_norm_f32";
-    if (int rc = grad_norm_impl(fn, const_cast<const float* const*>(grads), sizes, count, norm_dev, ws, ws_bytes,
-                                stream))
+    if (int rc = grad_norm_impl(fn, DF_DTYPE_FLOAT32, reinterpret_cast<const void* const*>(grads), sizes, count,
+                                norm_dev, ws, ws_bytes, stream))
         return rc;
     hipStream_t st = as_stream(stream);
     for (int i0 = 0; i0 < count;) {

@@ -574,6 +574,53 @@ int df_adam_update_absmax_f32(float* const* params, const float* const* grads, f
                               int timestep, const float* clip_norm_dev, float max_norm,
                               float* absmax_dev, void* stream);
 
+/* df_grad_norm_f32 over gradients of one dtype (fp32, bf16, f16; 2-byte ones
+ * at any element alignment), for df_adamw_update's clip_norm_dev; the same
+ * workspace.  No reference counterpart for the 2-byte types. */
+int df_grad_norm(int dtype, const void* const* grads, const int64_t* sizes, int count,
+                 float* norm_dev, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- AdamW over lists of tensors (decoupled weight decay; new: the
+ * reference's Adam couples it, dnn/optimizers/adam_optimizer.cu:24-30) ----
+ * One step, in place, over `count` tensors of sizes[i] elements (0: skipped);
+ * every array is a HOST array of `count` entries, the pointers in them DEVICE
+ * pointers aligned to their elements:
+ *   g = grad * f;  m = b1*m + (1-b1)*g;  v = b2*v + ((1-b2)*g)*g;
+ *   p = p*(1 - lr*wd) - (lr*(m / (1-b1^t))) / (sqrt(v / (1-b2^t)) + eps)
+ * every operation rounded to binary32 as written, IEEE division and square
+ * root; f = max_norm / norm when clip_norm_dev is non-NULL and norm =
+ * clip_norm_dev[0] > max_norm, else 1.
+ *  params       : fp32.
+ *  grads        : of grad_dtype, fp32, bf16 or f16.
+ *  m, v         : state_dtype DF_DTYPE_FLOAT32: fp32, the values (m_scale and
+ *                 v_scale are not used); DF_DTYPE_FP8E4M3: e4m3 codes, value i
+ *                 of a tensor being code * scale[i / 256] for m and
+ *                 (code * scale[i / 256])^2 for v, with df_adamw_scale_count(
+ *                 sizes[i]) fp32 scales in m_scale[i] and v_scale[i].  The
+ *                 update uses the new binary32 m and v; they are then kept as
+ *                 codes of m and of sqrt(v) at max / 448 over the finite
+ *                 values of each 256 (at least 2^-126; 1 where all are 0),
+ *                 rounded to nearest even and saturated, NaN as 0x7F, a
+ *                 sqrt(v) above 0 at least code 1.  All codes 0 at any finite
+ *                 scale is the state before the first step.
+ *  copies       : NULL, or per tensor the updated p in copy_dtype (bf16, f16).
+ *  weight_decay : wd per tensor, or NULL (0).
+ *  timestep     : t >= 1, the already-incremented step count; with
+ *                 timestep_dev non-NULL t is read there when the kernel runs
+ *                 (below 1: 1), and with lr_dev lr is: a captured call then
+ *                 follows both on replay.
+ *  absmax_dev   : NULL, or a device array: max |p| over the finite values of
+ *                 updated tensor i (0 for an empty one), for
+ *                 df_quantize_2d_batch_absmax.
+ * What is written (params, states, scales, copies) must not overlap. */
+int64_t df_adamw_scale_count(int64_t n);  /* ceil(n / 256) */
+int df_adamw_update(int count, const int64_t* sizes, float* const* params, int grad_dtype,
+                    const void* const* grads, int state_dtype, void* const* m, void* const* v,
+                    float* const* m_scale, float* const* v_scale, int copy_dtype, void* const* copies,
+                    float lr, float beta1, float beta2, float eps, const float* weight_decay,
+                    int timestep, const float* lr_dev, const int* timestep_dev,
+                    const float* clip_norm_dev, float max_norm, float* absmax_dev, void* stream);
+
 /* ---- tensor utilities behind dnn::tensor (dnn/core/tensor.cu:18-52) ---- */
 /* fill_kernel (tensor.cu:19): n elements of elem_bytes (1, 2 or 4) = *value */
 int df_fill(void* dst, int64_t n, int elem_bytes, const void* value_host, void* stream);
