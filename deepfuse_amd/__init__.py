@@ -114,6 +114,12 @@ _SIGS = {
     "df_fp8_gemm_bwd_absmax": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int,
                                         _vp, _vp, _vp, _c_int, _vp, _c_int, _c_int, _vp, _c_int, _c_int, _vp, _vp,
                                         _vp, _c_sz, _vp]),
+    "df_fp8_experts_fwd": (_c_int, [_vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp,
+                                    _c_int, _vp]),
+    "df_fp8_experts_dx": (_c_int, [_vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp,
+                                   _c_int, _vp]),
+    "df_fp8_experts_dw": (_c_int, [_vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp,
+                                   _c_int, _vp]),
     "df_fill": (_c_int, [_vp, _c_i64, _c_int, _vp, _vp]),
     "df_add": (_c_int, [_c_int, _vp, _vp, _vp, _c_i64, _vp]),
     "df_convert": (_c_int, [_c_int, _vp, _c_int, _vp, _c_i64, _vp]),
@@ -897,3 +903,126 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
              sv, int(ct), arrays[-1] if copies is not None else None, 0.0 if "lr" in scalars else float(lr), float(beta1),
              float(beta2), float(eps), wd, 0 if "timestep" in scalars else int(timestep), scalars.get("lr"),
              scalars.get("timestep"), scalars.get("clip_norm"), float(max_norm), _ptr(absmax), _stream())
+
+
+# ----------------------------------------------------------------------------
+# products grouped by expert
+# ----------------------------------------------------------------------------
+def _experts_args(fn: str, offsets, scale, scales, experts: int, count: int, **codes):
+    """Checks shared by the experts' products: devices, the offsets, the scales and the codes' layout."""
+    torch = _torch()
+    _check_gpu(fn, offsets=offsets, scale=scale, scales=scales, **codes)
+    _row_vector(fn, "offsets", offsets, experts + 1, torch.int32)
+    for name, t, n in (("scale", scale, 1), ("scales", scales, count)):
+        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{fn}: the {name} {tuple(t.shape)} {t.dtype} is not {n} contiguous fp32 values")
+    for name, t in codes.items():
+        if t.dtype != torch.uint8 or t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{fn}: {name} is not uint8 codes with contiguous rows")
+        if t.dim() == 3 and t.shape[0] > 1 and t.stride(0) != t.shape[1] * t.stride(1):
+            raise ValueError(f"{fn}: the experts of {name} do not follow each other")
+
+
+def _experts_out(fn: str, out, shape, dtype, device):
+    torch = _torch()
+    if out is None:
+        return torch.empty(shape, dtype=dtype or torch.bfloat16, device=device)
+    if tuple(out.shape) != tuple(shape) or (dtype is not None and out.dtype != dtype) or out.device != device:
+        raise ValueError(f"{fn}: out is {tuple(out.shape)} {out.dtype} on {out.device}, not {tuple(shape)} on {device}")
+    if out.dim() == 2:
+        _rows(fn, "out", out, shape, out.dtype)
+    elif not out.is_contiguous():
+        raise ValueError(f"{fn}: out is not contiguous")
+    return out
+
+
+def _experts_rows(fn: str, c_fn: str, a_q, w_q, offsets, red: int, sa, sw, out_dtype, out):
+    if a_q.dim() != 2 or w_q.dim() != 3:
+        raise ValueError(f"{fn}: codes of {a_q.dim()} and {w_q.dim()} dimensions, not 2 and 3")
+    experts, cols = w_q.shape[0], w_q.shape[1]
+    _experts_args(fn, offsets, sa, sw, experts, experts, rows=a_q, weights=w_q)
+    if a_q.shape[1] < red or w_q.shape[2] < red:
+        raise ValueError(f"{fn}: rows of {a_q.shape[1]} and {w_q.shape[2]} codes, fewer than {red}")
+    rows = a_q.shape[0]
+    out = _experts_out(fn, out, (rows, cols), out_dtype, a_q.device)
+    n, k = (cols, red) if c_fn == "df_fp8_experts_fwd" else (red, cols)
+    with _on(a_q):
+        call(c_fn, _ptr(a_q), a_q.stride(0), _ptr(w_q), w_q.stride(1), rows, n, k, experts, _ptr(offsets), _ptr(sa),
+             _ptr(sw), int(_in_dtype(out)), _ptr(out), out.stride(0), _stream())
+    return out
+
+
+def experts_fwd(x_q, w_q, offsets, K: int, sx, sw, out_dtype=None, out=None):
+    """Y [rows, N] of a Linear dealt to experts (df_fp8_experts_fwd): x_q
+    [rows, >=K] and w_q [experts, N, >=K] e4m3 codes, offsets int32
+    [experts + 1] (expert e has rows offsets[e] to offsets[e+1], on the
+    device), sx one scale, sw one per expert.  ``out`` keeps its rows that
+    belong to no expert; a new output (bf16 unless out_dtype says otherwise)
+    has them undefined."""
+    return _experts_rows("experts_fwd", "df_fp8_experts_fwd", x_q, w_q, offsets, K, sx, sw, out_dtype, out)
+
+
+def experts_dx(dy_q, wt_q, offsets, N: int, sdy, sw, out_dtype=None, out=None):
+    """dX [rows, K] (df_fp8_experts_dx): dy_q [rows, >=N] e5m2 codes, wt_q
+    [experts, K, >=N] the transposed e4m3 codes of each expert's weights."""
+    return _experts_rows("experts_dx", "df_fp8_experts_dx", dy_q, wt_q, offsets, N, sdy, sw, out_dtype, out)
+
+
+def experts_dw(dyt_q, xt_q, offsets, rows: int, sdy, sx, out_dtype=None, out=None):
+    """dW [experts, N, K] (df_fp8_experts_dw; fp32 unless out_dtype or ``out``
+    says otherwise): dyt_q [N, >=rows] e5m2 and xt_q [K, >=rows] e4m3, the
+    transposed codes of all rows."""
+    fn, torch = "experts_dw", _torch()
+    if dyt_q.dim() != 2 or xt_q.dim() != 2:
+        raise ValueError(f"{fn}: codes of {dyt_q.dim()} and {xt_q.dim()} dimensions, not 2")
+    if offsets.dim() != 1 or offsets.numel() < 1:
+        raise ValueError(f"{fn}: offsets {tuple(offsets.shape)} are not experts + 1 values")
+    experts = offsets.numel() - 1
+    _experts_args(fn, offsets, sdy, sx, experts, 1, dyt_q=dyt_q, xt_q=xt_q)
+    if dyt_q.shape[1] < rows or xt_q.shape[1] < rows:
+        raise ValueError(f"{fn}: rows of {dyt_q.shape[1]} and {xt_q.shape[1]} codes, fewer than {rows}")
+    N, K = dyt_q.shape[0], xt_q.shape[0]
+    if out is None and out_dtype is None:
+        out_dtype = torch.float32
+    out = _experts_out(fn, out, (experts, N, K), out_dtype, dyt_q.device)
+    with _on(dyt_q):
+        call("df_fp8_experts_dw", _ptr(dyt_q), dyt_q.stride(0), _ptr(xt_q), xt_q.stride(0), rows, N, K, experts,
+             _ptr(offsets), _ptr(sdy), _ptr(sx), int(_in_dtype(out)), _ptr(out), K, _stream())
+    return out
+
+
+def quantize_experts(w, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=True):
+    """Codes of the experts' weights w [experts, N, K] (contiguous fp32, bf16
+    or float16) at a just-in-time scale per expert, laid out for the products
+    above: returns (scales [experts], q [experts, N, ceil16(K)] or None, qt
+    [experts, K, ceil16(N)] or None)."""
+    fn, torch = "quantize_experts", _torch()
+    if w.dim() != 3 or not w.is_contiguous():
+        raise ValueError(f"{fn}: w {tuple(w.shape)} is not [experts, N, K] and contiguous")
+    if not (want_q or want_qt):
+        raise ValueError(f"{fn}: no codes wanted")
+    _check_gpu(fn, w=w)
+    E, N, K = w.shape
+    dt = int(_in_dtype(w))
+    with _on(w):
+        src = w.view(E, N * K)
+        if src.stride(0) * w.element_size() % 16:  # the batched quantize takes tensors at 16-byte boundaries
+            src = torch.nn.functional.pad(src, (0, -src.shape[1] % 16))
+        new = lambda r, c: torch.empty((E, r, round16(c)), dtype=torch.uint8, device=w.device)
+        q, qt = new(N, K) if want_q else None, new(K, N) if want_qt else None
+        sc = torch.empty(E, dtype=torch.float32, device=w.device)
+        ldq, ldqt = round16(K) if want_q else 0, round16(N) if want_qt else 0
+        if w.dtype == torch.float16:  # the batched quantize takes fp32 and bf16
+            ws = torch.empty(int(lib().df_quantize_2d_jit_workspace_bytes(N, K, 0)), dtype=torch.uint8, device=w.device)
+            for e in range(E):
+                call("df_quantize_2d_jit", dt, _ptr(src[e]), N, K, int(fmt), None, _ptr(sc[e:]),
+                     _ptr(q[e]) if want_q else None, ldq, _ptr(qt[e]) if want_qt else None, ldqt, None, _ptr(ws),
+                     ws.numel(), _stream())
+            return sc, q, qt
+        am = torch.empty(E, dtype=torch.float32, device=w.device)
+        ws = torch.empty(int(lib().df_quantize_2d_batch_workspace_bytes()), dtype=torch.uint8, device=w.device)
+        arr, ptrs = lambda v: (_c_int * E)(*[v] * E), lambda t: (_vp * E)(*[x.data_ptr() for x in t])
+        call("df_quantize_2d_batch", dt, E, ptrs(src), arr(N), arr(K), int(fmt), _ptr(am), _ptr(sc),
+             ptrs(q) if want_q else None, arr(ldq) if want_q else None, ptrs(qt) if want_qt else None,
+             arr(ldqt) if want_qt else None, _ptr(ws), ws.numel(), _stream())
+    return sc, q, qt

@@ -1,0 +1,342 @@
+// gemm_experts.hip -- the fp8 products of a Linear whose rows are dealt to
+// experts (a mixture of experts): rows sorted by expert, expert e owning rows
+// off[e] .. off[e+1) of the tokens, with weights of its own:
+//   forward  Y[i]  = X[i]  . W[e]^T * sx  * sw[e]      (e4m3 x e4m3)
+//   dX       dX[i] = dY[i] . W[e]   * sdy * sw[e]      (e5m2 x e4m3)
+//   dW       dW[e] = sum over e's rows of dY^T . X * sdy * sx   (e5m2 x e4m3)
+// The offsets are read on the device, so nothing waits for the host to learn
+// how the rows were dealt.  ROWS calls (forward, dX) cut the rows of each
+// expert into tiles; SUMS calls (dW) reduce over the tokens, whose range for
+// an expert starts and ends at any byte of the transposed operands' rows: the
+// bytes of the neighbouring experts in the first and last 16-byte chunk are
+// cleared on both operands (a neighbour's NaN would outlive a zero on one).
+//
+// Two ways to multiply.  The fp8 matrix instructions add their products in
+// groups of eight along K and drop what lies 13 bits below the largest of a
+// group (measured: 2^16 + 2^3 keeps both, 2^16 + 2^2 loses the second; across
+// groups and into the accumulator 23 bits are kept).  That is up to 7 * 2^-13
+// of a group's largest product, in random data about 1e-5 of a result: below a
+// 2-byte output's rounding, but not below an fp32 output's.  So calls with a
+// 2-byte output use them, and calls with an fp32 output widen the codes to
+// bf16 (exact, v_cvt_scalef32_pk_bf16_*) in registers, whose products the bf16
+// instructions add with all 23 bits, at half the matrix rate.
+//
+// Offsets are clamped into [0, rows] and to be non-decreasing per expert, so a
+// wrong one gives wrong values but no access outside the operands.
+//
+// The reference has no mixture of experts; per expert this is
+// fully_connected_forward_kernel, fc_backward_input and fc_backward_weights
+// (dnn/layers/fully_connected_layer.cu:14-89).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "df_common.hpp"
+#include "gemm_common.hpp"
+
+namespace dfk {
+
+namespace {
+
+constexpr int kMaxExperts = 1024;
+
+// One call.  ROWS: A [rows, lda], B [experts][N][ldb], C [rows, ldc], reduction K.
+// SUMS: A [M, lda], B [N, ldb], C [experts][M][ldc], reduction over the tokens.
+struct ExpertArgs {
+    const uint8_t* A;
+    const uint8_t* B;
+    void* C;
+    const int* off;
+    const float* sa;
+    const float* sb;
+    int lda, ldb, ldc, rows, M, N, K, experts, vec_out;
+};
+
+// expert e's rows, whatever the offsets hold
+__device__ __forceinline__ void expert_rows(const int* off, int e, int rows, int& lo, int& hi) {
+    lo = min(max(off[e], 0), rows);
+    hi = min(max(off[e + 1], lo), rows);
+}
+
+// bytes of a dword at byte position `pos` that lie in [lo, hi)
+__device__ __forceinline__ uint32_t keep_bytes(int pos, int lo, int hi) {
+    const int a = min(max(lo - pos, 0), 4) * 8, b = min(max(hi - pos, 0), 4) * 8;
+    const uint32_t upto = b == 32 ? ~0u : (1u << b) - 1u, below = a == 32 ? ~0u : (1u << a) - 1u;
+    return upto & ~below;
+}
+
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+
+// eight codes -> bf16, exact
+template <int FMT> __device__ __forceinline__ bf8 widen8(uint32_t lo, uint32_t hi) {
+    bf2 p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i < 2 ? lo : hi;
+        if constexpr (FMT == E4M3)
+            p[i] = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
+                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
+        else
+            p[i] = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, true)
+                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, false);
+    }
+    return bf8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+}
+
+// ------------------------------------------------------------ small tiles --
+// As gemm_small.hip's kernel: a block owns a 16*MT x 16*NT tile, its W waves
+// take the 128-byte K steps in turn and add up through LDS, in wave order.
+// ROWS: blockIdx.y is the expert, whose row tiles blockIdx.z, + gridDim.z, ...
+// the block computes.  SUMS: blockIdx.x is the tile, blockIdx.y the expert.
+// WIDE: codes are multiplied as bf16, eight of a lane's 32 at a time: which K
+// an instruction takes together is free as long as A and B agree.
+template <int FA, int FB, int MT, int NT, int W, int U, bool SUMS, bool WIDE>
+__global__ __launch_bounds__(64 * W) void experts_small_kernel(const ExpertArgs g, int c_dtype) {
+    constexpr int ROWS = 16 * MT, COLS = 16 * NT;
+    constexpr int NL = 2 * (MT + NT);  // loads of 8 rows x 128 bytes per step
+    constexpr int SLAB = NL * 1024;    // a wave's step: A rows, then B rows
+    constexpr int RSTR = COLS + 4;     // row of a partial tile (floats)
+    constexpr int RED = ROWS * RSTR * 4;
+    constexpr uint32_t kOOB = 0x80000000u;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[W * (SLAB > RED ? SLAB : RED)];
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int e = blockIdx.y;
+    int lo, hi;
+    expert_rows(g.off, e, g.rows, lo, hi);
+    const int tiles_n = (g.N + COLS - 1) / COLS;
+    const int n0 = (SUMS ? (int)(blockIdx.x % tiles_n) : (int)blockIdx.x) * COLS;
+    const int mbeg = SUMS ? (int)(blockIdx.x / tiles_n) * ROWS : lo + (int)blockIdx.z * ROWS;
+    const int mend = SUMS ? min(mbeg + 1, g.M) : hi;  // SUMS: one tile
+    // the reduction's bytes [k_lo, k_hi) of the operands' rows, in steps of 128 from kb
+    const int kb = SUMS ? lo & ~127 : 0, k_lo = SUMS ? lo : 0, k_hi = SUMS ? hi : g.K;
+    const int nk = (k_hi - kb + 127) >> 7;
+    const uint8_t* const Be = g.B + (SUMS ? 0 : (int64_t)e * g.N * g.ldb) + (int64_t)n0 * g.ldb;
+    const __amdgpu_buffer_rsrc_t rB = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)Be, (short)0, min(g.N - n0, COLS) * g.ldb, 0x00020000);
+    const float sab = g.sa[0] * g.sb[SUMS ? 0 : e];
+
+    // loads: lane l takes 16-byte chunk l%8 of row l/8 of each 8-row group
+    const int lr = lane >> 3, lc = (lane & 7) * 16;
+    const uint32_t oa = (uint32_t)lr * (uint32_t)g.lda + (uint32_t)lc;
+    const uint32_t ob = (uint32_t)lr * (uint32_t)g.ldb + (uint32_t)lc;
+    // slab: rows of 128 bytes, 16-byte chunk c of row r in slot c ^ (r/2 % 8)
+    uint8_t* const slab = lds + w * SLAB;
+    const int wr_even = lr * 128 + (((lane & 7) ^ (lr >> 1)) << 4);
+    const int wr_odd = wr_even ^ 64;
+    const int fr = lane & 15, fq = (lane >> 4) * 2, fs = (fr >> 1) & 7;
+    const int rd0 = fr * 128 + ((fq ^ fs) << 4), rd1 = fr * 128 + (((fq + 1) ^ fs) << 4);
+    // the lanes of a wave hand chunks to each other through the slab: LDS
+    // operations of a wave execute in order, the compiler must keep that order
+    auto lanes_meet = [] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    };
+
+    for (int m0 = mbeg; m0 < mend; m0 += SUMS ? ROWS : (int)gridDim.z * ROWS) {
+        const int mrows = min((SUMS ? g.M : hi) - m0, ROWS);
+        const __amdgpu_buffer_rsrc_t rA = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(g.A + (int64_t)m0 * g.lda), (short)0, mrows * g.lda, 0x00020000);
+        u32x4 buf[U][NL];
+        auto load = [&](u32x4* b, int s) {
+            const int k = kb + s * 128;  // past the last step: every chunk out of range
+            const bool in = k + lc < k_hi && (!SUMS || k + lc + 16 > k_lo);
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+                b[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                    rA, in ? oa + (uint32_t)(8 * i) * (uint32_t)g.lda + (uint32_t)k : kOOB, 0, 0));
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i)
+                b[2 * MT + i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                    rB, in ? ob + (uint32_t)(8 * i) * (uint32_t)g.ldb + (uint32_t)k : kOOB, 0, 0));
+        };
+        v4f acc[MT][NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        // fragment t (16 rows) of a step in registers, through its part of the slab
+        auto frag = [&](const u32x4* b, int t) -> v8i {
+            *reinterpret_cast<u32x4*>(slab + t * 2048 + wr_even) = b[2 * t];
+            *reinterpret_cast<u32x4*>(slab + t * 2048 + 1024 + wr_odd) = b[2 * t + 1];
+            lanes_meet();
+            const u32x4 x = *reinterpret_cast<const u32x4*>(slab + t * 2048 + rd0);
+            const u32x4 y = *reinterpret_cast<const u32x4*>(slab + t * 2048 + rd1);
+            v8i f;
+            f[0] = (int)x.x; f[1] = (int)x.y; f[2] = (int)x.z; f[3] = (int)x.w;
+            f[4] = (int)y.x; f[5] = (int)y.y; f[6] = (int)y.z; f[7] = (int)y.w;
+            return f;
+        };
+        auto step = [&](u32x4* b, int s) {
+            if (SUMS && (s == 0 || s == nk - 1)) {  // the neighbours' bytes of the edge chunks
+                const int k = kb + s * 128 + lc;
+                u32x4 keep;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) keep[d] = keep_bytes(k + 4 * d, k_lo, k_hi);
+#pragma unroll
+                for (int i = 0; i < NL; ++i) b[i] &= keep;
+            }
+            lanes_meet();  // the step before has read the slab
+            v8i fb[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) fb[j] = frag(b, MT + j);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const v8i fa = frag(b, i);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if constexpr (WIDE) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                widen8<FB>((uint32_t)fb[j][2 * q], (uint32_t)fb[j][2 * q + 1]),
+                                widen8<FA>((uint32_t)fa[2 * q], (uint32_t)fa[2 * q + 1]), acc[i][j], 0, 0, 0);
+                    } else {
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, acc[i][j], FB, FA, 0,
+                                                                                     0, 0, 0);
+                    }
+                }
+            }
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(buf[u], w + u * W);
+        for (int s = w; s < nk; s += W * U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (s + u * W < nk) step(buf[u], s + u * W);
+                load(buf[u], s + (u + U) * W);
+            }
+        }
+        // accumulators are C^T: lane l holds row l%16 and columns 4*(l/16) .. +4
+        __syncthreads();
+        float* const red = reinterpret_cast<float*>(lds);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                *reinterpret_cast<v4f*>(red + (w * ROWS + 16 * i + fr) * RSTR + 16 * j + 4 * (lane >> 4)) = acc[i][j];
+        __syncthreads();
+        for (int x = threadIdx.x; x < ROWS * COLS / 4; x += 64 * W) {
+            const int r = x / (COLS / 4), c = (x % (COLS / 4)) * 4, col = n0 + c;
+            if (r >= mrows || col >= g.N) continue;
+            v4f t = *reinterpret_cast<const v4f*>(red + r * RSTR + c);
+#pragma unroll
+            for (int v = 1; v < W; ++v) t += *reinterpret_cast<const v4f*>(red + (v * ROWS + r) * RSTR + c);
+            float o[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) o[y] = t[y] * sab;
+            auto put = [&](auto* p) {
+                using T = typename std::remove_reference<decltype(*p)>::type;
+                if (g.vec_out && col + 3 < g.N) {
+                    store4(p, o);
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        if (col + y < g.N) p[y] = OutCvt<T>::cvt(o[y]);
+                }
+            };
+            const int64_t at = ((SUMS ? (int64_t)e * g.M : 0) + m0 + r) * g.ldc + col;
+            if (c_dtype == DF_DTYPE_FLOAT32) put(static_cast<float*>(g.C) + at);
+            else if (c_dtype == DF_DTYPE_HALF) put(static_cast<f16_t*>(g.C) + at);
+            else put(static_cast<uint16_t*>(g.C) + at);
+        }
+        __syncthreads();  // the partial tiles are read before slabs go over them
+    }
+}
+
+template <int FA, bool SUMS, bool WIDE> void launch_small(const ExpertArgs& g, int c_dtype, hipStream_t st) {
+    if constexpr (SUMS) {
+        const dim3 grid(((g.N + 31) / 32) * ((g.M + 31) / 32), g.experts);
+        experts_small_kernel<FA, E4M3, 2, 2, 4, 2, true, WIDE><<<grid, 256, 0, st>>>(g, c_dtype);
+    } else {
+        const int per = (g.rows + g.experts - 1) / g.experts;  // rows of an expert if dealt evenly
+        if (per <= 16) {
+            const dim3 grid((g.N + 15) / 16, g.experts, 1);
+            experts_small_kernel<FA, E4M3, 1, 1, 4, 4, false, WIDE><<<grid, 256, 0, st>>>(g, c_dtype);
+        } else {
+            const dim3 grid((g.N + 31) / 32, g.experts, std::min((per + 31) / 32, 64));
+            experts_small_kernel<FA, E4M3, 2, 2, 4, 2, false, WIDE><<<grid, 256, 0, st>>>(g, c_dtype);
+        }
+    }
+}
+
+template <int FA, bool SUMS> void launch(ExpertArgs& g, int c_dtype, hipStream_t st) {
+    const int esz = c_dtype == DF_DTYPE_FLOAT32 ? 4 : 2;
+    g.vec_out = ((int64_t)g.ldc * esz) % 16 == 0 && aligned16(g.C);
+    if (c_dtype == DF_DTYPE_FLOAT32) launch_small<FA, SUMS, true>(g, c_dtype, st);
+    else launch_small<FA, SUMS, false>(g, c_dtype, st);
+}
+
+// Checks of one call; `empty`: nothing to compute.
+int check_call(const char* fn, const ExpertArgs& g, int K, bool sums, int c_dtype, bool& empty) {
+    DF_CHECK(g.rows >= 0 && g.M >= 0 && g.N >= 0 && K >= 0 && g.experts >= 0, DF_ERR_INVALID,
+             "%s: a negative size (rows=%d, experts=%d)", fn, g.rows, g.experts);
+    DF_CHECK(g.experts <= kMaxExperts, DF_ERR_UNSUPPORTED, "%s: %d experts (at most %d)", fn, g.experts, kMaxExperts);
+    DF_CHECK(c_dtype == DF_DTYPE_FLOAT32 || c_dtype == DF_DTYPE_BFLOAT16 || c_dtype == DF_DTYPE_HALF,
+             DF_ERR_UNSUPPORTED, "%s: output dtype %d not supported", fn, c_dtype);
+    DF_CHECK((int64_t)((g.N + 15) / 16) * (sums ? (g.M + 15) / 16 : 1) < (1ll << 31), DF_ERR_INVALID,
+             "%s: output too large", fn);
+    empty = g.experts == 0 || g.N == 0 || (sums ? g.M == 0 : g.rows == 0);
+    if (empty) return DF_OK;
+    DF_CHECK(g.ldc >= g.N, DF_ERR_INVALID, "%s: output leading dimension %d < %d", fn, g.ldc, g.N);
+    DF_CHECK(g.C && g.off && g.sa && g.sb, DF_ERR_INVALID, "%s: NULL pointer", fn);
+    const int red = sums ? g.rows : K;
+    DF_CHECK((g.A && g.B) || red == 0, DF_ERR_INVALID, "%s: NULL operand", fn);
+    DF_CHECK(red == 0 || (g.lda >= red && g.ldb >= red && g.lda % 16 == 0 && g.ldb % 16 == 0), DF_ERR_ALIGN,
+             "%s: operand leading dimensions %d and %d must be multiples of 16 and >= %d", fn, g.lda, g.ldb, red);
+    DF_CHECK(g.lda >= 0 && g.ldb >= 0 && g.lda < (1 << 23) && g.ldb < (1 << 23), DF_ERR_UNSUPPORTED,
+             "%s: operand leading dimensions %d and %d (below 2^23)", fn, g.lda, g.ldb);
+    DF_CHECK(aligned16(g.A) && aligned16(g.B), DF_ERR_ALIGN, "%s: operands must be 16-byte aligned", fn);
+    DF_CHECK(aligned4(g.off) && aligned4(g.sa) && aligned4(g.sb), DF_ERR_ALIGN, "%s: offsets or scales misaligned", fn);
+    DF_CHECK(((uintptr_t)g.C & (c_dtype == DF_DTYPE_FLOAT32 ? 3u : 1u)) == 0, DF_ERR_ALIGN,
+             "%s: output is not aligned to its elements", fn);
+    return DF_OK;
+}
+
+}  // namespace
+
+}  // namespace dfk
+
+using namespace dfk;
+
+extern "C" int df_fp8_experts_fwd(const uint8_t* Xq, int ldx, const uint8_t* Wq, int ldw, int rows, int N, int K,
+                                  int experts, const int* offsets_dev, const float* sx_dev, const float* sw_dev,
+                                  int y_dtype, void* Y, int ldy, void* stream) {
+    clear_error();
+    const char* fn = "df_fp8_experts_fwd";
+    ExpertArgs g{Xq, Wq, Y, offsets_dev, sx_dev, sw_dev, ldx, ldw, ldy, rows, 0, N, (K + 15) & ~15, experts, 0};
+    bool empty = false;
+    if (int rc = check_call(fn, g, K, false, y_dtype, empty)) return rc;
+    if (empty) return DF_OK;
+    launch<E4M3, false>(g, y_dtype, as_stream(stream));
+    return launch_status(fn);
+}
+
+extern "C" int df_fp8_experts_dx(const uint8_t* dYq, int lddy, const uint8_t* Wtq, int ldwt, int rows, int N, int K,
+                                 int experts, const int* offsets_dev, const float* sdy_dev, const float* sw_dev,
+                                 int dx_dtype, void* dX, int lddx, void* stream) {
+    clear_error();
+    const char* fn = "df_fp8_experts_dx";
+    ExpertArgs g{dYq, Wtq, dX, offsets_dev, sdy_dev, sw_dev, lddy, ldwt, lddx, rows, 0, K, (N + 15) & ~15, experts, 0};
+    bool empty = false;
+    if (int rc = check_call(fn, g, N, false, dx_dtype, empty)) return rc;
+    if (empty) return DF_OK;
+    launch<E5M2, false>(g, dx_dtype, as_stream(stream));
+    return launch_status(fn);
+}
+
+extern "C" int df_fp8_experts_dw(const uint8_t* dYtq, int lddyt, const uint8_t* Xtq, int ldxt, int rows, int N, int K,
+                                 int experts, const int* offsets_dev, const float* sdy_dev, const float* sx_dev,
+                                 int dw_dtype, void* dW, int lddw, void* stream) {
+    clear_error();
+    const char* fn = "df_fp8_experts_dw";
+    ExpertArgs g{dYtq, Xtq, dW, offsets_dev, sdy_dev, sx_dev, lddyt, ldxt, lddw, rows, N, K, 0, experts, 0};
+    bool empty = false;
+    if (int rc = check_call(fn, g, 0, true, dw_dtype, empty)) return rc;
+    if (empty) return DF_OK;
+    launch<E5M2, true>(g, dw_dtype, as_stream(stream));
+    return launch_status(fn);
+}

@@ -471,6 +471,44 @@ int df_fp8_gemm_bwd_absmax(const uint8_t* dYq, int lddy, const uint8_t* Wtq, int
                            float* dx_absmax_dev, float* dx_scale_dev,
                            void* ws, size_t ws_bytes, void* stream);
 
+/* ---- fp8 products grouped by expert (new: the reference has no mixture of
+ * experts; per expert these replace fully_connected_forward_kernel,
+ * fc_backward_input and fc_backward_weights,
+ * dnn/layers/fully_connected_layer.cu:14-89) ----
+ * The Linear of `experts` (<= 1024) experts with weights W[e] [N, K], over
+ * `rows` rows sorted by expert: expert e has rows offsets_dev[e] <= i <
+ * offsets_dev[e+1] (int32 [experts + 1] on the device, non-decreasing within
+ * [0, rows]; read there, never by the host).  Any number of rows per expert,
+ * none included.
+ *  df_fp8_experts_fwd : Y[i]  = (X[i]  . W[e]^T) * sx * sw[e], e4m3 x e4m3:
+ *                       Xq [rows, ldx], Wq [experts][N][ldw].
+ *  df_fp8_experts_dx  : dX[i] = (dY[i] . W[e]) * sdy * sw[e], e5m2 x e4m3:
+ *                       dYq [rows, lddy], Wtq [experts][K][ldwt] (the
+ *                       transposed codes of each W[e]).
+ *  df_fp8_experts_dw  : dW[e] = (sum over e's rows of dY[i]^T X[i]) * sdy *
+ *                       sx, e5m2 x e4m3: dYtq [N, lddyt] and Xtq [K, ldxt], the
+ *                       transposed codes of all rows; dW [experts][N][lddw],
+ *                       overwritten (zeros for an expert without rows).
+ * sx, sdy: device scalars; sw: device, one per expert.  Codes as
+ * df_quantize_2d and df_quantize_2d_batch write them: leading dimensions
+ * multiples of 16 below 2^23, 16-byte aligned, zero codes up to the next
+ * multiple of 16 of the reduction (the forward and dX; dW needs none).
+ * Outputs fp32, bf16 or f16, rounded once from fp32 accumulation.  An fp32
+ * output is the fp32 sum of exact products (bf16 matrix instructions); a
+ * 2-byte output takes the fp8 ones, twice as fast, which drop what lies 13
+ * bits below the largest of each eight products.  Rows of Y
+ * and dX that belong to no expert are left as they are.  Offsets outside
+ * [0, rows] or decreasing give wrong values, but no access out of bounds. */
+int df_fp8_experts_fwd(const uint8_t* Xq, int ldx, const uint8_t* Wq, int ldw, int rows, int N, int K,
+                       int experts, const int* offsets_dev, const float* sx_dev, const float* sw_dev,
+                       int y_dtype, void* Y, int ldy, void* stream);
+int df_fp8_experts_dx(const uint8_t* dYq, int lddy, const uint8_t* Wtq, int ldwt, int rows, int N,
+                      int K, int experts, const int* offsets_dev, const float* sdy_dev,
+                      const float* sw_dev, int dx_dtype, void* dX, int lddx, void* stream);
+int df_fp8_experts_dw(const uint8_t* dYtq, int lddyt, const uint8_t* Xtq, int ldxt, int rows, int N,
+                      int K, int experts, const int* offsets_dev, const float* sdy_dev,
+                      const float* sx_dev, int dw_dtype, void* dW, int lddw, void* stream);
+
 /* ---- layer weight streaming (new: the reference describes layer-serialized
  * execution, README.md:212-226, and has its host-side pieces in the NVMe
  * loader -- pinned cudaHostAlloc buffers, per-slot streams, cudaMemcpyAsync,
