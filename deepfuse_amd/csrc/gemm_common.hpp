@@ -1,5 +1,5 @@
 // gemm_common.hpp -- what the fp8 GEMM sources share (gemm_fp8.hip,
-// gemm_small.hip): operand and accumulator vector types, the output
+// gemm_small.hip, gemm_experts*.hip): operand and accumulator vector types, the output
 // conversions, the bias loads and the arguments of one NT GEMM.
 #pragma once
 
@@ -37,6 +37,61 @@ __device__ __forceinline__ void store4(f16_t* p, const float* v) {
     *reinterpret_cast<u32x2*>(p) = u32x2{f32_to_f16_rne(v[0]) | (f32_to_f16_rne(v[1]) << 16),
                                         f32_to_f16_rne(v[2]) | (f32_to_f16_rne(v[3]) << 16)};
 }
+
+// ---- what the persistent kernels share ----
+constexpr int kGroupM = 8;             // tile rows of a group of the tile order
+constexpr int kPBM = 256, kPBN = 256;  // persistent block tile
+constexpr int kPKB = 128;              // K bytes per DMA step
+constexpr int kPStage = (kPBM + kPBN) * kPKB;
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t pack_bf16_rne(float a, float b) {
+    const v2f f = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, v2bf));
+}
+
+// s_waitcnt immediate (gfx9 encoding): vmcnt(n), lgkmcnt(0), no expcnt wait
+__device__ __forceinline__ constexpr int waitcnt_vm_lgkm0(int n) {
+    return (n & 15) | ((n >> 4) << 14) | 0x70;
+}
+
+// The lane index, computed afresh where it is called.  The asm is opaque to
+// the optimiser, so offsets derived from it stay where they are used: taken
+// from threadIdx, the epilogue's per-lane offsets were hoisted out of the
+// tile loop and, at the main loop's register pressure, spilled; each reload
+// in the epilogue then waited on vmcnt(0), i.e. for the DMA in flight.
+__device__ __forceinline__ int fresh_lane() {
+    int l;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+    return l;
+}
+
+// Epilogue geometry for an output element of ES bytes: each 32-row block of
+// a wave's FMR*32 x 64 part passes through an LDS slab of SR rows.
+template <int ES, int FMR = 4>
+struct EpiGeom {
+    static constexpr int SR = ES == 2 ? 16 : 8;          // slab rows
+    static constexpr int SROW = 64 * ES + 16;            // padded slab row (bytes)
+    static constexpr int SLAB = SR * SROW;
+    static constexpr int NPASS = 32 / SR;                // slab passes per 32-row block
+    static constexpr int SPP = SR * 64 * ES / 1024;      // 16-byte stores per lane per pass
+    static constexpr int NST = FMR * NPASS * SPP;        // epilogue stores per wave
+};
+
+// Store mode of the persistent kernel's epilogue: 0 element stores, 1
+// 16-byte stores, 2 16-byte non-temporal stores.  One store instruction
+// writes whole 64-column row segments (128 bytes of bf16, 256 of fp32);
+// non-temporal stores are kept to rows that start on a 128-byte boundary, so
+// that no cache line is written in parts by several non-temporal stores (in
+// a probe that did so -- 8-byte non-temporal stores -- one output of sixteen
+// came back different, where plain stores matched).
+inline int epi_store_mode(const void* C, int64_t ldc_bytes) {
+    if (ldc_bytes % 16 != 0 || !aligned16(C)) return 0;
+    return (ldc_bytes % 128 == 0 && ((uintptr_t)C & 127u) == 0) ? 2 : 1;
+}
+
+template <typename T> struct Tag { using type = T; };
 
 struct GemmArgs {
     const uint8_t* A; int lda;

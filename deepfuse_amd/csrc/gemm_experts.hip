@@ -34,56 +34,11 @@
 
 #include "df_common.hpp"
 #include "gemm_common.hpp"
+#include "gemm_experts.hpp"
 
 namespace dfk {
 
 namespace {
-
-constexpr int kMaxExperts = 1024;
-
-// One call.  ROWS: A [rows, lda], B [experts][N][ldb], C [rows, ldc], reduction K.
-// SUMS: A [M, lda], B [N, ldb], C [experts][M][ldc], reduction over the tokens.
-struct ExpertArgs {
-    const uint8_t* A;
-    const uint8_t* B;
-    void* C;
-    const int* off;
-    const float* sa;
-    const float* sb;
-    int lda, ldb, ldc, rows, M, N, K, experts, vec_out;
-};
-
-// expert e's rows, whatever the offsets hold
-__device__ __forceinline__ void expert_rows(const int* off, int e, int rows, int& lo, int& hi) {
-    lo = min(max(off[e], 0), rows);
-    hi = min(max(off[e + 1], lo), rows);
-}
-
-// bytes of a dword at byte position `pos` that lie in [lo, hi)
-__device__ __forceinline__ uint32_t keep_bytes(int pos, int lo, int hi) {
-    const int a = min(max(lo - pos, 0), 4) * 8, b = min(max(hi - pos, 0), 4) * 8;
-    const uint32_t upto = b == 32 ? ~0u : (1u << b) - 1u, below = a == 32 ? ~0u : (1u << a) - 1u;
-    return upto & ~below;
-}
-
-typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
-
-// eight codes -> bf16, exact
-template <int FMT> __device__ __forceinline__ bf8 widen8(uint32_t lo, uint32_t hi) {
-    bf2 p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t w = i < 2 ? lo : hi;
-        if constexpr (FMT == E4M3)
-            p[i] = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
-                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false);
-        else
-            p[i] = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, true)
-                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, false);
-    }
-    return bf8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
-}
 
 // ------------------------------------------------------------ small tiles --
 // As gemm_small.hip's kernel: a block owns a 16*MT x 16*NT tile, its W waves
@@ -263,9 +218,34 @@ template <int FA, bool SUMS, bool WIDE> void launch_small(const ExpertArgs& g, i
     }
 }
 
+// Which kernel a call takes.
+struct TilePlan {
+    bool tiles, narrow;
+    int grid;
+};
+TilePlan plan(const ExpertArgs& g, bool sums) {
+    const int per = (g.rows + g.experts - 1) / g.experts;  // rows of an expert if dealt evenly
+    const int cus = std::max(device_cu_count(), 1);
+    TilePlan p{per >= 64 && g.N >= 128 && (!sums || g.M >= 128), false, 0};
+    if (!p.tiles) return p;
+    // tiles at most: ROWS end each expert with a partial one
+    const int64_t mt = sums ? (int64_t)g.experts * ((g.M + kPBM - 1) / kPBM)
+                            : g.rows / kPBM + std::min(g.experts, g.rows);
+    const int64_t wide = mt * ((g.N + kPBN - 1) / kPBN), slim = mt * ((g.N + 127) / 128);
+    p.narrow = wide < cus;
+    p.grid = (int)std::min<int64_t>(p.narrow ? slim : wide, cus);
+    return p;
+}
+
 template <int FA, bool SUMS> void launch(ExpertArgs& g, int c_dtype, hipStream_t st) {
-    const int esz = c_dtype == DF_DTYPE_FLOAT32 ? 4 : 2;
-    g.vec_out = ((int64_t)g.ldc * esz) % 16 == 0 && aligned16(g.C);
+    const int64_t ldc_bytes = (int64_t)g.ldc * (c_dtype == DF_DTYPE_FLOAT32 ? 4 : 2);
+    const TilePlan p = plan(g, SUMS);
+    if (p.tiles) {
+        g.vec_out = epi_store_mode(g.C, ldc_bytes);
+        launch_expert_tiles(FA, SUMS, p.narrow, c_dtype, g, p.grid, st);
+        return;
+    }
+    g.vec_out = ldc_bytes % 16 == 0 && aligned16(g.C);
     if (c_dtype == DF_DTYPE_FLOAT32) launch_small<FA, SUMS, true>(g, c_dtype, st);
     else launch_small<FA, SUMS, false>(g, c_dtype, st);
 }
@@ -277,8 +257,11 @@ int check_call(const char* fn, const ExpertArgs& g, int K, bool sums, int c_dtyp
     DF_CHECK(g.experts <= kMaxExperts, DF_ERR_UNSUPPORTED, "%s: %d experts (at most %d)", fn, g.experts, kMaxExperts);
     DF_CHECK(c_dtype == DF_DTYPE_FLOAT32 || c_dtype == DF_DTYPE_BFLOAT16 || c_dtype == DF_DTYPE_HALF,
              DF_ERR_UNSUPPORTED, "%s: output dtype %d not supported", fn, c_dtype);
-    DF_CHECK((int64_t)((g.N + 15) / 16) * (sums ? (g.M + 15) / 16 : 1) < (1ll << 31), DF_ERR_INVALID,
-             "%s: output too large", fn);
+    DF_CHECK((int64_t)((g.N + 15) / 16) * (sums ? (g.M + 15) / 16 : 1) < (1ll << 31) &&
+                 (int64_t)((g.N + 127) / 128) *
+                         (sums ? (int64_t)g.experts * ((g.M + 255) / 256) : (int64_t)g.rows / 256 + g.experts) <
+                     (1ll << 31),
+             DF_ERR_INVALID, "%s: output too large", fn);
     empty = g.experts == 0 || g.N == 0 || (sums ? g.M == 0 : g.rows == 0);
     if (empty) return DF_OK;
     DF_CHECK(g.ldc >= g.N, DF_ERR_INVALID, "%s: output leading dimension %d < %d", fn, g.ldc, g.N);

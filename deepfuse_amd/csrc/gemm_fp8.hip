@@ -44,7 +44,6 @@ namespace dfk {
 
 constexpr int kBK = 128;              // bytes of K per step = one MFMA depth
 constexpr int kLdsStride = kBK + 16;  // padded LDS row (bytes)
-constexpr int kGroupM = 8;
 
 __device__ __forceinline__ v8i lds_frag(const uint8_t* p) {
     const u32x4 lo = *reinterpret_cast<const u32x4*>(p);
@@ -432,47 +431,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void gemm_nt_dma128_kernel(
 // lanes per 128-byte row segment, non-temporal: the output streams past L2,
 // leaving it to the operand panels (2-3% less step time at config 4 than
 // plain stores).
-constexpr int kPBM = 256, kPBN = 256;  // persistent block tile
-constexpr int kPKB = 128;              // K bytes per DMA step
-constexpr int kPStage = (kPBM + kPBN) * kPKB;
 constexpr int kPBiasSlots = 3;
 constexpr int kPBiasSlot = 2048;
-
-typedef float v2f __attribute__((ext_vector_type(2)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ uint32_t pack_bf16_rne(float a, float b) {
-    const v2f f = {a, b};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, v2bf));
-}
-
-// s_waitcnt immediate (gfx9 encoding): vmcnt(n), lgkmcnt(0), no expcnt wait
-__device__ __forceinline__ constexpr int waitcnt_vm_lgkm0(int n) {
-    return (n & 15) | ((n >> 4) << 14) | 0x70;
-}
-
-// The lane index, computed afresh where it is called.  The asm is opaque to
-// the optimiser, so offsets derived from it stay where they are used: taken
-// from threadIdx, the epilogue's per-lane offsets were hoisted out of the
-// tile loop and, at the main loop's register pressure, spilled; each reload
-// in the epilogue then waited on vmcnt(0), i.e. for the DMA in flight.
-__device__ __forceinline__ int fresh_lane() {
-    int l;
-    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
-    return l;
-}
-
-// Epilogue geometry for an output element of ES bytes: each 32-row block of
-// a wave's FMR*32 x 64 part passes through an LDS slab of SR rows.
-template <int ES, int FMR = 4>
-struct EpiGeom {
-    static constexpr int SR = ES == 2 ? 16 : 8;          // slab rows
-    static constexpr int SROW = 64 * ES + 16;            // padded slab row (bytes)
-    static constexpr int SLAB = SR * SROW;
-    static constexpr int NPASS = 32 / SR;                // slab passes per 32-row block
-    static constexpr int SPP = SR * 64 * ES / 1024;      // 16-byte stores per lane per pass
-    static constexpr int NST = FMR * NPASS * SPP;        // epilogue stores per wave
-};
 
 // The second GEMM of a grouped launch (see gemm_sched.hpp): its operands,
 // output and scales; never split, no bias.
@@ -488,8 +448,6 @@ struct PProb {
 // cost of a work unit beyond its DMA steps (pipeline fill, epilogue), in
 // the steps of the grouped schedule
 constexpr int kUnitOverhead = 3;
-
-template <typename T> struct Tag { using type = T; };
 
 // NARROW: 256x128 tiles (one problem, unsplit).  The eight waves own 64x64
 // parts (4 x 2 waves, 2x2 MFMA tiles each); a DMA step moves the 256 A rows
@@ -1184,18 +1142,6 @@ static void launch_cfg(const GemmArgs& g) {
     splitk_reduce_kernel<OutT, BiasT><<<blocks, 256, 0, g.st>>>(g.ws, S_eff, g.M, g.N, g.sa, g.sb,
                                                                 static_cast<const BiasT*>(g.bias),
                                                                 static_cast<OutT*>(g.C), g.ldc, vec_red);
-}
-
-// Store mode of the persistent kernel's epilogue: 0 element stores, 1
-// 16-byte stores, 2 16-byte non-temporal stores.  One store instruction
-// writes whole 64-column row segments (128 bytes of bf16, 256 of fp32);
-// non-temporal stores are kept to rows that start on a 128-byte boundary, so
-// that no cache line is written in parts by several non-temporal stores (in
-// a probe that did so -- 8-byte non-temporal stores -- one output of sixteen
-// came back different, where plain stores matched).
-static int epi_store_mode(const void* C, int64_t ldc_bytes) {
-    if (ldc_bytes % 16 != 0 || !aligned16(C)) return 0;
-    return (ldc_bytes % 128 == 0 && ((uintptr_t)C & 127u) == 0) ? 2 : 1;
 }
 
 // The persistent kernel takes outputs with at least one 256x256 tile per CU
