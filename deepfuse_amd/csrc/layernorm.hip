@@ -129,34 +129,43 @@ template <typename T> __device__ __forceinline__ void store_chunk(T* row, int j,
     }
 }
 
+// sum over the wave by DPP: within rows of 16 lanes, then across them into lane
+// 63 (half the time of a butterfly through LDS)
 __device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+#define DF_DPP_ADD(CTRL) \
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true))
+    DF_DPP_ADD(0x111);  // row_shr:1
+    DF_DPP_ADD(0x112);  // row_shr:2
+    DF_DPP_ADD(0x114);  // row_shr:4
+    DF_DPP_ADD(0x118);  // row_shr:8: lane 15 of a row has the row's
+    DF_DPP_ADD(0x142);  // row_bcast:15
+    DF_DPP_ADD(0x143);  // row_bcast:31: lane 63 has the wave's
+#undef DF_DPP_ADD
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// Sum over the RT threads that share a row.  For a block's row the waves'
-// sums meet in LDS, in one of two slots in turn: a slot is written again only
-// after the barrier of the call between, which every wave reaches after its
-// reads of that slot.
-template <int RT> struct RowSum {
-    float (*red)[2][RT / 64];  // [slot][which][wave], LDS (unused for a wave's row)
+// Sum over the RT threads that share a row, in a block of GP such groups.  For
+// rows wider than a wave the waves' sums meet in LDS, in one of two slots in
+// turn: a slot is written again only after the barrier of the call between,
+// which every wave reaches after its reads of that slot.
+template <int RT, int GP = 1> struct RowSum {
+    float (*red)[2][GP][RT / 64];  // [slot][which][group][wave], LDS (unused for a wave's row)
     int slot = 0;
     __device__ __forceinline__ void two(float& a, float& b) {
         a = wave_add(a);
         b = wave_add(b);
         if constexpr (RT > 64) {
-            const int w = threadIdx.x >> 6;
+            const int gi = GP == 1 ? 0 : threadIdx.x / RT, w = (threadIdx.x % RT) >> 6;  // (uniform in a wave)
             if ((threadIdx.x & 63) == 0) {
-                red[slot][0][w] = a;
-                red[slot][1][w] = b;
+                red[slot][0][gi][w] = a;
+                red[slot][1][gi][w] = b;
             }
             __syncthreads();
             a = b = 0.0f;
 #pragma unroll
             for (int i = 0; i < RT / 64; ++i) {
-                a += red[slot][0][i];
-                b += red[slot][1][i];
+                a += red[slot][0][gi][i];
+                b += red[slot][1][gi][i];
             }
             slot ^= 1;
         }
@@ -170,8 +179,8 @@ template <int RT> struct RowSum {
 
 // mean and rstd of a row whose chunk k is get(k, values); values past the
 // row's end, which are 0, take mean 0, so that they add nothing
-template <typename T, int RT, int CH, typename Get>
-__device__ __forceinline__ void row_stats(const Get& get, int t, int cols, float eps, RowSum<RT>& rs, float& mean,
+template <typename T, int RT, int CH, typename Get, typename Sum>
+__device__ __forceinline__ void row_stats(const Get& get, int t, int cols, float eps, Sum& rs, float& mean,
                                           float& rstd) {
     constexpr int E = El<T>::E;
     float s = 0.0f, sq = 0.0f;
@@ -210,7 +219,7 @@ template <typename T, int RT, int CH>
 __global__ __launch_bounds__(RT == 64 ? 256 : RT) void ln_forward_kernel(const FwdArgs<T> a) {
     constexpr int E = El<T>::E;
     constexpr int RPB = RT == 64 ? 4 : 1;  // rows a block works on at once
-    __shared__ float red[2][2][RT / 64];
+    __shared__ float red[2][2][1][RT / 64];
     const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
     RowSum<RT> rs{red};
     u32x4 gw[CH], bw[CH], nx[CH], nr[CH];
@@ -224,7 +233,7 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void ln_forward_kernel(const F
         }
     };
     const int step = gridDim.x * RPB;
-    int r = blockIdx.x * RPB + (RT == 64 ? threadIdx.x >> 6 : 0);
+    int r = blockIdx.x * RPB + (RT == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
     if (r < a.rows) fetch(r);
     if (affine) {
 #pragma unroll
@@ -280,7 +289,7 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void ln_forward_kernel(const F
 // Rows wider than a block's registers: a block reads its row three times.
 constexpr int kWide = 1024;
 template <typename T> __global__ __launch_bounds__(kWide) void ln_forward_wide_kernel(const FwdArgs<T> a) {
-    __shared__ float red[2][2][kWide / 64];
+    __shared__ float red[2][2][1][kWide / 64];
     RowSum<kWide> rs{red};
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* xr = a.x + (int64_t)r * a.ldx;
@@ -325,24 +334,27 @@ template <typename T> struct BwdArgs {
     float eps;
 };
 
-// Rows a block of the kernel below works on at once.  A wave's rows: eight
-// waves, so that one block per CU leaves 256 partial sums to fold; the waves
-// add theirs in LDS first.
-constexpr int kBwdWaves = 8;
-
-// A thread keeps the same columns for all its rows, so gamma's and beta's
-// sums stay in its registers; they leave once, at the end, as one partial per
+// A block of NT threads works on NT / RT rows at once (512 threads, or 1024
+// for the widest rows: two blocks or one per CU).  A thread keeps the same
+// columns for all its rows, so gamma's and beta's sums stay in its registers;
+// at the end the row groups' sums meet in LDS and leave as one partial per
 // block (2 * cols values), which ln_fold_kernel adds in block order.
+// Two chunks a thread: with a wave to a row of 1600 bf16 values, four chunks
+// and their sums spilled 28 registers a lane, whose reloads waited for the
+// next row's loads: 98.5 us against 48.5 (16384 rows).
 // SUMS: gamma's and beta's gradients are wanted.
+constexpr int bwd_threads(int rt) { return rt > 512 ? rt : 512; }
 template <typename T, int RT, int CH, bool SUMS>
-__global__ __launch_bounds__(RT == 64 ? 64 * kBwdWaves : RT) void ln_backward_kernel(const BwdArgs<T> a) {
+__global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_kernel(const BwdArgs<T> a) {
     constexpr int E = El<T>::E;
-    constexpr int RPB = RT == 64 ? kBwdWaves : 1;
-    __shared__ float red[2][2][RT / 64];
-    const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
-    const int wave = threadIdx.x >> 6;
-    RowSum<RT> rs{red};
-    u32x4 gw[CH], nx[CH], ny[CH];
+    constexpr int GP = bwd_threads(RT) / RT;
+    __shared__ float red[2][2][GP][RT / 64];
+    const int t = threadIdx.x % RT, group = __builtin_amdgcn_readfirstlane(threadIdx.x / RT);
+    RowSum<RT, GP> rs{red};
+    // gamma, each thread's own chunks: in LDS, where reading them waits for no
+    // load under way, and takes no registers from row to row
+    __shared__ u32x4 gw[CH][bwd_threads(RT)];
+    u32x4 nx[CH], ny[CH];
     const bool affine = a.gamma != nullptr, add = a.dres != nullptr, given = a.mean != nullptr;
     float nmean = 0.0f, nrstd = 0.0f;
     auto fetch = [&](int r) __attribute__((always_inline)) {
@@ -357,33 +369,40 @@ __global__ __launch_bounds__(RT == 64 ? 64 * kBwdWaves : RT) void ln_backward_ke
     };
     float sg[CH][E], sb[CH][E];
 #pragma unroll
-    for (int k = 0; k < CH; ++k)
+    for (int k = 0; k < CH; ++k) {
+        nx[k] = ny[k] = u32x4{0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < E; ++e) sg[k][e] = sb[k][e] = 0.0f;
-    const int step = gridDim.x * RPB;
-    int r = blockIdx.x * RPB + (RT == 64 ? wave : 0);
+    }
+    const int step = gridDim.x * GP;
+    int r = blockIdx.x * GP + group;
     if (r < a.rows) fetch(r);
     if (affine) {
 #pragma unroll
-        for (int k = 0; k < CH; ++k) gw[k] = load_chunk<T>(a.gamma, t + RT * k, a.cols);
+        for (int k = 0; k < CH; ++k) gw[k][threadIdx.x] = load_chunk<T>(a.gamma, t + RT * k, a.cols);
     }
     const float inv = 1.0f / (float)a.cols;
-    for (; r < a.rows; r += step) {
+    // the block's groups go round together (they share barriers); a group past
+    // the last row works on zeros and stores nothing
+    for (int base = blockIdx.x * GP; base < a.rows; base += step, r += step) {
+        const bool live = GP == 1 || r < a.rows;
         u32x4 cx[CH], cy[CH], cr[CH];
         float mean = nmean, rstd = nrstd;
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
             cx[k] = nx[k];
             cy[k] = ny[k];
+            if (GP > 1 && !live) cx[k] = cy[k] = u32x4{0, 0, 0, 0};
         }
         // used only after the row's sums: no need to have it a row ahead
-        if (add) {
+        if (add && live) {
 #pragma unroll
             for (int k = 0; k < CH; ++k) cr[k] = load_chunk<T>(a.dres + (int64_t)r * a.lddr, t + RT * k, a.cols);
         }
         if (r + step < a.rows) fetch(r + step);
         if (!given)
             row_stats<T, RT, CH>([&](int k, float* o) { El<T>::widen(cx[k], o); }, t, a.cols, a.eps, rs, mean, rstd);
+        if (GP > 1 && !live) mean = rstd = 0.0f;
         // xh and g = dy * gamma of chunk k.  Past the row's end dy is 0, so
         // what xh holds there adds nothing as long as it is finite: mean and
         // rstd of a row with an infinity or a NaN are not, and neither are
@@ -392,7 +411,7 @@ __global__ __launch_bounds__(RT == 64 ? 64 * kBwdWaves : RT) void ln_backward_ke
             El<T>::widen(cx[k], xh);
             El<T>::widen(cy[k], d);
             float w[E];
-            if (affine) El<T>::widen(gw[k], w);
+            if (affine) El<T>::widen(gw[k][threadIdx.x], w);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 xh[e] = (xh[e] - mean) * rstd;
@@ -418,9 +437,8 @@ __global__ __launch_bounds__(RT == 64 ? 64 * kBwdWaves : RT) void ln_backward_ke
         rs.two(c1, c2);
         c1 *= inv;
         c2 *= inv;
-        // The terms again from the row as loaded: kept from the first pass,
-        // they would take 64 registers more of a 2-byte row of four chunks,
-        // which spilled 1.1 KB a lane.
+        if (!live) continue;
+        // the terms again from the row as loaded, not kept: registers
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
             __builtin_amdgcn_sched_barrier(0);
@@ -442,34 +460,34 @@ __global__ __launch_bounds__(RT == 64 ? 64 * kBwdWaves : RT) void ln_backward_ke
             og = a.dgamma;
             ob = a.dbeta;
         }
-        if constexpr (RT == 64) {
-            // the eight waves' sums in LDS, halves onto halves; a chunk's E
-            // values of lane t lie E apart by 64, without bank conflicts
-            __shared__ float slab[kBwdWaves / 2][2][CH * E * 64];
+        if constexpr (GP > 1) {
+            // the groups' sums in LDS, halves onto halves; a thread's values
+            // lie RT apart: no bank conflicts
+            __shared__ float slab[GP / 2][2][CH * E * RT];
 #pragma unroll
-            for (int half = kBwdWaves / 2; half > 0; half >>= 1) {
-                if (wave >= half && wave < 2 * half) {
+            for (int half = GP / 2; half > 0; half >>= 1) {
+                if (group >= half && group < 2 * half) {
 #pragma unroll
                     for (int k = 0; k < CH; ++k)
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
-                            slab[wave - half][0][(k * E + e) * 64 + t] = sg[k][e];
-                            slab[wave - half][1][(k * E + e) * 64 + t] = sb[k][e];
+                            slab[group - half][0][(k * E + e) * RT + t] = sg[k][e];
+                            slab[group - half][1][(k * E + e) * RT + t] = sb[k][e];
                         }
                 }
                 __syncthreads();
-                if (wave < half) {
+                if (group < half) {
 #pragma unroll
                     for (int k = 0; k < CH; ++k)
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
-                            sg[k][e] += slab[wave][0][(k * E + e) * 64 + t];
-                            sb[k][e] += slab[wave][1][(k * E + e) * 64 + t];
+                            sg[k][e] += slab[group][0][(k * E + e) * RT + t];
+                            sb[k][e] += slab[group][1][(k * E + e) * RT + t];
                         }
                 }
                 __syncthreads();
             }
-            if (wave != 0) return;
+            if (group != 0) return;
         }
 #pragma unroll
         for (int k = 0; k < CH; ++k)
@@ -521,7 +539,7 @@ __global__ __launch_bounds__(64 * kFoldWaves) void ln_fold_kernel(const float* _
 template <typename T>
 __global__ __launch_bounds__(kWide) void ln_stats_wide_kernel(const T* x, int rows, int cols, int ldx, float eps,
                                                               float* mean, float* rstd) {
-    __shared__ float red[2][2][kWide / 64];
+    __shared__ float red[2][2][1][kWide / 64];
     RowSum<kWide> rs{red};
     for (int r = blockIdx.x; r < rows; r += gridDim.x) {
         const T* xr = x + (int64_t)r * ldx;
@@ -556,7 +574,7 @@ template <typename T> __global__ __launch_bounds__(256) void ln_colsum_wide_kern
 }
 
 template <typename T> __global__ __launch_bounds__(kWide) void ln_dx_wide_kernel(const BwdArgs<T> a) {
-    __shared__ float red[2][2][kWide / 64];
+    __shared__ float red[2][2][1][kWide / 64];
     RowSum<kWide> rs{red};
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const T* yr = a.dy + (int64_t)r * a.lddy;
@@ -586,12 +604,13 @@ template <typename T> __global__ __launch_bounds__(kWide) void ln_dx_wide_kernel
 }
 
 // -------------------------------------------------------------------- plans --
-// Threads a row and chunks a thread: a wave while its registers hold the row,
-// then the smallest block that does; threads 0: too wide for either.
+// Threads a row and chunks a thread; threads 0: too wide for registers.  The
+// forward keeps a row in a wave while its registers hold it; the backward, with
+// its sums, keeps two chunks a thread.
 struct LnShape {
     int threads, chunks;
 };
-LnShape ln_shape(int cols, int esz) {
+LnShape fwd_shape(int cols, int esz) {
     const int n = (int)(((int64_t)cols * esz + 15) / 16);  // 16-byte chunks of a row
     if (n <= 64) return {64, 1};
     if (n <= 128) return {64, 2};
@@ -601,20 +620,29 @@ LnShape ln_shape(int cols, int esz) {
     if (n <= 2048) return {512, 4};
     return {0, 0};
 }
+LnShape bwd_shape(int cols, int esz) {
+    const int n = (int)(((int64_t)cols * esz + 15) / 16);
+    if (n <= 64) return {64, 1};
+    if (n <= 128) return {64, 2};
+    if (n <= 256) return {128, 2};
+    if (n <= 512) return {256, 2};
+    if (n <= 1024) return {512, 2};
+    if (n <= 2048) return {1024, 2};
+    return {0, 0};
+}
 
 constexpr int kMaxParts = 512;  // partial sums of gamma's and beta's gradients
 constexpr int kWideParts = 64;
 
-// blocks of the backward kernel: one per CU of eight waves (a wave's row or
-// 512 threads a row), two of 256 threads
+// blocks of the backward kernel: 16 waves per CU walk the rows
 int bwd_blocks(int rows, const LnShape& s) {
-    if (s.threads == 64) return std::min((rows + kBwdWaves - 1) / kBwdWaves, 256);
     if (s.threads == 0) return std::min(rows, kWideParts);
-    return std::min(rows, s.threads == 256 ? 512 : 256);
+    const int nt = bwd_threads(s.threads), per = nt / s.threads;
+    return std::min((rows + per - 1) / per, 256 * 1024 / nt);
 }
 
 template <typename T> void launch_forward(const FwdArgs<T>& a, hipStream_t st) {
-    const LnShape s = ln_shape(a.cols, (int)sizeof(T));
+    const LnShape s = fwd_shape(a.cols, (int)sizeof(T));
     // 16 waves per CU walk the rows
     const int grid = s.threads == 64 ? std::min((a.rows + 3) / 4, 1024)
                                      : std::min(a.rows, s.threads == 0 ? 512 : 256 * 1024 / s.threads);
@@ -635,7 +663,7 @@ template <typename T> void launch_forward(const FwdArgs<T>& a, hipStream_t st) {
 
 // `stat`: room for mean and rstd of every row (wide rows without given ones)
 template <typename T> void launch_backward(BwdArgs<T> a, float* stat, hipStream_t st) {
-    const LnShape s = ln_shape(a.cols, (int)sizeof(T));
+    const LnShape s = bwd_shape(a.cols, (int)sizeof(T));
     const int grid = bwd_blocks(a.rows, s);
     const bool sums = a.dgamma != nullptr;
     auto fold = [&](int parts) {
@@ -660,18 +688,18 @@ template <typename T> void launch_backward(BwdArgs<T> a, float* stat, hipStream_
         ln_dx_wide_kernel<T><<<rgrid, kWide, 0, st>>>(a);
         return;
     }
-#define DF_LN(RT, CH)                                                                        \
-    if (s.threads == RT && s.chunks == CH) {                                                 \
-        constexpr int NT = RT == 64 ? 64 * kBwdWaves : RT;                                   \
-        if (sums) ln_backward_kernel<T, RT, CH, true><<<grid, NT, 0, st>>>(a);               \
-        else ln_backward_kernel<T, RT, CH, false><<<grid, NT, 0, st>>>(a);                   \
+#define DF_LN(RT, CH)                                                          \
+    if (s.threads == RT && s.chunks == CH) {                                   \
+        constexpr int NT = bwd_threads(RT);                                    \
+        if (sums) ln_backward_kernel<T, RT, CH, true><<<grid, NT, 0, st>>>(a); \
+        else ln_backward_kernel<T, RT, CH, false><<<grid, NT, 0, st>>>(a);     \
     }
     DF_LN(64, 1)
     DF_LN(64, 2)
-    DF_LN(64, 4)
+    DF_LN(128, 2)
     DF_LN(256, 2)
-    DF_LN(256, 4)
-    DF_LN(512, 4)
+    DF_LN(512, 2)
+    DF_LN(1024, 2)
 #undef DF_LN
     if (sums && grid > 1) fold(grid);
 }
