@@ -298,3 +298,30 @@ def test_other_stream(dev):
         df.adamw_update(P, G, M, V, 1, weight_decay=0.0, **HYPER)
     torch.cuda.current_stream().wait_stream(s)
     assert same(host(P)[0], step32(p[0], g[0].numpy(), 0 * p[0], 0 * p[0], 1, 0.0)[0])
+
+
+@pytest.mark.parametrize("beta2,t", [(0.95, 100), (0.999, 1), (0.9999, 3)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_all_magnitudes_bit_exact(dev, bits, beta2, t):
+    """Whole units of values of each size, from subnormal to past 2^20, with zeros of both signs among them."""
+    rng = np.random.default_rng(11)
+    n = 256 * 4 * 40
+    size = np.repeat(np.exp2(np.linspace(-149, 40, n // 256)), 256)
+    g = (rng.standard_normal(n) * size).astype(F)
+    g[rng.random(n) < 0.05] = 0.0
+    g[rng.random(n) < 0.05] = -0.0
+    p = (rng.standard_normal(n) * np.exp2(rng.uniform(-40, 10, n))).astype(F)
+    p[rng.random(n) < 0.02] = -0.0
+    P, G = dev_list([p], dev), dev_list([g], dev)
+    M, V, MS, VS = df.adamw_state(P, bits)
+    m = v = np.zeros(n, F)
+    for k in range(2):
+        df.adamw_update(P, G, M, V, t + k, lr=3e-3, beta2=beta2, weight_decay=0.1, m_scales=MS, v_scales=VS)
+        p, m, v = step32(p, g, m, v, t + k, 0.1, beta2=beta2)
+        assert same(host(P)[0], p), k
+        if bits == 32:
+            assert same(host(M)[0], m) and same(host(V)[0], v), k
+        else:
+            (cm, sm), (cv, sv) = keep8(m), keep8(v, root=True)
+            assert same(host(M)[0], cm) and same(host(V)[0], cv) and same(host(MS)[0], sm) and same(host(VS)[0], sv), k
+            m, v = widen(sm, cm), widen(sv, cv, root=True)
