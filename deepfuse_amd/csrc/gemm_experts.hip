@@ -218,28 +218,49 @@ template <int FA, bool SUMS, bool WIDE> void launch_small(const ExpertArgs& g, i
     }
 }
 
-// Which kernel a call takes.
+// Which kernel a call takes; the host knows the rows, not how they were dealt,
+// and goes by `per`, an expert's rows if dealt evenly.  Measured (us a call,
+// small tiles against large ones):
+//  ROWS, 2-byte output, 8 experts 1600 -> 6400: per 32 26.4 / 27.2, per 64
+//    36.7 / 24.7; 32 experts 1600 -> 1600: 26.5 / 27.3 and 38.3 / 22.9; fp32
+//    output (half the matrix rate, which small tiles do not feel), 8 experts:
+//    per 64 38.5 / 46.1, per 128 63.7 / 46.2.  Outputs of 64 columns leave half
+//    a large tile idle: 8 experts 1600 -> 64, per 1024: 11.2 / 15.1.
+//  SUMS: large tiles write dW in whole row segments: 8 experts 6400 x 1600,
+//    per 16: 220 / 74; few outputs of long reductions want more blocks: 8 experts
+//    256 x 256, per 1024: 9.2 / 20.9; 64 experts 256 x 256 (4096 small tiles),
+//    per 256: 20.1 / 15.4; 64 experts 128 x 128 (1024): 9.2 / 12.7.
+// 256 x 128 tiles where the rounds of blocks over the CUs come out cheaper, as
+// for the dense products (a narrow step takes 0.6 of a wide one; 3 and 2 steps
+// of overhead a tile).  8 experts 6400 -> 1600, per 64: 54.7 / 39.3 wide against
+// narrow; 1600 -> 6400, per 2048: 172 / 211.
 struct TilePlan {
     bool tiles, narrow;
     int grid;
 };
-TilePlan plan(const ExpertArgs& g, bool sums) {
-    const int per = (g.rows + g.experts - 1) / g.experts;  // rows of an expert if dealt evenly
+TilePlan plan(const ExpertArgs& g, bool sums, bool wide_codes) {
+    const int per = (g.rows + g.experts - 1) / g.experts;
     const int cus = std::max(device_cu_count(), 1);
-    TilePlan p{per >= 64 && g.N >= 128 && (!sums || g.M >= 128), false, 0};
+    TilePlan p{false, false, 0};
+    if (sums) p.tiles = (int64_t)g.experts * ((g.M + 31) / 32) * ((g.N + 31) / 32) > 8 * (int64_t)cus;
+    else p.tiles = per > (wide_codes ? 96 : 32) && g.N > 64;
     if (!p.tiles) return p;
-    // tiles at most: ROWS end each expert with a partial one
+    const int64_t wn = (g.N + kPBN - 1) / kPBN, sn = (g.N + 127) / 128;
+    // row tiles: ROWS end each expert with a partial one, half of one on average
     const int64_t mt = sums ? (int64_t)g.experts * ((g.M + kPBM - 1) / kPBM)
-                            : g.rows / kPBM + std::min(g.experts, g.rows);
-    const int64_t wide = mt * ((g.N + kPBN - 1) / kPBN), slim = mt * ((g.N + 127) / 128);
-    p.narrow = wide < cus;
-    p.grid = (int)std::min<int64_t>(p.narrow ? slim : wide, cus);
+                            : g.rows / kPBM + (std::min(g.experts, g.rows) + 1) / 2;
+    const int64_t steps = ((sums ? per : g.K) + kPKB - 1) / kPKB + (sums ? 1 : 0);
+    const int64_t wr = (mt * wn + cus - 1) / cus, sr = (mt * sn + cus - 1) / cus;
+    p.narrow = (double)sr * (0.6 * (double)steps + 2.0) < (double)wr * ((double)steps + 3.0);
+    // at most this many units; blocks without one return at once
+    const int64_t most = (sums ? mt : g.rows / kPBM + std::min(g.experts, g.rows)) * (p.narrow ? sn : wn);
+    p.grid = (int)std::min<int64_t>(most, cus);
     return p;
 }
 
 template <int FA, bool SUMS> void launch(ExpertArgs& g, int c_dtype, hipStream_t st) {
     const int64_t ldc_bytes = (int64_t)g.ldc * (c_dtype == DF_DTYPE_FLOAT32 ? 4 : 2);
-    const TilePlan p = plan(g, SUMS);
+    const TilePlan p = plan(g, SUMS, c_dtype == DF_DTYPE_FLOAT32);
     if (p.tiles) {
         g.vec_out = epi_store_mode(g.C, ldc_bytes);
         launch_expert_tiles(FA, SUMS, p.narrow, c_dtype, g, p.grid, st);

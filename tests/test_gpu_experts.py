@@ -301,3 +301,28 @@ def test_operands_past_32_bits(dev):
     xt[K - 1, :E] = one
     dw = df.experts_dw(dyt, xt, off, E, s, s, out_dtype=torch.bfloat16)
     assert (dw[:, N - 1, K - 1] == 1).all() and dw[E - 1].sum() == 1 and dw[E // 2].sum() == 1
+
+
+# per side of the choice of kernel: 32 rows an expert (2-byte outputs), 96 (fp32), 64 output columns, 2048 small tiles of dW;
+# few tiles and many, wide and narrow ones
+@pytest.mark.parametrize("counts,K,N", [
+    ([32, 32, 32], 144, 65), ([33, 33, 33], 144, 65), ([33, 40, 35], 160, 64), ([96] * 3, 272, 200), ([97] * 3, 272, 200),
+    ([0, 200, 100, 1], 130, 129), ([64] * 40, 256, 264), ([1] * 70, 192, 160), ([0] * 40 + [7], 260, 300),
+    ([300] * 9, 1040, 1300), ([129, 383, 640], 1600, 2000), ([0, 0, 2000], 800, 1600), ([13] * 9, 1200, 1000),
+    ([127, 128, 129, 255, 256, 257, 15, 16, 17], 520, 1100),
+])
+def test_exact_around_the_plan(dev, counts, K, N):
+    check_exact(Case(dev, counts, K, N, seed=N), dtypes=(torch.float32, torch.bfloat16))
+
+
+def test_no_reduction(dev):
+    """K of no codes and experts without rows on large tiles: zeros, every row of an expert written."""
+    off = torch.tensor([0, 100, 400], dtype=torch.int32, device=dev)
+    s, sw = torch.ones(1, device=dev), torch.ones(2, device=dev)
+    z = lambda *shape: torch.zeros(*shape, dtype=torch.uint8, device=dev)
+    for dt in (torch.float32, torch.bfloat16):
+        y = torch.full((450, 300), 3.0, dtype=dt, device=dev)
+        df.experts_fwd(z(450, 16)[:, :0], z(2, 300, 16)[..., :0], off, 0, s, sw, out=y)
+        assert (y[:400] == 0).all() and (y[400:] == 3).all()
+        dw = df.experts_dw(z(2000, 16)[:, :0], z(2000, 16)[:, :0], off * 0, 0, s, s, out_dtype=dt)
+        assert dw.shape == (2, 2000, 2000) and (dw == 0).all()
