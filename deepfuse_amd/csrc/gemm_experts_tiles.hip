@@ -83,6 +83,8 @@ __device__ __forceinline__ int find_expert(const int* first, int v, int lane) {
     return 16 * n1 + __builtin_popcountll(m & 0xFFFFull);
 }
 
+typedef u32x4 u32x4_el __attribute__((aligned(2)));
+
 template <int FA, int FB, typename OutT, bool SUMS, bool WIDE, bool NARROW>
 __global__ __launch_bounds__(512, 1) void experts_tile_kernel(const ExpertArgs g) {
     constexpr int FM = NARROW ? 2 : 4, FN = 2;    // 32x32 MFMA tiles per wave
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(512, 1) void experts_tile_kernel(const ExpertArgs g
 
     // Stores a finished unit: scale and conversion in registers, then each
     // 32-row block through the wave's LDS slab and out as 16-byte stores of
-    // whole row segments (vec_out 2: non-temporal).  Whether the wave's part
+    // whole row segments (vec_out 2: non-temporal; see epi_store_mode).  Whether the wave's part
     // lay wholly inside the output, i.e. whether it issued all its stores.
     auto store_unit = [&](const Unit& u, float sab) __attribute__((always_inline)) -> bool {
         constexpr int ES = (int)sizeof(OutT);
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(512, 1) void experts_tile_kernel(const ExpertArgs g
         constexpr int RPS = 64 / CPR;
         const int srow = el / CPR, rc = el % CPR;
         const int scol = colw + rc * (16 / ES);
-        const bool col_full = g.vec_out && scol + 16 / ES <= g.N;
+        const bool col_full = scol + 16 / ES <= g.N;
         const int my_sr = efr % G::SR, my_pass = efr / G::SR;
         typedef typename std::conditional<ES == 2, u32x2, f32x4>::type Pk;
         // LDS operations of one wave execute in order, so a pass's reads see
@@ -423,8 +425,9 @@ __global__ __launch_bounds__(512, 1) void experts_tile_kernel(const ExpertArgs g
                     if (row < u.mend) {
                         OutT* dst = C + (int64_t)row * g.ldc + scol;
                         if (col_full) {
+                            // rows at any element's boundary: 16-byte stores all the same
                             if (g.vec_out == 2) __builtin_nontemporal_store(val, reinterpret_cast<u32x4*>(dst));
-                            else *reinterpret_cast<u32x4*>(dst) = val;
+                            else *reinterpret_cast<u32x4_el*>(dst) = val;
                         } else {
                             const OutT* ev = reinterpret_cast<const OutT*>(&val);
 #pragma unroll
