@@ -716,13 +716,14 @@ def _check_gpu(fn: str, **tensors):
             continue
         if not t.is_cuda:
             raise ValueError(f"{fn}: {name} is on {t.device}, not on a GPU")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"{fn}: {name} is on {t.device}, others on {dev}")
-        dev = t.device
+        at = t.get_device()
+        if dev is not None and at != dev:
+            raise ValueError(f"{fn}: {name} is on {t.device}, others on GPU {dev}")
+        dev = at
 
 
 def _check_like(fn: str, name: str, t, shape, dtype):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    if t.shape != shape or t.dtype is not dtype:
         raise ValueError(f"{fn}: {name} is {tuple(t.shape)} {t.dtype}, not {tuple(shape)} {dtype}")
 
 
@@ -730,10 +731,10 @@ def _rows(fn: str, name: str, t, shape, dtype) -> int:
     """The leading dimension of a [rows, cols] operand whose rows are
     contiguous and do not overlap."""
     _check_like(fn, name, t, shape, dtype)
-    rows, cols = shape
-    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
-        raise ValueError(f"{fn}: {name} with strides {tuple(t.stride())} has no contiguous rows of its own")
-    return max(t.stride(0), cols) if rows > 1 else cols
+    (rows, cols), (ld, step) = shape, t.stride()
+    if cols > 1 and step != 1 or rows > 1 and ld < cols:
+        raise ValueError(f"{fn}: {name} with strides {(ld, step)} has no contiguous rows of its own")
+    return ld if rows > 1 else cols
 
 
 def _row_vector(fn: str, name: str, t, n: int, dtype):
