@@ -14,8 +14,11 @@ Reference mapping (SensorVista/DeepFuse):
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import enum
+import itertools
+import operator
 import os
 import re
 
@@ -801,22 +804,32 @@ def layernorm_backward(dy, x, gamma=None, mean=None, rstd=None, eps=1e-5, dresid
 # ----------------------------------------------------------------------------
 # AdamW over lists of tensors, states in 32 or in 8 bits
 # ----------------------------------------------------------------------------
-def _list_of(fn: str, what: str, tensors, sizes, dtype, dev):
-    """Checks a list of contiguous tensors of one dtype on the GPU ``dev``, of the given sizes."""
+_dtype_of = operator.attrgetter("dtype")
+
+
+def _list_of(fn: str, what: str, tensors, sizes, dtype, at: int):
+    """Checks a list of contiguous tensors of one dtype on GPU ``at``, of the
+    given sizes; returns their addresses.  A map over the list per question:
+    half the time of asking tensor by tensor."""
+    T = _torch().Tensor
     if len(tensors) != len(sizes):
         raise ValueError(f"{fn}: {len(tensors)} {what} for {len(sizes)} parameters")
-    for t, n in zip(tensors, sizes):
-        if t.dtype is not dtype or t.numel() != n or not t.is_contiguous() or t.device != dev or not t.is_cuda:
-            i = next(i for i, u in enumerate(tensors) if u is t)
-            raise ValueError(f"{fn}: {what}[{i}] ({tuple(t.shape)} {t.dtype} on {t.device}) is not a contiguous {dtype} "
-                             f"tensor of {n} values on {dev}" + ("" if t.is_cuda else ", a GPU"))
+    if not (list(map(T.numel, tensors)) == sizes and set(map(_dtype_of, tensors)) == {dtype}
+            and all(map(T.is_contiguous, tensors)) and set(map(T.get_device, tensors)) == {at}):
+        for i, (t, n) in enumerate(zip(tensors, sizes)):
+            if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.get_device() != at:
+                raise ValueError(f"{fn}: {what}[{i}] ({tuple(t.shape)} {t.dtype} on {t.device}) is not a contiguous "
+                                 f"{dtype} tensor of {n} values on GPU {at}")
+    return array.array("Q", map(T.data_ptr, tensors))
 
 
 def _grad_norm16(grads, clip):
     fn, torch = "grad_norm", _torch()
     if clip is not None:
         raise TypeError(f"{fn}: {grads[0].dtype} gradients are not clipped in place (give adamw_update the norm)")
-    _list_of(fn, "grads", grads, [t.numel() for t in grads], grads[0].dtype, grads[0].device)
+    if not grads[0].is_cuda:
+        raise ValueError(f"{fn}: the gradients are on {grads[0].device}, not on a GPU")
+    _list_of(fn, "grads", grads, [t.numel() for t in grads], grads[0].dtype, grads[0].get_device())
     sizes = _sizes(grads)
     with _on(grads[0]):
         ws = torch.empty(int(lib().df_grad_norm_workspace_bytes(len(grads), sizes)), dtype=torch.uint8,
@@ -861,29 +874,31 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
     eight = m_scales is not None
     if eight != (v_scales is not None):
         raise ValueError(f"{fn}: m_scales and v_scales go together")
+    if not params[0].is_cuda:
+        raise ValueError(f"{fn}: the parameters are on {params[0].device}, not on a GPU")
     gt = _in_dtype(grads[0]) if grads else DType.FLOAT32
     state = torch.float8_e4m3fn if eight else torch.float32
-    sizes, dev = [p.numel() for p in params], params[0].device
-    _list_of(fn, "params", params, sizes, torch.float32, dev)
-    _list_of(fn, "grads", grads, sizes, grads[0].dtype if grads else None, dev)
-    _list_of(fn, "ms", ms, sizes, state, dev)
-    _list_of(fn, "vs", vs, sizes, state, dev)
-    written = [params, ms, vs]
+    sizes, at = [p.numel() for p in params], params[0].get_device()
+    p = _list_of(fn, "params", params, sizes, torch.float32, at)
+    g = _list_of(fn, "grads", grads, sizes, grads[0].dtype if grads else None, at)
+    m = _list_of(fn, "ms", ms, sizes, state, at)
+    v = _list_of(fn, "vs", vs, sizes, state, at)
+    written, sm, sv, c = [p, m, v], None, None, None
     if eight:
         blocks = [-(-k // 256) for k in sizes]
-        _list_of(fn, "m_scales", m_scales, blocks, torch.float32, dev)
-        _list_of(fn, "v_scales", v_scales, blocks, torch.float32, dev)
-        written += [m_scales, v_scales]
+        sm = _list_of(fn, "m_scales", m_scales, blocks, torch.float32, at)
+        sv = _list_of(fn, "v_scales", v_scales, blocks, torch.float32, at)
+        written += [sm, sv]
     ct = DType.FLOAT32
     if copies is not None:
         ct = _in_dtype(copies[0]) if copies else ct
         if ct == DType.FLOAT32:
             raise TypeError(f"{fn}: copies are bf16 or float16")
-        _list_of(fn, "copies", copies, sizes, copies[0].dtype, dev)
-        written.append(copies)
-    arrays = [_ptrs(ts) for ts in written]
-    at = [a for arr in arrays for a, k in zip(arr, sizes) if k]
-    if len(set(at)) != len(at):
+        c = _list_of(fn, "copies", copies, sizes, copies[0].dtype, at)
+        written.append(c)
+    if 0 in sizes:  # empty tensors share an address
+        written = [[a for a, k in zip(arr, sizes) if k] for arr in written]
+    if len(set(itertools.chain(*written))) != sum(map(len, written)):
         raise ValueError(f"{fn}: a tensor that the step writes is listed twice")
     if isinstance(weight_decay, (int, float)):
         wd = (_c_f * n)(*[weight_decay] * n)
@@ -892,21 +907,22 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
             raise ValueError(f"{fn}: {len(weight_decay)} weight decays for {n} parameters")
         wd = (_c_f * n)(*weight_decay)
     scalars = {}
-    for name, v, dt in (("timestep", timestep, torch.int32), ("lr", lr, torch.float32), ("clip_norm", clip_norm, torch.float32)):
-        if isinstance(v, torch.Tensor):
-            if v.numel() != 1 or v.dtype != dt or v.device != params[0].device:
+    for name, x, dt in (("timestep", timestep, torch.int32), ("lr", lr, torch.float32),
+                        ("clip_norm", clip_norm, torch.float32)):
+        if isinstance(x, torch.Tensor):
+            if x.numel() != 1 or x.dtype != dt or x.device != params[0].device:
                 raise ValueError(f"{fn}: {name} is not one {dt} on {params[0].device}")
-            scalars[name] = v.data_ptr()
+            scalars[name] = x.data_ptr()
     if absmax is not None and (absmax.dtype != torch.float32 or absmax.numel() < n or not absmax.is_contiguous()
                                or absmax.device != params[0].device):
         raise ValueError(f"{fn}: absmax is not {n} contiguous fp32 values on {params[0].device}")
-    p, m, v = arrays[:3]
-    sm, sv = arrays[3:5] if eight else (None, None)
+    at_of = lambda arr: None if arr is None else arr.buffer_info()[0]
     with _on(params[0]):
-        call("df_adamw_update", n, (_c_i64 * n)(*sizes), p, int(gt), _ptrs(grads), int(DType.FP8E4M3 if eight else DType.FLOAT32), m, v, sm,
-             sv, int(ct), arrays[-1] if copies is not None else None, 0.0 if "lr" in scalars else float(lr), float(beta1),
-             float(beta2), float(eps), wd, 0 if "timestep" in scalars else int(timestep), scalars.get("lr"),
-             scalars.get("timestep"), scalars.get("clip_norm"), float(max_norm), _ptr(absmax), _stream())
+        call("df_adamw_update", n, (_c_i64 * n)(*sizes), at_of(p), int(gt), at_of(g),
+             int(DType.FP8E4M3 if eight else DType.FLOAT32), at_of(m), at_of(v), at_of(sm), at_of(sv), int(ct), at_of(c),
+             0.0 if "lr" in scalars else float(lr), float(beta1), float(beta2), float(eps), wd,
+             0 if "timestep" in scalars else int(timestep), scalars.get("lr"), scalars.get("timestep"),
+             scalars.get("clip_norm"), float(max_norm), _ptr(absmax), _stream())
 
 
 # ----------------------------------------------------------------------------
