@@ -16,6 +16,11 @@
 // launches norm_size threads per block, which fails beyond 1024 (GPT-2 XL's
 // 1600).
 //
+// Addition: gradient(grad_output) is the true backward, which the reference
+// lacks: the gradient of the last forward's input, with gamma's and beta's in
+// gradients() (overwritten; a FullyConnectedLayer's are too).  Training mode
+// only.
+//
 // The fused producer: FullyConnectedLayer::forward(input, norm) quantizes
 // LayerNorm(input) straight into the Linear's fp8 operands without
 // materialising the normalised tensor.
@@ -39,6 +44,7 @@ public:
 
     tensor<T> forward(const tensor<T>& input) override;
     tensor<T> backward(const tensor<T>& grad_output) override;
+    tensor<T> gradient(const tensor<T>& grad_output);
 
     std::vector<tensor<T>*> parameters() override;
     std::vector<tensor<T>*> gradients() override;
@@ -68,7 +74,9 @@ private:
     tensor<T> grad_gamma_;
     tensor<T> grad_beta_;
     std::optional<tensor<T>> input_cache_;
-    void* ws_ = nullptr;  // row statistics (device), grown on demand
+    void* workspace(size_t need);
+
+    void* ws_ = nullptr;  // row statistics, partial sums (device), grown on demand
     size_t ws_bytes_ = 0;
 };
 

@@ -55,20 +55,26 @@ tensor<T> LayerNormLayer<T>::forward(const tensor<T>& input) {
     note_input(input);
     tensor<T> output(input.shape());
     if (rows == 0) return output;
-    const size_t need = df_layernorm_workspace_bytes(rows, norm_size_, 0, 0);
+    void* ws = workspace(df_layernorm_workspace_bytes(rows, norm_size_, 0, 0));
+    CHECK_DF_EX(df_layernorm(dtype_traits<T>::value, input.data(), rows, norm_size_, norm_size_,
+                             affine_ ? gamma_.data() : nullptr, affine_ ? beta_.data() : nullptr, epsilon_,
+                             output.data(), norm_size_, ws, ws_bytes_, st()));
+    return output;
+}
+
+template <typename T>
+void* LayerNormLayer<T>::workspace(size_t need) {
     if (need > ws_bytes_) {
         if (ws_) {
             CHECK_HIP_EX(hipStreamSynchronize(Hip::stream()));
             CHECK_HIP_EX(hipFree(ws_));
             ws_ = nullptr;
+            ws_bytes_ = 0;
         }
         CHECK_HIP_EX(hipMalloc(&ws_, need));
         ws_bytes_ = need;
     }
-    CHECK_DF_EX(df_layernorm(dtype_traits<T>::value, input.data(), rows, norm_size_, norm_size_,
-                             affine_ ? gamma_.data() : nullptr, affine_ ? beta_.data() : nullptr, epsilon_,
-                             output.data(), norm_size_, ws_, ws_bytes_, st()));
-    return output;
+    return ws_;
 }
 
 // the reference's backward (.cu:82-90): the incoming gradient, copied
@@ -77,6 +83,32 @@ tensor<T> LayerNormLayer<T>::backward(const tensor<T>& grad_output) {
     if (this->training_enabled_ && !input_cache_.has_value())
         throw std::runtime_error("LayerNormLayer: input_cache_ is empty in backward().");
     return grad_output.clone();
+}
+
+template <typename T>
+tensor<T> LayerNormLayer<T>::gradient(const tensor<T>& grad_output) {
+    if (!this->training_enabled_ || !input_cache_.has_value())
+        throw std::runtime_error("LayerNormLayer: gradient() needs training mode and a forward() before it.");
+    const tensor<T>& x = *input_cache_;
+    if (grad_output.size() != x.size())
+        throw std::invalid_argument("LayerNormLayer: gradient of " + std::to_string(grad_output.size()) +
+                                    " values for an input of " + std::to_string(x.size()));
+    const int rows = rows_of(x);
+    tensor<T> dx(x.shape());
+    // gamma's and beta's sums are fp32: behind the workspace unless T is
+    const size_t sums = affine_ ? 2 * (size_t)norm_size_ * sizeof(float) : 0;
+    const size_t need = (df_layernorm_backward_workspace_bytes(rows, norm_size_) + 15) & ~(size_t)15;
+    char* ws = static_cast<char*>(workspace(need + sums));
+    float* dgamma = affine_ ? reinterpret_cast<float*>(ws + need) : nullptr;
+    float* dbeta = affine_ ? dgamma + norm_size_ : nullptr;
+    CHECK_DF_EX(df_layernorm_backward(dtype_traits<T>::value, grad_output.data(), norm_size_, x.data(), norm_size_, rows,
+                                      norm_size_, affine_ ? gamma_.data() : nullptr, nullptr, nullptr, epsilon_, nullptr,
+                                      0, dx.data(), norm_size_, dgamma, dbeta, ws, need, st()));
+    if (affine_) {
+        CHECK_DF_EX(df_convert(DF_DTYPE_FLOAT32, dgamma, dtype_traits<T>::value, grad_gamma_.data(), norm_size_, st()));
+        CHECK_DF_EX(df_convert(DF_DTYPE_FLOAT32, dbeta, dtype_traits<T>::value, grad_beta_.data(), norm_size_, st()));
+    }
+    return dx;
 }
 
 template <typename T>

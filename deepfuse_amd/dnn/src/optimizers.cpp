@@ -1,5 +1,6 @@
-// optimizers.cpp -- AdamOptimizer<float> and utils::clip_grad_norm<float> of
-// the C++ drop-in, on df_adam_update_f32 / df_clip_grad_norm_f32.
+// optimizers.cpp -- AdamOptimizer<float>, AdamWOptimizer<float> and
+// utils::clip_grad_norm<float> of the C++ drop-in, on df_adam_update_f32,
+// df_adamw_update and df_clip_grad_norm_f32.
 //
 // Reference: dnn/optimizers/adam_optimizer.cu:83-130 and
 // dnn/utils/clip_grad_norm.cu:31-62.
@@ -9,6 +10,7 @@
 #include "dnn/core/hip.hpp"
 #include "dnn/core/tensor.hpp"
 #include "dnn/optimizers/adam_optimizer.hpp"
+#include "dnn/optimizers/adamw_optimizer.hpp"
 #include "dnn/utils/common.hpp"
 
 namespace dnn {
@@ -162,5 +164,97 @@ const float* AdamOptimizer<float>::step_clipped(float max_norm) {
 }
 
 template class AdamOptimizer<float>;
+
+template <>
+AdamWOptimizer<float>::AdamWOptimizer(float learning_rate, float beta1, float beta2, float epsilon, float weight_decay,
+                                      int state_bits)
+    : learning_rate_(learning_rate), beta1_(beta1), beta2_(beta2), epsilon_(epsilon), weight_decay_(weight_decay),
+      state_bits_(state_bits) {
+    if (state_bits != 32 && state_bits != 8)
+        throw std::invalid_argument("AdamWOptimizer: states in " + std::to_string(state_bits) + " bits (8 or 32)");
+}
+
+template <>
+void AdamWOptimizer<float>::update_parameters(const std::vector<tensor<float>*>& parameters,
+                                              const std::vector<tensor<float>*>& gradients) {
+    Optimizer<float>::update_parameters(parameters, gradients);
+    for (auto* param : parameters) {
+        if (state_.find(param) != state_.end()) continue;
+        State s;
+        if (state_bits_ == 32) {
+            s.m = std::make_unique<tensor<float>>(param->shape());
+            s.v = std::make_unique<tensor<float>>(param->shape());
+            s.m->fill(0.0f);
+            s.v->fill(0.0f);
+        } else {
+            const std::vector<int> blocks{(int)df_adamw_scale_count(param->size())};
+            s.mq = std::make_unique<tensor<uint8_t>>(param->shape());
+            s.vq = std::make_unique<tensor<uint8_t>>(param->shape());
+            s.m_scale = std::make_unique<tensor<float>>(blocks);
+            s.v_scale = std::make_unique<tensor<float>>(blocks);
+            s.mq->fill(0);
+            s.vq->fill(0);
+            s.m_scale->fill(1.0f);
+            s.v_scale->fill(1.0f);
+        }
+        state_.emplace(param, std::move(s));
+    }
+}
+
+template <>
+void AdamWOptimizer<float>::zero_grad() {
+    for (auto* grad : this->gradients_) grad->fill(0.0f);
+}
+
+template <>
+void AdamWOptimizer<float>::launch(const float* clip_norm, float max_norm) {
+    const auto& params = this->parameters_;
+    const auto& grads = this->gradients_;
+    if (grads.size() < params.size())
+        throw std::invalid_argument("AdamWOptimizer::step: fewer gradients than parameters");
+    const size_t n = params.size();
+    std::vector<float*> p(n), ms(n), vs(n);
+    std::vector<void*> m(n), v(n);
+    std::vector<const void*> g(n);
+    std::vector<int64_t> sizes(n);
+    std::vector<float> wd(n);
+    for (size_t i = 0; i < n; ++i) {
+        if (grads[i]->size() != params[i]->size())
+            throw std::invalid_argument("AdamWOptimizer::step: gradient " + std::to_string(i) +
+                                        " differs in size from its parameter");
+        for (size_t k = 0; k < i; ++k)
+            if (params[k] == params[i])
+                throw std::invalid_argument("AdamWOptimizer::step: parameter " + std::to_string(i) + " is listed twice");
+        State& s = state_.at(params[i]);
+        p[i] = params[i]->data();
+        g[i] = grads[i]->data();
+        m[i] = s.m ? static_cast<void*>(s.m->data()) : s.mq->data();
+        v[i] = s.v ? static_cast<void*>(s.v->data()) : s.vq->data();
+        ms[i] = s.m_scale ? s.m_scale->data() : nullptr;
+        vs[i] = s.v_scale ? s.v_scale->data() : nullptr;
+        sizes[i] = params[i]->size();
+        const auto d = decay_.find(params[i]);
+        wd[i] = d == decay_.end() ? weight_decay_ : d->second;
+    }
+    ++timestep_;
+    CHECK_DF_EX(df_adamw_update((int)n, sizes.data(), p.data(), DF_DTYPE_FLOAT32, g.data(),
+                                state_bits_ == 8 ? DF_DTYPE_FP8E4M3 : DF_DTYPE_FLOAT32, m.data(), v.data(), ms.data(),
+                                vs.data(), DF_DTYPE_FLOAT32, nullptr, learning_rate_, beta1_, beta2_, epsilon_, wd.data(),
+                                timestep_, nullptr, nullptr, clip_norm, max_norm, nullptr, stream_arg()));
+}
+
+template <>
+void AdamWOptimizer<float>::step() {
+    launch(nullptr, 0.0f);
+}
+
+template <>
+const float* AdamWOptimizer<float>::step_clipped(float max_norm) {
+    const float* norm = device_norm(this->gradients_, false, max_norm);
+    launch(norm, max_norm);
+    return norm;
+}
+
+template class AdamWOptimizer<float>;
 
 }  // namespace dnn

@@ -27,6 +27,7 @@
 #include "dnn/layers/fully_connected_layer.hpp"
 #include "dnn/layers/layer_norm_layer.hpp"
 #include "dnn/optimizers/adam_optimizer.hpp"
+#include "dnn/optimizers/adamw_optimizer.hpp"
 #include "dnn/utils/common.hpp"
 #include "mini_test.hpp"
 
@@ -134,6 +135,7 @@ using Fp8TensorTest = HipFixture;
 using FullyConnectedLayerTest = HipFixture;
 using AdamOptimizerTest = HipFixture;
 using LayerNormLayerTest = HipFixture;
+using AdamWOptimizerTest = HipFixture;
 using ClipGradNormTest = HipFixture;
 
 }  // namespace
@@ -1075,6 +1077,77 @@ TEST_F(LayerNormLayerTest, BackwardPassesTheGradientThrough) {
     EXPECT_TRUE(download(ln.backward(g)) == gh);
 }
 
+// gradient() against the formula in binary64: dx, and gamma's and beta's sums.
+template <typename T>
+void check_norm_gradient(int rows, int C, bool affine, double step, void (*up)(tensor<T>&, const std::vector<float>&),
+                         std::vector<float> (*down)(const tensor<T>&)) {
+    LayerNormLayer<T> ln(C, 1e-5f, affine, true);
+    tensor<T> x({rows, C}), gy({rows, C}), gamma({C});
+    up(x, uniform((size_t)rows * C, -2.0f, 3.0f, 301));
+    up(gy, uniform((size_t)rows * C, -1.0f, 1.0f, 302));
+    up(gamma, uniform(C, 0.5f, 1.5f, 303));
+    std::vector<float> gh(C, 1.0f);
+    if (affine) {
+        gh = down(gamma);
+        up(*ln.parameters()[0], gh);
+    }
+    EXPECT_THROW(ln.gradient(gy), std::runtime_error);  // no forward yet
+    ln.forward(x);
+    const auto xh = down(x), gyh = down(gy), dx = down(ln.gradient(gy));
+    std::vector<double> dg(C, 0.0), db(C, 0.0), ag(C, 0.0);
+    for (int r = 0; r < rows; ++r) {
+        const float *xr = &xh[(size_t)r * C], *gr = &gyh[(size_t)r * C];
+        double mean = 0, var = 0, c1 = 0, c2 = 0, big = 0;
+        for (int c = 0; c < C; ++c) mean += xr[c];
+        mean /= C;
+        for (int c = 0; c < C; ++c) var += (xr[c] - mean) * (xr[c] - mean);
+        const double rstd = 1.0 / std::sqrt(var / C + 1e-5);
+        for (int c = 0; c < C; ++c) {
+            const double n = (xr[c] - mean) * rstd, g = (double)gr[c] * gh[c];
+            c1 += g / C;
+            c2 += g * n / C;
+            big = std::max(big, std::abs(g) * (1 + std::abs(n)));
+            dg[c] += gr[c] * n;
+            ag[c] += std::abs(gr[c] * n) + std::abs(gr[c]);
+            db[c] += gr[c];
+        }
+        for (int c = 0; c < C; ++c) {
+            const double n = (xr[c] - mean) * rstd, want = rstd * ((double)gr[c] * gh[c] - c1 - n * c2);
+            // one rounding to T, and 64 binary32 roundings of the terms
+            EXPECT_LE(std::abs(dx[(size_t)r * C + c] - want), step * std::abs(want) + 64 * 6e-8 * 4 * rstd * big);
+        }
+    }
+    if (!affine) return;
+    const auto a = down(*ln.gradients()[0]), b = down(*ln.gradients()[1]);
+    for (int c = 0; c < C; ++c) {
+        EXPECT_LE(std::abs(a[c] - dg[c]), step * std::abs(dg[c]) + (64 + rows) * 6e-8 * ag[c]);
+        EXPECT_LE(std::abs(b[c] - db[c]), step * std::abs(db[c]) + (64 + rows) * 6e-8 * ag[c]);
+    }
+}
+
+void up_f32(tensor<float>& t, const std::vector<float>& v) { t.upload(v.data()); }
+std::vector<float> down_f32(const tensor<float>& t) { return download(t); }
+std::vector<float> down_bf16(const tensor<bfloat16>& t) { return download_f(t); }
+std::vector<float> down_f16(const tensor<__half>& t) { return download_f(t); }
+
+TEST_F(LayerNormLayerTest, GradientMatchesFormula) {
+    check_norm_gradient<float>(37, 96, true, 6e-8, up_f32, down_f32);
+    check_norm_gradient<float>(5, 771, false, 6e-8, up_f32, down_f32);
+    check_norm_gradient<bfloat16>(33, 200, true, 0.00390625, upload_bf16, down_bf16);
+    check_norm_gradient<__half>(20, 64, true, 0.00048828125, upload_f16, down_f16);
+}
+
+TEST_F(LayerNormLayerTest, GradientRefusals) {
+    LayerNormLayer<float> eval(16), ln(16, 1e-5f, true, true);
+    tensor<float> x({4, 16}), g({3, 16});
+    x.fill(1.0f);
+    g.fill(1.0f);
+    eval.forward(x);
+    EXPECT_THROW(eval.gradient(x), std::runtime_error);  // not in training mode
+    ln.forward(x);
+    EXPECT_THROW(ln.gradient(g), std::invalid_argument);
+}
+
 TEST_F(LayerNormLayerTest, SaveLoadRoundTrip) {
     LayerNormLayer<float> a(24), b(24);
     const auto g = uniform(24, 0.5f, 1.5f, 106);
@@ -1364,6 +1437,104 @@ TEST_F(AdamOptimizerTest, LinearLayerStepsMatchOracle) {
         EXPECT_TRUE(download(opt.second_moment(params[i])) == v[i]);
     }
     EXPECT_EQ(opt.timestep(), 3);
+}
+
+// One AdamW step of one value, each operation rounded to binary32.
+void adamw_value(float& p, float g, float& m, float& v, float lr, float wd, int t, float f) {
+    const float b1 = 0.9f, b2 = 0.95f, eps = 1e-8f;
+    const float c1 = 1.0f - (float)std::pow((double)b1, t), c2 = 1.0f - (float)std::pow((double)b2, t);
+    volatile float ge = g * f;
+    volatile float m1 = b1 * m, m2 = (1.0f - b1) * ge, v1 = b2 * v, v2 = (1.0f - b2) * ge;
+    volatile float v3 = v2 * ge;
+    m = m1 + m2;
+    v = v1 + v3;
+    volatile float mh = m / c1, vh = v / c2, lw = lr * wd;
+    volatile float keep = 1.0f - lw, root = std::sqrt(vh), num = lr * mh;
+    volatile float den = root + eps, pk = p * keep;
+    volatile float step = num / den;
+    p = pk - step;
+}
+
+TEST_F(AdamWOptimizerTest, StepsMatchFormulaBitForBit) {
+    const std::vector<std::vector<int>> shapes{{33, 40}, {257}, {3}};
+    std::vector<std::unique_ptr<tensor<float>>> ps, gs;
+    std::vector<tensor<float>*> pp, gp;
+    std::vector<std::vector<float>> p, g, m, v;
+    for (size_t i = 0; i < shapes.size(); ++i) {
+        ps.push_back(std::make_unique<tensor<float>>(shapes[i]));
+        gs.push_back(std::make_unique<tensor<float>>(shapes[i]));
+        p.push_back(uniform(ps[i]->size(), -1.0f, 1.0f, 401 + i));
+        g.push_back(uniform(ps[i]->size(), -0.1f, 0.1f, 411 + i));
+        ps[i]->upload(p[i].data());
+        gs[i]->upload(g[i].data());
+        m.emplace_back(p[i].size(), 0.0f);
+        v.emplace_back(p[i].size(), 0.0f);
+        pp.push_back(ps[i].get());
+        gp.push_back(gs[i].get());
+    }
+    AdamWOptimizer<float> opt(0.01f, 0.9f, 0.95f, 1e-8f, 0.1f);
+    opt.update_parameters(pp, gp);
+    opt.set_weight_decay(pp[1], 0.0f);
+    for (int t = 1; t <= 3; ++t) {
+        opt.step();
+        for (size_t i = 0; i < p.size(); ++i)
+            for (size_t k = 0; k < p[i].size(); ++k)
+                adamw_value(p[i][k], g[i][k], m[i][k], v[i][k], 0.01f, i == 1 ? 0.0f : 0.1f, t, 1.0f);
+    }
+    for (size_t i = 0; i < p.size(); ++i) EXPECT_TRUE(download(*ps[i]) == p[i]);
+    EXPECT_EQ(opt.timestep(), 3);
+    // clipped: the gradients keep their values
+    const float* norm = opt.step_clipped(0.5f);
+    float nv = 0.0f;
+    CHECK_HIP_EX(hipMemcpy(&nv, norm, sizeof(float), hipMemcpyDeviceToHost));
+    EXPECT_GT(nv, 0.5f);
+    for (size_t i = 0; i < p.size(); ++i) {
+        for (size_t k = 0; k < p[i].size(); ++k)
+            adamw_value(p[i][k], g[i][k], m[i][k], v[i][k], 0.01f, i == 1 ? 0.0f : 0.1f, 4, 0.5f / nv);
+        EXPECT_TRUE(download(*ps[i]) == p[i]);
+        EXPECT_TRUE(download(*gs[i]) == g[i]);
+    }
+}
+
+// 8-bit states: the first step, whose states start at zero, equals the 32-bit
+// one bit for bit; later ones stay within what half a step of the codes (2^-4
+// of m and of sqrt(v)) moves an update.
+TEST_F(AdamWOptimizerTest, EightBitStates) {
+    tensor<float> a({500}), b({500}), g({500});
+    const auto p0 = uniform(500, -1.0f, 1.0f, 421), g0 = uniform(500, 0.5f, 1.0f, 422);
+    a.upload(p0.data());
+    b.upload(p0.data());
+    g.upload(g0.data());
+    AdamWOptimizer<float> full(0.01f), small(0.01f, 0.9f, 0.999f, 1e-8f, 0.01f, 8);
+    EXPECT_EQ(small.state_bits(), 8);
+    full.update_parameters({&a}, {&g});
+    small.update_parameters({&b}, {&g});
+    full.step();
+    small.step();
+    EXPECT_TRUE(download(a) == download(b));
+    for (int t = 2; t <= 4; ++t) {
+        full.step();
+        small.step();
+        const auto x = download(a), y = download(b);
+        // m / sqrt(v) is 1 with a steady gradient; both have been kept to 2^-4
+        // t-1 times before step t, so that step is off by at most 2 (t-1) / 16
+        // of the rate, and the steps so far by t (t-1) / 16 (a quarter more for
+        // products of such errors)
+        for (int i = 0; i < 500; ++i) EXPECT_LE(std::abs(x[i] - y[i]), 0.01f * t * (t - 1) / 16.0f * 1.25f);
+    }
+}
+
+TEST_F(AdamWOptimizerTest, Refusals) {
+    EXPECT_THROW(AdamWOptimizer<float>(0.01f, 0.9f, 0.999f, 1e-8f, 0.0f, 16), std::invalid_argument);
+    tensor<float> p({4}), g({4}), bad({5});
+    AdamWOptimizer<float> opt;
+    opt.update_parameters({&p}, {});
+    EXPECT_THROW(opt.step(), std::invalid_argument);
+    opt.update_parameters({&p}, {&bad});
+    EXPECT_THROW(opt.step(), std::invalid_argument);
+    opt.update_parameters({&p, &p}, {&g, &g});
+    EXPECT_THROW(opt.step(), std::invalid_argument);
+    EXPECT_EQ(opt.timestep(), 0);
 }
 
 // step_clipped(max_norm) == clip_grad_norm(grads, max_norm) + step(), except
