@@ -946,14 +946,14 @@ def _experts_args(fn: str, offsets, scale, scales, experts: int, count: int, **c
 def _experts_out(fn: str, out, shape, dtype, device):
     torch = _torch()
     if out is None:
-        return torch.empty(shape, dtype=dtype or torch.bfloat16, device=device)
+        return torch.empty(shape, dtype=dtype or torch.bfloat16, device=device), shape[-1]
     if tuple(out.shape) != tuple(shape) or (dtype is not None and out.dtype != dtype) or out.device != device:
         raise ValueError(f"{fn}: out is {tuple(out.shape)} {out.dtype} on {out.device}, not {tuple(shape)} on {device}")
     if out.dim() == 2:
-        _rows(fn, "out", out, shape, out.dtype)
-    elif not out.is_contiguous():
+        return out, _rows(fn, "out", out, shape, out.dtype)
+    if not out.is_contiguous():
         raise ValueError(f"{fn}: out is not contiguous")
-    return out
+    return out, shape[-1]
 
 
 def _experts_rows(fn: str, c_fn: str, a_q, w_q, offsets, red: int, sa, sw, out_dtype, out):
@@ -964,11 +964,11 @@ def _experts_rows(fn: str, c_fn: str, a_q, w_q, offsets, red: int, sa, sw, out_d
     if a_q.shape[1] < red or w_q.shape[2] < red:
         raise ValueError(f"{fn}: rows of {a_q.shape[1]} and {w_q.shape[2]} codes, fewer than {red}")
     rows = a_q.shape[0]
-    out = _experts_out(fn, out, (rows, cols), out_dtype, a_q.device)
+    out, ld = _experts_out(fn, out, (rows, cols), out_dtype, a_q.device)
     n, k = (cols, red) if c_fn == "df_fp8_experts_fwd" else (red, cols)
     with _on(a_q):
         call(c_fn, _ptr(a_q), a_q.stride(0), _ptr(w_q), w_q.stride(1), rows, n, k, experts, _ptr(offsets), _ptr(sa),
-             _ptr(sw), int(_in_dtype(out)), _ptr(out), out.stride(0), _stream())
+             _ptr(sw), int(_in_dtype(out)), _ptr(out), ld, _stream())
     return out
 
 
@@ -1004,7 +1004,7 @@ def experts_dw(dyt_q, xt_q, offsets, rows: int, sdy, sx, out_dtype=None, out=Non
     N, K = dyt_q.shape[0], xt_q.shape[0]
     if out is None and out_dtype is None:
         out_dtype = torch.float32
-    out = _experts_out(fn, out, (experts, N, K), out_dtype, dyt_q.device)
+    out, _ = _experts_out(fn, out, (experts, N, K), out_dtype, dyt_q.device)
     with _on(dyt_q):
         call("df_fp8_experts_dw", _ptr(dyt_q), dyt_q.stride(0), _ptr(xt_q), xt_q.stride(0), rows, N, K, experts,
              _ptr(offsets), _ptr(sdy), _ptr(sx), int(_in_dtype(out)), _ptr(out), K, _stream())
@@ -1024,6 +1024,10 @@ def quantize_experts(w, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=True):
     _check_gpu(fn, w=w)
     E, N, K = w.shape
     dt = int(_in_dtype(w))
+    if w.numel() == 0:  # nothing to measure: the rule's scale of no values is 1
+        none = lambda r, c: torch.zeros((E, r, round16(c)), dtype=torch.uint8, device=w.device)
+        return (torch.ones(E, dtype=torch.float32, device=w.device), none(N, K) if want_q else None,
+                none(K, N) if want_qt else None)
     with _on(w):
         src = w.view(E, N * K)
         if src.stride(0) * w.element_size() % 16:  # the batched quantize takes tensors at 16-byte boundaries

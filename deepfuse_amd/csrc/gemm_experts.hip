@@ -275,6 +275,7 @@ template <int FA, bool SUMS> void launch(ExpertArgs& g, int c_dtype, hipStream_t
 int check_call(const char* fn, const ExpertArgs& g, int K, bool sums, int c_dtype, bool& empty) {
     DF_CHECK(g.rows >= 0 && g.M >= 0 && g.N >= 0 && K >= 0 && g.experts >= 0, DF_ERR_INVALID,
              "%s: a negative size (rows=%d, experts=%d)", fn, g.rows, g.experts);
+    DF_CHECK(g.rows <= 0x7FFF0000, DF_ERR_INVALID, "%s: %d rows", fn, g.rows);  // row counters step past the last
     DF_CHECK(g.experts <= kMaxExperts, DF_ERR_UNSUPPORTED, "%s: %d experts (at most %d)", fn, g.experts, kMaxExperts);
     DF_CHECK(c_dtype == DF_DTYPE_FLOAT32 || c_dtype == DF_DTYPE_BFLOAT16 || c_dtype == DF_DTYPE_HALF,
              DF_ERR_UNSUPPORTED, "%s: output dtype %d not supported", fn, c_dtype);

@@ -708,6 +708,15 @@ bool ln_dtype(int dtype) {
     return dtype == DF_DTYPE_FLOAT32 || dtype == DF_DTYPE_BFLOAT16 || dtype == DF_DTYPE_HALF;
 }
 
+// row and column counters step past the last by at most 2^13
+constexpr int kMostRows = 0x7FFF0000;
+
+// An output over an input: the same rows exactly, or a row would be written
+// before another wave reads it.
+bool same_rows(const void* out, int ldo, const void* in, int ldi, int rows) {
+    return !out || out != in || ldo == ldi || rows == 1;
+}
+
 bool el_aligned(const void* p, int dtype) { return ((uintptr_t)p & (dtype == DF_DTYPE_FLOAT32 ? 3u : 1u)) == 0; }
 
 }  // namespace
@@ -721,7 +730,8 @@ extern "C" int df_layernorm_forward(int dtype, const void* x, int rows, int cols
                                     void* y, int ldy, float* mean, float* rstd, void* stream) {
     clear_error();
     const char* fn = "df_layernorm_forward";
-    DF_CHECK(rows >= 0 && cols >= 0, DF_ERR_INVALID, "%s: bad shape rows=%d cols=%d", fn, rows, cols);
+    DF_CHECK(rows >= 0 && cols >= 0 && rows <= kMostRows && cols <= kMostRows, DF_ERR_INVALID,
+             "%s: bad shape rows=%d cols=%d", fn, rows, cols);
     DF_CHECK(ln_dtype(dtype), DF_ERR_UNSUPPORTED, "%s: dtype %d not supported", fn, dtype);
     DF_CHECK((gamma == nullptr) == (beta == nullptr), DF_ERR_INVALID, "%s: gamma and beta go together", fn);
     DF_CHECK(eps >= 0.0f, DF_ERR_INVALID, "%s: eps < 0", fn);
@@ -731,6 +741,9 @@ extern "C" int df_layernorm_forward(int dtype, const void* x, int rows, int cols
     DF_CHECK(!sum || sum != y, DF_ERR_INVALID, "%s: sum and y are the same buffer", fn);
     DF_CHECK(ldx >= cols && ldy >= cols && (!residual || ldr >= cols) && (!sum || lds >= cols), DF_ERR_INVALID,
              "%s: a leading dimension is below cols=%d", fn, cols);
+    DF_CHECK(same_rows(sum, lds, x, ldx, rows) && same_rows(sum, lds, residual, ldr, rows) &&
+                 same_rows(y, ldy, x, ldx, rows) && same_rows(y, ldy, residual, ldr, rows),
+             DF_ERR_INVALID, "%s: an output lies over an input with another leading dimension", fn);
     for (const void* p : {x, residual, (const void*)sum, gamma, beta, (const void*)y})
         DF_CHECK(el_aligned(p, dtype), DF_ERR_ALIGN, "%s: a pointer is not aligned to its elements", fn);
     DF_CHECK(aligned4(mean) && aligned4(rstd), DF_ERR_ALIGN, "%s: mean or rstd misaligned", fn);
@@ -759,7 +772,8 @@ extern "C" int df_layernorm_backward(int dtype, const void* dy, int lddy, const 
                                      void* ws, size_t ws_bytes, void* stream) {
     clear_error();
     const char* fn = "df_layernorm_backward";
-    DF_CHECK(rows >= 0 && cols >= 0, DF_ERR_INVALID, "%s: bad shape rows=%d cols=%d", fn, rows, cols);
+    DF_CHECK(rows >= 0 && cols >= 0 && rows <= kMostRows && cols <= kMostRows, DF_ERR_INVALID,
+             "%s: bad shape rows=%d cols=%d", fn, rows, cols);
     DF_CHECK(ln_dtype(dtype), DF_ERR_UNSUPPORTED, "%s: dtype %d not supported", fn, dtype);
     DF_CHECK((mean == nullptr) == (rstd == nullptr), DF_ERR_INVALID, "%s: mean and rstd go together", fn);
     DF_CHECK((dgamma == nullptr) == (dbeta == nullptr), DF_ERR_INVALID, "%s: dgamma and dbeta go together", fn);
@@ -768,6 +782,9 @@ extern "C" int df_layernorm_backward(int dtype, const void* dy, int lddy, const 
     DF_CHECK(rows == 0 || (dy && x && dx), DF_ERR_INVALID, "%s: dy, x or dx is NULL", fn);
     DF_CHECK(rows == 0 || (lddy >= cols && ldx >= cols && lddx >= cols && (!dresidual || lddr >= cols)),
              DF_ERR_INVALID, "%s: a leading dimension is below cols=%d", fn, cols);
+    DF_CHECK(same_rows(dx, lddx, dy, lddy, rows) && same_rows(dx, lddx, x, ldx, rows) &&
+                 same_rows(dx, lddx, dresidual, lddr, rows),
+             DF_ERR_INVALID, "%s: dx lies over an input with another leading dimension", fn);
     for (const void* p : {dy, x, gamma, dresidual, (const void*)dx})
         DF_CHECK(el_aligned(p, dtype), DF_ERR_ALIGN, "%s: a pointer is not aligned to its elements", fn);
     DF_CHECK(aligned4(mean) && aligned4(rstd) && aligned4(dgamma) && aligned4(dbeta), DF_ERR_ALIGN,

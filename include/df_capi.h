@@ -293,8 +293,8 @@ int df_layernorm_quantize_delayed(int dtype, const void* x, int rows, int cols, 
  *                         mean, var and rstd of s as above;
  *                         y = fma((s - mean) * rstd, gamma, beta), rounded
  *                         once.  mean and rstd (fp32 [rows]) may be NULL.
- *                         sum may be x or residual, y may be x or residual;
- *                         sum and y differ.
+ *                         sum may be x or residual, y may be x or residual
+ *                         (with its leading dimension); sum and y differ.
  *  df_layernorm_backward: with xh = (x - mean) * rstd and g = dy * gamma,
  *                         dx = rstd * (g - mean(g) - xh * mean(g * xh))
  *                         + dresidual (NULL: none; the gradient that reaches
@@ -303,8 +303,8 @@ int df_layernorm_quantize_delayed(int dtype, const void* x, int rows, int cols, 
  *                         fp32 [cols], overwritten (both NULL: not wanted).
  *                         x is the forward's s.  mean and rstd NULL: taken
  *                         from x at eps again (after df_layernorm_quantize,
- *                         which keeps none).  dx may be dy, x or dresidual.
- *                         No rows: dgamma and dbeta are zeroed.  ws:
+ *                         which keeps none).  dx may be dy, x or dresidual
+ *                         (with its leading dimension).  No rows: dgamma and dbeta are zeroed.  ws:
  *                         df_layernorm_backward_workspace_bytes(rows, cols)
  *                         bytes, 16-byte aligned.  The column sums add rows in
  *                         a fixed order: deterministic. */

@@ -16,7 +16,7 @@ def rows_call(fn, a=FAKE, lda=32, w=FAKE, ldw=32, rows=8, N=32, K=32, experts=4,
 
 @pytest.mark.parametrize("fn", ["df_fp8_experts_fwd", "df_fp8_experts_dx"])
 @pytest.mark.parametrize("status,kw", [
-    (-1, dict(rows=-1)), (-1, dict(N=-1, K=-1)), (-1, dict(experts=-1)), (-2, dict(experts=1025)),
+    (-1, dict(rows=-1)), (-1, dict(rows=0x7FFFFFFF)), (-1, dict(N=-1, K=-1)), (-1, dict(experts=-1)), (-2, dict(experts=1025)),
     (-2, dict(dt=int(DType.INT8))), (-1, dict(ldo=31)), (-1, dict(off=None)), (-1, dict(s=None)), (-1, dict(sw=None)),
     (-1, dict(out=None)), (-1, dict(a=None)), (-1, dict(w=None)), (-4, dict(lda=24)), (-4, dict(ldw=16)),
     (-4, dict(a=FAKE + 8)), (-4, dict(w=FAKE + 8)), (-2, dict(ldw=1 << 23)), (-4, dict(off=FAKE + 2)), (-4, dict(out=FAKE + 2)),

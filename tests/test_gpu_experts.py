@@ -247,6 +247,9 @@ def test_quantize_experts(dev):
                 a, b = df.quantize_2d(we, s, Fmt.E4M3, want_qt=True)
                 assert sc[e] == s[0] and torch.equal(q[e], a) and torch.equal(qt[e], b)
             assert df.quantize_experts(w, want_qt=False)[2] is None
+    for shape in ((0, 4, 8), (2, 0, 8), (2, 4, 0)):
+        sc, q, qt = df.quantize_experts(torch.zeros(shape, device=dev))
+        assert (sc == 1).all() and q.shape == (*shape[:2], df.round16(shape[2])) and not q.any() and not qt.any()
 
 
 @pytest.mark.parametrize("counts", [[20, 0, 31, 13], [700, 900, 650]])

@@ -9,8 +9,8 @@ FAKE = 0x1000  # never dereferenced: each call fails its checks first
 F32, BF = int(DType.FLOAT32), int(DType.BFLOAT16)
 
 
-def fwd(dtype=F32, x=FAKE, rows=4, cols=8, ldx=8, res=None, ldr=0, sum=None, lds=0, gamma=FAKE, beta=FAKE, eps=1e-5, y=FAKE,
-        ldy=8, mean=None, rstd=None):
+def fwd(dtype=F32, x=FAKE, rows=4, cols=8, ldx=8, res=None, ldr=0, sum=None, lds=0, gamma=FAKE, beta=FAKE, eps=1e-5,
+        y=FAKE, ldy=8, mean=None, rstd=None):
     return df.lib().df_layernorm_forward(dtype, x, rows, cols, ldx, res, ldr, sum, lds, gamma, beta, eps, y, ldy, mean, rstd,
                                          None)
 
@@ -26,7 +26,8 @@ def bwd(dtype=F32, dy=FAKE, lddy=8, x=FAKE, ldx=8, rows=4, cols=8, gamma=FAKE, m
     (-1, dict(eps=float("nan"))), (-1, dict(sum=FAKE + 64)), (-1, dict(x=None)), (-1, dict(y=None)), (-1, dict(ldx=7)),
     (-1, dict(ldy=7)), (-1, dict(res=FAKE, ldr=7)), (-1, dict(res=FAKE, ldr=8, sum=FAKE, lds=8, y=FAKE)),
     (-1, dict(res=FAKE, ldr=8, sum=FAKE + 64, lds=7)), (-4, dict(x=FAKE + 2)), (-4, dict(dtype=BF, y=FAKE + 1)),
-    (-4, dict(mean=FAKE + 2)), (0, dict(rows=0, x=None, y=None)), (0, dict(cols=0, ldx=0, ldy=0)),
+    (-1, dict(rows=0x7FFFFFFF)), (-1, dict(y=FAKE, ldy=9)), (-1, dict(res=FAKE + 64, ldr=9, sum=FAKE, lds=9, y=FAKE + 128)),
+    (-1, dict(res=FAKE + 64, ldr=9, sum=FAKE + 64, lds=8, y=FAKE + 128)), (-4, dict(mean=FAKE + 2)), (0, dict(rows=0, x=None, y=None)), (0, dict(cols=0, ldx=0, ldy=0)),
 ])
 def test_forward_refusals(status, kw):
     assert fwd(**kw) == status
@@ -37,6 +38,7 @@ def test_forward_refusals(status, kw):
 @pytest.mark.parametrize("status,kw", [
     (-1, dict(rows=-1)), (-1, dict(cols=-1)), (-2, dict(dtype=int(DType.FP8E4M3))), (-1, dict(mean=None)),
     (-1, dict(dg=None)), (-1, dict(eps=-1.0)), (-1, dict(dy=None)), (-1, dict(x=None)), (-1, dict(dx=None)),
+    (-1, dict(cols=0x7FFFFFFF, lddy=0x7FFFFFFF)), (-1, dict(dx=FAKE, lddx=9)), (-1, dict(dr=FAKE, lddr=9)),
     (-1, dict(lddy=7)), (-1, dict(ldx=0)), (-1, dict(lddx=7)), (-1, dict(dr=FAKE, lddr=7)), (-4, dict(dy=FAKE + 2)),
     (-4, dict(dg=FAKE + 1)), (-5, dict(ws=None)), (-5, dict(ws=FAKE + 8)), (-5, dict(wsb=4 * 8 * 8 - 1)),
     (0, dict(cols=0, dy=None, x=None, dx=None, ws=None, wsb=0)),
