@@ -87,6 +87,21 @@ typedef f32x4 f32x4_el __attribute__((aligned(4)));
 typedef u32x2 u32x2_el __attribute__((aligned(2)));
 typedef uint32_t u32_el __attribute__((aligned(1)));
 
+// Lists larger than the 256 MB Infinity Cache stream past it: two GPT-2 XL
+// blocks (61.5M values, 8-bit states, 1 GB moved) 194 us against 205 with
+// plain accesses.  Smaller ones stay in it for whoever reads the parameters
+// next: one GPT-2 small block (7M values, 32-bit states) 30.6 us plain, 34.7
+// past the cache.
+constexpr int64_t kColdBytes = (int64_t)256 << 20;
+template <bool NT, typename V> __device__ __forceinline__ auto ldv(const V* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool NT, typename V, typename X> __device__ __forceinline__ void stv(V* p, X v) {
+    if constexpr (NT) __builtin_nontemporal_store((V)v, p);
+    else *p = v;
+}
+
 // maximum over the wave (VALU only): rows of 16 lanes, then across them
 __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
 #define DF_DPP_MAX(CTRL) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true))
@@ -110,7 +125,9 @@ template <> __device__ __forceinline__ float grad_one<f16_t>(const f16_t* p) {
 // four gradients as loaded, and widened
 template <typename G> struct Grad4 {
     u32x2 w;
-    __device__ __forceinline__ void load(const G* p) { w = *reinterpret_cast<const u32x2_el*>(p); }
+    template <bool NT> __device__ __forceinline__ void load(const G* p) {
+        w = ldv<NT>(reinterpret_cast<const u32x2_el*>(p));
+    }
     __device__ __forceinline__ void widen(float* g) const {
         if constexpr (std::is_same<G, uint16_t>::value) {
             g[0] = __uint_as_float(w.x << 16); g[1] = __uint_as_float(w.x & 0xFFFF0000u);
@@ -125,7 +142,9 @@ template <typename G> struct Grad4 {
 };
 template <> struct Grad4<float> {
     f32x4 w;
-    __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const f32x4_el*>(p); }
+    template <bool NT> __device__ __forceinline__ void load(const float* p) {
+        w = ldv<NT>(reinterpret_cast<const f32x4_el*>(p));
+    }
     __device__ __forceinline__ void widen(float* g) const {
 #pragma unroll
         for (int e = 0; e < 4; ++e) g[e] = w[e];
@@ -183,8 +202,8 @@ __device__ __forceinline__ float root_normal(float x) {  // x: 0 or in [2^-62, 2
 }
 
 // COPY: DF_DTYPE_BFLOAT16 or DF_DTYPE_HALF: the updated parameters are also
-// written in that type; -1: not.
-template <typename G, bool S8, int COPY>
+// written in that type; -1: not.  NT: the list is larger than the cache.
+template <typename G, bool S8, int COPY, bool NT>
 __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const WHyper h) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int lo = 0, hi = L.count - 1;  // the tensor that owns this block: the last with first <= blockIdx.x
@@ -298,16 +317,16 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
 #pragma unroll
                 for (int u = 0; u < kUnits; ++u) {
                     const int64_t i = u0 + u * stride + lane * 4;
-                    rg[u].load(gp + i);
-                    rp[u] = *reinterpret_cast<const f32x4_el*>(t.p + i);
+                    rg[u].template load<NT>(gp + i);
+                    rp[u] = ldv<NT>(reinterpret_cast<const f32x4_el*>(t.p + i));
                     if constexpr (S8) {
-                        cm[u] = *reinterpret_cast<const u32_el*>(static_cast<const uint8_t*>(t.m) + i);
-                        cv[u] = *reinterpret_cast<const u32_el*>(static_cast<const uint8_t*>(t.v) + i);
+                        cm[u] = ldv<NT>(reinterpret_cast<const u32_el*>(static_cast<const uint8_t*>(t.m) + i));
+                        cv[u] = ldv<NT>(reinterpret_cast<const u32_el*>(static_cast<const uint8_t*>(t.v) + i));
                         sm[u] = t.ms[(u0 + u * stride) >> 8];
                         sv[u] = t.vs[(u0 + u * stride) >> 8];
                     } else {
-                        rm[u] = *reinterpret_cast<const f32x4_el*>(static_cast<const float*>(t.m) + i);
-                        rv[u] = *reinterpret_cast<const f32x4_el*>(static_cast<const float*>(t.v) + i);
+                        rm[u] = ldv<NT>(reinterpret_cast<const f32x4_el*>(static_cast<const float*>(t.m) + i));
+                        rv[u] = ldv<NT>(reinterpret_cast<const f32x4_el*>(static_cast<const float*>(t.v) + i));
                     }
                 }
 #pragma unroll
@@ -333,24 +352,24 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
                     const bool plain = moments(g, m, v);
                     if (plain) update(std::true_type{}, p, m, v, root);
                     else update(std::false_type{}, p, m, v, root);
-                    *reinterpret_cast<f32x4_el*>(t.p + i) = f32x4{p[0], p[1], p[2], p[3]};
+                    stv<NT>(reinterpret_cast<f32x4_el*>(t.p + i), f32x4{p[0], p[1], p[2], p[3]});
                     if constexpr (COPY >= 0)
-                        *reinterpret_cast<u32x2_el*>(t.copy + i) =
-                            u32x2{copy_bits<COPY>(p[0]) | (copy_bits<COPY>(p[1]) << 16),
-                                  copy_bits<COPY>(p[2]) | (copy_bits<COPY>(p[3]) << 16)};
+                        stv<NT>(reinterpret_cast<u32x2_el*>(t.copy + i),
+                                u32x2{copy_bits<COPY>(p[0]) | (copy_bits<COPY>(p[1]) << 16),
+                                      copy_bits<COPY>(p[2]) | (copy_bits<COPY>(p[3]) << 16)});
                     if constexpr (S8) {
                         float s0, s1;
                         const uint32_t c0 = encode(m, std::false_type{}, plain, s0);
                         const uint32_t c1 = encode(root, std::true_type{}, plain, s1);
-                        *reinterpret_cast<u32_el*>(static_cast<uint8_t*>(t.m) + i) = c0;
-                        *reinterpret_cast<u32_el*>(static_cast<uint8_t*>(t.v) + i) = c1;
+                        stv<NT>(reinterpret_cast<u32_el*>(static_cast<uint8_t*>(t.m) + i), c0);
+                        stv<NT>(reinterpret_cast<u32_el*>(static_cast<uint8_t*>(t.v) + i), c1);
                         if (lane == 0) {
                             t.ms[(u0 + u * stride) >> 8] = s0;
                             t.vs[(u0 + u * stride) >> 8] = s1;
                         }
                     } else {
-                        *reinterpret_cast<f32x4_el*>(static_cast<float*>(t.m) + i) = f32x4{m[0], m[1], m[2], m[3]};
-                        *reinterpret_cast<f32x4_el*>(static_cast<float*>(t.v) + i) = f32x4{v[0], v[1], v[2], v[3]};
+                        stv<NT>(reinterpret_cast<f32x4_el*>(static_cast<float*>(t.m) + i), f32x4{m[0], m[1], m[2], m[3]});
+                        stv<NT>(reinterpret_cast<f32x4_el*>(static_cast<float*>(t.v) + i), f32x4{v[0], v[1], v[2], v[3]});
                     }
                 }
                 continue;
@@ -433,17 +452,22 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
     }
 }
 
-template <typename G, bool S8>
+template <typename G, bool S8, bool NT>
 void launch_copy(int copy_dtype, int blocks, const WList& L, const WHyper& h, hipStream_t st) {
-    if (copy_dtype == DF_DTYPE_BFLOAT16) adamw_kernel<G, S8, DF_DTYPE_BFLOAT16><<<blocks, kWThreads, 0, st>>>(L, h);
-    else if (copy_dtype == DF_DTYPE_HALF) adamw_kernel<G, S8, DF_DTYPE_HALF><<<blocks, kWThreads, 0, st>>>(L, h);
-    else adamw_kernel<G, S8, -1><<<blocks, kWThreads, 0, st>>>(L, h);
+    if (copy_dtype == DF_DTYPE_BFLOAT16)
+        adamw_kernel<G, S8, DF_DTYPE_BFLOAT16, NT><<<blocks, kWThreads, 0, st>>>(L, h);
+    else if (copy_dtype == DF_DTYPE_HALF)
+        adamw_kernel<G, S8, DF_DTYPE_HALF, NT><<<blocks, kWThreads, 0, st>>>(L, h);
+    else
+        adamw_kernel<G, S8, -1, NT><<<blocks, kWThreads, 0, st>>>(L, h);
 }
 
-template <typename G> void launch_state(bool s8, int copy_dtype, int blocks, const WList& L, const WHyper& h,
-                                        hipStream_t st) {
-    if (s8) launch_copy<G, true>(copy_dtype, blocks, L, h, st);
-    else launch_copy<G, false>(copy_dtype, blocks, L, h, st);
+template <typename G>
+void launch_state(bool s8, bool cold, int copy_dtype, int blocks, const WList& L, const WHyper& h, hipStream_t st) {
+    if (s8 && cold) launch_copy<G, true, true>(copy_dtype, blocks, L, h, st);
+    else if (s8) launch_copy<G, true, false>(copy_dtype, blocks, L, h, st);
+    else if (cold) launch_copy<G, false, true>(copy_dtype, blocks, L, h, st);
+    else launch_copy<G, false, false>(copy_dtype, blocks, L, h, st);
 }
 
 }  // namespace
@@ -476,11 +500,12 @@ extern "C" int df_adamw_update(int count, const int64_t* sizes, float* const* pa
     DF_CHECK(aligned4(lr_dev) && aligned4(timestep_dev) && aligned4(clip_norm_dev) && aligned4(absmax_dev),
              DF_ERR_ALIGN, "%s: a device scalar is not 4-byte aligned", fn);
     const unsigned gmask = grad_dtype == DF_DTYPE_FLOAT32 ? 3u : 1u;
-    int64_t total = 0;
+    int64_t total = 0, values = 0;
     for (int i = 0; i < count; ++i) {
         DF_CHECK(sizes[i] >= 0, DF_ERR_INVALID, "%s: sizes[%d] = %lld is negative", fn, i, (long long)sizes[i]);
         if (sizes[i] == 0) continue;
         total += (sizes[i] + kSpan - 1) / kSpan;
+        values += sizes[i];
         DF_CHECK(total < (1ll << 31), DF_ERR_INVALID, "%s: too many elements", fn);
         DF_CHECK(params[i] && grads[i] && m[i] && v[i] && (!s8 || (m_scale[i] && v_scale[i])) && (!copies || copies[i]),
                  DF_ERR_INVALID, "%s: a pointer of tensor %d is NULL", fn, i);
@@ -505,6 +530,9 @@ extern "C" int df_adamw_update(int count, const int64_t* sizes, float* const* pa
     h.absmax = reinterpret_cast<uint32_t*>(absmax_dev);
     hipStream_t st = as_stream(stream);
     if (total == 0 && (!absmax_dev || count == 0)) return DF_OK;
+    // bytes a value occupies, states and copy included
+    const int64_t each = 4 + (s8 ? 2 : 8) + (grad_dtype == DF_DTYPE_FLOAT32 ? 4 : 2) + (copies ? 2 : 0);
+    const bool cold = values * each > kColdBytes;
     if (absmax_dev) {
         const uint32_t zero = 0;
         if (int rc = df_fill(absmax_dev, count, 4, &zero, stream)) return rc;  // empty tensors stay at 0
@@ -526,9 +554,9 @@ extern "C" int df_adamw_update(int count, const int64_t* sizes, float* const* pa
         L.first[c] = blocks;
         L.count = c;
         const int cd = copies ? copy_dtype : -1;
-        if (grad_dtype == DF_DTYPE_FLOAT32) launch_state<float>(s8, cd, blocks, L, h, st);
-        else if (grad_dtype == DF_DTYPE_HALF) launch_state<f16_t>(s8, cd, blocks, L, h, st);
-        else launch_state<uint16_t>(s8, cd, blocks, L, h, st);
+        if (grad_dtype == DF_DTYPE_FLOAT32) launch_state<float>(s8, cold, cd, blocks, L, h, st);
+        else if (grad_dtype == DF_DTYPE_HALF) launch_state<f16_t>(s8, cold, cd, blocks, L, h, st);
+        else launch_state<uint16_t>(s8, cold, cd, blocks, L, h, st);
     }
     return launch_status(fn);
 }

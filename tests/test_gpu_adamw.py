@@ -325,3 +325,28 @@ def test_all_magnitudes_bit_exact(dev, bits, beta2, t):
             (cm, sm), (cv, sv) = keep8(m), keep8(v, root=True)
             assert same(host(M)[0], cm) and same(host(V)[0], cv) and same(host(MS)[0], sm) and same(host(VS)[0], sv), k
             m, v = widen(sm, cm), widen(sv, cv, root=True)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("gdt,copy", [(torch.float32, None), (torch.bfloat16, torch.float16), (torch.float16, torch.bfloat16)])
+def test_lists_larger_than_the_cache(dev, bits, gdt, copy):
+    """The same tensors next to one that takes the list past 256 MB: equal bits."""
+    sizes = [8192 * 3 + 700, 1025, 40_000]
+    p, g = make(sizes, 12, gdt)
+    big = 40_000_000
+    runs = []
+    for extra in (0, big):
+        P, G = dev_list(p, dev), [t.to(dev) for t in g]
+        if extra:
+            P.append(torch.ones(extra, device=dev))
+            G.append(torch.full((extra,), 1e-3, dtype=gdt, device=dev))
+        M, V, MS, VS = df.adamw_state(P, bits)
+        C = None if copy is None else [torch.zeros_like(t, dtype=copy) for t in P]
+        for t in (1, 2):
+            df.adamw_update(P, G, M, V, t, weight_decay=0.1, m_scales=MS, v_scales=VS, copies=C, **HYPER)
+        runs.append([x[:3] for x in (P, M, V, MS, VS, C) if x is not None])
+        if extra:  # all values of the filler are alike, and so are their updates
+            assert (P[3] == P[3][0]).all() and (bits == 32 or (MS[3] == MS[3][0]).all())
+            assert copy is None or (C[3] == P[3][0].to(copy)).all()
+    for a, b in zip(*runs):
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
