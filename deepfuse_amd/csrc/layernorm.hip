@@ -94,13 +94,15 @@ template <> struct El<f16_t> {
 };
 
 // chunk j of a row of `cols` values at any element-aligned address; values
-// past the row's end are not read and count as 0
+// past the row's end are not read and count as 0.  Non-temporal: nothing reads
+// a norm's inputs again soon (16384 x 1600 bf16 with the residual: forward 46.1
+// us against 48.2, backward 53.4 against 54.3)
 template <typename T> __device__ __forceinline__ u32x4 load_chunk(const T* row, int j, int cols) {
     constexpr int E = El<T>::E;
     const int c = j * E;
     u32x4 w = {0, 0, 0, 0};
     if (c + E <= cols) {
-        w = *reinterpret_cast<const u32x4_el*>(row + c);
+        w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_el*>(row + c));
     } else if (c < cols) {
 #pragma unroll
         for (int e = 0; e < E - 1; ++e) {
@@ -345,7 +347,7 @@ template <typename T> struct BwdArgs {
 // SUMS: gamma's and beta's gradients are wanted.
 constexpr int bwd_threads(int rt) { return rt > 512 ? rt : 512; }
 template <typename T, int RT, int CH, bool SUMS>
-__global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_kernel(const BwdArgs<T> a) {
+__device__ __forceinline__ void backward_rows(const BwdArgs<T>& a, int blocks) {
     constexpr int E = El<T>::E;
     constexpr int GP = bwd_threads(RT) / RT;
     __shared__ float red[2][2][GP][RT / 64];
@@ -374,9 +376,12 @@ __global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_kernel(const B
 #pragma unroll
         for (int e = 0; e < E; ++e) sg[k][e] = sb[k][e] = 0.0f;
     }
-    const int step = gridDim.x * GP;
+    const int step = blocks * GP;
     int r = blockIdx.x * GP + group;
-    if (r < a.rows) fetch(r);
+    // a row ahead, but where 1024 threads leave no registers for it (12800 bf16
+    // columns: 672 us with it, 418 without, at 16384 rows)
+    constexpr bool AHEAD = RT < 1024;
+    if (AHEAD && r < a.rows) fetch(r);
     if (affine) {
 #pragma unroll
         for (int k = 0; k < CH; ++k) gw[k][threadIdx.x] = load_chunk<T>(a.gamma, t + RT * k, a.cols);
@@ -386,6 +391,7 @@ __global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_kernel(const B
     // the last row works on zeros and stores nothing
     for (int base = blockIdx.x * GP; base < a.rows; base += step, r += step) {
         const bool live = GP == 1 || r < a.rows;
+        if (!AHEAD) fetch(r);
         u32x4 cx[CH], cy[CH], cr[CH];
         float mean = nmean, rstd = nrstd;
 #pragma unroll
@@ -399,7 +405,7 @@ __global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_kernel(const B
 #pragma unroll
             for (int k = 0; k < CH; ++k) cr[k] = load_chunk<T>(a.dres + (int64_t)r * a.lddr, t + RT * k, a.cols);
         }
-        if (r + step < a.rows) fetch(r + step);
+        if (AHEAD && r + step < a.rows) fetch(r + step);
         if (!given)
             row_stats<T, RT, CH>([&](int k, float* o) { El<T>::widen(cx[k], o); }, t, a.cols, a.eps, rs, mean, rstd);
         if (GP > 1 && !live) mean = rstd = 0.0f;
@@ -456,7 +462,7 @@ __global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_kernel(const B
     if constexpr (SUMS) {
         float* og = a.part + (int64_t)blockIdx.x * 2 * a.cols;
         float* ob = og + a.cols;
-        if (gridDim.x == 1) {
+        if (blocks == 1) {
             og = a.dgamma;
             ob = a.dbeta;
         }
@@ -499,6 +505,65 @@ __global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_kernel(const B
                     ob[c] = sb[k][e];
                 }
             }
+    }
+}
+
+template <typename T, int RT, int CH, bool SUMS>
+__global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_kernel(const BwdArgs<T> a) {
+    backward_rows<T, RT, CH, SUMS>(a, gridDim.x);
+}
+
+// Few rows, their statistics given: dx and the column sums in one launch.  The
+// blocks behind the first `row_blocks` take 32 columns each and read dy and x
+// again (from the L2 the rows' blocks fill), a wave two rows at a time, so the
+// sums need neither partials nor a second launch.
+constexpr int kOnceCols = 32, kOnceLoads = 8;
+template <typename T, int RT, int CH>
+__global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_once_kernel(const BwdArgs<T> a, int row_blocks) {
+    if ((int)blockIdx.x < row_blocks) {
+        backward_rows<T, RT, CH, false>(a, row_blocks);
+        return;
+    }
+    constexpr int W = bwd_threads(RT) / 64;
+    __shared__ float red[W][2][kOnceCols];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane % kOnceCols;
+    const int c = ((int)blockIdx.x - row_blocks) * kOnceCols + i;
+    float sg = 0.0f, sb = 0.0f;
+    auto row = [&](int r, float d, float x) {
+        sg = __builtin_fmaf(d, (x - a.mean[r]) * a.rstd[r], sg);
+        sb += d;
+    };
+    if (c < a.cols) {
+        constexpr int STEP = 2 * W;
+        int r = 2 * w + lane / kOnceCols;
+        for (; r + (kOnceLoads - 1) * STEP < a.rows; r += kOnceLoads * STEP) {
+            float d[kOnceLoads], x[kOnceLoads];
+#pragma unroll
+            for (int k = 0; k < kOnceLoads; ++k) {
+                d[k] = El<T>::one(a.dy + (int64_t)(r + k * STEP) * a.lddy + c);
+                x[k] = El<T>::one(a.x + (int64_t)(r + k * STEP) * a.ldx + c);
+            }
+#pragma unroll
+            for (int k = 0; k < kOnceLoads; ++k) row(r + k * STEP, d[k], x[k]);
+        }
+        for (; r < a.rows; r += STEP)
+            row(r, El<T>::one(a.dy + (int64_t)r * a.lddy + c), El<T>::one(a.x + (int64_t)r * a.ldx + c));
+    }
+    sg += __shfl_xor(sg, 32, 64);
+    sb += __shfl_xor(sb, 32, 64);
+    if (lane < kOnceCols) {
+        red[w][0][i] = sg;
+        red[w][1][i] = sb;
+    }
+    __syncthreads();
+    if (w == 0 && lane < kOnceCols && c < a.cols) {
+#pragma unroll
+        for (int v = 1; v < W; ++v) {
+            sg += red[v][0][i];
+            sb += red[v][1][i];
+        }
+        a.dgamma[c] = sg;
+        a.dbeta[c] = sb;
     }
 }
 
@@ -631,14 +696,22 @@ LnShape bwd_shape(int cols, int esz) {
     return {0, 0};
 }
 
+// Rows up to which dx and the column sums share a launch (us, two launches
+// against one, bf16): 64 x 768 8.0 / 4.0, 512 x 768 8.1 / 4.5, 1024 x 1600
+// 11.7 / 8.1, 2048 x 1600 18.3 / 20.3; rows of a block or more leave large
+// partials: 512 x 6400 38.5 / 13.1, 2048 x 6400 53.4 / 37.2, 4096 x 6400 73.9 / 68.8.
+int once_rows(int threads) { return threads < 512 ? 1024 : 4096; }
 constexpr int kMaxParts = 512;  // partial sums of gamma's and beta's gradients
 constexpr int kWideParts = 64;
 
 // blocks of the backward kernel: 16 waves per CU walk the rows
 int bwd_blocks(int rows, const LnShape& s) {
     if (s.threads == 0) return std::min(rows, kWideParts);
+    // (four times round at least before there are more than 256: each leaves
+    // 2 * cols partial sums.  2048 x 1600 bf16: 14.7 us with 256 blocks, 18.4
+    // with 512; 8192 x 1600: 37.4 and 33.0)
     const int nt = bwd_threads(s.threads), per = nt / s.threads;
-    return std::min((rows + per - 1) / per, 256 * 1024 / nt);
+    return std::min((rows + per - 1) / per, std::min(256 * 1024 / nt, std::max(256, rows / (4 * per))));
 }
 
 template <typename T> void launch_forward(const FwdArgs<T>& a, hipStream_t st) {
@@ -674,6 +747,10 @@ template <typename T> void launch_backward(BwdArgs<T> a, float* stat, hipStream_
         if (sums) fold(0);
         return;
     }
+    // rows and columns in one launch, unless dx lies over dy or x, which the
+    // columns' blocks read: then these go first
+    const bool once = sums && a.mean && grid > 1 && s.threads > 0 && a.rows <= once_rows(s.threads);
+    const bool over = a.dx == a.dy || a.dx == a.x;
     if (s.threads == 0) {
         const int rgrid = std::min(a.rows, 512);
         if (!a.mean) {
@@ -691,6 +768,16 @@ template <typename T> void launch_backward(BwdArgs<T> a, float* stat, hipStream_
 #define DF_LN(RT, CH)                                                          \
     if (s.threads == RT && s.chunks == CH) {                                   \
         constexpr int NT = bwd_threads(RT);                                    \
+        if (once) {                                                            \
+            const int cb = (a.cols + kOnceCols - 1) / kOnceCols;               \
+            if (over) {                                                        \
+                ln_backward_once_kernel<T, RT, CH><<<cb, NT, 0, st>>>(a, 0);   \
+                ln_backward_kernel<T, RT, CH, false><<<grid, NT, 0, st>>>(a);  \
+            } else {                                                           \
+                ln_backward_once_kernel<T, RT, CH><<<grid + cb, NT, 0, st>>>(a, grid); \
+            }                                                                  \
+            return;                                                            \
+        }                                                                      \
         if (sums) ln_backward_kernel<T, RT, CH, true><<<grid, NT, 0, st>>>(a); \
         else ln_backward_kernel<T, RT, CH, false><<<grid, NT, 0, st>>>(a);     \
     }
