@@ -131,6 +131,23 @@ def test_many_rows(dev, dtype, rows, cols):
     assert torch.equal(alone[0], back[0]) and alone[1] is None and alone[2] is None
 
 
+@pytest.mark.parametrize("rows,cols,over", [(1024, 771, None), (1025, 771, None), (1024, 771, "dy"), (4096, 4200, None),
+                                            (4097, 4200, None), (4096, 4200, "s"), (9, 771, None), (8, 771, None)])
+def test_both_sides_of_one_launch(dev, rows, cols, over):
+    """Rows around the most whose dx and column sums share a launch, and around
+    one block's; dx over what the columns' sums read; the same call again."""
+    t = inputs(dev, rows, cols, torch.bfloat16, seed=rows + cols)
+    s, dy = t["x"], t["dy"]
+    _, _, mean, rstd = df.layernorm_forward(s, t["gamma"], t["beta"], 1e-5)
+    want = df.layernorm_backward(dy, s, t["gamma"], mean, rstd, dresidual=t["dr"])
+    check_backward(want, dy, s, t["gamma"], mean, rstd, t["dr"])
+    u = {"dy": dy.clone(), "s": s.clone()}
+    dx = torch.empty_like(s) if over is None else u[over]
+    dg, db = torch.empty(cols, device=dev), torch.empty(cols, device=dev)
+    c_backward(df.DType.BFLOAT16, u["dy"], u["s"], t["gamma"], mean, rstd, t["dr"], dx, dg, db)
+    assert torch.equal(dx, want[0]) and torch.equal(dg, want[1]) and torch.equal(db, want[2])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("cols,pad", [(771, 5), (1600, 1), (1600, 8), (2500, 3), (17000, 7)])
 def test_strided_rows(dev, dtype, cols, pad):
