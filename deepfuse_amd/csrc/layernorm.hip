@@ -93,25 +93,45 @@ template <> struct El<f16_t> {
     }
 };
 
-// chunk j of a row of `cols` values at any element-aligned address; values
-// past the row's end are not read and count as 0.  Non-temporal: nothing reads
-// a norm's inputs again soon (16384 x 1600 bf16 with the residual: forward 46.1
-// us against 48.2, backward 53.4 against 54.3)
+// Chunk j of a row of `cols` values at any element-aligned address, as one
+// load: where the row ends inside it, the 16 bytes up to the row's end, which
+// place_chunk() moves down when the values are used.  Put together from single
+// values at the load, the last chunk made its wave wait for all loads under way,
+// the next row's too: 16384 x 2500 bf16 took 128 us backward and 105
+// forward, and takes 81 and 67 so (2496 columns: 79 and 66).  Rows at odd
+// addresses alone cost nothing.  Plain loads: non-temporal ones drop the lines
+// that neighbouring rows share (1000 x 771 bf16 backward 11.4 us against 8.6).
 template <typename T> __device__ __forceinline__ u32x4 load_chunk(const T* row, int j, int cols) {
     constexpr int E = El<T>::E;
     const int c = j * E;
     u32x4 w = {0, 0, 0, 0};
-    if (c + E <= cols) {
-        w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_el*>(row + c));
-    } else if (c < cols) {
+    if (cols >= E) {
+        // (a 32-bit offset on the row's address, the same for every tensor)
+        const uint32_t at = (uint32_t)min(c, cols - E) * (uint32_t)sizeof(T);
+        if (c < cols) w = *reinterpret_cast<const u32x4_el*>(reinterpret_cast<const char*>(row) + at);
+    } else if (j == 0) {  // a row shorter than a chunk
 #pragma unroll
         for (int e = 0; e < E - 1; ++e) {
-            if (c + e < cols) {
-                if constexpr (sizeof(T) == 4) w[e] = __builtin_bit_cast(uint32_t, row[c + e]);
-                else w[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, row[c + e]) << (16 * (e & 1));
+            if (e < cols) {
+                if constexpr (sizeof(T) == 4) w[e] = __builtin_bit_cast(uint32_t, row[e]);
+                else w[e >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, row[e]) << (16 * (e & 1));
             }
         }
     }
+    return w;
+}
+
+// chunk j as load_chunk() gave it, its values in their places; those past the
+// row's end are 0
+template <typename T> __device__ __forceinline__ u32x4 place_chunk(u32x4 w, int j, int cols) {
+    constexpr int E = El<T>::E;
+    const int over = j * E + E - cols;  // values past the row's end, if 1 to E - 1
+    if (over <= 0 || over >= E || cols < E) return w;
+    const int half = sizeof(T) == 4 ? 2 * over : over;  // 16-bit places to move, 1 to 7
+    if (half & 4) w = u32x4{w[2], w[3], 0, 0};
+    if (half & 2) w = u32x4{w[1], w[2], w[3], 0};
+    if (half & 1)
+        w = u32x4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16};
     return w;
 }
 
@@ -163,11 +183,19 @@ template <int RT, int GP = 1> struct RowSum {
                 red[slot][1][gi][w] = b;
             }
             __syncthreads();
-            a = b = 0.0f;
+            if constexpr (RT >= 1024) {
+                // a wave's sums to a lane: all 32 in every lane took registers that
+                // the backward spilled (12800 bf16 columns: 627 us against 333)
+                const int l = threadIdx.x & 63;
+                a = wave_add(l < RT / 64 ? red[slot][0][gi][l] : 0.0f);
+                b = wave_add(l < RT / 64 ? red[slot][1][gi][l] : 0.0f);
+            } else {
+                a = b = 0.0f;
 #pragma unroll
-            for (int i = 0; i < RT / 64; ++i) {
-                a += red[slot][0][gi][i];
-                b += red[slot][1][gi][i];
+                for (int i = 0; i < RT / 64; ++i) {
+                    a += red[slot][0][gi][i];
+                    b += red[slot][1][gi][i];
+                }
             }
             slot ^= 1;
         }
@@ -240,18 +268,23 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void ln_forward_kernel(const F
     if (affine) {
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
-            gw[k] = load_chunk<T>(a.gamma, t + RT * k, a.cols);
-            bw[k] = load_chunk<T>(a.beta, t + RT * k, a.cols);
+            gw[k] = place_chunk<T>(load_chunk<T>(a.gamma, t + RT * k, a.cols), t + RT * k, a.cols);
+            bw[k] = place_chunk<T>(load_chunk<T>(a.beta, t + RT * k, a.cols), t + RT * k, a.cols);
         }
     }
+    // a row's last chunk is loaded with values of the chunk before it, which
+    // another wave may own, and the sum may lie over x: no wave stores of the
+    // first row before all have its loads on their way (later rows' loads come
+    // before the barriers of the row before them)
+    if constexpr (RT > 64) __syncthreads();
     for (; r < a.rows; r += step) {
         float v[CH][E];
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
-            El<T>::widen(nx[k], v[k]);
+            El<T>::widen(place_chunk<T>(nx[k], t + RT * k, a.cols), v[k]);
             if (add) {
                 float q[E];
-                El<T>::widen(nr[k], q);
+                El<T>::widen(place_chunk<T>(nr[k], t + RT * k, a.cols), q);
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[k][e] += q[e];
                 // the statistics are those of the sum as stored
@@ -341,9 +374,10 @@ template <typename T> struct BwdArgs {
 // columns for all its rows, so gamma's and beta's sums stay in its registers;
 // at the end the row groups' sums meet in LDS and leave as one partial per
 // block (2 * cols values), which ln_fold_kernel adds in block order.
-// Two chunks a thread: with a wave to a row of 1600 bf16 values, four chunks
-// and their sums spilled 28 registers a lane, whose reloads waited for the
-// next row's loads: 98.5 us against 48.5 (16384 rows).
+// Two chunks a thread and no row ahead: the sums leave no registers for more.
+// Four chunks (a wave to a row of 1600 bf16 values) spilled 28 a lane, 98.5 us
+// against 48.5 at 16384 rows; the next row's loads, of which the 16 waves of a
+// CU hide as much, fewer: 1600 columns 54 against 51, 12800 467 against 333.
 // SUMS: gamma's and beta's gradients are wanted.
 constexpr int bwd_threads(int rt) { return rt > 512 ? rt : 512; }
 template <typename T, int RT, int CH, bool SUMS>
@@ -356,32 +390,19 @@ __device__ __forceinline__ void backward_rows(const BwdArgs<T>& a, int blocks) {
     // gamma, each thread's own chunks: in LDS, where reading them waits for no
     // load under way, and takes no registers from row to row
     __shared__ u32x4 gw[CH][bwd_threads(RT)];
-    u32x4 nx[CH], ny[CH];
     const bool affine = a.gamma != nullptr, add = a.dres != nullptr, given = a.mean != nullptr;
-    float nmean = 0.0f, nrstd = 0.0f;
-    auto fetch = [&](int r) __attribute__((always_inline)) {
-#pragma unroll
-        for (int k = 0; k < CH; ++k) nx[k] = load_chunk<T>(a.x + (int64_t)r * a.ldx, t + RT * k, a.cols);
-#pragma unroll
-        for (int k = 0; k < CH; ++k) ny[k] = load_chunk<T>(a.dy + (int64_t)r * a.lddy, t + RT * k, a.cols);
-        if (given) {
-            nmean = a.mean[r];
-            nrstd = a.rstd[r];
-        }
-    };
+    // The chunk in which the rows end holds this many values of the chunk before
+    // it (a chunk behind it: all).  They stay where they were loaded, gamma's
+    // likewise (moving them cost registers that were spilled: 16384 x 1600 70 us
+    // against 51), count for neither sum and are not stored.
+    auto borrowed = [&](int k) { return a.cols < E ? 0 : max(0, (t + RT * k) * E + E - a.cols); };
     float sg[CH][E], sb[CH][E];
 #pragma unroll
-    for (int k = 0; k < CH; ++k) {
-        nx[k] = ny[k] = u32x4{0, 0, 0, 0};
+    for (int k = 0; k < CH; ++k)
 #pragma unroll
         for (int e = 0; e < E; ++e) sg[k][e] = sb[k][e] = 0.0f;
-    }
     const int step = blocks * GP;
     int r = blockIdx.x * GP + group;
-    // a row ahead, but where 1024 threads leave no registers for it (12800 bf16
-    // columns: 672 us with it, 418 without, at 16384 rows)
-    constexpr bool AHEAD = RT < 1024;
-    if (AHEAD && r < a.rows) fetch(r);
     if (affine) {
 #pragma unroll
         for (int k = 0; k < CH; ++k) gw[k][threadIdx.x] = load_chunk<T>(a.gamma, t + RT * k, a.cols);
@@ -391,23 +412,27 @@ __device__ __forceinline__ void backward_rows(const BwdArgs<T>& a, int blocks) {
     // the last row works on zeros and stores nothing
     for (int base = blockIdx.x * GP; base < a.rows; base += step, r += step) {
         const bool live = GP == 1 || r < a.rows;
-        if (!AHEAD) fetch(r);
         u32x4 cx[CH], cy[CH], cr[CH];
-        float mean = nmean, rstd = nrstd;
+        float mean = 0.0f, rstd = 0.0f;
 #pragma unroll
-        for (int k = 0; k < CH; ++k) {
-            cx[k] = nx[k];
-            cy[k] = ny[k];
-            if (GP > 1 && !live) cx[k] = cy[k] = u32x4{0, 0, 0, 0};
-        }
-        // used only after the row's sums: no need to have it a row ahead
-        if (add && live) {
+        for (int k = 0; k < CH; ++k) cx[k] = cy[k] = u32x4{0, 0, 0, 0};
+        if (live) {
 #pragma unroll
-            for (int k = 0; k < CH; ++k) cr[k] = load_chunk<T>(a.dres + (int64_t)r * a.lddr, t + RT * k, a.cols);
+            for (int k = 0; k < CH; ++k) cx[k] = load_chunk<T>(a.x + (int64_t)r * a.ldx, t + RT * k, a.cols);
+#pragma unroll
+            for (int k = 0; k < CH; ++k) cy[k] = load_chunk<T>(a.dy + (int64_t)r * a.lddy, t + RT * k, a.cols);
+            if (add) {
+#pragma unroll
+                for (int k = 0; k < CH; ++k) cr[k] = load_chunk<T>(a.dres + (int64_t)r * a.lddr, t + RT * k, a.cols);
+            }
+            if (given) {
+                mean = a.mean[r];
+                rstd = a.rstd[r];
+            }
         }
-        if (AHEAD && r + step < a.rows) fetch(r + step);
         if (!given)
-            row_stats<T, RT, CH>([&](int k, float* o) { El<T>::widen(cx[k], o); }, t, a.cols, a.eps, rs, mean, rstd);
+            row_stats<T, RT, CH>([&](int k, float* o) { El<T>::widen(place_chunk<T>(cx[k], t + RT * k, a.cols), o); },
+                                 t, a.cols, a.eps, rs, mean, rstd);
         if (GP > 1 && !live) mean = rstd = 0.0f;
         // xh and g = dy * gamma of chunk k.  Past the row's end dy is 0, so
         // what xh holds there adds nothing as long as it is finite: mean and
@@ -430,6 +455,12 @@ __device__ __forceinline__ void backward_rows(const BwdArgs<T>& a, int blocks) {
             __builtin_amdgcn_sched_barrier(0);  // one chunk's terms at a time: registers
             float xh[E], d[E], g[E];
             terms(k, xh, d, g);
+            const int over = borrowed(k);
+            if (over > 0) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (e < over) g[e] = 0.0f;
+            }
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 if (SUMS) {
@@ -456,7 +487,8 @@ __device__ __forceinline__ void backward_rows(const BwdArgs<T>& a, int blocks) {
                 g[e] = rstd * (g[e] - __builtin_fmaf(xh[e], c2, c1));
                 if (add) g[e] += q[e];
             }
-            store_chunk<T>(a.dx + (int64_t)r * a.lddx, t + RT * k, a.cols, El<T>::narrow(g));
+            store_chunk<T>(a.dx + (int64_t)r * a.lddx, t + RT * k, a.cols,
+                           place_chunk<T>(El<T>::narrow(g), t + RT * k, a.cols));
         }
     }
     if constexpr (SUMS) {
@@ -499,8 +531,8 @@ __device__ __forceinline__ void backward_rows(const BwdArgs<T>& a, int blocks) {
         for (int k = 0; k < CH; ++k)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const int c = (t + RT * k) * E + e;
-                if (c < a.cols) {
+                const int c = (t + RT * k) * E + e - borrowed(k);
+                if (e >= borrowed(k) && c < a.cols) {
                     og[c] = sg[k][e];
                     ob[c] = sb[k][e];
                 }
@@ -697,10 +729,10 @@ LnShape bwd_shape(int cols, int esz) {
 }
 
 // Rows up to which dx and the column sums share a launch (us, two launches
-// against one, bf16): 64 x 768 8.0 / 4.0, 512 x 768 8.1 / 4.5, 1024 x 1600
-// 11.7 / 8.1, 2048 x 1600 18.3 / 20.3; rows of a block or more leave large
-// partials: 512 x 6400 38.5 / 13.1, 2048 x 6400 53.4 / 37.2, 4096 x 6400 73.9 / 68.8.
-int once_rows(int threads) { return threads < 512 ? 1024 : 4096; }
+// against one, bf16): 64 x 768 8.7 / 4.3, 512 x 768 9.4 / 4.9, 1024 x 768 10.2 /
+// 7.1, 2048 x 768 12.1 / 13.2; 1024 x 6400 29.0 / 17.8, 4096 x 6400 61 / 82;
+// 1024 x 12800 46.9 / 42.6, 2048 x 12800 66 / 82.
+constexpr int kOnceRows = 1024;
 constexpr int kMaxParts = 512;  // partial sums of gamma's and beta's gradients
 constexpr int kWideParts = 64;
 
@@ -708,8 +740,8 @@ constexpr int kWideParts = 64;
 int bwd_blocks(int rows, const LnShape& s) {
     if (s.threads == 0) return std::min(rows, kWideParts);
     // (four times round at least before there are more than 256: each leaves
-    // 2 * cols partial sums.  2048 x 1600 bf16: 14.7 us with 256 blocks, 18.4
-    // with 512; 8192 x 1600: 37.4 and 33.0)
+    // 2 * cols partial sums.  2048 x 1600 bf16: 16.7 us with 256 blocks, 19.4
+    // with 512; 8192 x 1600: 35.7 and 33.6)
     const int nt = bwd_threads(s.threads), per = nt / s.threads;
     return std::min((rows + per - 1) / per, std::min(256 * 1024 / nt, std::max(256, rows / (4 * per))));
 }
@@ -749,7 +781,7 @@ template <typename T> void launch_backward(BwdArgs<T> a, float* stat, hipStream_
     }
     // rows and columns in one launch, unless dx lies over dy or x, which the
     // columns' blocks read: then these go first
-    const bool once = sums && a.mean && grid > 1 && s.threads > 0 && a.rows <= once_rows(s.threads);
+    const bool once = sums && a.mean && grid > 1 && s.threads > 0 && a.rows <= kOnceRows;
     const bool over = a.dx == a.dy || a.dx == a.x;
     if (s.threads == 0) {
         const int rgrid = std::min(a.rows, 512);
