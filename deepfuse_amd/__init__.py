@@ -747,6 +747,13 @@ def _row_vector(fn: str, name: str, t, n: int, dtype):
             raise ValueError(f"{fn}: {name} is not contiguous")
 
 
+def _plain(t, shape, dtype, at: int) -> bool:
+    """Absent, or a contiguous tensor of this shape and type on GPU ``at``: the
+    usual argument, seen in one test.  What is not gets its questions one by
+    one, for the layouts allowed beyond this and the error's text."""
+    return t is None or t.shape == shape and t.dtype is dtype and t.is_contiguous() and t.get_device() == at
+
+
 def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, residual=None):
     """LayerNorm over the last dim of a 2-D fp32/bf16/f16 tensor for training
     (df_layernorm_forward): returns (y, s, mean, rstd), where s = x + residual
@@ -755,20 +762,25 @@ def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, residual=None):
     fn, torch = "layernorm_forward", _torch()
     if x.dim() != 2:
         raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
-    _check_gpu(fn, x=x, gamma=gamma, beta=beta, residual=residual)
-    rows, cols = x.shape
-    dt, ldx = int(_in_dtype(x)), _rows(fn, "x", x, x.shape, x.dtype)
-    ldr = 0 if residual is None else _rows(fn, "residual", residual, x.shape, x.dtype)
-    _row_vector(fn, "gamma", gamma, cols, x.dtype)
-    _row_vector(fn, "beta", beta, cols, x.dtype)
+    shape, dtype, at = x.shape, x.dtype, x.get_device()
+    rows, cols = shape
+    ldx = ldr = cols
+    if not (at >= 0 and x.is_contiguous() and _plain(residual, shape, dtype, at) and _plain(gamma, (cols,), dtype, at)
+            and _plain(beta, (cols,), dtype, at)):
+        _check_gpu(fn, x=x, gamma=gamma, beta=beta, residual=residual)
+        ldx = _rows(fn, "x", x, shape, dtype)
+        ldr = cols if residual is None else _rows(fn, "residual", residual, shape, dtype)
+        _row_vector(fn, "gamma", gamma, cols, dtype)
+        _row_vector(fn, "beta", beta, cols, dtype)
+    dt = _in_dtype(x)
     with _on(x):
-        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-        s = x if residual is None else torch.empty_like(y)
-        mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+        y = x.new_empty(shape)
+        s = x if residual is None else x.new_empty(shape)
+        mean = x.new_empty(rows, dtype=torch.float32)
         rstd = torch.empty_like(mean)
-        call("df_layernorm_forward", dt, _ptr(x), rows, cols, ldx, _ptr(residual), ldr,
-             None if residual is None else _ptr(s), cols, _ptr(gamma), _ptr(beta), float(eps), _ptr(y), cols,
-             _ptr(mean), _ptr(rstd), _stream())
+        call("df_layernorm_forward", dt, x.data_ptr(), rows, cols, ldx, _ptr(residual), ldr,
+             None if residual is None else s.data_ptr(), cols, _ptr(gamma), _ptr(beta), float(eps), y.data_ptr(), cols,
+             mean.data_ptr(), rstd.data_ptr(), _stream())
     return y, s, mean, rstd
 
 
@@ -781,23 +793,29 @@ def layernorm_backward(dy, x, gamma=None, mean=None, rstd=None, eps=1e-5, dresid
     fn, torch = "layernorm_backward", _torch()
     if x.dim() != 2:
         raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
-    _check_gpu(fn, dy=dy, x=x, gamma=gamma, mean=mean, rstd=rstd, dresidual=dresidual)
-    rows, cols = x.shape
-    dt, ldx, lddy = int(_in_dtype(x)), _rows(fn, "x", x, x.shape, x.dtype), _rows(fn, "dy", dy, x.shape, x.dtype)
-    lddr = 0 if dresidual is None else _rows(fn, "dresidual", dresidual, x.shape, x.dtype)
-    _row_vector(fn, "gamma", gamma, cols, x.dtype)
-    _row_vector(fn, "mean", mean, rows, torch.float32)
-    _row_vector(fn, "rstd", rstd, rows, torch.float32)
+    shape, dtype, at = x.shape, x.dtype, x.get_device()
+    rows, cols = shape
+    ldx = lddy = lddr = cols
+    if not (at >= 0 and x.is_contiguous() and _plain(dy, shape, dtype, at) and _plain(dresidual, shape, dtype, at)
+            and _plain(gamma, (cols,), dtype, at) and _plain(mean, (rows,), torch.float32, at)
+            and _plain(rstd, (rows,), torch.float32, at)):
+        _check_gpu(fn, dy=dy, x=x, gamma=gamma, mean=mean, rstd=rstd, dresidual=dresidual)
+        ldx, lddy = _rows(fn, "x", x, shape, dtype), _rows(fn, "dy", dy, shape, dtype)
+        lddr = cols if dresidual is None else _rows(fn, "dresidual", dresidual, shape, dtype)
+        _row_vector(fn, "gamma", gamma, cols, dtype)
+        _row_vector(fn, "mean", mean, rows, torch.float32)
+        _row_vector(fn, "rstd", rstd, rows, torch.float32)
+    dt = _in_dtype(x)
     with _on(x):
-        dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-        dg = torch.empty(cols, dtype=torch.float32, device=x.device) if sums else None
+        dx = x.new_empty(shape)
+        dg = x.new_empty(cols, dtype=torch.float32) if sums else None
         db = torch.empty_like(dg) if sums else None
         # not a cached one: a captured graph keeps the workspace it was given
-        ws = torch.empty(int(lib().df_layernorm_backward_workspace_bytes(rows, cols)), dtype=torch.uint8,
-                         device=x.device)
-        call("df_layernorm_backward", dt, _ptr(dy), lddy, _ptr(x), ldx, rows, cols, _ptr(gamma), _ptr(mean),
-             _ptr(rstd), float(eps), _ptr(dresidual), lddr, _ptr(dx), cols, _ptr(dg), _ptr(db), _ptr(ws),
-             ws.numel(), _stream())
+        nws = lib().df_layernorm_backward_workspace_bytes(rows, cols)
+        ws = x.new_empty(nws, dtype=torch.uint8)
+        call("df_layernorm_backward", dt, dy.data_ptr(), lddy, x.data_ptr(), ldx, rows, cols, _ptr(gamma), _ptr(mean),
+             _ptr(rstd), float(eps), _ptr(dresidual), lddr, dx.data_ptr(), cols, _ptr(dg), _ptr(db), ws.data_ptr(), nws,
+             _stream())
     return dx, dg, db
 
 
@@ -807,20 +825,27 @@ def layernorm_backward(dy, x, gamma=None, mean=None, rstd=None, eps=1e-5, dresid
 _dtype_of = operator.attrgetter("dtype")
 
 
-def _list_of(fn: str, what: str, tensors, sizes, dtype, at: int):
-    """Checks a list of contiguous tensors of one dtype on GPU ``at``, of the
-    given sizes; returns their addresses.  A map over the list per question:
-    half the time of asking tensor by tensor."""
-    T = _torch().Tensor
-    if len(tensors) != len(sizes):
-        raise ValueError(f"{fn}: {len(tensors)} {what} for {len(sizes)} parameters")
-    if not (list(map(T.numel, tensors)) == sizes and set(map(_dtype_of, tensors)) == {dtype}
-            and all(map(T.is_contiguous, tensors)) and set(map(T.get_device, tensors)) == {at}):
-        for i, (t, n) in enumerate(zip(tensors, sizes)):
-            if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.get_device() != at:
-                raise ValueError(f"{fn}: {what}[{i}] ({tuple(t.shape)} {t.dtype} on {t.device}) is not a contiguous "
-                                 f"{dtype} tensor of {n} values on GPU {at}")
-    return array.array("Q", map(T.data_ptr, tensors))
+def _lists(fn: str, at: int, lists):
+    """Checks lists of contiguous tensors on GPU ``at``, given as (name,
+    tensors, sizes, dtype), sizes one per parameter in each; returns all their
+    addresses in order.  A map over all tensors per question: half the time of
+    asking tensor by tensor."""
+    T, n = _torch().Tensor, len(lists[0][2])
+    every, want, dtypes = [], [], []
+    for what, tensors, sizes, dtype in lists:
+        if len(tensors) != n:
+            raise ValueError(f"{fn}: {len(tensors)} {what} for {n} parameters")
+        every += tensors
+        want += sizes
+        dtypes += [dtype] * n
+    if not (list(map(T.numel, every)) == want and list(map(_dtype_of, every)) == dtypes
+            and all(map(T.is_contiguous, every)) and set(map(T.get_device, every)) == {at}):
+        for what, tensors, sizes, dtype in lists:
+            for i, (t, k) in enumerate(zip(tensors, sizes)):
+                if t.dtype != dtype or t.numel() != k or not t.is_contiguous() or t.get_device() != at:
+                    raise ValueError(f"{fn}: {what}[{i}] ({tuple(t.shape)} {t.dtype} on {t.device}) is not a "
+                                     f"contiguous {dtype} tensor of {k} values on GPU {at}")
+    return array.array("Q", map(T.data_ptr, every))
 
 
 def _grad_norm16(grads, clip):
@@ -829,7 +854,7 @@ def _grad_norm16(grads, clip):
         raise TypeError(f"{fn}: {grads[0].dtype} gradients are not clipped in place (give adamw_update the norm)")
     if not grads[0].is_cuda:
         raise ValueError(f"{fn}: the gradients are on {grads[0].device}, not on a GPU")
-    _list_of(fn, "grads", grads, [t.numel() for t in grads], grads[0].dtype, grads[0].get_device())
+    _lists(fn, grads[0].get_device(), [("grads", grads, [t.numel() for t in grads], grads[0].dtype)])
     sizes = _sizes(grads)
     with _on(grads[0]):
         ws = torch.empty(int(lib().df_grad_norm_workspace_bytes(len(grads), sizes)), dtype=torch.uint8,
@@ -879,27 +904,27 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
     gt = _in_dtype(grads[0]) if grads else DType.FLOAT32
     state = torch.float8_e4m3fn if eight else torch.float32
     sizes, at = [p.numel() for p in params], params[0].get_device()
-    p = _list_of(fn, "params", params, sizes, torch.float32, at)
-    g = _list_of(fn, "grads", grads, sizes, grads[0].dtype if grads else None, at)
-    m = _list_of(fn, "ms", ms, sizes, state, at)
-    v = _list_of(fn, "vs", vs, sizes, state, at)
-    written, sm, sv, c = [p, m, v], None, None, None
+    lists = [("params", params, sizes, torch.float32), ("grads", grads, sizes, grads[0].dtype if grads else None),
+             ("ms", ms, sizes, state), ("vs", vs, sizes, state)]
     if eight:
         blocks = [-(-k // 256) for k in sizes]
-        sm = _list_of(fn, "m_scales", m_scales, blocks, torch.float32, at)
-        sv = _list_of(fn, "v_scales", v_scales, blocks, torch.float32, at)
-        written += [sm, sv]
+        lists += [("m_scales", m_scales, blocks, torch.float32), ("v_scales", v_scales, blocks, torch.float32)]
     ct = DType.FLOAT32
     if copies is not None:
         ct = _in_dtype(copies[0]) if copies else ct
         if ct == DType.FLOAT32:
             raise TypeError(f"{fn}: copies are bf16 or float16")
-        c = _list_of(fn, "copies", copies, sizes, copies[0].dtype, at)
-        written.append(c)
+        lists.append(("copies", copies, sizes, copies[0].dtype))
+    addresses = _lists(fn, at, lists)
+    written = addresses[:n] + addresses[2 * n:]  # all but the gradients
     if 0 in sizes:  # empty tensors share an address
-        written = [[a for a, k in zip(arr, sizes) if k] for arr in written]
-    if len(set(itertools.chain(*written))) != sum(map(len, written)):
+        written = [a for a, k in zip(written, itertools.cycle(sizes)) if k]
+    if len(set(written)) != len(written):
         raise ValueError(f"{fn}: a tensor that the step writes is listed twice")
+    first = addresses.buffer_info()[0]
+    p, g, m, v = (first + 8 * n * i for i in range(4))
+    sm, sv = (first + 32 * n, first + 40 * n) if eight else (None, None)
+    c = None if copies is None else first + 8 * n * (len(lists) - 1)
     if isinstance(weight_decay, (int, float)):
         wd = (_c_f * n)(*[weight_decay] * n)
     else:
@@ -916,11 +941,9 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
     if absmax is not None and (absmax.dtype != torch.float32 or absmax.numel() < n or not absmax.is_contiguous()
                                or absmax.device != params[0].device):
         raise ValueError(f"{fn}: absmax is not {n} contiguous fp32 values on {params[0].device}")
-    at_of = lambda arr: None if arr is None else arr.buffer_info()[0]
     with _on(params[0]):
-        call("df_adamw_update", n, (_c_i64 * n)(*sizes), at_of(p), int(gt), at_of(g),
-             int(DType.FP8E4M3 if eight else DType.FLOAT32), at_of(m), at_of(v), at_of(sm), at_of(sv), int(ct), at_of(c),
-             0.0 if "lr" in scalars else float(lr), float(beta1), float(beta2), float(eps), wd,
+        call("df_adamw_update", n, (_c_i64 * n)(*sizes), p, gt, g, DType.FP8E4M3 if eight else DType.FLOAT32, m, v, sm,
+             sv, ct, c, 0.0 if "lr" in scalars else float(lr), float(beta1), float(beta2), float(eps), wd,
              0 if "timestep" in scalars else int(timestep), scalars.get("lr"), scalars.get("timestep"),
              scalars.get("clip_norm"), float(max_norm), _ptr(absmax), _stream())
 
@@ -931,7 +954,10 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
 def _experts_args(fn: str, offsets, scale, scales, experts: int, count: int, **codes):
     """Checks shared by the experts' products: devices, the offsets, the scales and the codes' layout."""
     torch = _torch()
-    _check_gpu(fn, offsets=offsets, scale=scale, scales=scales, **codes)
+    at = offsets.get_device()
+    if not (at >= 0 and scale.get_device() == at and scales.get_device() == at
+            and all(t.get_device() == at for t in codes.values())):
+        _check_gpu(fn, offsets=offsets, scale=scale, scales=scales, **codes)
     _row_vector(fn, "offsets", offsets, experts + 1, torch.int32)
     for name, t, n in (("scale", scale, 1), ("scales", scales, count)):
         if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
@@ -967,8 +993,8 @@ def _experts_rows(fn: str, c_fn: str, a_q, w_q, offsets, red: int, sa, sw, out_d
     out, ld = _experts_out(fn, out, (rows, cols), out_dtype, a_q.device)
     n, k = (cols, red) if c_fn == "df_fp8_experts_fwd" else (red, cols)
     with _on(a_q):
-        call(c_fn, _ptr(a_q), a_q.stride(0), _ptr(w_q), w_q.stride(1), rows, n, k, experts, _ptr(offsets), _ptr(sa),
-             _ptr(sw), int(_in_dtype(out)), _ptr(out), ld, _stream())
+        call(c_fn, a_q.data_ptr(), a_q.stride(0), w_q.data_ptr(), w_q.stride(1), rows, n, k, experts,
+             offsets.data_ptr(), sa.data_ptr(), sw.data_ptr(), _in_dtype(out), out.data_ptr(), ld, _stream())
     return out
 
 
