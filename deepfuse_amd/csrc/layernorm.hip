@@ -546,49 +546,63 @@ __global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_kernel(const B
 }
 
 // Few rows, their statistics given: dx and the column sums in one launch.  The
-// blocks behind the first `row_blocks` take 32 columns each and read dy and x
-// again (from the L2 the rows' blocks fill), a wave two rows at a time, so the
-// sums need neither partials nor a second launch.
-constexpr int kOnceCols = 32, kOnceLoads = 8;
+// blocks behind the first `row_blocks` take a few columns each and read dy and
+// x again (from the L2 the rows' blocks fill), a wave two or four rows at a
+// time, so the sums need neither partials nor a second launch.  Eight rows'
+// loads at a time, the last eight too: one by one, they took as long as the rest
+// (1000 x 771 bf16 8.2 us, 6.7 so).  16 columns a block for narrow rows, which
+// leave CUs idle (1024 x 768 7.2 us with 32, 6.7 with 16), 32 for wide ones
+// (1024 x 6400 17.4 and 23.7).
+constexpr int kOnceLoads = 8;
+constexpr int once_cols(int rt) { return rt <= 128 ? 16 : 32; }
 template <typename T, int RT, int CH>
 __global__ __launch_bounds__(bwd_threads(RT), 4) void ln_backward_once_kernel(const BwdArgs<T> a, int row_blocks) {
     if ((int)blockIdx.x < row_blocks) {
         backward_rows<T, RT, CH, false>(a, row_blocks);
         return;
     }
-    constexpr int W = bwd_threads(RT) / 64;
-    __shared__ float red[W][2][kOnceCols];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane % kOnceCols;
-    const int c = ((int)blockIdx.x - row_blocks) * kOnceCols + i;
+    constexpr int W = bwd_threads(RT) / 64, CW = once_cols(RT);
+    __shared__ float red[W][2][CW];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane % CW;
+    const int c = ((int)blockIdx.x - row_blocks) * CW + i;
     float sg = 0.0f, sb = 0.0f;
-    auto row = [&](int r, float d, float x) {
-        sg = __builtin_fmaf(d, (x - a.mean[r]) * a.rstd[r], sg);
-        sb += d;
-    };
     if (c < a.cols) {
-        constexpr int STEP = 2 * W;
-        int r = 2 * w + lane / kOnceCols;
-        for (; r + (kOnceLoads - 1) * STEP < a.rows; r += kOnceLoads * STEP) {
-            float d[kOnceLoads], x[kOnceLoads];
+        constexpr int STEP = 64 / CW * W;
+        // kOnceLoads rows from r0; LAST: only those that there are
+        auto rows = [&](int r0, auto last) __attribute__((always_inline)) {
+            constexpr bool LAST = decltype(last)::value;
+            float d[kOnceLoads], x[kOnceLoads], m[kOnceLoads], q[kOnceLoads];
 #pragma unroll
             for (int k = 0; k < kOnceLoads; ++k) {
-                d[k] = El<T>::one(a.dy + (int64_t)(r + k * STEP) * a.lddy + c);
-                x[k] = El<T>::one(a.x + (int64_t)(r + k * STEP) * a.ldx + c);
+                const int r = LAST ? min(r0 + k * STEP, a.rows - 1) : r0 + k * STEP;
+                d[k] = El<T>::one(a.dy + (int64_t)r * a.lddy + c);
+                x[k] = El<T>::one(a.x + (int64_t)r * a.ldx + c);
+                m[k] = a.mean[r];
+                q[k] = a.rstd[r];
             }
 #pragma unroll
-            for (int k = 0; k < kOnceLoads; ++k) row(r + k * STEP, d[k], x[k]);
-        }
-        for (; r < a.rows; r += STEP)
-            row(r, El<T>::one(a.dy + (int64_t)r * a.lddy + c), El<T>::one(a.x + (int64_t)r * a.ldx + c));
+            for (int k = 0; k < kOnceLoads; ++k) {
+                if (!LAST || r0 + k * STEP < a.rows) {
+                    sg = __builtin_fmaf(d[k], (x[k] - m[k]) * q[k], sg);
+                    sb += d[k];
+                }
+            }
+        };
+        int r = threadIdx.x / CW;
+        for (; r + (kOnceLoads - 1) * STEP < a.rows; r += kOnceLoads * STEP) rows(r, std::false_type{});
+        if (r < a.rows) rows(r, std::true_type{});
     }
-    sg += __shfl_xor(sg, 32, 64);
-    sb += __shfl_xor(sb, 32, 64);
-    if (lane < kOnceCols) {
+#pragma unroll
+    for (int off = CW; off < 64; off <<= 1) {
+        sg += __shfl_xor(sg, off, 64);
+        sb += __shfl_xor(sb, off, 64);
+    }
+    if (lane < CW) {
         red[w][0][i] = sg;
         red[w][1][i] = sb;
     }
     __syncthreads();
-    if (w == 0 && lane < kOnceCols && c < a.cols) {
+    if (w == 0 && lane < CW && c < a.cols) {
 #pragma unroll
         for (int v = 1; v < W; ++v) {
             sg += red[v][0][i];
@@ -730,9 +744,9 @@ LnShape bwd_shape(int cols, int esz) {
 }
 
 // Rows up to which dx and the column sums share a launch (us, two launches
-// against one, bf16): 64 x 768 8.7 / 4.3, 512 x 768 9.4 / 4.9, 1024 x 768 10.2 /
-// 7.1, 2048 x 768 12.1 / 13.2; 1024 x 6400 29.0 / 17.8, 4096 x 6400 61 / 82;
-// 1024 x 12800 46.9 / 42.6, 2048 x 12800 66 / 82.
+// against one, bf16): 64 x 768 8.7 / 4.3, 512 x 768 10.3 / 4.9, 1024 x 768 10.0 /
+// 6.7, 2048 x 768 11.5 / 13.2; 1024 x 6400 29.2 / 17.4, 4096 x 6400 61 / 82;
+// 1024 x 12800 47.4 / 42.6, 2048 x 12800 66 / 82.
 constexpr int kOnceRows = 1024;
 constexpr int kMaxParts = 512;  // partial sums of gamma's and beta's gradients
 constexpr int kWideParts = 64;
@@ -802,7 +816,7 @@ template <typename T> void launch_backward(BwdArgs<T> a, float* stat, hipStream_
     if (s.threads == RT && s.chunks == CH) {                                   \
         constexpr int NT = bwd_threads(RT);                                    \
         if (once) {                                                            \
-            const int cb = (a.cols + kOnceCols - 1) / kOnceCols;               \
+            const int cb = (a.cols + once_cols(RT) - 1) / once_cols(RT);       \
             if (over) {                                                        \
                 ln_backward_once_kernel<T, RT, CH><<<cb, NT, 0, st>>>(a, 0);   \
                 ln_backward_kernel<T, RT, CH, false><<<grid, NT, 0, st>>>(a);  \
