@@ -41,10 +41,49 @@ namespace dfk {
 namespace {
 
 // ------------------------------------------------------------ small tiles --
+// Row tile v of all experts' tiles of ROWS rows, counted through: its expert,
+// that one's rows [lo, hi) and the tile's first; false behind the last.  The
+// same for every lane of the wave (a lane counts an expert's tiles).
+template <int ROWS>
+__device__ __forceinline__ bool row_tile(const ExpertArgs& g, int v, int lane, int& e, int& lo, int& hi, int& m0) {
+    for (int base = 0; base < g.experts; base += 64) {
+        int a = 0, b = 0;
+        if (base + lane < g.experts) expert_rows(g.off, base + lane, g.rows, a, b);
+        const int mine = (b - a + ROWS - 1) / ROWS;
+        int upto = mine;  // summed up over the lanes: within rows of 16, then across them
+#define DF_SCAN(CTRL, ROWS_IN) upto += __builtin_amdgcn_update_dpp(0, upto, CTRL, ROWS_IN, 0xF, false)
+        DF_SCAN(0x111, 0xF);  // row_shr:1
+        DF_SCAN(0x112, 0xF);
+        DF_SCAN(0x114, 0xF);
+        DF_SCAN(0x118, 0xF);  // row_shr:8
+        DF_SCAN(0x142, 0xA);  // row_bcast:15 into the second and fourth row
+        DF_SCAN(0x143, 0xC);  // row_bcast:31 into the upper half
+#undef DF_SCAN
+        const int all = __builtin_amdgcn_readlane(upto, 63);
+        if (v < all) {
+            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > v));
+            e = base + l;
+            lo = __builtin_amdgcn_readlane(a, l);
+            hi = __builtin_amdgcn_readlane(b, l);
+            m0 = lo + (v - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l))) * ROWS;
+            return true;
+        }
+        v -= all;
+    }
+    return false;
+}
+
 // As gemm_small.hip's kernel: a block owns a 16*MT x 16*NT tile, its W waves
 // take the 128-byte K steps in turn and add up through LDS, in wave order.
-// ROWS: blockIdx.y is the expert, whose row tiles blockIdx.z, + gridDim.z, ...
-// the block computes.  SUMS: blockIdx.x is the tile, blockIdx.y the expert.
+// ROWS: blockIdx.x is the column tile.  Tiles of 16 rows, for experts of a few
+// rows: blockIdx.y is the expert.  Tiles of 32: all experts' row tiles, counted
+// through, are the block's from blockIdx.y in steps of gridDim.y, so that an
+// expert that got most rows keeps no block longer than others (936 rows over 45
+// experts, 300 of them one's, 1408 -> 448: 30.5 us with blocks bound to experts,
+// 14.8 so; even shares mostly take 0.3 us more, and up to 15% where blocks side
+// by side read the same weights from memory.  Counted in order of the tiles'
+// place in their expert, or with a column's tiles on one XCD: slower elsewhere).
+// SUMS: blockIdx.x is the tile, blockIdx.y the expert.
 // WIDE: codes are multiplied as bf16, eight of a lane's 32 at a time: which K
 // an instruction takes together is free as long as A and B agree.
 template <int FA, int FB, int MT, int NT, int W, int U, bool SUMS, bool WIDE>
@@ -55,23 +94,12 @@ __global__ __launch_bounds__(64 * W) void experts_small_kernel(const ExpertArgs 
     constexpr int RSTR = COLS + 4;     // row of a partial tile (floats)
     constexpr int RED = ROWS * RSTR * 4;
     constexpr uint32_t kOOB = 0x80000000u;
+    constexpr bool COUNTED = !SUMS && MT > 1;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[W * (SLAB > RED ? SLAB : RED)];
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int e = blockIdx.y;
-    int lo, hi;
-    expert_rows(g.off, e, g.rows, lo, hi);
     const int tiles_n = (g.N + COLS - 1) / COLS;
     const int n0 = (SUMS ? (int)(blockIdx.x % tiles_n) : (int)blockIdx.x) * COLS;
-    const int mbeg = SUMS ? (int)(blockIdx.x / tiles_n) * ROWS : lo + (int)blockIdx.z * ROWS;
-    const int mend = SUMS ? min(mbeg + 1, g.M) : hi;  // SUMS: one tile
-    // the reduction's bytes [k_lo, k_hi) of the operands' rows, in steps of 128 from kb
-    const int kb = SUMS ? lo & ~127 : 0, k_lo = SUMS ? lo : 0, k_hi = SUMS ? hi : g.K;
-    const int nk = (k_hi - kb + 127) >> 7;
-    const uint8_t* const Be = g.B + (SUMS ? 0 : (int64_t)e * g.N * g.ldb) + (int64_t)n0 * g.ldb;
-    const __amdgpu_buffer_rsrc_t rB = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)Be, (short)0, min(g.N - n0, COLS) * g.ldb, 0x00020000);
-    const float sab = g.sa[0] * g.sb[SUMS ? 0 : e];
 
     // loads: lane l takes 16-byte chunk l%8 of row l/8 of each 8-row group
     const int lr = lane >> 3, lc = (lane & 7) * 16;
@@ -91,7 +119,23 @@ __global__ __launch_bounds__(64 * W) void experts_small_kernel(const ExpertArgs 
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
     };
 
-    for (int m0 = mbeg; m0 < mend; m0 += SUMS ? ROWS : (int)gridDim.z * ROWS) {
+    for (int v = COUNTED ? (int)blockIdx.y : 0;; v += COUNTED ? (int)gridDim.y : 1) {
+        int e, lo, hi, m0;
+        if constexpr (COUNTED) {
+            if (!row_tile<ROWS>(g, v, lane, e, lo, hi, m0)) return;  // the whole block
+        } else {
+            e = blockIdx.y;
+            expert_rows(g.off, e, g.rows, lo, hi);
+            m0 = SUMS ? (int)(blockIdx.x / tiles_n) * ROWS : lo + v * ROWS;
+            if (!SUMS && m0 >= hi) return;
+        }
+        // the reduction's bytes [k_lo, k_hi) of the operands' rows, in steps of 128 from kb
+        const int kb = SUMS ? lo & ~127 : 0, k_lo = SUMS ? lo : 0, k_hi = SUMS ? hi : g.K;
+        const int nk = (k_hi - kb + 127) >> 7;
+        const uint8_t* const Be = g.B + (SUMS ? 0 : (int64_t)e * g.N * g.ldb) + (int64_t)n0 * g.ldb;
+        const __amdgpu_buffer_rsrc_t rB = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)Be, (short)0, min(g.N - n0, COLS) * g.ldb, 0x00020000);
+        const float sab = g.sa[0] * g.sb[SUMS ? 0 : e];
         const int mrows = min((SUMS ? g.M : hi) - m0, ROWS);
         const __amdgpu_buffer_rsrc_t rA = __builtin_amdgcn_make_buffer_rsrc(
             (void*)(g.A + (int64_t)m0 * g.lda), (short)0, mrows * g.lda, 0x00020000);
@@ -198,6 +242,7 @@ __global__ __launch_bounds__(64 * W) void experts_small_kernel(const ExpertArgs 
             else if (c_dtype == DF_DTYPE_HALF) put(static_cast<f16_t*>(g.C) + at);
             else put(static_cast<uint16_t*>(g.C) + at);
         }
+        if (SUMS) return;
         __syncthreads();  // the partial tiles are read before slabs go over them
     }
 }
@@ -207,33 +252,38 @@ template <int FA, bool SUMS, bool WIDE> void launch_small(const ExpertArgs& g, i
         const dim3 grid(((g.N + 31) / 32) * ((g.M + 31) / 32), g.experts);
         experts_small_kernel<FA, E4M3, 2, 2, 4, 2, true, WIDE><<<grid, 256, 0, st>>>(g, c_dtype);
     } else {
-        const int per = (g.rows + g.experts - 1) / g.experts;  // rows of an expert if dealt evenly
-        if (per <= 16) {
-            const dim3 grid((g.N + 15) / 16, g.experts, 1);
+        if ((g.rows + g.experts - 1) / g.experts <= 16) {
+            const dim3 grid((g.N + 15) / 16, g.experts);
             experts_small_kernel<FA, E4M3, 1, 1, 4, 4, false, WIDE><<<grid, 256, 0, st>>>(g, c_dtype);
         } else {
-            const dim3 grid((g.N + 31) / 32, g.experts, std::min((per + 31) / 32, 64));
+            // at most this many row tiles; blocks behind the last return at once
+            const int64_t most = (int64_t)g.rows / 32 + std::min(g.experts, g.rows);
+            const dim3 grid((g.N + 31) / 32, (int)std::min<int64_t>(most, 65535));
             experts_small_kernel<FA, E4M3, 2, 2, 4, 2, false, WIDE><<<grid, 256, 0, st>>>(g, c_dtype);
         }
     }
 }
 
 // Which kernel a call takes; the host knows the rows, not how they were dealt,
-// and goes by `per`, an expert's rows if dealt evenly.  Measured (us a call,
-// small tiles against large ones):
-//  ROWS, 2-byte output, 8 experts 1600 -> 6400: per 32 26.4 / 27.2, per 64
-//    36.7 / 24.7; 32 experts 1600 -> 1600: 26.5 / 27.3 and 38.3 / 22.9; fp32
-//    output (half the matrix rate, which small tiles do not feel), 8 experts:
-//    per 64 38.5 / 46.1, per 128 63.7 / 46.2.  Outputs of 64 columns leave half
-//    a large tile idle: 8 experts 1600 -> 64, per 1024: 11.2 / 15.1.
+// and counts row tiles as if dealt evenly.
+//  ROWS: by the time either would take, in us, a step being 128 of K.  Large
+//    tiles: 5 + 1.2 for each wide step (0.72 for a narrow one; 2.05 times as much
+//    on bf16 instructions) and round of blocks over the CUs, with 3 steps of
+//    overhead a tile (2.8 narrow).  Small tiles of 32 x 32: 4 + 0.12 for each
+//    step (its latency) + 0.35e-3 for each tile and step, with 10 steps of
+//    overhead a tile.  Measured, us a call, small against large:
+//      bf16 out, 1 expert 4160 -> 2112: per 48 9.0 / 27.4, per 320 17.9 / 35.6;
+//      8 experts 1600 -> 6400: per 24 25.5 / 34.3, per 96 50.2 / 30.6; 1600 ->
+//      1600: per 48 14.3 / 15.5, per 96 18.3 / 16.7; 16 experts 768 -> 256: per
+//      160 8.4 / 10.4, per 320 13.1 / 11.1.  fp32 out, 8 experts 1600 -> 6400:
+//      per 48 40.0 / 47.3, per 160 77 / 46; 1600 -> 1600: per 160 24.8 / 26.8.
 //  SUMS: large tiles write dW in whole row segments: 8 experts 6400 x 1600,
 //    per 16: 220 / 74; few outputs of long reductions want more blocks: 8 experts
 //    256 x 256, per 1024: 9.2 / 20.9; 64 experts 256 x 256 (4096 small tiles),
 //    per 256: 20.1 / 15.4; 64 experts 128 x 128 (1024): 9.2 / 12.7.
 // 256 x 128 tiles where the rounds of blocks over the CUs come out cheaper, as
-// for the dense products (a narrow step takes 0.6 of a wide one; 3 and 2 steps
-// of overhead a tile).  8 experts 6400 -> 1600, per 64: 54.7 / 39.3 wide against
-// narrow; 1600 -> 6400, per 2048: 172 / 211.
+// for the dense products.  8 experts 6400 -> 1600, per 64: 54.7 / 39.3 wide
+// against narrow; 1600 -> 6400, per 2048: 172 / 211.
 struct TilePlan {
     bool tiles, narrow;
     int grid;
@@ -242,16 +292,23 @@ TilePlan plan(const ExpertArgs& g, bool sums, bool wide_codes) {
     const int per = (g.rows + g.experts - 1) / g.experts;
     const int cus = std::max(device_cu_count(), 1);
     TilePlan p{false, false, 0};
-    if (sums) p.tiles = (int64_t)g.experts * ((g.M + 31) / 32) * ((g.N + 31) / 32) > 8 * (int64_t)cus;
-    else p.tiles = per > (wide_codes ? 96 : 32) && g.N > 64;
-    if (!p.tiles) return p;
     const int64_t wn = (g.N + kPBN - 1) / kPBN, sn = (g.N + 127) / 128;
     // row tiles: ROWS end each expert with a partial one, half of one on average
-    const int64_t mt = sums ? (int64_t)g.experts * ((g.M + kPBM - 1) / kPBM)
-                            : g.rows / kPBM + (std::min(g.experts, g.rows) + 1) / 2;
+    const int64_t some = std::min(g.experts, g.rows);
+    auto row_tiles = [&](int tile) { return std::max(some, g.rows / tile + (some + 1) / 2); };
+    const int64_t mt = sums ? (int64_t)g.experts * ((g.M + kPBM - 1) / kPBM) : row_tiles(kPBM);
     const int64_t steps = ((sums ? per : g.K) + kPKB - 1) / kPKB + (sums ? 1 : 0);
     const int64_t wr = (mt * wn + cus - 1) / cus, sr = (mt * sn + cus - 1) / cus;
-    p.narrow = (double)sr * (0.6 * (double)steps + 2.0) < (double)wr * ((double)steps + 3.0);
+    const double wide = (double)wr * ((double)steps + 3.0), narrow = (double)sr * (0.6 * (double)steps + 2.0);
+    p.narrow = narrow < wide;
+    if (sums) {
+        p.tiles = (int64_t)g.experts * ((g.M + 31) / 32) * ((g.N + 31) / 32) > 8 * (int64_t)cus;
+    } else {
+        const double small = 4.0 + 0.12 * (double)steps +
+                             0.35e-3 * (double)(row_tiles(32) * ((g.N + 31) / 32)) * ((double)steps + 10.0);
+        p.tiles = 5.0 + (wide_codes ? 2.46 : 1.2) * std::min(wide, narrow) < small;
+    }
+    if (!p.tiles) return p;
     // at most this many units; blocks without one return at once
     const int64_t most = (sums ? mt : g.rows / kPBM + std::min(g.experts, g.rows)) * (p.narrow ? sn : wn);
     p.grid = (int)std::min<int64_t>(most, cus);
