@@ -329,3 +329,24 @@ def test_no_reduction(dev):
         assert (y[:400] == 0).all() and (y[400:] == 3).all()
         dw = df.experts_dw(z(2000, 16)[:, :0], z(2000, 16)[:, :0], off * 0, 0, s, s, out_dtype=dt)
         assert dw.shape == (2, 2000, 2000) and (dw == 0).all()
+
+
+# sides of the choice by estimated time, and row tiles counted through more
+# experts than a wave has lanes, most of them empty
+@pytest.mark.parametrize("counts,K,N", [
+    ([2000], 1024, 512), ([3000], 1024, 512), ([0] * 64 + [2200] + [0] * 60 + [40, 33] + [0] * 8, 160, 100),
+    ([0] * 130 + [2300], 160, 36), ([900, 3, 0, 2, 1], 300, 200), ([1, 2, 0, 3, 900], 300, 200), ([31, 33, 32, 1] * 20, 96, 40),
+], ids=lambda v: str(v)[:20])
+def test_exact_uneven(dev, counts, K, N):
+    check_exact(Case(dev, counts, K, N, seed=N, behind=5), dtypes=(torch.float32, torch.bfloat16))
+
+
+def test_no_reduction_many_columns(dev):
+    """K of no codes, on large tiles in the forward too."""
+    off = torch.tensor([0, 100, 400], dtype=torch.int32, device=dev)
+    s, sw = torch.ones(1, device=dev), torch.ones(2, device=dev)
+    z = lambda *shape: torch.zeros(*shape, dtype=torch.uint8, device=dev)
+    for dt in (torch.float32, torch.bfloat16):
+        y = torch.full((450, 12000), 3.0, dtype=dt, device=dev)
+        df.experts_fwd(z(450, 16)[:, :0], z(2, 12000, 16)[..., :0], off, 0, s, sw, out=y)
+        assert (y[:400] == 0).all() and (y[400:] == 3).all()
