@@ -954,10 +954,13 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
 def _experts_args(fn: str, offsets, scale, scales, experts: int, count: int, **codes):
     """Checks shared by the experts' products: devices, the offsets, the scales and the codes' layout."""
     torch = _torch()
-    at = offsets.get_device()
-    if not (at >= 0 and scale.get_device() == at and scales.get_device() == at
-            and all(t.get_device() == at for t in codes.values())):
-        _check_gpu(fn, offsets=offsets, scale=scale, scales=scales, **codes)
+    at, (a, b) = offsets.get_device(), codes.values()
+    if (at >= 0 and _plain(a, a.shape, torch.uint8, at) and _plain(b, b.shape, torch.uint8, at)
+            and _plain(offsets, (experts + 1,), torch.int32, at) and scale.numel() == 1
+            and _plain(scale, scale.shape, torch.float32, at) and scales.numel() == count
+            and _plain(scales, scales.shape, torch.float32, at)):
+        return
+    _check_gpu(fn, offsets=offsets, scale=scale, scales=scales, **codes)
     _row_vector(fn, "offsets", offsets, experts + 1, torch.int32)
     for name, t, n in (("scale", scale, 1), ("scales", scales, count)):
         if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
@@ -969,10 +972,10 @@ def _experts_args(fn: str, offsets, scale, scales, experts: int, count: int, **c
             raise ValueError(f"{fn}: the experts of {name} do not follow each other")
 
 
-def _experts_out(fn: str, out, shape, dtype, device):
-    torch = _torch()
+def _experts_out(fn: str, out, shape, dtype, like):
     if out is None:
-        return torch.empty(shape, dtype=dtype or torch.bfloat16, device=device), shape[-1]
+        return like.new_empty(shape, dtype=dtype or _torch().bfloat16), shape[-1]
+    device = like.device
     if tuple(out.shape) != tuple(shape) or (dtype is not None and out.dtype != dtype) or out.device != device:
         raise ValueError(f"{fn}: out is {tuple(out.shape)} {out.dtype} on {out.device}, not {tuple(shape)} on {device}")
     if out.dim() == 2:
@@ -990,7 +993,7 @@ def _experts_rows(fn: str, c_fn: str, a_q, w_q, offsets, red: int, sa, sw, out_d
     if a_q.shape[1] < red or w_q.shape[2] < red:
         raise ValueError(f"{fn}: rows of {a_q.shape[1]} and {w_q.shape[2]} codes, fewer than {red}")
     rows = a_q.shape[0]
-    out, ld = _experts_out(fn, out, (rows, cols), out_dtype, a_q.device)
+    out, ld = _experts_out(fn, out, (rows, cols), out_dtype, a_q)
     n, k = (cols, red) if c_fn == "df_fp8_experts_fwd" else (red, cols)
     with _on(a_q):
         call(c_fn, a_q.data_ptr(), a_q.stride(0), w_q.data_ptr(), w_q.stride(1), rows, n, k, experts,
@@ -1030,10 +1033,10 @@ def experts_dw(dyt_q, xt_q, offsets, rows: int, sdy, sx, out_dtype=None, out=Non
     N, K = dyt_q.shape[0], xt_q.shape[0]
     if out is None and out_dtype is None:
         out_dtype = torch.float32
-    out, _ = _experts_out(fn, out, (experts, N, K), out_dtype, dyt_q.device)
+    out, _ = _experts_out(fn, out, (experts, N, K), out_dtype, dyt_q)
     with _on(dyt_q):
-        call("df_fp8_experts_dw", _ptr(dyt_q), dyt_q.stride(0), _ptr(xt_q), xt_q.stride(0), rows, N, K, experts,
-             _ptr(offsets), _ptr(sdy), _ptr(sx), int(_in_dtype(out)), _ptr(out), K, _stream())
+        call("df_fp8_experts_dw", dyt_q.data_ptr(), dyt_q.stride(0), xt_q.data_ptr(), xt_q.stride(0), rows, N, K,
+             experts, offsets.data_ptr(), sdy.data_ptr(), sx.data_ptr(), _in_dtype(out), out.data_ptr(), K, _stream())
     return out
 
 
