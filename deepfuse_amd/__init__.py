@@ -951,15 +951,30 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
 # ----------------------------------------------------------------------------
 # products grouped by expert
 # ----------------------------------------------------------------------------
+def _codes_ld(fn: str, name: str, t) -> int:
+    """The leading dimension of codes, a matrix or one per expert.  The stride
+    of a dimension of one is arbitrary and says nothing."""
+    rows, ld = t.shape[-2], t.stride(-2)
+    if t.dim() == 3 and t.shape[0] > 1:
+        if rows == 1:
+            return t.stride(0)
+        if t.stride(0) != rows * ld:
+            raise ValueError(f"{fn}: the experts of {name} do not follow each other")
+    return t.shape[-1] if rows == 1 and (ld < t.shape[-1] or ld % 16) else ld
+
+
 def _experts_args(fn: str, offsets, scale, scales, experts: int, count: int, **codes):
-    """Checks shared by the experts' products: devices, the offsets, the scales and the codes' layout."""
+    """Checks shared by the experts' products: devices, the offsets, the scales
+    and the codes' layout; returns the codes' leading dimensions."""
     torch = _torch()
     at, (a, b) = offsets.get_device(), codes.values()
     if (at >= 0 and _plain(a, a.shape, torch.uint8, at) and _plain(b, b.shape, torch.uint8, at)
             and _plain(offsets, (experts + 1,), torch.int32, at) and scale.numel() == 1
             and _plain(scale, scale.shape, torch.float32, at) and scales.numel() == count
             and _plain(scales, scales.shape, torch.float32, at)):
-        return
+        lda, ldb = a.shape[-1], b.shape[-1]
+        if not (lda % 16 or ldb % 16):
+            return lda, ldb
     _check_gpu(fn, offsets=offsets, scale=scale, scales=scales, **codes)
     _row_vector(fn, "offsets", offsets, experts + 1, torch.int32)
     for name, t, n in (("scale", scale, 1), ("scales", scales, count)):
@@ -968,8 +983,7 @@ def _experts_args(fn: str, offsets, scale, scales, experts: int, count: int, **c
     for name, t in codes.items():
         if t.dtype != torch.uint8 or t.shape[-1] > 1 and t.stride(-1) != 1:
             raise ValueError(f"{fn}: {name} is not uint8 codes with contiguous rows")
-        if t.dim() == 3 and t.shape[0] > 1 and t.stride(0) != t.shape[1] * t.stride(1):
-            raise ValueError(f"{fn}: the experts of {name} do not follow each other")
+    return tuple(_codes_ld(fn, name, t) for name, t in codes.items())
 
 
 def _experts_out(fn: str, out, shape, dtype, like):
@@ -989,14 +1003,14 @@ def _experts_rows(fn: str, c_fn: str, a_q, w_q, offsets, red: int, sa, sw, out_d
     if a_q.dim() != 2 or w_q.dim() != 3:
         raise ValueError(f"{fn}: codes of {a_q.dim()} and {w_q.dim()} dimensions, not 2 and 3")
     experts, cols = w_q.shape[0], w_q.shape[1]
-    _experts_args(fn, offsets, sa, sw, experts, experts, rows=a_q, weights=w_q)
+    lda, ldw = _experts_args(fn, offsets, sa, sw, experts, experts, rows=a_q, weights=w_q)
     if a_q.shape[1] < red or w_q.shape[2] < red:
         raise ValueError(f"{fn}: rows of {a_q.shape[1]} and {w_q.shape[2]} codes, fewer than {red}")
     rows = a_q.shape[0]
     out, ld = _experts_out(fn, out, (rows, cols), out_dtype, a_q)
     n, k = (cols, red) if c_fn == "df_fp8_experts_fwd" else (red, cols)
     with _on(a_q):
-        call(c_fn, a_q.data_ptr(), a_q.stride(0), w_q.data_ptr(), w_q.stride(1), rows, n, k, experts,
+        call(c_fn, a_q.data_ptr(), lda, w_q.data_ptr(), ldw, rows, n, k, experts,
              offsets.data_ptr(), sa.data_ptr(), sw.data_ptr(), _in_dtype(out), out.data_ptr(), ld, _stream())
     return out
 
@@ -1027,7 +1041,7 @@ def experts_dw(dyt_q, xt_q, offsets, rows: int, sdy, sx, out_dtype=None, out=Non
     if offsets.dim() != 1 or offsets.numel() < 1:
         raise ValueError(f"{fn}: offsets {tuple(offsets.shape)} are not experts + 1 values")
     experts = offsets.numel() - 1
-    _experts_args(fn, offsets, sdy, sx, experts, 1, dyt_q=dyt_q, xt_q=xt_q)
+    lddy, ldx = _experts_args(fn, offsets, sdy, sx, experts, 1, dyt_q=dyt_q, xt_q=xt_q)
     if dyt_q.shape[1] < rows or xt_q.shape[1] < rows:
         raise ValueError(f"{fn}: rows of {dyt_q.shape[1]} and {xt_q.shape[1]} codes, fewer than {rows}")
     N, K = dyt_q.shape[0], xt_q.shape[0]
@@ -1035,8 +1049,7 @@ def experts_dw(dyt_q, xt_q, offsets, rows: int, sdy, sx, out_dtype=None, out=Non
         out_dtype = torch.float32
     out, _ = _experts_out(fn, out, (experts, N, K), out_dtype, dyt_q)
     with _on(dyt_q):
-        call("df_fp8_experts_dw", dyt_q.data_ptr(), dyt_q.stride(0), xt_q.data_ptr(), xt_q.stride(0), rows, N, K,
-             experts, offsets.data_ptr(), sdy.data_ptr(), sx.data_ptr(), _in_dtype(out), out.data_ptr(), K, _stream())
+        call("df_fp8_experts_dw", dyt_q.data_ptr(), lddy, xt_q.data_ptr(), ldx, rows, N, K, experts, offsets.data_ptr(), sdy.data_ptr(), sx.data_ptr(), _in_dtype(out), out.data_ptr(), K, _stream())
     return out
 
 
