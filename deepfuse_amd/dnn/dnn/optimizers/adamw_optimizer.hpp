@@ -7,8 +7,10 @@
 // bias gradients; one df_adamw_update call updates the whole list.
 //
 // state_bits 32: the moments in binary32; 8: as e4m3 codes with a scale per 256
-// values (a quarter of the memory; see include/df_capi.h).  Moments of a
-// parameter start at zero when update_parameters first lists it.
+// values (a quarter of the memory; see include/df_capi.h).  A parameter is known
+// by its tensor's address, its moments start at zero when update_parameters
+// first lists it, or lists it with another size; step() refuses one whose size
+// changed after that (tensor::load gives a tensor another shape and buffer).
 // set_weight_decay(param, wd) gives one parameter a decay of its own (0 for
 // biases and norms, usually).  step_clipped(max_norm) is step() on gradients
 // clipped to that global norm, which keep their values.
@@ -45,6 +47,7 @@ private:
         std::unique_ptr<tensor<T>> m, v;                // 32 bits
         std::unique_ptr<tensor<uint8_t>> mq, vq;        // 8 bits: codes
         std::unique_ptr<tensor<float>> m_scale, v_scale;
+        int64_t size() const { return m ? m->size() : mq->size(); }
     };
     void launch(const float* clip_norm, float max_norm);
 

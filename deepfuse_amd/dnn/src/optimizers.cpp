@@ -179,7 +179,8 @@ void AdamWOptimizer<float>::update_parameters(const std::vector<tensor<float>*>&
                                               const std::vector<tensor<float>*>& gradients) {
     Optimizer<float>::update_parameters(parameters, gradients);
     for (auto* param : parameters) {
-        if (state_.find(param) != state_.end()) continue;
+        const auto it = state_.find(param);
+        if (it != state_.end() && it->second.size() == param->size()) continue;
         State s;
         if (state_bits_ == 32) {
             s.m = std::make_unique<tensor<float>>(param->shape());
@@ -197,7 +198,7 @@ void AdamWOptimizer<float>::update_parameters(const std::vector<tensor<float>*>&
             s.m_scale->fill(1.0f);
             s.v_scale->fill(1.0f);
         }
-        state_.emplace(param, std::move(s));
+        state_.insert_or_assign(param, std::move(s));
     }
 }
 
@@ -226,6 +227,9 @@ void AdamWOptimizer<float>::launch(const float* clip_norm, float max_norm) {
             if (params[k] == params[i])
                 throw std::invalid_argument("AdamWOptimizer::step: parameter " + std::to_string(i) + " is listed twice");
         State& s = state_.at(params[i]);
+        if (s.size() != params[i]->size())
+            throw std::invalid_argument("AdamWOptimizer::step: parameter " + std::to_string(i) +
+                                        " changed its size since update_parameters listed it");
         p[i] = params[i]->data();
         g[i] = grads[i]->data();
         m[i] = s.m ? static_cast<void*>(s.m->data()) : s.mq->data();

@@ -1537,6 +1537,41 @@ TEST_F(AdamWOptimizerTest, Refusals) {
     EXPECT_EQ(opt.timestep(), 0);
 }
 
+// A listed tensor that takes another size under its address: step() refuses it
+// until update_parameters lists it again, with moments of the new size at zero.
+TEST_F(AdamWOptimizerTest, ListedTensorTakesAnotherSize) {
+    for (const int bits : {32, 8}) {
+        for (const int n : {5000, 40}) {
+            tensor<float> p({300}), g({300}), q({n}), h({n});
+            p.fill(1.0f);
+            g.fill(0.5f);
+            AdamWOptimizer<float> opt(0.01f, 0.9f, 0.999f, 1e-8f, 0.01f, bits), fresh(0.01f, 0.9f, 0.999f, 1e-8f, 0.01f, bits);
+            opt.update_parameters({&p}, {&g});
+            const auto pv = uniform(n, -1.0f, 1.0f, 431), gv = uniform(n, -0.1f, 0.1f, 432);
+            for (auto* t : {&p, &q}) {
+                *t = tensor<float>({n});
+                t->upload(pv.data());
+            }
+            for (auto* t : {&g, &h}) {
+                *t = tensor<float>({n});
+                t->upload(gv.data());
+            }
+            EXPECT_THROW(opt.step(), std::invalid_argument);
+            EXPECT_THROW(opt.step_clipped(1.0f), std::invalid_argument);
+            EXPECT_TRUE(download(p) == pv);
+            EXPECT_EQ(opt.timestep(), 0);
+            opt.update_parameters({&p}, {&g});
+            fresh.update_parameters({&q}, {&h});
+            for (int t = 0; t < 2; ++t) {
+                opt.step();
+                fresh.step();
+                opt.update_parameters({&p}, {&g});  // the same size: the moments stay
+            }
+            EXPECT_TRUE(download(p) == download(q));
+        }
+    }
+}
+
 // step_clipped(max_norm) == clip_grad_norm(grads, max_norm) + step(), except
 // that the gradients keep their values.
 TEST_F(AdamOptimizerTest, StepClippedEqualsClipThenStep) {
