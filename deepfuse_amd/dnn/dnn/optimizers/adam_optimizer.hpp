@@ -8,6 +8,10 @@
 // weight and bias gradients; one df_adam_update_f32 call updates the whole
 // list (the reference launches one kernel per tensor).
 //
+// A parameter is known by its tensor's address.  Where update_parameters lists
+// it with another size than before, its moments start at zero again; step()
+// refuses one whose size changed after that.
+//
 // Addition: step_clipped(max_norm) is utils::clip_grad_norm(gradients(),
 // max_norm) followed by step(), with the clip factor applied inside the
 // update instead of rewriting the gradients (they keep their unclipped

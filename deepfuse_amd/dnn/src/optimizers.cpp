@@ -108,13 +108,14 @@ void AdamOptimizer<float>::update_parameters(const std::vector<tensor<float>*>& 
                                              const std::vector<tensor<float>*>& gradients) {
     Optimizer<float>::update_parameters(parameters, gradients);
     for (auto* param : parameters) {
-        if (m_.find(param) == m_.end()) {
+        const auto it = m_.find(param);
+        if (it == m_.end() || it->second->size() != param->size()) {
             auto m_buf = std::make_unique<tensor<float>>(param->shape());
             auto v_buf = std::make_unique<tensor<float>>(param->shape());
             m_buf->fill(0.0f);
             v_buf->fill(0.0f);
-            m_.emplace(param, std::move(m_buf));
-            v_.emplace(param, std::move(v_buf));
+            m_.insert_or_assign(param, std::move(m_buf));
+            v_.insert_or_assign(param, std::move(v_buf));
         }
     }
 }
@@ -138,6 +139,9 @@ void AdamOptimizer<float>::launch(const float* clip_norm, float max_norm) {
         if (grads[i]->size() != params[i]->size())
             throw std::invalid_argument("AdamOptimizer::step: gradient " + std::to_string(i) +
                                         " differs in size from its parameter");
+        if (m_.at(params[i])->size() != params[i]->size())
+            throw std::invalid_argument("AdamOptimizer::step: parameter " + std::to_string(i) +
+                                        " changed its size since update_parameters listed it");
         p[i] = params[i]->data();
         g[i] = grads[i]->data();
         m[i] = m_.at(params[i])->data();

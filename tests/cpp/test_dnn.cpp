@@ -1572,6 +1572,36 @@ TEST_F(AdamWOptimizerTest, ListedTensorTakesAnotherSize) {
     }
 }
 
+// As AdamWOptimizerTest.ListedTensorTakesAnotherSize.
+TEST_F(AdamOptimizerTest, ListedTensorTakesAnotherSize) {
+    for (const int n : {5000, 40}) {
+        tensor<float> p({300}), g({300}), q({n}), h({n});
+        p.fill(1.0f);
+        g.fill(0.5f);
+        AdamOptimizer<float> opt(0.01f), fresh(0.01f);
+        opt.update_parameters({&p}, {&g});
+        const auto pv = uniform(n, -1.0f, 1.0f, 441), gv = uniform(n, -0.1f, 0.1f, 442);
+        for (auto* t : {&p, &q}) {
+            *t = tensor<float>({n});
+            t->upload(pv.data());
+        }
+        for (auto* t : {&g, &h}) {
+            *t = tensor<float>({n});
+            t->upload(gv.data());
+        }
+        EXPECT_THROW(opt.step(), std::invalid_argument);
+        EXPECT_TRUE(download(p) == pv);
+        opt.update_parameters({&p}, {&g});
+        fresh.update_parameters({&q}, {&h});
+        EXPECT_EQ(opt.first_moment(&p).size(), n);
+        EXPECT_EQ(opt.second_moment(&p).size(), n);
+        opt.step();
+        fresh.step();
+        opt.update_parameters({&p}, {&g});  // the same size: the moments stay
+        EXPECT_TRUE(download(opt.first_moment(&p)) == download(fresh.first_moment(&q)));
+    }
+}
+
 // step_clipped(max_norm) == clip_grad_norm(grads, max_norm) + step(), except
 // that the gradients keep their values.
 TEST_F(AdamOptimizerTest, StepClippedEqualsClipThenStep) {
