@@ -889,9 +889,10 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
     all.  ``weight_decay`` is one number or one per tensor; ``timestep`` an int
     or an int32 device tensor and ``lr`` a number or an fp32 device tensor,
     read when the kernel runs (a captured step follows them on replay).
-    ``clip_norm`` (a device norm from :func:`grad_norm`) applies max_norm /
-    norm to the gradients; ``absmax`` (fp32 of len(params)) receives max |p|
-    of each updated tensor."""
+    ``clip_norm`` (a device norm from :func:`grad_norm`, a tensor) applies
+    max_norm / norm to the gradients where the norm is larger than max_norm,
+    which then has to be above 0; ``absmax`` (fp32 of len(params)) receives
+    max |p| of each updated tensor."""
     fn, torch = "adamw_update", _torch()
     n = len(params)
     if n == 0:
@@ -938,6 +939,11 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
             if x.numel() != 1 or x.dtype != dt or x.device != params[0].device:
                 raise ValueError(f"{fn}: {name} is not one {dt} on {params[0].device}")
             scalars[name] = x.data_ptr()
+    if clip_norm is not None:
+        if "clip_norm" not in scalars:
+            raise TypeError(f"{fn}: clip_norm is a device norm (a tensor), not {type(clip_norm).__name__}")
+        if not max_norm > 0:
+            raise ValueError(f"{fn}: max_norm = {max_norm} with a clip_norm (a limit above 0)")
     if absmax is not None and (absmax.dtype != torch.float32 or absmax.numel() < n or not absmax.is_contiguous()
                                or absmax.device != params[0].device):
         raise ValueError(f"{fn}: absmax is not {n} contiguous fp32 values on {params[0].device}")

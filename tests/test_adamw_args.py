@@ -86,3 +86,14 @@ def test_python_refusals():
     df.adamw_update([], [], [], [], 1)
     with pytest.raises(TypeError, match="not clipped"):
         df.grad_norm([torch.zeros(4, dtype=torch.bfloat16)], clip=1.0)
+
+
+def test_clip_needs_a_device_norm_and_a_limit():
+    """A number in the norm's place would clip nothing, a norm without a limit would zero every gradient."""
+    ok = lambda: [fake(4)]
+    for norm in (50.0, 1, torch.nn.Identity(), [fake(1)]):
+        with pytest.raises(TypeError, match="clip_norm"):
+            df.adamw_update(ok(), ok(), ok(), ok(), 1, clip_norm=norm, max_norm=1.0)
+    for kw in (dict(), dict(max_norm=0.0), dict(max_norm=-1.0), dict(max_norm=float("nan"))):
+        with pytest.raises(ValueError, match="max_norm"):
+            df.adamw_update(ok(), ok(), ok(), ok(), 1, clip_norm=fake(1), **kw)
