@@ -123,13 +123,18 @@ __global__ __launch_bounds__(kOThreads) void sumsq_kernel(const NormList L, doub
     if (threadIdx.x == 0) partial[part0 + b] = acc;
 }
 
-// The same for 2-byte gradients (their squares are exact in binary32), eight
-// values per 16-byte load; any element alignment.
+// The same for 2-byte gradients, eight values per 16-byte load; any element
+// alignment.  They are squared in binary64, exactly: bf16 has binary32's range,
+// so a square in binary32 overflows above 2^64 and loses bits below 2^-63.
 typedef u32x4 u32x4_el __attribute__((aligned(2)));
 template <typename T> static __device__ __forceinline__ float widen16(uint32_t h);
 template <> __device__ __forceinline__ float widen16<uint16_t>(uint32_t h) { return bf16_to_f32(h); }
 template <> __device__ __forceinline__ float widen16<f16_t>(uint32_t h) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+template <typename T> static __device__ __forceinline__ double sq16(uint32_t h) {
+    const double x = (double)widen16<T>(h);
+    return x * x;
 }
 template <typename T>
 __global__ __launch_bounds__(kOThreads) void sumsq16_kernel(const NormList L, double* __restrict__ partial,
@@ -150,9 +155,9 @@ __global__ __launch_bounds__(kOThreads) void sumsq16_kernel(const NormList L, do
 #pragma unroll
             for (int k = 0; k < kLoads; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc += sq(widen16<T>(r[k][i] & 0xFFFFu)) + sq(widen16<T>(r[k][i] >> 16));
+                for (int i = 0; i < 4; ++i) acc += sq16<T>(r[k][i] & 0xFFFFu) + sq16<T>(r[k][i] >> 16);
         } else {
-            for (int64_t i = base + threadIdx.x; i < n; i += kOThreads) acc += sq(widen16<T>(x[i]));
+            for (int64_t i = base + threadIdx.x; i < n; i += kOThreads) acc += sq16<T>(x[i]);
             break;
         }
     }

@@ -613,8 +613,8 @@ int df_adam_update_absmax_f32(float* const* params, const float* const* grads, f
                               float* absmax_dev, void* stream);
 
 /* df_grad_norm_f32 over gradients of one dtype (fp32, bf16, f16; 2-byte ones
- * at any element alignment), for df_adamw_update's clip_norm_dev; the same
- * workspace.  No reference counterpart for the 2-byte types. */
+ * at any element alignment, squared exactly), for df_adamw_update's
+ * clip_norm_dev; the same workspace.  No reference counterpart for the 2-byte types. */
 int df_grad_norm(int dtype, const void* const* grads, const int64_t* sizes, int count,
                  float* norm_dev, void* ws, size_t ws_bytes, void* stream);
 
