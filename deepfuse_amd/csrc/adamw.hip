@@ -82,10 +82,11 @@ __host__ __device__ inline float bias_corr(float beta, int t) {
     return 1.0f - (float)r;
 }
 
-// 16, 8 or 4 bytes at element alignment
-typedef f32x4 f32x4_el __attribute__((aligned(4)));
-typedef u32x2 u32x2_el __attribute__((aligned(2)));
-typedef uint32_t u32_el __attribute__((aligned(1)));
+// 16, 8 or 4 bytes at element alignment (in structs: a template argument loses
+// a type's alignment)
+struct F4 { typedef f32x4 V __attribute__((aligned(4))); };
+struct H4 { typedef u32x2 V __attribute__((aligned(2))); };
+struct B4 { typedef uint32_t V __attribute__((aligned(1))); };
 
 // Lists larger than the 256 MB Infinity Cache stream past it: two GPT-2 XL
 // blocks (61.5M values, 8-bit states, 1 GB moved) 194 us against 205 with
@@ -93,13 +94,15 @@ typedef uint32_t u32_el __attribute__((aligned(1)));
 // next: one GPT-2 small block (7M values, 32-bit states) 30.6 us plain, 34.7
 // past the cache.
 constexpr int64_t kColdBytes = (int64_t)256 << 20;
-template <bool NT, typename V> __device__ __forceinline__ auto ldv(const V* p) {
-    if constexpr (NT) return __builtin_nontemporal_load(p);
-    else return *p;
+template <bool NT, typename A> __device__ __forceinline__ auto ldv(const void* p) {
+    const typename A::V* const q = static_cast<const typename A::V*>(p);
+    if constexpr (NT) return __builtin_nontemporal_load(q);
+    else return *q;
 }
-template <bool NT, typename V, typename X> __device__ __forceinline__ void stv(V* p, X v) {
-    if constexpr (NT) __builtin_nontemporal_store((V)v, p);
-    else *p = v;
+template <bool NT, typename A, typename X> __device__ __forceinline__ void stv(void* p, X v) {
+    typename A::V* const q = static_cast<typename A::V*>(p);
+    if constexpr (NT) __builtin_nontemporal_store(v, q);
+    else *q = v;
 }
 
 // maximum over the wave (VALU only): rows of 16 lanes, then across them
@@ -126,7 +129,7 @@ template <> __device__ __forceinline__ float grad_one<f16_t>(const f16_t* p) {
 template <typename G> struct Grad4 {
     u32x2 w;
     template <bool NT> __device__ __forceinline__ void load(const G* p) {
-        w = ldv<NT>(reinterpret_cast<const u32x2_el*>(p));
+        w = ldv<NT, H4>(p);
     }
     __device__ __forceinline__ void widen(float* g) const {
         if constexpr (std::is_same<G, uint16_t>::value) {
@@ -143,7 +146,7 @@ template <typename G> struct Grad4 {
 template <> struct Grad4<float> {
     f32x4 w;
     template <bool NT> __device__ __forceinline__ void load(const float* p) {
-        w = ldv<NT>(reinterpret_cast<const f32x4_el*>(p));
+        w = ldv<NT, F4>(p);
     }
     __device__ __forceinline__ void widen(float* g) const {
 #pragma unroll
@@ -318,15 +321,15 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
                 for (int u = 0; u < kUnits; ++u) {
                     const int64_t i = u0 + u * stride + lane * 4;
                     rg[u].template load<NT>(gp + i);
-                    rp[u] = ldv<NT>(reinterpret_cast<const f32x4_el*>(t.p + i));
+                    rp[u] = ldv<NT, F4>(t.p + i);
                     if constexpr (S8) {
-                        cm[u] = ldv<NT>(reinterpret_cast<const u32_el*>(static_cast<const uint8_t*>(t.m) + i));
-                        cv[u] = ldv<NT>(reinterpret_cast<const u32_el*>(static_cast<const uint8_t*>(t.v) + i));
+                        cm[u] = ldv<NT, B4>(static_cast<const uint8_t*>(t.m) + i);
+                        cv[u] = ldv<NT, B4>(static_cast<const uint8_t*>(t.v) + i);
                         sm[u] = t.ms[(u0 + u * stride) >> 8];
                         sv[u] = t.vs[(u0 + u * stride) >> 8];
                     } else {
-                        rm[u] = ldv<NT>(reinterpret_cast<const f32x4_el*>(static_cast<const float*>(t.m) + i));
-                        rv[u] = ldv<NT>(reinterpret_cast<const f32x4_el*>(static_cast<const float*>(t.v) + i));
+                        rm[u] = ldv<NT, F4>(static_cast<const float*>(t.m) + i);
+                        rv[u] = ldv<NT, F4>(static_cast<const float*>(t.v) + i);
                     }
                 }
 #pragma unroll
@@ -352,24 +355,24 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
                     const bool plain = moments(g, m, v);
                     if (plain) update(std::true_type{}, p, m, v, root);
                     else update(std::false_type{}, p, m, v, root);
-                    stv<NT>(reinterpret_cast<f32x4_el*>(t.p + i), f32x4{p[0], p[1], p[2], p[3]});
+                    stv<NT, F4>(t.p + i, f32x4{p[0], p[1], p[2], p[3]});
                     if constexpr (COPY >= 0)
-                        stv<NT>(reinterpret_cast<u32x2_el*>(t.copy + i),
+                        stv<NT, H4>(t.copy + i,
                                 u32x2{copy_bits<COPY>(p[0]) | (copy_bits<COPY>(p[1]) << 16),
                                       copy_bits<COPY>(p[2]) | (copy_bits<COPY>(p[3]) << 16)});
                     if constexpr (S8) {
                         float s0, s1;
                         const uint32_t c0 = encode(m, std::false_type{}, plain, s0);
                         const uint32_t c1 = encode(root, std::true_type{}, plain, s1);
-                        stv<NT>(reinterpret_cast<u32_el*>(static_cast<uint8_t*>(t.m) + i), c0);
-                        stv<NT>(reinterpret_cast<u32_el*>(static_cast<uint8_t*>(t.v) + i), c1);
+                        stv<NT, B4>(static_cast<uint8_t*>(t.m) + i, c0);
+                        stv<NT, B4>(static_cast<uint8_t*>(t.v) + i, c1);
                         if (lane == 0) {
                             t.ms[(u0 + u * stride) >> 8] = s0;
                             t.vs[(u0 + u * stride) >> 8] = s1;
                         }
                     } else {
-                        stv<NT>(reinterpret_cast<f32x4_el*>(static_cast<float*>(t.m) + i), f32x4{m[0], m[1], m[2], m[3]});
-                        stv<NT>(reinterpret_cast<f32x4_el*>(static_cast<float*>(t.v) + i), f32x4{v[0], v[1], v[2], v[3]});
+                        stv<NT, F4>(static_cast<float*>(t.m) + i, f32x4{m[0], m[1], m[2], m[3]});
+                        stv<NT, F4>(static_cast<float*>(t.v) + i, f32x4{v[0], v[1], v[2], v[3]});
                     }
                 }
                 continue;

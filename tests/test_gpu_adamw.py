@@ -350,3 +350,29 @@ def test_lists_larger_than_the_cache(dev, bits, gdt, copy):
             assert copy is None or (C[3] == P[3][0].to(copy)).all()
     for a, b in zip(*runs):
         assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("gdt,copy", [(torch.float32, None), (torch.bfloat16, torch.float16)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_views_past_the_cache(dev, bits, gdt, copy):
+    """A list past 256 MB of which one tensor, its gradient, states and copy lie at odd elements: equal to plain ones."""
+    n, big = 8192 * 2 + 1300, 40_000_000
+    p, g = make([n], 13, gdt)
+    at = lambda t, k: torch.cat([t.view(torch.uint8).new_zeros(k * t.element_size()), t.view(torch.uint8).reshape(-1),
+                                 t.view(torch.uint8).new_zeros(16)])[k * t.element_size():][:t.numel() * t.element_size()].view(t.dtype)
+    runs = []
+    for k in (0, 1, 3):
+        P, G = [at(t, k) for t in dev_list(p, dev)], [at(t.to(dev), k) for t in g]
+        st = [None if x is None else [at(x[0], k)] for x in df.adamw_state(P, bits)]
+        C = None if copy is None else [at(torch.zeros(n, dtype=copy, device=dev), k)]
+        assert P[0].data_ptr() % 16 == 4 * k % 16 and st[0][0].data_ptr() % 16 == (k if bits == 8 else 4 * k) % 16
+        fill = torch.ones(big, device=dev)
+        more = df.adamw_state([fill], bits)
+        args = [P + [fill], G + [torch.zeros(big, dtype=gdt, device=dev)]]
+        M, V, MS, VS = (None if x is None else x + y for x, y in zip(st, more))
+        copies = None if C is None else C + [torch.zeros(big, dtype=copy, device=dev)]
+        for t in (1, 2):
+            df.adamw_update(*args, M, V, t, weight_decay=0.1, m_scales=MS, v_scales=VS, copies=copies, **HYPER)
+        runs.append([x[0].clone() for x in (P, M, V, MS, VS, copies) if x is not None])
+    for other in runs[1:]:
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(runs[0], other))
