@@ -55,6 +55,7 @@ class DFError(RuntimeError):
 
 
 _c_int, _c_i64, _c_sz, _c_f = ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
+_c_u32 = ctypes.c_uint32
 _vp = ctypes.c_void_p
 
 # name -> (restype, argtypes); every function declared in df_capi.h
@@ -168,6 +169,8 @@ _SIGS = {
     "df_adamw_scale_count": (_c_i64, [_c_i64]),
     "df_adamw_update": (_c_int, [_c_int, _vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _c_f, _c_f,
                                  _c_f, _c_f, _vp, _c_int, _vp, _vp, _vp, _c_f, _vp, _vp]),
+    "df_adamw_update_dithered": (_c_int, [_c_int, _vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _c_f,
+                                          _c_f, _c_f, _c_f, _vp, _c_int, _vp, _vp, _vp, _c_f, _vp, _c_u32, _vp]),
 }
 
 _lib = None
@@ -868,7 +871,7 @@ def _grad_norm16(grads, clip):
 def adamw_state(params, bits: int = 32):
     """(ms, vs, m_scales, v_scales) for :func:`adamw_update` before the first
     step: fp32 zeros and no scales (None), or with ``bits=8`` e4m3 zeros and
-    an fp32 scale per 256 values."""
+    an fp32 scale per 256 values (to be updated with ``dither``: see there)."""
     torch = _torch()
     if bits == 32:
         return [torch.zeros_like(p) for p in params], [torch.zeros_like(p) for p in params], None, None
@@ -881,7 +884,7 @@ def adamw_state(params, bits: int = 32):
 
 
 def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
-                 m_scales=None, v_scales=None, copies=None, clip_norm=None, max_norm=0.0, absmax=None):
+                 m_scales=None, v_scales=None, copies=None, clip_norm=None, max_norm=0.0, absmax=None, dither=None):
     """One AdamW step (df_adamw_update) over contiguous fp32 parameters, in
     place on params, the states (fp32, or float8_e4m3fn with m_scales and
     v_scales: see :func:`adamw_state`) and ``copies`` (bf16 or float16, the
@@ -892,7 +895,15 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
     ``clip_norm`` (a device norm from :func:`grad_norm`, a tensor) applies
     max_norm / norm to the gradients where the norm is larger than max_norm,
     which then has to be above 0; ``absmax`` (fp32 of len(params)) receives
-    max |p| of each updated tensor."""
+    max |p| of each updated tensor.
+
+    ``dither`` (an int, the seed of the draws; it may stay the same, the step
+    count is drawn on too) rounds 8-bit states up or down at random in proportion
+    (df_adamw_update_dithered).  Without it they are rounded to nearest: exact
+    for one step, but a root of v moves by at most (1 - beta2) / 2 a step, its
+    codes lie 6 to 12% apart, and one that falls goes back to its code: after
+    gradients have become smaller it stays too large (up to ten times after a
+    tenfold fall), and the steps too small.  A training run gives ``dither``."""
     fn, torch = "adamw_update", _torch()
     n = len(params)
     if n == 0:
@@ -900,6 +911,8 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
     eight = m_scales is not None
     if eight != (v_scales is not None):
         raise ValueError(f"{fn}: m_scales and v_scales go together")
+    if dither is not None and not eight:
+        raise ValueError(f"{fn}: dither without 8-bit states")
     if not params[0].is_cuda:
         raise ValueError(f"{fn}: the parameters are on {params[0].device}, not on a GPU")
     gt = _in_dtype(grads[0]) if grads else DType.FLOAT32
@@ -948,10 +961,14 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
                                or absmax.device != params[0].device):
         raise ValueError(f"{fn}: absmax is not {n} contiguous fp32 values on {params[0].device}")
     with _on(params[0]):
-        call("df_adamw_update", n, (_c_i64 * n)(*sizes), p, gt, g, DType.FP8E4M3 if eight else DType.FLOAT32, m, v, sm,
-             sv, ct, c, 0.0 if "lr" in scalars else float(lr), float(beta1), float(beta2), float(eps), wd,
-             0 if "timestep" in scalars else int(timestep), scalars.get("lr"), scalars.get("timestep"),
-             scalars.get("clip_norm"), float(max_norm), _ptr(absmax), _stream())
+        args = (n, (_c_i64 * n)(*sizes), p, gt, g, DType.FP8E4M3 if eight else DType.FLOAT32, m, v, sm,
+                sv, ct, c, 0.0 if "lr" in scalars else float(lr), float(beta1), float(beta2), float(eps), wd,
+                0 if "timestep" in scalars else int(timestep), scalars.get("lr"), scalars.get("timestep"),
+                scalars.get("clip_norm"), float(max_norm), _ptr(absmax))
+        if dither is None:
+            call("df_adamw_update", *args, _stream())
+        else:
+            call("df_adamw_update_dithered", *args, int(dither) & 0xFFFFFFFF, _stream())
 
 
 # ----------------------------------------------------------------------------

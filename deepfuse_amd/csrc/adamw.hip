@@ -12,9 +12,24 @@
 // finite values; v as codes of sqrt(v), which the update needs anyway: e4m3
 // spans 2^-9 to 448, so the square root covers 2^35 of v in one block.  A v
 // above 0 never goes to code 0: the next step would divide its m by eps alone.
-// The update itself uses the binary32 m and v; only what is kept is rounded
-// (to 4 significant bits: off by at most 2^-4 of the value, or 2^-10 of the
-// scale).
+// The update itself uses the binary32 m and v; only what is kept is rounded, to
+// 4 significant bits.
+//
+// To nearest, what one step keeps is off by at most 2^-4 of the value (or 2^-10
+// of the scale), but the next step starts from there.  A step lowers a root by
+// at most (1 - b2)/2 of itself, 2.5% at b2 = 0.95 and 0.05% at 0.999, and codes
+// lie 6 to 12% apart: rounded to nearest, a falling root goes back to its code
+// until the scale moves.  Half a block's gradients falling tenfold leave its
+// roots up to ten times too large, for good where the gradients are steady.
+// Dithered rounding (df_adamw_update_dithered) takes the upper of two codes with
+// the probability of the value's place between them, so that a root moves as
+// often as it should.  Its noise: a move of a share d of a code gap w is made with
+// probability d, variance d w^2 at most, and dies away by b2 a step; with d w <= 2
+// (1 - b2)/2 of the root (its own move and the scale's) and w <= 1/8 of it that is
+// a variance of (1 - b2)/8 a step over 1 - b2^2, or 1 / (8 (1 + b2)): a standard
+// deviation of a quarter of the root at most, however near b2 is to 1 (measured:
+// 0.12 to 0.17, a third in the middle of a tenfold fall).  Two GPT-2 XL blocks (61.5M
+// values) 214 us dithered, 194 to nearest.
 //
 // Bound by HBM: 24 bytes and the gradient per element with binary32 states,
 // 12.1 and the gradient with 8-bit ones.  A wave takes 256 values at a time,
@@ -65,6 +80,8 @@ struct WList {
 struct WHyper {
     float lr, b1, b2, omb1, omb2, eps, max_norm;
     float bc1, bc2;         // 1 - beta^t, unless step is given
+    int t;                  // likewise, and
+    uint32_t seed;          // for the dither
     const float* lr_dev;
     const int* step;
     const float* norm;
@@ -166,6 +183,32 @@ __device__ __forceinline__ float block_scale(uint32_t am) {
     return am ? __builtin_fmaxf(a / 448.0f, 0x1p-126f) : 1.0f;
 }
 
+// ---- dithered rounding ----
+// 32 bits from 32: xor-shifts and odd multipliers in turn (the first digits of
+// the square roots of 2 and 3).
+__device__ __forceinline__ uint32_t mix(uint32_t x) {
+    x ^= x >> 16;
+    x *= 0x6A09E667u;
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+// the draw of value i under a key of its own for each seed, step and tensor
+__device__ __forceinline__ uint32_t draw(uint32_t key, int64_t i) {
+    return mix(key + (uint32_t)i * 0x9E3779B9u + (uint32_t)(i >> 32) * 0xBB67AE85u);
+}
+
+// y to one of the e4m3 values next to it by 16 random bits r, at most 448: r is
+// added below the 3 bits of mantissa that stay, and the others are cut.  Below
+// 2^-6 e4m3 is even, in steps of 2^-9, as from 2^-6 to 2^-5: such a value goes
+// there and back.  r stands for the middle of its interval, so that a value of
+// e4m3 stays.
+__device__ __forceinline__ float dither_e4m3(float y, uint32_t r) {
+    const float a = __builtin_fabsf(y), up = a < 0x1p-6f ? 0x1p-6f : 0.0f;
+    const float n = __uint_as_float((__float_as_uint(a + up) + (r << 4) + 8u) & 0xFFF00000u) - up;
+    return __builtin_copysignf(__builtin_fminf(n, 448.0f), y);
+}
+
 template <int COPY> __device__ __forceinline__ uint32_t copy_bits(float v) {
     return COPY == DF_DTYPE_HALF ? f32_to_f16_rne(v) : f32_to_bf16_rne(v);
 }
@@ -206,7 +249,8 @@ __device__ __forceinline__ float root_normal(float x) {  // x: 0 or in [2^-62, 2
 
 // COPY: DF_DTYPE_BFLOAT16 or DF_DTYPE_HALF: the updated parameters are also
 // written in that type; -1: not.  NT: the list is larger than the cache.
-template <typename G, bool S8, int COPY, bool NT>
+// DITHER: 8-bit states are rounded by dither.
+template <typename G, bool S8, int COPY, bool NT, bool DITHER>
 __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const WHyper h) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int lo = 0, hi = L.count - 1;  // the tensor that owns this block: the last with first <= blockIdx.x
@@ -229,6 +273,9 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
     }
     const float keep = 1.0f - lr * L.wd[lo];
     uint32_t am = 0;
+    uint32_t key = 0;
+    if constexpr (DITHER)
+        key = mix(mix(mix(h.seed) + (uint32_t)(h.step ? max(h.step[0], 1) : h.t)) + (uint32_t)L.idx[lo]);
 
     const ByShared by1{bc1, 1.0f / bc1}, by2{bc2, 1.0f / bc2};
     const float lr64 = lr * 0x1p-64f;
@@ -273,7 +320,8 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
         }
     };
     // codes and scale of a unit's values; ROOT: roots, which above 0 go to code 1 at least
-    auto encode = [&](const float* x, auto root, bool plain, float& s) __attribute__((always_inline)) -> uint32_t {
+    auto encode = [&](const float* x, auto root, bool plain, float& s, const uint32_t* rnd)
+                      __attribute__((always_inline)) -> uint32_t {
         constexpr bool ROOT = decltype(root)::value;
         uint32_t a = 0;
         if (plain) {  // no NaN or infinity among them
@@ -285,6 +333,21 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
         }
         s = block_scale(wave_umax(a));
         float y[4];
+        if constexpr (DITHER) {
+            const float inv = 1.0f / s;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                y[e] = x[e] * inv;
+                if (ROOT) y[e] = x[e] > 0.0f ? __builtin_fmaxf(y[e], 0x1p-9f) : y[e];
+                const float z = dither_e4m3(y[e], ROOT ? rnd[e] >> 16 : rnd[e] & 0xFFFFu);
+                y[e] = plain || __builtin_fabsf(y[e]) <= 448.0f ? z : y[e];  // others are saturated or NaN
+            }
+            if (plain) {
+                const int lo2 = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+                return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo2, true);
+            }
+            return encode2_hw<E4M3>(y[0], y[1]) | (encode2_hw<E4M3>(y[2], y[3]) << 16);
+        }
         if (plain && s >= 0x1p-40f && s <= 0x1p40f) {
             // quotients of at most 448 (so no clamp); one whose remainders
             // underflow is below 2^-17 and goes to code 0 whatever its last bits
@@ -362,8 +425,13 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
                                       copy_bits<COPY>(p[2]) | (copy_bits<COPY>(p[3]) << 16)});
                     if constexpr (S8) {
                         float s0, s1;
-                        const uint32_t c0 = encode(m, std::false_type{}, plain, s0);
-                        const uint32_t c1 = encode(root, std::true_type{}, plain, s1);
+                        uint32_t rnd[4] = {};
+                        if constexpr (DITHER) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) rnd[e] = draw(key, i + e);
+                        }
+                        const uint32_t c0 = encode(m, std::false_type{}, plain, s0, rnd);
+                        const uint32_t c1 = encode(root, std::true_type{}, plain, s1, rnd);
                         stv<NT, B4>(static_cast<uint8_t*>(t.m) + i, c0);
                         stv<NT, B4>(static_cast<uint8_t*>(t.v) + i, c1);
                         if (lane == 0) {
@@ -412,8 +480,13 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (ub + lane * 4 + e >= t.n) m[e] = root[e] = 0.0f;
-                    c0 = encode(m, std::false_type{}, false, s0);
-                    c1 = encode(root, std::true_type{}, false, s1);
+                    uint32_t rnd[4] = {};
+                    if constexpr (DITHER) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) rnd[e] = draw(key, ub + lane * 4 + e);
+                    }
+                    c0 = encode(m, std::false_type{}, false, s0, rnd);
+                    c1 = encode(root, std::true_type{}, false, s1, rnd);
                     if (lane == 0) {
                         t.ms[ub >> 8] = s0;
                         t.vs[ub >> 8] = s1;
@@ -455,22 +528,30 @@ __global__ __launch_bounds__(kWThreads) void adamw_kernel(const WList L, const W
     }
 }
 
-template <typename G, bool S8, bool NT>
+enum Kept { kBits32, kBits8, kBits8Dithered };  // how states are kept
+
+template <typename G, Kept K, bool NT>
 void launch_copy(int copy_dtype, int blocks, const WList& L, const WHyper& h, hipStream_t st) {
+    constexpr bool S8 = K != kBits32, D = K == kBits8Dithered;
     if (copy_dtype == DF_DTYPE_BFLOAT16)
-        adamw_kernel<G, S8, DF_DTYPE_BFLOAT16, NT><<<blocks, kWThreads, 0, st>>>(L, h);
+        adamw_kernel<G, S8, DF_DTYPE_BFLOAT16, NT, D><<<blocks, kWThreads, 0, st>>>(L, h);
     else if (copy_dtype == DF_DTYPE_HALF)
-        adamw_kernel<G, S8, DF_DTYPE_HALF, NT><<<blocks, kWThreads, 0, st>>>(L, h);
+        adamw_kernel<G, S8, DF_DTYPE_HALF, NT, D><<<blocks, kWThreads, 0, st>>>(L, h);
     else
-        adamw_kernel<G, S8, -1, NT><<<blocks, kWThreads, 0, st>>>(L, h);
+        adamw_kernel<G, S8, -1, NT, D><<<blocks, kWThreads, 0, st>>>(L, h);
+}
+
+template <typename G, Kept K>
+void launch_cold(bool cold, int copy_dtype, int blocks, const WList& L, const WHyper& h, hipStream_t st) {
+    if (cold) launch_copy<G, K, true>(copy_dtype, blocks, L, h, st);
+    else launch_copy<G, K, false>(copy_dtype, blocks, L, h, st);
 }
 
 template <typename G>
-void launch_state(bool s8, bool cold, int copy_dtype, int blocks, const WList& L, const WHyper& h, hipStream_t st) {
-    if (s8 && cold) launch_copy<G, true, true>(copy_dtype, blocks, L, h, st);
-    else if (s8) launch_copy<G, true, false>(copy_dtype, blocks, L, h, st);
-    else if (cold) launch_copy<G, false, true>(copy_dtype, blocks, L, h, st);
-    else launch_copy<G, false, false>(copy_dtype, blocks, L, h, st);
+void launch_state(Kept kept, bool cold, int copy_dtype, int blocks, const WList& L, const WHyper& h, hipStream_t st) {
+    if (kept == kBits32) launch_cold<G, kBits32>(cold, copy_dtype, blocks, L, h, st);
+    else if (kept == kBits8) launch_cold<G, kBits8>(cold, copy_dtype, blocks, L, h, st);
+    else launch_cold<G, kBits8Dithered>(cold, copy_dtype, blocks, L, h, st);
 }
 
 }  // namespace
@@ -481,19 +562,18 @@ using namespace dfk;
 
 extern "C" int64_t df_adamw_scale_count(int64_t n) { return n <= 0 ? 0 : (n + kUnit - 1) / kUnit; }
 
-extern "C" int df_adamw_update(int count, const int64_t* sizes, float* const* params, int grad_dtype,
-                               const void* const* grads, int state_dtype, void* const* m, void* const* v,
-                               float* const* m_scale, float* const* v_scale, int copy_dtype, void* const* copies,
-                               float lr, float beta1, float beta2, float eps, const float* weight_decay, int timestep,
-                               const float* lr_dev, const int* timestep_dev, const float* clip_norm_dev,
-                               float max_norm, float* absmax_dev, void* stream) {
-    clear_error();
-    const char* fn = "df_adamw_update";
+static int update(const char* fn, bool dither, uint32_t seed, int count, const int64_t* sizes, float* const* params,
+                  int grad_dtype, const void* const* grads, int state_dtype, void* const* m, void* const* v,
+                  float* const* m_scale, float* const* v_scale, int copy_dtype, void* const* copies, float lr,
+                  float beta1, float beta2, float eps, const float* weight_decay, int timestep, const float* lr_dev,
+                  const int* timestep_dev, const float* clip_norm_dev, float max_norm, float* absmax_dev,
+                  void* stream) {
     DF_CHECK(count >= 0, DF_ERR_INVALID, "%s: count = %d is negative", fn, count);
     DF_CHECK(grad_dtype == DF_DTYPE_FLOAT32 || grad_dtype == DF_DTYPE_BFLOAT16 || grad_dtype == DF_DTYPE_HALF,
              DF_ERR_UNSUPPORTED, "%s: gradient dtype %d not supported", fn, grad_dtype);
     DF_CHECK(state_dtype == DF_DTYPE_FLOAT32 || state_dtype == DF_DTYPE_FP8E4M3, DF_ERR_UNSUPPORTED,
              "%s: state dtype %d not supported", fn, state_dtype);
+    DF_CHECK(!dither || state_dtype == DF_DTYPE_FP8E4M3, DF_ERR_UNSUPPORTED, "%s: only 8-bit states are dithered", fn);
     DF_CHECK(!copies || copy_dtype == DF_DTYPE_BFLOAT16 || copy_dtype == DF_DTYPE_HALF, DF_ERR_UNSUPPORTED,
              "%s: copy dtype %d not supported", fn, copy_dtype);
     const bool s8 = state_dtype == DF_DTYPE_FP8E4M3;
@@ -527,6 +607,8 @@ extern "C" int df_adamw_update(int count, const int64_t* sizes, float* const* pa
     h.max_norm = max_norm;
     h.bc1 = bias_corr(beta1, timestep);
     h.bc2 = bias_corr(beta2, timestep);
+    h.t = timestep;
+    h.seed = seed;
     h.lr_dev = lr_dev;
     h.step = timestep_dev;
     h.norm = clip_norm_dev;
@@ -557,9 +639,35 @@ extern "C" int df_adamw_update(int count, const int64_t* sizes, float* const* pa
         L.first[c] = blocks;
         L.count = c;
         const int cd = copies ? copy_dtype : -1;
-        if (grad_dtype == DF_DTYPE_FLOAT32) launch_state<float>(s8, cold, cd, blocks, L, h, st);
-        else if (grad_dtype == DF_DTYPE_HALF) launch_state<f16_t>(s8, cold, cd, blocks, L, h, st);
-        else launch_state<uint16_t>(s8, cold, cd, blocks, L, h, st);
+        const Kept kept = !s8 ? kBits32 : dither ? kBits8Dithered : kBits8;
+        if (grad_dtype == DF_DTYPE_FLOAT32) launch_state<float>(kept, cold, cd, blocks, L, h, st);
+        else if (grad_dtype == DF_DTYPE_HALF) launch_state<f16_t>(kept, cold, cd, blocks, L, h, st);
+        else launch_state<uint16_t>(kept, cold, cd, blocks, L, h, st);
     }
     return launch_status(fn);
+}
+
+extern "C" int df_adamw_update(int count, const int64_t* sizes, float* const* params, int grad_dtype,
+                               const void* const* grads, int state_dtype, void* const* m, void* const* v,
+                               float* const* m_scale, float* const* v_scale, int copy_dtype, void* const* copies,
+                               float lr, float beta1, float beta2, float eps, const float* weight_decay, int timestep,
+                               const float* lr_dev, const int* timestep_dev, const float* clip_norm_dev,
+                               float max_norm, float* absmax_dev, void* stream) {
+    clear_error();
+    return update("df_adamw_update", false, 0, count, sizes, params, grad_dtype, grads, state_dtype, m, v,
+                  m_scale, v_scale, copy_dtype, copies, lr, beta1, beta2, eps, weight_decay, timestep, lr_dev,
+                  timestep_dev, clip_norm_dev, max_norm, absmax_dev, stream);
+}
+
+extern "C" int df_adamw_update_dithered(int count, const int64_t* sizes, float* const* params, int grad_dtype,
+                                        const void* const* grads, int state_dtype, void* const* m, void* const* v,
+                                        float* const* m_scale, float* const* v_scale, int copy_dtype, void* const* copies,
+                                        float lr, float beta1, float beta2, float eps, const float* weight_decay, int timestep,
+                                        const float* lr_dev, const int* timestep_dev, const float* clip_norm_dev,
+                                        float max_norm, float* absmax_dev, uint32_t seed,
+                                        void* stream) {
+    clear_error();
+    return update("df_adamw_update_dithered", true, seed, count, sizes, params, grad_dtype, grads, state_dtype, m, v,
+                  m_scale, v_scale, copy_dtype, copies, lr, beta1, beta2, eps, weight_decay, timestep, lr_dev,
+                  timestep_dev, clip_norm_dev, max_norm, absmax_dev, stream);
 }

@@ -7,7 +7,8 @@
 // bias gradients; one df_adamw_update call updates the whole list.
 //
 // state_bits 32: the moments in binary32; 8: as e4m3 codes with a scale per 256
-// values (a quarter of the memory; see include/df_capi.h).  A parameter is known
+// values, dithered (a quarter of the memory; see df_adamw_update_dithered in
+// include/df_capi.h).  A parameter is known
 // by its tensor's address, its moments start at zero when update_parameters
 // first lists it, or lists it with another size; step() refuses one whose size
 // changed after that (tensor::load gives a tensor another shape and buffer).

@@ -245,10 +245,17 @@ void AdamWOptimizer<float>::launch(const float* clip_norm, float max_norm) {
         wd[i] = d == decay_.end() ? weight_decay_ : d->second;
     }
     ++timestep_;
-    CHECK_DF_EX(df_adamw_update((int)n, sizes.data(), p.data(), DF_DTYPE_FLOAT32, g.data(),
-                                state_bits_ == 8 ? DF_DTYPE_FP8E4M3 : DF_DTYPE_FLOAT32, m.data(), v.data(), ms.data(),
-                                vs.data(), DF_DTYPE_FLOAT32, nullptr, learning_rate_, beta1_, beta2_, epsilon_, wd.data(),
-                                timestep_, nullptr, nullptr, clip_norm, max_norm, nullptr, stream_arg()));
+    if (state_bits_ == 8)
+        CHECK_DF_EX(df_adamw_update_dithered((int)n, sizes.data(), p.data(), DF_DTYPE_FLOAT32, g.data(),
+                                             DF_DTYPE_FP8E4M3, m.data(), v.data(), ms.data(), vs.data(),
+                                             DF_DTYPE_FLOAT32, nullptr, learning_rate_, beta1_, beta2_, epsilon_,
+                                             wd.data(), timestep_, nullptr, nullptr, clip_norm, max_norm, nullptr,
+                                             /*seed=*/0, stream_arg()));
+    else
+        CHECK_DF_EX(df_adamw_update((int)n, sizes.data(), p.data(), DF_DTYPE_FLOAT32, g.data(), DF_DTYPE_FLOAT32,
+                                    m.data(), v.data(), nullptr, nullptr, DF_DTYPE_FLOAT32, nullptr, learning_rate_,
+                                    beta1_, beta2_, epsilon_, wd.data(), timestep_, nullptr, nullptr, clip_norm,
+                                    max_norm, nullptr, stream_arg()));
 }
 
 template <>

@@ -641,6 +641,12 @@ int df_grad_norm(int dtype, const void* const* grads, const int64_t* sizes, int 
  *                 rounded to nearest even and saturated, NaN as 0x7F, a
  *                 sqrt(v) above 0 at least code 1.  All codes 0 at any finite
  *                 scale is the state before the first step.
+ *                 This is exact for one step, but does not follow many: a step
+ *                 lowers sqrt(v) by at most (1-b2)/2 of itself, its codes lie 6
+ *                 to 12% apart, and a falling one is rounded back to its code
+ *                 until the scale moves.  Where half of a block's gradients
+ *                 fall tenfold, their sqrt(v) stays up to ten times too large.
+ *                 To train with 8-bit states: df_adamw_update_dithered.
  *  copies       : NULL, or per tensor the updated p in copy_dtype (bf16, f16).
  *  weight_decay : wd per tensor, or NULL (0).
  *  timestep     : t >= 1, the already-incremented step count; with
@@ -650,7 +656,18 @@ int df_grad_norm(int dtype, const void* const* grads, const int64_t* sizes, int 
  *  absmax_dev   : NULL, or a device array: max |p| over the finite values of
  *                 updated tensor i (0 for an empty one), for
  *                 df_quantize_2d_batch_absmax.
- * What is written (params, states, scales, copies) must not overlap. */
+ * What is written (params, states, scales, copies) must not overlap, nor lie
+ * over another tensor's gradients.
+ *  df_adamw_update_dithered: the same with states of DF_DTYPE_FP8E4M3 only, m
+ *                 and sqrt(v) rounded up or down at random: q = x * (1 / scale)
+ *                 (after the raise to code 1) goes to the larger in magnitude
+ *                 of the two e4m3 values next to it with the probability of its
+ *                 place between them, so what is kept is right on average and
+ *                 moves by as much as it should over many steps, with a noise
+ *                 of a quarter of sqrt(v) at most (one standard deviation; a
+ *                 third while it falls fast), however near b2 is to 1.  The draws come from a hash of seed, t, the tensor's
+ *                 place in the list and the value's in the tensor: the same
+ *                 call gives the same codes, and one seed serves all steps. */
 int64_t df_adamw_scale_count(int64_t n);  /* ceil(n / 256) */
 int df_adamw_update(int count, const int64_t* sizes, float* const* params, int grad_dtype,
                     const void* const* grads, int state_dtype, void* const* m, void* const* v,
@@ -658,6 +675,13 @@ int df_adamw_update(int count, const int64_t* sizes, float* const* params, int g
                     float lr, float beta1, float beta2, float eps, const float* weight_decay,
                     int timestep, const float* lr_dev, const int* timestep_dev,
                     const float* clip_norm_dev, float max_norm, float* absmax_dev, void* stream);
+int df_adamw_update_dithered(int count, const int64_t* sizes, float* const* params, int grad_dtype,
+                             const void* const* grads, int state_dtype, void* const* m, void* const* v,
+                             float* const* m_scale, float* const* v_scale, int copy_dtype,
+                             void* const* copies, float lr, float beta1, float beta2, float eps,
+                             const float* weight_decay, int timestep, const float* lr_dev,
+                             const int* timestep_dev, const float* clip_norm_dev, float max_norm,
+                             float* absmax_dev, uint32_t seed, void* stream);
 
 /* ---- tensor utilities behind dnn::tensor (dnn/core/tensor.cu:18-52) ---- */
 /* fill_kernel (tensor.cu:19): n elements of elem_bytes (1, 2 or 4) = *value */

@@ -1602,6 +1602,45 @@ TEST_F(AdamOptimizerTest, ListedTensorTakesAnotherSize) {
     }
 }
 
+// Gradients that fall tenfold for half of the values: the steps with 8-bit
+// states follow those with 32-bit ones.  A kept root has a standard deviation
+// of at most a quarter, so 1 / root lies above 1 / its mean by 1/16 on average,
+// and the mean over 1024 values (they are drawn apart) within 0.25 / 32 * 6 of
+// that.  A root that stayed would leave steps of a tenth.
+TEST_F(AdamWOptimizerTest, EightBitStatesFollowAFall) {
+    constexpr int n = 2048;
+    tensor<float> a({n}), b({n}), g({n});
+    a.fill(0.0f);
+    b.fill(0.0f);
+    AdamWOptimizer<float> full(0.01f, 0.9f, 0.99f, 1e-8f, 0.0f), small(0.01f, 0.9f, 0.99f, 1e-8f, 0.0f, 8);
+    full.update_parameters({&a}, {&g});
+    small.update_parameters({&b}, {&g});
+    std::vector<float> gh(n, 1.0f), x0, y0;
+    for (int t = 1; t <= 1500; ++t) {
+        if (t == 1 || t == 301) {
+            for (int i = 0; t > 1 && i < n; ++i)
+                if (i % 256 >= 128) gh[i] = 0.1f;
+            g.upload(gh.data());
+        }
+        full.step();
+        small.step();
+        if (t == 1300) {
+            x0 = download(a);
+            y0 = download(b);
+        }
+    }
+    const auto x = download(a), y = download(b);
+    double moved[2][2] = {};
+    for (int i = 0; i < n; ++i) {
+        moved[i % 256 >= 128][0] += x[i] - x0[i];
+        moved[i % 256 >= 128][1] += y[i] - y0[i];
+    }
+    for (const auto& m : moved) {
+        EXPECT_GT(m[1] / m[0], 1 - 0.05);
+        EXPECT_LT(m[1] / m[0], 1 + 0.0625 + 0.05);
+    }
+}
+
 // step_clipped(max_norm) == clip_grad_norm(grads, max_norm) + step(), except
 // that the gradients keep their values.
 TEST_F(AdamOptimizerTest, StepClippedEqualsClipThenStep) {

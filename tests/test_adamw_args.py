@@ -97,3 +97,16 @@ def test_clip_needs_a_device_norm_and_a_limit():
     for kw in (dict(), dict(max_norm=0.0), dict(max_norm=-1.0), dict(max_norm=float("nan"))):
         with pytest.raises(ValueError, match="max_norm"):
             df.adamw_update(ok(), ok(), ok(), ok(), 1, clip_norm=fake(1), **kw)
+
+
+def test_dither_refusals():
+    sizes = (ctypes.c_int64 * 1)(4)
+    f = lambda st=E4, n=sizes, t=1, ms=one(): df.lib().df_adamw_update_dithered(
+        1, n, one(), F32, one(), st, one(), one(), ms, one(), 0, None, 1e-3, 0.9, 0.99, 1e-8, None, t, None, None, None, 0.0,
+        None, 7, None)
+    assert f(st=F32) == -2 and f(st=BF) == -2 and f(t=0) == -1 and f(ms=None) == -1 and f(n=(ctypes.c_int64 * 1)(-1)) == -1
+    assert "df_adamw_update_dithered" in df.lib().df_last_error_string().decode()
+    assert f(n=(ctypes.c_int64 * 1)(0)) == 0
+    ok = lambda: [fake(4)]
+    with pytest.raises(ValueError, match="dither"):
+        df.adamw_update(ok(), ok(), ok(), ok(), 1, dither=0)
