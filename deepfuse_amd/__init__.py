@@ -728,6 +728,13 @@ def _check_gpu(fn: str, **tensors):
         dev = at
 
 
+def _fits(fn: str, *sizes: int):
+    """Sizes and strides that the C interface can take: ctypes would cut a
+    larger one to its low 32 bits."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise ValueError(f"{fn}: a size or stride of {max(sizes)}, past 32 bits")
+
+
 def _check_like(fn: str, name: str, t, shape, dtype):
     if t.shape != shape or t.dtype is not dtype:
         raise ValueError(f"{fn}: {name} is {tuple(t.shape)} {t.dtype}, not {tuple(shape)} {dtype}")
@@ -740,7 +747,10 @@ def _rows(fn: str, name: str, t, shape, dtype) -> int:
     (rows, cols), (ld, step) = shape, t.stride()
     if cols > 1 and step != 1 or rows > 1 and ld < cols:
         raise ValueError(f"{fn}: {name} with strides {(ld, step)} has no contiguous rows of its own")
-    return ld if rows > 1 else cols
+    if rows <= 1:
+        return cols
+    _fits(fn, ld)
+    return ld
 
 
 def _row_vector(fn: str, name: str, t, n: int, dtype):
@@ -767,6 +777,7 @@ def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, residual=None):
         raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
     shape, dtype, at = x.shape, x.dtype, x.get_device()
     rows, cols = shape
+    _fits(fn, rows, cols)
     ldx = ldr = cols
     if not (at >= 0 and x.is_contiguous() and _plain(residual, shape, dtype, at) and _plain(gamma, (cols,), dtype, at)
             and _plain(beta, (cols,), dtype, at)):
@@ -798,6 +809,7 @@ def layernorm_backward(dy, x, gamma=None, mean=None, rstd=None, eps=1e-5, dresid
         raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
     shape, dtype, at = x.shape, x.dtype, x.get_device()
     rows, cols = shape
+    _fits(fn, rows, cols)
     ldx = lddy = lddr = cols
     if not (at >= 0 and x.is_contiguous() and _plain(dy, shape, dtype, at) and _plain(dresidual, shape, dtype, at)
             and _plain(gamma, (cols,), dtype, at) and _plain(mean, (rows,), torch.float32, at)
@@ -1030,6 +1042,7 @@ def _experts_rows(fn: str, c_fn: str, a_q, w_q, offsets, red: int, sa, sw, out_d
     if a_q.shape[1] < red or w_q.shape[2] < red:
         raise ValueError(f"{fn}: rows of {a_q.shape[1]} and {w_q.shape[2]} codes, fewer than {red}")
     rows = a_q.shape[0]
+    _fits(fn, rows, cols, red, experts, lda, ldw)
     out, ld = _experts_out(fn, out, (rows, cols), out_dtype, a_q)
     n, k = (cols, red) if c_fn == "df_fp8_experts_fwd" else (red, cols)
     with _on(a_q):
@@ -1068,6 +1081,7 @@ def experts_dw(dyt_q, xt_q, offsets, rows: int, sdy, sx, out_dtype=None, out=Non
     if dyt_q.shape[1] < rows or xt_q.shape[1] < rows:
         raise ValueError(f"{fn}: rows of {dyt_q.shape[1]} and {xt_q.shape[1]} codes, fewer than {rows}")
     N, K = dyt_q.shape[0], xt_q.shape[0]
+    _fits(fn, rows, N, K, experts, lddy, ldx)
     if out is None and out_dtype is None:
         out_dtype = torch.float32
     out, _ = _experts_out(fn, out, (experts, N, K), out_dtype, dyt_q)
@@ -1088,6 +1102,7 @@ def quantize_experts(w, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=True):
         raise ValueError(f"{fn}: no codes wanted")
     _check_gpu(fn, w=w)
     E, N, K = w.shape
+    _fits(fn, E, N, K)
     dt = int(_in_dtype(w))
     if w.numel() == 0:  # nothing to measure: the rule's scale of no values is 1
         none = lambda r, c: torch.zeros((E, r, round16(c)), dtype=torch.uint8, device=w.device)
