@@ -43,7 +43,9 @@ namespace {
 // ------------------------------------------------------------ small tiles --
 // Row tile v of all experts' tiles of ROWS rows, counted through: its expert,
 // that one's rows [lo, hi) and the tile's first; false behind the last.  The
-// same for every lane of the wave (a lane counts an expert's tiles).
+// same for every lane of the wave (a lane counts an expert's tiles).  v is below
+// most_tiles(): up to the first lane past it the counts are right even where
+// later ones of overlapping offsets pass 32 bits.
 template <int ROWS>
 __device__ __forceinline__ bool row_tile(const ExpertArgs& g, int v, int lane, int& e, int& lo, int& hi, int& m0) {
     for (int base = 0; base < g.experts; base += 64) {
@@ -59,16 +61,16 @@ __device__ __forceinline__ bool row_tile(const ExpertArgs& g, int v, int lane, i
         DF_SCAN(0x142, 0xA);  // row_bcast:15 into the second and fourth row
         DF_SCAN(0x143, 0xC);  // row_bcast:31 into the upper half
 #undef DF_SCAN
-        const int all = __builtin_amdgcn_readlane(upto, 63);
-        if (v < all) {
-            const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > v));
+        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > v);
+        if (past) {
+            const int l = __builtin_ctzll(past);
             e = base + l;
             lo = __builtin_amdgcn_readlane(a, l);
             hi = __builtin_amdgcn_readlane(b, l);
             m0 = lo + (v - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l))) * ROWS;
             return true;
         }
-        v -= all;
+        v -= __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
@@ -119,10 +121,11 @@ __global__ __launch_bounds__(64 * W) void experts_small_kernel(const ExpertArgs 
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
     };
 
+    const int most = COUNTED ? most_tiles(g.rows, g.experts, ROWS) : 0;
     for (int v = COUNTED ? (int)blockIdx.y : 0;; v += COUNTED ? (int)gridDim.y : 1) {
         int e, lo, hi, m0;
         if constexpr (COUNTED) {
-            if (!row_tile<ROWS>(g, v, lane, e, lo, hi, m0)) return;  // the whole block
+            if (v >= most || !row_tile<ROWS>(g, v, lane, e, lo, hi, m0)) return;  // the whole block
         } else {
             e = blockIdx.y;
             expert_rows(g.off, e, g.rows, lo, hi);
@@ -257,8 +260,7 @@ template <int FA, bool SUMS, bool WIDE> void launch_small(const ExpertArgs& g, i
             experts_small_kernel<FA, E4M3, 1, 1, 4, 4, false, WIDE><<<grid, 256, 0, st>>>(g, c_dtype);
         } else {
             // at most this many row tiles; blocks behind the last return at once
-            const int64_t most = (int64_t)g.rows / 32 + std::min(g.experts, g.rows);
-            const dim3 grid((g.N + 31) / 32, (int)std::min<int64_t>(most, 65535));
+            const dim3 grid((g.N + 31) / 32, std::min(most_tiles(g.rows, g.experts, 32), 65535));
             experts_small_kernel<FA, E4M3, 2, 2, 4, 2, false, WIDE><<<grid, 256, 0, st>>>(g, c_dtype);
         }
     }
@@ -310,7 +312,7 @@ TilePlan plan(const ExpertArgs& g, bool sums, bool wide_codes) {
     }
     if (!p.tiles) return p;
     // at most this many units; blocks without one return at once
-    const int64_t most = (sums ? mt : g.rows / kPBM + std::min(g.experts, g.rows)) * (p.narrow ? sn : wn);
+    const int64_t most = (sums ? mt : most_tiles(g.rows, g.experts, kPBM)) * (p.narrow ? sn : wn);
     p.grid = (int)std::min<int64_t>(most, cus);
     return p;
 }

@@ -27,6 +27,13 @@ __device__ __forceinline__ void expert_rows(const int* off, int e, int rows, int
     hi = min(max(off[e + 1], lo), rows);
 }
 
+// The most tiles of `tile` rows that experts' rows take, dealt in any way.
+// Offsets that overlap may give more, up to one of all rows per expert: tiles
+// from here on are not worked on, and counts of them may pass 32 bits.
+__host__ __device__ __forceinline__ int most_tiles(int rows, int experts, int tile) {
+    return rows / tile + (experts < rows ? experts : rows);
+}
+
 // bytes of a dword at byte position `pos` that lie in [lo, hi)
 __device__ __forceinline__ uint32_t keep_bytes(int pos, int lo, int hi) {
     const int a = min(max(lo - pos, 0), 4) * 8, b = min(max(hi - pos, 0), 4) * 8;

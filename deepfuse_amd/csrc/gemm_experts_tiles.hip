@@ -40,7 +40,9 @@ __device__ __forceinline__ void fixed_rows(const ExpertArgs& g, int e, int& lo, 
 }
 
 // Block-wide: tiles of 256 rows before each expert, into first[0..kMaxExperts]
-// (INT_MAX behind the last).
+// (INT_MAX behind the last).  Sums stay at kCountCap, so that overlapping offsets
+// do not wrap them: each is right up to there, past most_tiles() (below 2^24).
+constexpr int kCountCap = 0x3FFFFFFF;
 __device__ __forceinline__ void count_tiles(const ExpertArgs& g, int* first, int* waves) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
     int c[2], sum = 0;
@@ -59,11 +61,11 @@ __device__ __forceinline__ void count_tiles(const ExpertArgs& g, int* first, int
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const int o = __shfl_up(s, off, 64);
-        if (lane >= off) s += o;
+        if (lane >= off) s = min(s + o, kCountCap);
     }
     if (lane == 63) waves[w] = s;
     __syncthreads();
-    for (int i = 0; i < w; ++i) s += waves[i];
+    for (int i = 0; i < w; ++i) s = min(s + waves[i], kCountCap);
     int at = s - sum;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -106,8 +108,9 @@ __global__ __launch_bounds__(512, 1) void experts_tile_kernel(const ExpertArgs g
     const int tiles_n = (g.N + BN - 1) / BN;
     const int tiles_m = SUMS ? (g.M + kPBM - 1) / kPBM : 0;
     if constexpr (!SUMS) count_tiles(g, first, reinterpret_cast<int*>(lds));
-    const int nunits =
-        SUMS ? g.experts * tiles_m * tiles_n : __builtin_amdgcn_readfirstlane(first[g.experts]) * tiles_n;
+    const int nunits = SUMS ? g.experts * tiles_m * tiles_n
+                            : min(__builtin_amdgcn_readfirstlane(first[g.experts]),
+                                  most_tiles(g.rows, g.experts, kPBM)) * tiles_n;
 
     const int P = gridDim.x;
     const int q = P >> 3, rr = P & 7;

@@ -74,3 +74,23 @@ def test_one_row_dw(dev):
         for e, (lo, hi) in enumerate(((0, 30), (30, 61))):
             assert torch.equal(a[e, 0].double(), d(many[E4], E4)[:, lo:hi] @ d(one[E5], E5)[lo:hi])
             assert torch.equal(b[e, :, 0].double(), d(many[E5], E5)[:, lo:hi] @ d(one[E4], E4)[lo:hi])
+
+
+@pytest.mark.parametrize("rows,E,K,N", [(3000, 1024, 16, 40), (3000, 64, 256, 1600), (40_000, 100, 64, 36), (9000, 30, 512, 1600)])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_overlapping_offsets(dev, rows, E, K, N, dt):
+    """Every other expert claims all rows: values mean nothing, but nothing outside the output is written, the call ends
+    as soon as a right one would, and a right one after it is right."""
+    g = torch.Generator(device=dev).manual_seed(rows)
+    x, w = codes(g, dev, (rows, K), E4), codes(g, dev, (E, N, K), E4)
+    s, sw = torch.ones(1, device=dev), torch.ones(E, device=dev)
+    room = torch.full((rows + 600, N), 5.0, dtype=dt, device=dev)
+    out = room[300:300 + rows]
+    for bad in ([0, rows] * E, [rows, -3] * E, [0] + [rows] * E, [2 ** 31 - 1, -2 ** 31] * E):
+        df.experts_fwd(x, w, torch.tensor(bad[:E + 1], dtype=torch.int64).to(torch.int32).to(dev), K, s, sw, out=out)
+        assert (room[:300] == 5).all() and (room[300 + rows:] == 5).all()
+    cut = torch.linspace(0, rows, E + 1, device=dev).int()
+    df.experts_fwd(x, w, cut, K, s, sw, out=out)
+    b = cut.tolist()
+    ref = torch.cat([x[lo:hi].view(E4).float() @ w[e].view(E4).float().t() for e, (lo, hi) in enumerate(zip(b, b[1:]))])
+    assert torch.equal(out, ref.to(dt))
