@@ -1110,8 +1110,9 @@ def quantize_experts(w, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=True):
                 none(K, N) if want_qt else None)
     with _on(w):
         src = w.view(E, N * K)
-        if src.stride(0) * w.element_size() % 16:  # the batched quantize takes tensors at 16-byte boundaries
-            src = torch.nn.functional.pad(src, (0, -src.shape[1] % 16))
+        if N * K * w.element_size() % 16 or w.data_ptr() % 16:  # the quantize calls take tensors at 16-byte boundaries
+            src = w.new_empty((E, round16(N * K)))
+            src[:, :N * K].copy_(w.view(E, N * K))
         new = lambda r, c: torch.empty((E, r, round16(c)), dtype=torch.uint8, device=w.device)
         q, qt = new(N, K) if want_q else None, new(K, N) if want_qt else None
         sc = torch.empty(E, dtype=torch.float32, device=w.device)

@@ -89,3 +89,18 @@ def test_experts_apart(calls):
             with pytest.raises(ValueError, match="follow"):
                 rows_call("experts_fwd", fake(8, 32), w, 32)
     assert not calls
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(3, 4, 8), (3, 5, 7), (1, 4, 8)])
+@pytest.mark.parametrize("offset", [0, 1, 3])
+def test_weights_at_any_element(calls, dtype, shape, offset):
+    """Experts' weights that start at any element are quantized from 16-byte boundaries, with their values."""
+    n = shape[0] * shape[1] * shape[2]
+    base = torch.arange(64 + n).to(dtype)
+    start = -(base.data_ptr() % 16) // base.element_size() % 8 + offset
+    w = base[start:start + n].view(shape).as_subclass(Fake)
+    df.quantize_experts(w)
+    ptrs = [list(c[3]) for c in calls if c[0] == "df_quantize_2d_batch"]
+    ptrs = ptrs[0] if ptrs else [c[2] for c in calls]
+    assert len(ptrs) == shape[0] and all(p % 16 == 0 for p in ptrs)

@@ -76,6 +76,19 @@ def test_one_row_dw(dev):
             assert torch.equal(b[e, :, 0].double(), d(many[E5], E5)[:, lo:hi] @ d(one[E4], E4)[lo:hi])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("E,N,K", [(3, 40, 96), (5, 37, 51), (1, 16, 16)])
+def test_quantize_weights_at_any_element(dev, dtype, E, N, K):
+    g = torch.Generator(device=dev).manual_seed(E)
+    w = torch.randn(E, N, K, generator=g, device=dev).to(dtype)
+    want = df.quantize_experts(w)
+    for off in (1, 3, 8):
+        base = torch.full((E * N * K + 16,), 1e4, device=dev).to(dtype)
+        view = base[off:off + E * N * K].view(E, N, K)
+        view.copy_(w)
+        assert all(torch.equal(a, b) for a, b in zip(df.quantize_experts(view), want)), off
+
+
 @pytest.mark.parametrize("rows,E,K,N", [(3000, 1024, 16, 40), (3000, 64, 256, 1600), (40_000, 100, 64, 36), (9000, 30, 512, 1600)])
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 def test_overlapping_offsets(dev, rows, E, K, N, dt):
