@@ -728,10 +728,13 @@ def _check_gpu(fn: str, **tensors):
         dev = at
 
 
+_INT_MAX = 0x7FFFFFFF
+
+
 def _fits(fn: str, *sizes: int):
     """Sizes and strides that the C interface can take: ctypes would cut a
-    larger one to its low 32 bits."""
-    if max(sizes) > 0x7FFFFFFF:
+    larger one to its low 32 bits.  (Asked where one of them, or-ed, is.)"""
+    if max(sizes) > _INT_MAX:
         raise ValueError(f"{fn}: a size or stride of {max(sizes)}, past 32 bits")
 
 
@@ -777,7 +780,8 @@ def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, residual=None):
         raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
     shape, dtype, at = x.shape, x.dtype, x.get_device()
     rows, cols = shape
-    _fits(fn, rows, cols)
+    if (rows | cols) > _INT_MAX:
+        _fits(fn, rows, cols)
     ldx = ldr = cols
     if not (at >= 0 and x.is_contiguous() and _plain(residual, shape, dtype, at) and _plain(gamma, (cols,), dtype, at)
             and _plain(beta, (cols,), dtype, at)):
@@ -809,7 +813,8 @@ def layernorm_backward(dy, x, gamma=None, mean=None, rstd=None, eps=1e-5, dresid
         raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
     shape, dtype, at = x.shape, x.dtype, x.get_device()
     rows, cols = shape
-    _fits(fn, rows, cols)
+    if (rows | cols) > _INT_MAX:
+        _fits(fn, rows, cols)
     ldx = lddy = lddr = cols
     if not (at >= 0 and x.is_contiguous() and _plain(dy, shape, dtype, at) and _plain(dresidual, shape, dtype, at)
             and _plain(gamma, (cols,), dtype, at) and _plain(mean, (rows,), torch.float32, at)
@@ -1042,7 +1047,8 @@ def _experts_rows(fn: str, c_fn: str, a_q, w_q, offsets, red: int, sa, sw, out_d
     if a_q.shape[1] < red or w_q.shape[2] < red:
         raise ValueError(f"{fn}: rows of {a_q.shape[1]} and {w_q.shape[2]} codes, fewer than {red}")
     rows = a_q.shape[0]
-    _fits(fn, rows, cols, red, experts, lda, ldw)
+    if (rows | cols | red | experts | lda | ldw) > _INT_MAX:
+        _fits(fn, rows, cols, red, experts, lda, ldw)
     out, ld = _experts_out(fn, out, (rows, cols), out_dtype, a_q)
     n, k = (cols, red) if c_fn == "df_fp8_experts_fwd" else (red, cols)
     with _on(a_q):
@@ -1053,7 +1059,8 @@ def _experts_rows(fn: str, c_fn: str, a_q, w_q, offsets, red: int, sa, sw, out_d
 
 def experts_fwd(x_q, w_q, offsets, K: int, sx, sw, out_dtype=None, out=None):
     """Y [rows, N] of a Linear dealt to experts (df_fp8_experts_fwd): x_q
-    [rows, >=K] and w_q [experts, N, >=K] e4m3 codes, offsets int32
+    [rows, >=K] and w_q [experts, N, >=K] e4m3 codes, zero from K to the next
+    multiple of 16 as the quantize calls leave them, offsets int32
     [experts + 1] (expert e has rows offsets[e] to offsets[e+1], on the
     device), sx one scale, sw one per expert.  ``out`` keeps its rows that
     belong to no expert; a new output (bf16 unless out_dtype says otherwise)
@@ -1063,7 +1070,8 @@ def experts_fwd(x_q, w_q, offsets, K: int, sx, sw, out_dtype=None, out=None):
 
 def experts_dx(dy_q, wt_q, offsets, N: int, sdy, sw, out_dtype=None, out=None):
     """dX [rows, K] (df_fp8_experts_dx): dy_q [rows, >=N] e5m2 codes, wt_q
-    [experts, K, >=N] the transposed e4m3 codes of each expert's weights."""
+    [experts, K, >=N] the transposed e4m3 codes of each expert's weights, both
+    zero from N to the next multiple of 16."""
     return _experts_rows("experts_dx", "df_fp8_experts_dx", dy_q, wt_q, offsets, N, sdy, sw, out_dtype, out)
 
 
@@ -1081,7 +1089,8 @@ def experts_dw(dyt_q, xt_q, offsets, rows: int, sdy, sx, out_dtype=None, out=Non
     if dyt_q.shape[1] < rows or xt_q.shape[1] < rows:
         raise ValueError(f"{fn}: rows of {dyt_q.shape[1]} and {xt_q.shape[1]} codes, fewer than {rows}")
     N, K = dyt_q.shape[0], xt_q.shape[0]
-    _fits(fn, rows, N, K, experts, lddy, ldx)
+    if (rows | N | K | experts | lddy | ldx) > _INT_MAX:
+        _fits(fn, rows, N, K, experts, lddy, ldx)
     if out is None and out_dtype is None:
         out_dtype = torch.float32
     out, _ = _experts_out(fn, out, (experts, N, K), out_dtype, dyt_q)

@@ -95,7 +95,7 @@ tensor<T> LayerNormLayer<T>::gradient(const tensor<T>& grad_output) {
                                     " values for an input of " + std::to_string(x.size()));
     const int rows = rows_of(x);
     tensor<T> dx(x.shape());
-    // gamma's and beta's sums are fp32: behind the workspace unless T is
+    // gamma's and beta's sums, fp32 whatever T is, lie behind the workspace
     const size_t sums = affine_ ? 2 * (size_t)norm_size_ * sizeof(float) : 0;
     const size_t need = (df_layernorm_backward_workspace_bytes(rows, norm_size_) + 15) & ~(size_t)15;
     char* ws = static_cast<char*>(workspace(need + sums));
