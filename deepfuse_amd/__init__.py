@@ -21,6 +21,7 @@ import itertools
 import operator
 import os
 import re
+import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdeepfuse_amd.so")
@@ -900,6 +901,17 @@ def adamw_state(params, bits: int = 32):
             [ones(p) for p in params])
 
 
+_nearest_told = False
+
+
+def _tell_nearest(fn: str):
+    """Once a process: what 8-bit states without ``dither`` do."""
+    global _nearest_told
+    _nearest_told = True
+    warnings.warn(f"{fn}: 8-bit states rounded to nearest do not follow v where it falls (steps stay too small); "
+                  "give dither=<seed> to train", stacklevel=3)
+
+
 def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
                  m_scales=None, v_scales=None, copies=None, clip_norm=None, max_norm=0.0, absmax=None, dither=None):
     """One AdamW step (df_adamw_update) over contiguous fp32 parameters, in
@@ -920,7 +932,8 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
     for one step, but a root of v moves by at most (1 - beta2) / 2 a step, its
     codes lie 6 to 12% apart, and one that falls goes back to its code: after
     gradients have become smaller it stays too large (up to ten times after a
-    tenfold fall), and the steps too small.  A training run gives ``dither``."""
+    tenfold fall), and the steps too small.  A training run gives ``dither``;
+    the first call without it warns."""
     fn, torch = "adamw_update", _torch()
     n = len(params)
     if n == 0:
@@ -930,6 +943,8 @@ def adamw_update(params, grads, ms, vs, timestep, lr=1e-3, beta1=0.9, beta2=0.99
         raise ValueError(f"{fn}: m_scales and v_scales go together")
     if dither is not None and not eight:
         raise ValueError(f"{fn}: dither without 8-bit states")
+    if eight and dither is None and not _nearest_told:
+        _tell_nearest(fn)
     if not params[0].is_cuda:
         raise ValueError(f"{fn}: the parameters are on {params[0].device}, not on a GPU")
     gt = _in_dtype(grads[0]) if grads else DType.FLOAT32

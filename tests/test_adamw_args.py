@@ -1,6 +1,7 @@
 """Refusals of df_adamw_update, df_grad_norm and their Python forms (CPU only:
 none launches a kernel)."""
 import ctypes
+import warnings
 
 import pytest
 import torch
@@ -110,3 +111,22 @@ def test_dither_refusals():
     ok = lambda: [fake(4)]
     with pytest.raises(ValueError, match="dither"):
         df.adamw_update(ok(), ok(), ok(), ok(), 1, dither=0)
+
+
+def test_nearest_warns_once(monkeypatch):
+    """8-bit states without dither: said once; 32-bit ones and dithered ones say nothing."""
+    monkeypatch.setattr(df, "_nearest_told", False)
+    codes = lambda: [torch.zeros(4).to(torch.float8_e4m3fn).as_subclass(Fake)]
+    ok = lambda: [fake(4)]
+    bad = dict(clip_norm=1.0)  # ends the call before the library
+    run = lambda **kw: pytest.raises(TypeError, df.adamw_update, ok(), ok(), codes(), codes(), 1, m_scales=[fake(1)],
+                                     v_scales=[fake(1)], **bad, **kw)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        run(dither=0)
+        pytest.raises(TypeError, df.adamw_update, ok(), ok(), ok(), ok(), 1, **bad)
+    with pytest.warns(UserWarning, match="dither"):
+        run()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        run()
