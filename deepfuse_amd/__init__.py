@@ -18,6 +18,7 @@ import array
 import ctypes
 import enum
 import itertools
+import math
 import operator
 import os
 import re
@@ -797,6 +798,9 @@ def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, residual=None):
         s = x if residual is None else x.new_empty(shape)
         mean = x.new_empty(rows, dtype=torch.float32)
         rstd = torch.empty_like(mean)
+        if cols == 0:  # the library writes nothing; a mean over no values is none
+            mean.fill_(math.nan)
+            rstd.fill_(math.nan)
         call("df_layernorm_forward", dt, x.data_ptr(), rows, cols, ldx, _ptr(residual), ldr,
              None if residual is None else s.data_ptr(), cols, _ptr(gamma), _ptr(beta), float(eps), y.data_ptr(), cols,
              mean.data_ptr(), rstd.data_ptr(), _stream())

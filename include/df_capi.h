@@ -295,6 +295,7 @@ int df_layernorm_quantize_delayed(int dtype, const void* x, int rows, int cols, 
  *                         once.  mean and rstd (fp32 [rows]) may be NULL.
  *                         sum may be x or residual, y may be x or residual
  *                         (with its leading dimension); sum and y differ.
+ *                         No rows or no columns: nothing is written.
  *  df_layernorm_backward: with xh = (x - mean) * rstd and g = dy * gamma,
  *                         dx = rstd * (g - mean(g) - xh * mean(g * xh))
  *                         + dresidual (NULL: none; the gradient that reaches

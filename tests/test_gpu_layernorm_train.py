@@ -277,3 +277,18 @@ def test_rows_behind_the_call_stay(dev):
                 t["gamma"].data_ptr(), t["beta"].data_ptr(), 1e-5, y.data_ptr(), cols + 6, None, None, st)
         assert (y[9:] == 7).all() and (y[:, cols:] == 7).all()
         assert torch.equal(y[:9, :cols], df.layernorm_forward(t["x"], t["gamma"], t["beta"])[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_no_columns(dev, dtype):
+    """Statistics over no values are NaN, not what the memory held; no rows give empty ones."""
+    torch.full((1 << 16,), 3.0, device=dev)  # freed: what the allocator hands out next
+    for rows in (5, 300):
+        x = torch.empty(rows, 0, dtype=dtype, device=dev)
+        y, s, mean, rstd = df.layernorm_forward(x, residual=x)
+        assert y.shape == s.shape == (rows, 0) and mean.shape == rstd.shape == (rows,)
+        assert mean.isnan().all() and rstd.isnan().all()
+        dx, dg, db = df.layernorm_backward(x, s, None, mean, rstd)
+        assert dx.shape == (rows, 0) and dg.shape == db.shape == (0,)
+    y, s, mean, rstd = df.layernorm_forward(torch.empty(0, 7, dtype=dtype, device=dev))
+    assert y.shape == (0, 7) and mean.shape == rstd.shape == (0,)
