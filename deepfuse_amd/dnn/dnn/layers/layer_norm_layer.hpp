@@ -18,8 +18,9 @@
 //
 // Addition: gradient(grad_output) is the true backward, which the reference
 // lacks: the gradient of the last forward's input, with gamma's and beta's in
-// gradients() (overwritten; a FullyConnectedLayer's are too).  Training mode
-// only.
+// gradients() (overwritten; a FullyConnectedLayer's are too; zero before the
+// first call, so that an optimizer step after backward() alone moves neither).
+// Training mode only.
 //
 // The fused producer: FullyConnectedLayer::forward(input, norm) quantizes
 // LayerNorm(input) straight into the Linear's fp8 operands without

@@ -28,6 +28,8 @@ LayerNormLayer<T>::LayerNormLayer(int norm_size, float epsilon, bool affine, boo
     if (affine_) {
         gamma_.fill(static_cast<T>(1.0f));
         beta_.fill(static_cast<T>(0.0f));
+        grad_gamma_.zero();
+        grad_beta_.zero();
     }
 }
 

@@ -1137,6 +1137,21 @@ TEST_F(LayerNormLayerTest, GradientMatchesFormula) {
     check_norm_gradient<__half>(20, 64, true, 0.00048828125, upload_f16, down_f16);
 }
 
+TEST_F(LayerNormLayerTest, GradientsAreZeroBeforeGradient) {
+    for (int k = 0; k < 4; ++k) {
+        {
+            tensor<float> a({777}), b({777}), c({777}), d({777});  // freed memory that holds values
+            for (auto* t : {&a, &b, &c, &d}) t->fill(3.0f);
+        }
+        LayerNormLayer<float> ln(777, 1e-5f, true, true);
+        tensor<float> x({2, 777});
+        x.fill(1.0f);
+        ln.forward(x);
+        ln.backward(x);
+        for (auto* g : ln.gradients()) EXPECT_TRUE(download(*g) == std::vector<float>(777, 0.0f));
+    }
+}
+
 TEST_F(LayerNormLayerTest, GradientRefusals) {
     LayerNormLayer<float> eval(16), ln(16, 1e-5f, true, true);
     tensor<float> x({4, 16}), g({3, 16});
