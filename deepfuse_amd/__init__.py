@@ -1114,7 +1114,8 @@ def experts_dw(dyt_q, xt_q, offsets, rows: int, sdy, sx, out_dtype=None, out=Non
         out_dtype = torch.float32
     out, _ = _experts_out(fn, out, (experts, N, K), out_dtype, dyt_q)
     with _on(dyt_q):
-        call("df_fp8_experts_dw", dyt_q.data_ptr(), lddy, xt_q.data_ptr(), ldx, rows, N, K, experts, offsets.data_ptr(), sdy.data_ptr(), sx.data_ptr(), _in_dtype(out), out.data_ptr(), K, _stream())
+        call("df_fp8_experts_dw", dyt_q.data_ptr(), lddy, xt_q.data_ptr(), ldx, rows, N, K, experts,
+             offsets.data_ptr(), sdy.data_ptr(), sx.data_ptr(), _in_dtype(out), out.data_ptr(), K, _stream())
     return out
 
 

@@ -661,11 +661,11 @@ extern "C" int df_adamw_update(int count, const int64_t* sizes, float* const* pa
 
 extern "C" int df_adamw_update_dithered(int count, const int64_t* sizes, float* const* params, int grad_dtype,
                                         const void* const* grads, int state_dtype, void* const* m, void* const* v,
-                                        float* const* m_scale, float* const* v_scale, int copy_dtype, void* const* copies,
-                                        float lr, float beta1, float beta2, float eps, const float* weight_decay, int timestep,
-                                        const float* lr_dev, const int* timestep_dev, const float* clip_norm_dev,
-                                        float max_norm, float* absmax_dev, uint32_t seed,
-                                        void* stream) {
+                                        float* const* m_scale, float* const* v_scale, int copy_dtype,
+                                        void* const* copies, float lr, float beta1, float beta2, float eps,
+                                        const float* weight_decay, int timestep, const float* lr_dev,
+                                        const int* timestep_dev, const float* clip_norm_dev, float max_norm,
+                                        float* absmax_dev, uint32_t seed, void* stream) {
     clear_error();
     return update("df_adamw_update_dithered", true, seed, count, sizes, params, grad_dtype, grads, state_dtype, m, v,
                   m_scale, v_scale, copy_dtype, copies, lr, beta1, beta2, eps, weight_decay, timestep, lr_dev,
