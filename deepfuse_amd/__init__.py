@@ -126,6 +126,17 @@ _SIGS = {
                                    _c_int, _vp]),
     "df_fp8_experts_dw": (_c_int, [_vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp,
                                    _c_int, _vp]),
+    "df_quantize_blocks": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp, _c_int,
+                                    _vp, _c_int, _vp, _c_int, _vp]),
+    "df_fp8_gemm_blocks": (_c_int, [_c_int, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp,
+                                    _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp]),
+    "df_rmsnorm_forward": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_f, _vp, _c_int,
+                                    _vp, _vp]),
+    "df_rmsnorm_quantize": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_f, _vp, _c_int,
+                                     _vp, _c_int, _vp, _c_int, _c_int, _vp, _c_int, _vp]),
+    "df_rmsnorm_backward_workspace_bytes": (_c_sz, [_c_int, _c_int]),
+    "df_rmsnorm_backward": (_c_int, [_c_int, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _vp, _vp, _c_f, _vp, _c_int, _vp,
+                                     _c_int, _vp, _vp, _c_sz, _vp]),
     "df_fill": (_c_int, [_vp, _c_i64, _c_int, _vp, _vp]),
     "df_add": (_c_int, [_c_int, _vp, _vp, _vp, _c_i64, _vp]),
     "df_convert": (_c_int, [_c_int, _vp, _c_int, _vp, _c_i64, _vp]),
@@ -1160,3 +1171,8 @@ def quantize_experts(w, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=True):
              ptrs(q) if want_q else None, arr(ldq) if want_q else None, ptrs(qt) if want_qt else None,
              arr(ldqt) if want_qt else None, _ptr(ws), ws.numel(), _stream())
     return sc, q, qt
+
+
+# fp8 with a scale per 128 values, the root-mean-square norm
+from .blocks import (block_scales, gemm_blocks, quantize_blocks, rmsnorm_backward,  # noqa: E402,F401
+                     rmsnorm_forward, rmsnorm_quantize)

@@ -1,0 +1,250 @@
+"""fp8 codes with a scale per 128 values, and what makes and reads them: the
+quantizer, the products of a Linear, the root-mean-square norm in front of it.
+
+Codes are float8_e4m3fn or float8_e5m2 tensors whose rows start at multiples of
+16 bytes.  Scales are [blocks, rows]: scales[b, r] belongs to columns 128 b to
+128 b + 127 of row r, as float8_e8m0fnu (powers of two, which the matrix
+instructions apply by themselves) or fp32 numbers, each block's starting at a
+multiple of 16 bytes.  The calls here lay both out so; :func:`block_scales`
+brings scales from elsewhere into that form.
+"""
+from __future__ import annotations
+
+from . import (DType, Fmt, _check_gpu, _check_like, _fits, _in_dtype, _INT_MAX, _on, _plain, _ptr, _row_vector, _rows,
+               _stream, _torch, call, lib, round16)
+
+BLOCK = 128  # values that share a scale
+SCALE_F32, SCALE_E8M0 = 0, 1  # df_scale_kind
+
+
+def _kind(fn: str, dtype) -> int:
+    torch = _torch()
+    if dtype is torch.float8_e8m0fnu:
+        return SCALE_E8M0
+    if dtype is torch.float32:
+        return SCALE_F32
+    raise TypeError(f"{fn}: scales are float8_e8m0fnu or float32, not {dtype}")
+
+
+def _code_dtype(fmt):
+    torch = _torch()
+    return torch.float8_e4m3fn if Fmt(fmt) == Fmt.E4M3 else torch.float8_e5m2
+
+
+def _new_scales(like, blocks: int, rows: int, dtype):
+    """[blocks, rows], each block's at a multiple of 16 bytes."""
+    step = 16 if dtype.itemsize == 1 else 4
+    ld = -(-rows // step) * step
+    return like.new_empty((blocks, ld), dtype=dtype)[:, :rows], ld
+
+
+def _scales_ld(fn: str, name: str, s, blocks: int, rows: int, dtype) -> int:
+    """The leading dimension of scales, checked to lie as the library reads
+    them: 16 bytes at a time, the last ones of a block too."""
+    if s.shape != (blocks, rows) or s.dtype is not dtype:
+        raise ValueError(f"{fn}: {name} is {tuple(s.shape)} {s.dtype}, not {(blocks, rows)} {dtype}")
+    size = dtype.itemsize
+    need = -(-rows * size // 16) * 16 // size  # of one block
+    ld = s.stride(0) if blocks > 1 else need
+    end = s.storage_offset() + (blocks - 1) * ld + need
+    if (rows > 1 and s.stride(1) != 1 or ld < rows or ld * size % 16 or s.data_ptr() % 16
+            or end * size > s.untyped_storage().nbytes()):
+        raise ValueError(f"{fn}: {name} with strides {s.stride()} does not lie as block_scales() leaves it")
+    return ld
+
+
+def block_scales(scales, rows: int | None = None):
+    """Scales as others keep them, [rows, blocks], or for codes of ``rows``
+    rows [ceil(rows / 128), blocks] (one per 128 x 128 square), as the products
+    read them: [blocks, rows].  A copy, made once when weights are loaded."""
+    fn, torch = "block_scales", _torch()
+    _kind(fn, scales.dtype)
+    if scales.dim() != 2:
+        raise ValueError(f"{fn}: scales of {scales.dim()} dimensions, not 2")
+    raw = scales.view(torch.uint8) if scales.dtype.itemsize == 1 else scales
+    if rows is not None:
+        if raw.shape[0] != -(-rows // BLOCK):
+            raise ValueError(f"{fn}: {raw.shape[0]} rows of scales for {rows} rows of codes, 128 to a scale")
+        raw = raw.repeat_interleave(BLOCK, 0)[:rows]
+    out, _ = _new_scales(scales, raw.shape[1], raw.shape[0], scales.dtype)
+    out.view(raw.dtype).copy_(raw.t())
+    return out
+
+
+def quantize_blocks(x, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=False, square=False, scale_dtype=None):
+    """A 2-D fp32/bf16/f16 tensor [R, C] to fp8 codes with a scale per 128 values
+    (df_quantize_blocks): returns (q [R, ceil16(C)], s [ceil(C/128), R], qt [C,
+    ceil16(R)], st [ceil(R/128), C]), None where not wanted.  q shares a scale
+    among 128 columns of a row, qt among 128 rows of a column; with ``square``
+    (weights) both have one scale per 128 x 128.  Scales are powers of two
+    (float8_e8m0fnu) unless ``scale_dtype`` is float32."""
+    fn, torch = "quantize_blocks", _torch()
+    if x.dim() != 2:
+        raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
+    if not (want_q or want_qt):
+        raise ValueError(f"{fn}: no codes wanted")
+    scale_dtype = scale_dtype or torch.float8_e8m0fnu
+    kind, codes = _kind(fn, scale_dtype), _code_dtype(fmt)
+    rows, cols = x.shape
+    if (rows | cols) > _INT_MAX:
+        _fits(fn, rows, cols)
+    _check_gpu(fn, x=x)
+    ldx = cols if x.is_contiguous() else _rows(fn, "x", x, x.shape, x.dtype)
+    dt = _in_dtype(x)
+    with _on(x):
+        q = s = qt = st = None
+        ldq = lds = ldqt = ldst = 0
+        if want_q:
+            ldq = round16(cols)
+            q = x.new_empty((rows, ldq), dtype=codes)
+            s, lds = _new_scales(x, -(-cols // BLOCK), rows, scale_dtype)
+        if want_qt:
+            ldqt = round16(rows)
+            qt = x.new_empty((cols, ldqt), dtype=codes)
+            st, ldst = _new_scales(x, -(-rows // BLOCK), cols, scale_dtype)
+        if rows and cols:
+            call("df_quantize_blocks", dt, x.data_ptr(), rows, cols, ldx, int(fmt), kind, int(bool(square)), _ptr(q), ldq,
+                 _ptr(s), lds, _ptr(qt), ldqt, _ptr(st), ldst, _stream())
+    return q, s, qt, st
+
+
+def _codes(fn: str, name: str, t, red: int, formats):
+    """Format and leading dimension of an operand's codes."""
+    if t.dim() != 2 or t.dtype not in formats:
+        raise ValueError(f"{fn}: {name} {tuple(t.shape)} {t.dtype} is not a matrix of {' or '.join(map(str, formats))}")
+    rows, width = t.shape
+    ld = t.stride(0) if rows > 1 else -(-width // 16) * 16
+    if width < red or width > 1 and t.stride(1) != 1 or ld < width or ld % 16 or t.data_ptr() % 16:
+        raise ValueError(f"{fn}: {name} {tuple(t.shape)} with strides {t.stride()} has no rows of {red} codes at "
+                         "multiples of 16 bytes")
+    return ld
+
+
+def gemm_blocks(a_q, sa, b_q, sb, K: int, bias=None, out_dtype=None, out=None):
+    """C [M, N] = A . B^T with a scale per 128 of K (df_fp8_gemm_blocks): a_q [M,
+    >=K] e4m3 or e5m2 codes with scales sa [ceil(K/128), M], b_q [N, >=K] e4m3
+    codes with scales sb [ceil(K/128), N], both zero from K to the next multiple
+    of 16; plus bias [N] (fp32, bf16 or f16).  A new C is bf16 unless ``out_dtype``
+    says otherwise; ``out`` is a C to write.  With :func:`quantize_blocks`' results
+    of x [M, K], w [N, K] (square) and dy [M, N]:
+    y = gemm_blocks(xq, sx, wq, sw, K), dx = gemm_blocks(dyq, sdy, wqt, swt, N),
+    dw = gemm_blocks(dyqt, sdyt, xqt, sxt, M)."""
+    fn, torch = "gemm_blocks", _torch()
+    e4, e5 = torch.float8_e4m3fn, torch.float8_e5m2
+    if K < 0:
+        raise ValueError(f"{fn}: K = {K}")
+    lda, ldb = _codes(fn, "a_q", a_q, K, (e4, e5)), _codes(fn, "b_q", b_q, K, (e4,))
+    M, N, blocks = a_q.shape[0], b_q.shape[0], -(-K // BLOCK)
+    kind = _kind(fn, sa.dtype)
+    ldsa, ldsb = _scales_ld(fn, "sa", sa, blocks, M, sa.dtype), _scales_ld(fn, "sb", sb, blocks, N, sa.dtype)
+    _check_gpu(fn, a_q=a_q, sa=sa, b_q=b_q, sb=sb, bias=bias, out=out)
+    if (M | N | K | lda | ldb | ldsa | ldsb) > _INT_MAX:
+        _fits(fn, M, N, K, lda, ldb, ldsa, ldsb)
+    bias_dt = DType.FLOAT32
+    if bias is not None:
+        bias_dt = _in_dtype(bias)
+        _row_vector(fn, "bias", bias, N, bias.dtype)
+    with _on(a_q):
+        if out is None:
+            out, ldc = a_q.new_empty((M, N), dtype=out_dtype or torch.bfloat16), N
+        else:
+            ldc = _rows(fn, "out", out, (M, N), out_dtype or out.dtype)
+        call("df_fp8_gemm_blocks", int(Fmt.E4M3 if a_q.dtype is e4 else Fmt.E5M2), a_q.data_ptr(), lda, b_q.data_ptr(), ldb,
+             M, N, K, kind, sa.data_ptr(), ldsa, sb.data_ptr(), ldsb, int(bias_dt), _ptr(bias), int(_in_dtype(out)),
+             out.data_ptr(), ldc, _stream())
+    return out
+
+
+# ----------------------------------------------------------------------------
+# root-mean-square norm
+# ----------------------------------------------------------------------------
+def _norm_args(fn: str, x, gamma, residual):
+    if x.dim() != 2:
+        raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
+    shape, dtype, at = x.shape, x.dtype, x.get_device()
+    rows, cols = shape
+    if (rows | cols) > _INT_MAX:
+        _fits(fn, rows, cols)
+    ldx = ldr = cols
+    if not (at >= 0 and x.is_contiguous() and _plain(residual, shape, dtype, at) and _plain(gamma, (cols,), dtype, at)):
+        _check_gpu(fn, x=x, gamma=gamma, residual=residual)
+        ldx = _rows(fn, "x", x, shape, dtype)
+        ldr = cols if residual is None else _rows(fn, "residual", residual, shape, dtype)
+        _row_vector(fn, "gamma", gamma, cols, dtype)
+    return rows, cols, ldx, ldr
+
+
+def rmsnorm_forward(x, gamma=None, eps=1e-5, residual=None):
+    """Root-mean-square norm over the last dim of a 2-D fp32/bf16/f16 tensor
+    (df_rmsnorm_forward): returns (y, s, rstd), where s = x + residual is what the
+    norm saw (x itself without a residual) and rstd its rows' fp32 statistic: what
+    :func:`rmsnorm_backward` takes."""
+    fn, torch = "rmsnorm_forward", _torch()
+    rows, cols, ldx, ldr = _norm_args(fn, x, gamma, residual)
+    dt = _in_dtype(x)
+    with _on(x):
+        y = x.new_empty((rows, cols))
+        s = x if residual is None else x.new_empty((rows, cols))
+        rstd = x.new_empty(rows, dtype=torch.float32)
+        if cols == 0:  # the library writes nothing; a mean over no values is none
+            rstd.fill_(float("nan"))
+        call("df_rmsnorm_forward", dt, x.data_ptr(), rows, cols, ldx, _ptr(residual), ldr,
+             None if residual is None else s.data_ptr(), cols, _ptr(gamma), float(eps), y.data_ptr(), cols,
+             rstd.data_ptr(), _stream())
+    return y, s, rstd
+
+
+def rmsnorm_quantize(x, gamma=None, eps=1e-5, residual=None, fmt: Fmt = Fmt.E4M3, want_y=False, scale_dtype=None):
+    """:func:`rmsnorm_forward` whose output is fp8 codes with a scale per 128
+    columns, the operand of :func:`gemm_blocks` (df_rmsnorm_quantize): returns (q
+    [R, ceil16(C)], scales [ceil(C/128), R], s, rstd), with ``want_y`` y in x's type
+    behind them.  Codes come from y in fp32, not from y as rounded."""
+    fn, torch = "rmsnorm_quantize", _torch()
+    rows, cols, ldx, ldr = _norm_args(fn, x, gamma, residual)
+    scale_dtype = scale_dtype or torch.float8_e8m0fnu
+    kind, codes, dt = _kind(fn, scale_dtype), _code_dtype(fmt), _in_dtype(x)
+    ldq = round16(cols)
+    with _on(x):
+        q = x.new_empty((rows, ldq), dtype=codes)
+        sc, ldsc = _new_scales(x, -(-cols // BLOCK), rows, scale_dtype)
+        s = x if residual is None else x.new_empty((rows, cols))
+        y = x.new_empty((rows, cols)) if want_y else None
+        rstd = x.new_empty(rows, dtype=torch.float32)
+        if cols == 0:
+            rstd.fill_(float("nan"))
+        call("df_rmsnorm_quantize", dt, x.data_ptr(), rows, cols, ldx, _ptr(residual), ldr,
+             None if residual is None else s.data_ptr(), cols, _ptr(gamma), float(eps), _ptr(y), cols, rstd.data_ptr(),
+             int(fmt), q.data_ptr(), ldq, kind, sc.data_ptr(), ldsc, _stream())
+    return (q, sc, s, rstd, y) if want_y else (q, sc, s, rstd)
+
+
+def rmsnorm_backward(dy, x, gamma=None, rstd=None, eps=1e-5, dresidual=None, sums=True):
+    """The gradients of :func:`rmsnorm_forward` (df_rmsnorm_backward), x being what
+    the norm saw: returns (dx, dgamma), the last in fp32 (None with
+    ``sums=False``).  Without rstd it is taken from x at eps again.  ``dresidual``
+    (the gradient that reaches the residual stream past the norm) is added to dx."""
+    fn, torch = "rmsnorm_backward", _torch()
+    if x.dim() != 2:
+        raise ValueError(f"{fn}: x has {x.dim()} dimensions, not 2")
+    shape, dtype, at = x.shape, x.dtype, x.get_device()
+    rows, cols = shape
+    if (rows | cols) > _INT_MAX:
+        _fits(fn, rows, cols)
+    ldx = lddy = lddr = cols
+    if not (at >= 0 and x.is_contiguous() and _plain(dy, shape, dtype, at) and _plain(dresidual, shape, dtype, at)
+            and _plain(gamma, (cols,), dtype, at) and _plain(rstd, (rows,), torch.float32, at)):
+        _check_gpu(fn, dy=dy, x=x, gamma=gamma, rstd=rstd, dresidual=dresidual)
+        ldx, lddy = _rows(fn, "x", x, shape, dtype), _rows(fn, "dy", dy, shape, dtype)
+        lddr = cols if dresidual is None else _rows(fn, "dresidual", dresidual, shape, dtype)
+        _row_vector(fn, "gamma", gamma, cols, dtype)
+        _row_vector(fn, "rstd", rstd, rows, torch.float32)
+    dt = _in_dtype(x)
+    with _on(x):
+        dx = x.new_empty(shape)
+        dg = x.new_empty(cols, dtype=torch.float32) if sums else None
+        # not a cached one: a captured graph keeps the workspace it was given
+        nws = lib().df_rmsnorm_backward_workspace_bytes(rows, cols)
+        ws = x.new_empty(nws, dtype=torch.uint8)
+        call("df_rmsnorm_backward", dt, dy.data_ptr(), lddy, x.data_ptr(), ldx, rows, cols, _ptr(gamma), _ptr(rstd),
+             float(eps), _ptr(dresidual), lddr, dx.data_ptr(), cols, _ptr(dg), ws.data_ptr(), nws, _stream())
+    return dx, dg

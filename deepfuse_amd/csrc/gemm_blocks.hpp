@@ -1,0 +1,56 @@
+// gemm_blocks.hpp -- what the products with a scale per 128 of the reduction share
+// (gemm_blocks.hip: entry point, plan and small tiles; gemm_blocks_tiles.hip: large
+// tiles).
+#pragma once
+
+#include "block_scale.hpp"
+#include "df_common.hpp"
+#include "gemm_common.hpp"
+
+namespace dfk {
+
+// C [M, ldc] = sum over blocks b of sa[b][m] * sb[b][n] * (A . B^T over block b) + bias;
+// A [M, lda], B [N, ldb], K rounded up to 16, scales [blocks][ldsa / ldsb].
+struct BlocksArgs {
+    const uint8_t* A;
+    const uint8_t* B;
+    void* C;
+    const void* sa;
+    const void* sb;
+    const void* bias;
+    int lda, ldb, ldc, ldsa, ldsb, M, N, K, bias_dtype, vec_out;
+};
+
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+
+// eight codes -> bf16, times the power of two `scale` (exact while the result is
+// in bf16's range)
+template <int FMT> __device__ __forceinline__ bf8 widen8_scaled(uint32_t lo, uint32_t hi, float scale) {
+    bf2 p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i < 2 ? lo : hi;
+        if constexpr (FMT == E4M3)
+            p[i] = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true)
+                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false);
+        else
+            p[i] = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, scale, true)
+                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, scale, false);
+    }
+    return bf8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+}
+
+// bytes of `blocks` blocks' scales of a matrix of `rows` rows: what may be read
+inline int64_t scales_extent(int64_t blocks, int64_t ld, int64_t rows, int bytes) {
+    const int64_t row = (rows * bytes + 15) & ~(int64_t)15;
+    return blocks == 0 ? 0 : (blocks - 1) * ld * bytes + row;
+}
+
+__device__ __forceinline__ float bias_at(const void* bias, int dtype, int i) {
+    if (dtype == DF_DTYPE_FLOAT32) return bias_ld(static_cast<const float*>(bias), i);
+    if (dtype == DF_DTYPE_HALF) return bias_ld(static_cast<const f16_t*>(bias), i);
+    return bias_ld(static_cast<const uint16_t*>(bias), i);
+}
+
+}  // namespace dfk

@@ -47,6 +47,10 @@ typedef enum {
 /* ---- fp8 formats (OCP OFP8 v1.0) ---- */
 typedef enum { DF_FMT_E4M3 = 0, DF_FMT_E5M2 = 1 } df_fp8_format;
 
+/* ---- kinds of scales where 128 values share one (df_quantize_blocks): fp32,
+ * or a power of two as its biased exponent, 2^(byte - 127) in one byte ---- */
+typedef enum { DF_SCALE_F32 = 0, DF_SCALE_E8M0 = 1 } df_scale_kind;
+
 /* ---- element types: values 0-4 are the reference's own enum
  * OnnxLoader::DType (dnn/utils/onnx_loader.cuh:16-22); 5 and 6 extend it
  * with the two 1-byte fp8 formats; 7 is int32 (the reference's tensor<int>,
@@ -509,6 +513,76 @@ int df_fp8_experts_dx(const uint8_t* dYq, int lddy, const uint8_t* Wtq, int ldwt
 int df_fp8_experts_dw(const uint8_t* dYtq, int lddyt, const uint8_t* Xtq, int ldxt, int rows, int N,
                       int K, int experts, const int* offsets_dev, const float* sdy_dev,
                       const float* sx_dev, int dw_dtype, void* dW, int lddw, void* stream);
+
+/* ---- fp8 with a scale per 128 values (new: the reference has no fp8) ----
+ * Scales lie as the products read them, blocks of the reduction first: a matrix
+ * of codes [rows, ld] that is reduced over its columns has scales [ceil(cols /
+ * 128)][ld_scales], the one of row r and columns 128 b .. 128 b + 127 at b *
+ * ld_scales + r.  ld_scales * (4 or 1 bytes) is a multiple of 16, the pointer
+ * 16-byte aligned, and each block's scales are readable up to the next multiple of
+ * 16 bytes (of any value).  Kinds (df_scale_kind):
+ *   DF_SCALE_F32  : absmax / FMAX, 1 where the absmax is 0 (rule D1/D2 of a block).
+ *   DF_SCALE_E8M0 : the smallest power of two that keeps absmax / s <= FMAX, as
+ *                   2^(byte - 127), at least 2^-127; 1 (byte 127) where the absmax
+ *                   is 0.  x / s is exact.  Byte 255 is no scale.
+ * absmax is over finite values; codes as for a whole tensor (top of this file).
+ *
+ * df_quantize_blocks: x [rows, ldx] (fp32, bf16 or f16, at any element's address)
+ * to row codes q [rows, ldq] with scales [ceil(cols/128)][ld_scales], and / or
+ * transposed codes qt [cols, ldqt] with scales_t [ceil(rows/128)][ld_scales_t],
+ * whose blocks are 128 rows of a column; either pair may be NULL.  square: one
+ * scale per 128 x 128 (weights: both kinds of codes then stand for the same
+ * values), written for each of its rows (columns) all the same.  Codes are zero
+ * up to the next multiple of 16 columns (rows).  At most 128 * 65535 rows. */
+int df_quantize_blocks(int dtype, const void* x, int rows, int cols, int ldx, int fmt, int scale_kind, int square,
+                       uint8_t* q, int ldq, void* scales, int ld_scales,
+                       uint8_t* qt, int ldqt, void* scales_t, int ld_scales_t, void* stream);
+
+/* Products on such codes (forward, dX and dW of a Linear):
+ *   C[m][n] = sum over blocks b of 128 of K of sa[b][m] * sb[b][n] * (sum over k
+ *             in b of A[m][k] * B[n][k]) + bias[n]
+ * A [M, lda] in fmt_a (e4m3 or e5m2), B [N, ldb] e4m3, codes zero from K up to the
+ * next multiple of 16; leading dimensions multiples of 16 below 2^23, 16-byte
+ * aligned; scales of one kind, sa [ceil(K/128)][ldsa] and sb [ceil(K/128)][ldsb],
+ * as above, each below 2^31 bytes.  bias (fp32, bf16 or f16, [N]) may be NULL.  C
+ * fp32, bf16 or f16, rounded once from fp32 accumulation; an fp32 one is the fp32
+ * sum of exact products (bf16 matrix instructions), a 2-byte one takes the fp8
+ * ones (see df_fp8_experts_fwd).  K == 0 gives the bias, or 0.
+ *   forward : Xq, sx (row codes) and Wq, sw      ; M tokens, N outputs, K inputs
+ *   dX      : dYq, sdy (row codes) and Wtq, swt  ; M tokens, N inputs, K outputs
+ *   dW      : dYtq, sdyt and Xtq, sxt            ; M outputs, N inputs, K tokens */
+int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const uint8_t* B, int ldb, int M, int N, int K,
+                       int scale_kind, const void* sa, int ldsa, const void* sb, int ldsb, int bias_dtype,
+                       const void* bias, int c_dtype, void* C, int ldc, void* stream);
+
+/* ---- root-mean-square norm (new: the reference has LayerNorm only,
+ * dnn/layers/layer_norm_layer.cu:26-90) ----
+ * Rows of cols values in dtype (fp32, bf16, f16), at any element's address:
+ *  df_rmsnorm_forward : s = x + residual rounded to dtype (s = x without one),
+ *     rstd = 1 / sqrt(mean(s^2) + eps), y = s * rstd * gamma.  residual and gamma
+ *     may be NULL (gamma 1); sum (needs a residual) receives s, rstd (float[rows])
+ *     the statistic; either may be NULL.  sum and y may lie over x or the
+ *     residual with the same leading dimension (not both over one).
+ *  df_rmsnorm_quantize: the same y as fp8 codes q [rows, ldq], zero up to the next
+ *     multiple of 16, with a scale per 128 columns (scales as
+ *     df_quantize_blocks's, from y in fp32); y itself is written too unless NULL.
+ *     q and scales lie over no other argument.
+ *  df_rmsnorm_backward: with xh = x * rstd, g = dy * gamma (x being what the norm
+ *     saw): dx = rstd * (g - xh * mean(g * xh)) + dresidual, dgamma[cols] =
+ *     sum over rows of dy * xh (fp32; NULL: not wanted).  rstd NULL: taken from x
+ *     at eps again.  dx may lie over dy, x or dresidual with the same leading
+ *     dimension.  ws: df_rmsnorm_backward_workspace_bytes(rows, cols), 16-byte
+ *     aligned.  rows == 0 gives dgamma = 0. */
+int df_rmsnorm_forward(int dtype, const void* x, int rows, int cols, int ldx, const void* residual, int ldr,
+                       void* sum, int lds, const void* gamma, float eps, void* y, int ldy, float* rstd,
+                       void* stream);
+int df_rmsnorm_quantize(int dtype, const void* x, int rows, int cols, int ldx, const void* residual, int ldr,
+                        void* sum, int lds, const void* gamma, float eps, void* y, int ldy, float* rstd,
+                        int fmt, uint8_t* q, int ldq, int scale_kind, void* scales, int ld_scales, void* stream);
+size_t df_rmsnorm_backward_workspace_bytes(int rows, int cols);
+int df_rmsnorm_backward(int dtype, const void* dy, int lddy, const void* x, int ldx, int rows, int cols,
+                        const void* gamma, const float* rstd, float eps, const void* dresidual, int lddr,
+                        void* dx, int lddx, float* dgamma, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- layer weight streaming (new: the reference describes layer-serialized
  * execution, README.md:212-226, and has its host-side pieces in the NVMe
