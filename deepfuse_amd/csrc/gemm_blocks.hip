@@ -205,6 +205,38 @@ template <int FA, bool E8, bool WIDE> void launch_small(const BlocksArgs& g, int
         blocks_small_kernel<FA, E8, WIDE, 2, 2, 4, 2><<<tiles(32, 32), 256, 0, st>>>(g, c_dtype, ea, eb);
 }
 
+// Which kernel a call takes, by the time each would take, in us; a step is 128 of
+// K.  Large tiles: rounds of blocks over the CUs.
+struct BlocksPlan {
+    int fm;  // 0: small tiles
+    int grid;
+};
+BlocksPlan plan(const BlocksArgs& g, bool e8, bool wide) {
+    const int cus = std::max(device_cu_count(), 1);
+    const double steps = (double)((g.K + 127) / 128);
+    auto tiles = [&](int r, int c) { return (int64_t)((g.M + r - 1) / r) * ((g.N + c - 1) / c); };
+    double best = 4.0 + 0.12 * steps + 0.35e-3 * (double)tiles(32, 32) * (steps + 10.0);
+    BlocksPlan p{0, 0};
+    if (g.K == 0) return p;
+    auto offer = [&](int fm, int r, int c, double step, double over) {
+        const int64_t n = tiles(r, c), rounds = (n + cus - 1) / cus;
+        const double t = 5.0 + (double)rounds * (wide ? 2.05 : 1.0) * (step * steps + over);
+        if (t < best) {
+            best = t;
+            p = {fm, (int)std::min<int64_t>(n, cus)};
+        }
+    };
+    if (e8) {
+        offer(4, 256, 256, 1.2, 3.6);
+        offer(2, 256, 128, 0.72, 2.4);
+        offer(1, 128, 128, 0.5, 1.8);
+    } else {
+        offer(2, 256, 128, 1.1, 2.4);
+        offer(1, 128, 128, 0.7, 1.8);
+    }
+    return p;
+}
+
 }  // namespace
 
 }  // namespace dfk
@@ -243,10 +275,16 @@ extern "C" int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const ui
     DF_CHECK(ea < (1ll << 31) && eb < (1ll << 31), DF_ERR_UNSUPPORTED, "%s: scales of 2^31 bytes or more", fn);
     BlocksArgs g{A, B, C, sa, sb, bias, lda, ldb, ldc, ldsa, ldsb, M, N, (K + 15) & ~15, bias_dtype, 0};
     const int64_t ldc_bytes = (int64_t)ldc * (c_dtype == DF_DTYPE_FLOAT32 ? 4 : 2);
-    g.vec_out = ldc_bytes % 16 == 0 && aligned16(C);
     if (K == 0) g.lda = g.ldb = g.ldsa = g.ldsb = 0;  // (not checked then, and nothing is read)
     const hipStream_t st = as_stream(stream);
     const bool wide = c_dtype == DF_DTYPE_FLOAT32, e8 = scale_kind == DF_SCALE_E8M0;
+    const BlocksPlan p = plan(g, e8, wide);
+    if (p.fm) {
+        g.vec_out = epi_store_mode(C, ldc_bytes);
+        launch_block_tiles(fmt_a, e8, p.fm, c_dtype, g, (int)ea, (int)eb, p.grid, st);
+        return launch_status(fn);
+    }
+    g.vec_out = ldc_bytes % 16 == 0 && aligned16(C);
     auto go = [&](auto fa, auto e, auto wd) {
         launch_small<decltype(fa)::value, decltype(e)::value, decltype(wd)::value>(g, c_dtype, (int)ea, (int)eb, st);
     };

@@ -53,4 +53,9 @@ __device__ __forceinline__ float bias_at(const void* bias, int dtype, int i) {
     return bias_ld(static_cast<const uint16_t*>(bias), i);
 }
 
+// gemm_blocks_tiles.hip: the persistent kernel on 256 x 256 (fm 4, power-of-two
+// scales only), 256 x 128 (2) or 128 x 128 tiles (1); vec_out: an epi_store_mode.
+void launch_block_tiles(int fmt_a, bool e8, int fm, int c_dtype, const BlocksArgs& g, int extent_a, int extent_b, int grid,
+                        hipStream_t st);
+
 }  // namespace dfk
