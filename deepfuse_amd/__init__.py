@@ -130,6 +130,10 @@ _SIGS = {
                                     _vp, _c_int, _vp, _c_int, _vp]),
     "df_fp8_gemm_blocks": (_c_int, [_c_int, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp,
                                     _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp]),
+    "df_moe_layer_workspace_bytes": (_c_sz, [_c_int, _c_int, _c_int]),
+    "df_moe_layer": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _c_int,
+                              _vp, _c_int, _vp, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp,
+                              _c_sz, _vp]),
     "df_rmsnorm_forward": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_f, _vp, _c_int,
                                     _vp, _vp]),
     "df_rmsnorm_quantize": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_f, _vp, _c_int,
@@ -1174,5 +1178,5 @@ def quantize_experts(w, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=True):
 
 
 # fp8 with a scale per 128 values, the root-mean-square norm
-from .blocks import (block_scales, gemm_blocks, quantize_blocks, rmsnorm_backward,  # noqa: E402,F401
-                     rmsnorm_forward, rmsnorm_quantize)
+from .blocks import (block_scales, gemm_blocks, moe_layer, quantize_blocks, quantize_experts_blocks,  # noqa: E402,F401
+                     rmsnorm_backward, rmsnorm_forward, rmsnorm_quantize)

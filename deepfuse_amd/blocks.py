@@ -156,6 +156,100 @@ def gemm_blocks(a_q, sa, b_q, sb, K: int, bias=None, out_dtype=None, out=None):
 
 
 # ----------------------------------------------------------------------------
+# a mixture-of-experts layer for a few tokens
+# ----------------------------------------------------------------------------
+ACTIVATIONS = {"swiglu": 0, "geglu": 1, "gelu": 2}  # df_activation
+
+
+def quantize_experts_blocks(w, scale_dtype=None):
+    """Experts' weights w [experts, R, C] (fp32, bf16 or float16) to e4m3 codes with a
+    scale per 128 x 128: returns (q [experts, R, ceil16(C)], s [experts, ceil(C/128),
+    R]), as :func:`moe_layer` takes them."""
+    fn, torch = "quantize_experts_blocks", _torch()
+    if w.dim() != 3 or not w.is_contiguous():
+        raise ValueError(f"{fn}: w {tuple(w.shape)} is not [experts, R, C] and contiguous")
+    scale_dtype = scale_dtype or torch.float8_e8m0fnu
+    kind = _kind(fn, scale_dtype)
+    _check_gpu(fn, w=w)
+    E, R, C = w.shape
+    _fits(fn, E, R, C)
+    dt = _in_dtype(w)
+    with _on(w):
+        q = w.new_empty((E, R, round16(C)), dtype=torch.float8_e4m3fn)
+        step = 16 // scale_dtype.itemsize
+        ld = -(-R // step) * step
+        s = w.new_empty((E, -(-C // BLOCK), ld), dtype=scale_dtype)
+        for e in range(E if R and C else 0):
+            call("df_quantize_blocks", dt, w[e].data_ptr(), R, C, C, int(Fmt.E4M3), kind, 1, q[e].data_ptr(), q.shape[2],
+                 s[e].data_ptr(), ld, None, 0, None, 0, _stream())
+    return q, s[:, :, :R]
+
+
+def _expert_weights(fn: str, n: int, w, s, rows: int, cols: int, experts: int):
+    """Leading dimensions of experts' codes and scales, checked."""
+    torch = _torch()
+    if w.dim() != 3 or w.dtype is not torch.float8_e4m3fn or w.shape[0] != experts or w.shape[1] != rows or w.shape[2] < cols:
+        raise ValueError(f"{fn}: w{n} is {tuple(w.shape)} {w.dtype}, not e4m3 codes of {(experts, rows, cols)}")
+    ldw = w.stride(1) if rows > 1 else w.stride(0) if experts > 1 else -(-w.shape[2] // 16) * 16
+    if (w.shape[2] > 1 and w.stride(2) != 1 or ldw < w.shape[2] or ldw % 16 or w.data_ptr() % 16
+            or experts > 1 and w.stride(0) != rows * ldw):
+        raise ValueError(f"{fn}: w{n} with strides {w.stride()} has no rows at multiples of 16 bytes, expert behind expert")
+    blocks, size = -(-cols // BLOCK), s.dtype.itemsize
+    if s.dim() != 3 or s.shape != (experts, blocks, rows):
+        raise ValueError(f"{fn}: s{n} is {tuple(s.shape)}, not {(experts, blocks, rows)}")
+    need = -(-rows * size // 16) * 16 // size
+    lds = s.stride(1) if blocks > 1 else s.stride(0) if experts > 1 else need
+    end = s.storage_offset() + (experts * blocks - 1) * lds + need
+    if (rows > 1 and s.stride(2) != 1 or lds < rows or lds * size % 16 or s.data_ptr() % 16
+            or experts > 1 and s.stride(0) != blocks * lds or end * size > s.untyped_storage().nbytes()):
+        raise ValueError(f"{fn}: s{n} with strides {s.stride()} does not lie as quantize_experts_blocks() leaves it")
+    return ldw, lds
+
+
+def moe_layer(x, logits, w1, s1, w2, s2, top_k: int, activation: str = "swiglu", renormalize: bool = True):
+    """A whole mixture-of-experts layer for a few tokens (df_moe_layer): x [T, H] bf16
+    or float16, T <= 64, logits [T, experts] of the router (fp32, bf16 or float16), w1
+    [experts, 2 N, >=H] (gate's rows, then up's; [experts, N, >=H] for "gelu") and w2
+    [experts, H, >=N] e4m3 codes with scales s1, s2 (:func:`quantize_experts_blocks`).
+    Each token goes to the ``top_k`` experts of its largest logits, weighted by the
+    softmax over them (over all experts without ``renormalize``); a logit of -inf or NaN
+    is never chosen.  Returns (y [T, H], ids int32 [T, top_k], weights fp32 [T, top_k]);
+    an id is -1 where no expert was left."""
+    fn, torch = "moe_layer", _torch()
+    if x.dim() != 2 or logits.dim() != 2 or logits.shape[0] != x.shape[0]:
+        raise ValueError(f"{fn}: x {tuple(x.shape)} and logits {tuple(logits.shape)} are not [tokens, H] and [tokens, experts]")
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{fn}: x is {x.dtype}, not bfloat16 or float16")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{fn}: activation {activation!r} is none of {', '.join(ACTIVATIONS)}")
+    (tokens, H), experts = x.shape, logits.shape[1]
+    N = w2.shape[-1] if w2.dim() == 3 else 0
+    if w1.dim() == 3:  # w2's rows may be padded, w1's are not
+        N = w1.shape[1] if activation == "gelu" else w1.shape[1] // 2
+    _check_gpu(fn, x=x, logits=logits, w1=w1, s1=s1, w2=w2, s2=s2)
+    kind = _kind(fn, s1.dtype)
+    if s2.dtype is not s1.dtype:
+        raise ValueError(f"{fn}: s1 is {s1.dtype} and s2 {s2.dtype}")
+    ldw1, lds1 = _expert_weights(fn, 1, w1, s1, N if activation == "gelu" else 2 * N, H, experts)
+    ldw2, lds2 = _expert_weights(fn, 2, w2, s2, H, N, experts)
+    ldx, ldl = _rows(fn, "x", x, x.shape, x.dtype), _rows(fn, "logits", logits, logits.shape, logits.dtype)
+    dt, lt = _in_dtype(x), _in_dtype(logits)
+    if max(H, 2 * N, ldw1, ldw2, lds1, lds2) > _INT_MAX:
+        _fits(fn, H, 2 * N, ldw1, ldw2, lds1, lds2)
+    with _on(x):
+        y = x.new_empty((tokens, H))
+        ids = x.new_empty((tokens, top_k), dtype=torch.int32)
+        weights = x.new_empty((tokens, top_k), dtype=torch.float32)
+        # not a cached one: a captured graph keeps the workspace it was given
+        nws = lib().df_moe_layer_workspace_bytes(tokens, top_k, N)
+        ws = x.new_empty(nws, dtype=torch.uint8)
+        call("df_moe_layer", dt, x.data_ptr(), ldx, tokens, H, N, experts, top_k, lt, logits.data_ptr(), ldl,
+             int(bool(renormalize)), ACTIVATIONS[activation], w1.data_ptr(), ldw1, w2.data_ptr(), ldw2, kind, s1.data_ptr(),
+             lds1, s2.data_ptr(), lds2, y.data_ptr(), H, ids.data_ptr(), weights.data_ptr(), ws.data_ptr(), nws, _stream())
+    return y, ids, weights
+
+
+# ----------------------------------------------------------------------------
 # root-mean-square norm
 # ----------------------------------------------------------------------------
 def _norm_args(fn: str, x, gamma, residual):

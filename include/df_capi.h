@@ -555,6 +555,36 @@ int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const uint8_t* B, i
                        int scale_kind, const void* sa, int ldsa, const void* sb, int ldsb, int bias_dtype,
                        const void* bias, int c_dtype, void* C, int ldc, void* stream);
 
+/* ---- a mixture-of-experts layer for a few tokens (new: the reference has no
+ * mixture of experts) ----
+ *   ids[t][j]     = the expert with the j-th largest of token t's logits (ties: the
+ *                   lower index), j < top_k
+ *   weights[t][j] = softmax of those logits, over the chosen (renormalize) or over
+ *                   all experts
+ *   y[t] = sum over j of weights[t][j] * W2[e] . act(W1[e] . x[t]),  e = ids[t][j]
+ * An expert whose logit is -infinity or NaN is not chosen: where fewer than top_k can
+ * be, the id is -1 and the weight 0; a token without experts gives 0.
+ *  x [tokens, ldx] bf16 or f16 (dtype), y [tokens, ldy] likewise: H values a token.
+ *  logits [tokens, ld_logits] in logits_dtype (fp32, bf16, f16).
+ *  act: DF_ACT_SWIGLU silu(g) * u, DF_ACT_GEGLU gelu(g) * u, with g the first N and u
+ *      the last N of W1's 2 N rows; DF_ACT_GELU with W1's N rows.  gelu is the tanh form.
+ *  W1 [experts][2 N or N][ldw1], W2 [experts][H][ldw2]: e4m3 codes, zero from H (N) up
+ *      to the next multiple of 16; s1 [experts][ceil(H/128)][lds1], s2 [experts]
+ *      [ceil(N/128)][lds2], scales as df_quantize_blocks's row codes', each expert's
+ *      behind the one before.
+ * Sums in fp32, the inner values kept to 16 bits of significand, y rounded once.
+ * At most 64 tokens, 256 experts, top_k 16, and 2^31 bytes of codes an expert.
+ * y and ids, weights [tokens * top_k] overlap no input.  ws:
+ * df_moe_layer_workspace_bytes(tokens, top_k, N), 16-byte aligned (0: sizes not
+ * taken).  Two launches for one token, three for more. */
+typedef enum { DF_ACT_SWIGLU = 0, DF_ACT_GEGLU = 1, DF_ACT_GELU = 2 } df_activation;
+size_t df_moe_layer_workspace_bytes(int tokens, int top_k, int N);
+int df_moe_layer(int dtype, const void* x, int ldx, int tokens, int H, int N, int experts, int top_k,
+                 int logits_dtype, const void* logits, int ld_logits, int renormalize, int act,
+                 const uint8_t* W1, int ldw1, const uint8_t* W2, int ldw2, int scale_kind, const void* s1, int lds1,
+                 const void* s2, int lds2, void* y, int ldy, int* ids, float* weights, void* ws, size_t ws_bytes,
+                 void* stream);
+
 /* ---- root-mean-square norm (new: the reference has LayerNorm only,
  * dnn/layers/layer_norm_layer.cu:26-90) ----
  * Rows of cols values in dtype (fp32, bf16, f16), at any element's address:
