@@ -130,7 +130,7 @@ _SIGS = {
                                     _vp, _c_int, _vp, _c_int, _vp]),
     "df_fp8_gemm_blocks": (_c_int, [_c_int, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp,
                                     _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp]),
-    "df_moe_layer_workspace_bytes": (_c_sz, [_c_int, _c_int, _c_int]),
+    "df_moe_layer_workspace_bytes": (_c_sz, [_c_int] * 5),
     "df_moe_layer": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _c_int,
                               _vp, _c_int, _vp, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp,
                               _c_sz, _vp]),

@@ -241,7 +241,7 @@ def moe_layer(x, logits, w1, s1, w2, s2, top_k: int, activation: str = "swiglu",
         ids = x.new_empty((tokens, top_k), dtype=torch.int32)
         weights = x.new_empty((tokens, top_k), dtype=torch.float32)
         # not a cached one: a captured graph keeps the workspace it was given
-        nws = lib().df_moe_layer_workspace_bytes(tokens, top_k, N)
+        nws = lib().df_moe_layer_workspace_bytes(tokens, H, N, experts, top_k)
         ws = x.new_empty(nws, dtype=torch.uint8)
         call("df_moe_layer", dt, x.data_ptr(), ldx, tokens, H, N, experts, top_k, lt, logits.data_ptr(), ldl,
              int(bool(renormalize)), ACTIVATIONS[activation], w1.data_ptr(), ldw1, w2.data_ptr(), ldw2, kind, s1.data_ptr(),

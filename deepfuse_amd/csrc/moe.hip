@@ -42,17 +42,22 @@ namespace {
 
 constexpr int kMoeTokens = 64, kMoeExperts = 256, kMoeTop = 16;
 constexpr int kMoePairs = kMoeTokens * kMoeTop;
-constexpr int kMoeUnits = kMoePairs / 16 + kMoeExperts;  // more than there can be
+constexpr int kMoeUnits = kMoePairs / 4 + kMoeExperts;  // more than there can be, of either size
 constexpr uint32_t kOOB = 0x80000000u;
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
-// What routing leaves for the products, at the workspace's start.
+// What routing leaves for the products, at the workspace's start: the pairs t * top + j
+// by expert, then token, and lists of units, an expert's next few of them, for either
+// product.
+struct MoeUnits {
+    int n;
+    int expert[kMoeUnits], first[kMoeUnits], count[kMoeUnits];  // (first: in `sorted`)
+};
 struct MoePlan {
-    int units;
-    int expert[kMoeUnits], first[kMoeUnits], count[kMoeUnits];  // a unit's expert, its pairs in `sorted`
-    int sorted[kMoePairs];                                      // pairs t * top + j by expert, then token
+    MoeUnits up, down;
+    int sorted[kMoePairs];
 };
 
 struct MoeArgs {
@@ -61,7 +66,8 @@ struct MoeArgs {
     void* y; int* ids; float* weights;
     MoePlan* plan;
     uint16_t* hi; uint16_t* lo;  // [pairs][ldh] bf16
-    int tokens, H, N, experts, top, ldx, ldl, ldy, ldw1, ldw2, lds1, lds2, ldh, act, renormalize, x_dtype, l_dtype;
+    float* part; int* arrived;   // W2 split: [splits][tokens][H16] sums, blocks done per column tile
+    int tokens, H, N, experts, top, ldx, ldl, ldy, ldw1, ldw2, lds1, lds2, ldh, act, renormalize, x_dtype, l_dtype, splits, up_size, down_size;
 };
 
 // ------------------------------------------------------------------ routing --
@@ -71,28 +77,32 @@ __device__ __forceinline__ float load_as_float(const void* p, int dtype, int64_t
     return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
 }
 
-template <typename F> __device__ __forceinline__ uint32_t wave_fold(uint32_t v, const F& f) {
-#define DF_FOLD(CTRL) v = f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xF, 0xF, false))
-    DF_FOLD(0x111);  // row_shr:1 .. 8, then row_bcast:15 and :31: lane 63 has the wave's
-    DF_FOLD(0x112);
-    DF_FOLD(0x114);
-    DF_FOLD(0x118);
-    DF_FOLD(0x142);
-    DF_FOLD(0x143);
+// f over the 16 lanes of a DPP row, the same in each of them (a butterfly: quad_perm
+// by 1 and 2, row_half_mirror, row_mirror)
+template <typename T, typename F> __device__ __forceinline__ T row_fold(T v, const F& f) {
+#define DF_FOLD(CTRL) \
+    v = f(v, __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true)))
+    DF_FOLD(0xB1);
+    DF_FOLD(0x4E);
+    DF_FOLD(0x141);
+    DF_FOLD(0x140);
 #undef DF_FOLD
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    return v;
 }
 
-// One wave: token t's choices, the j-th in lane j: its expert and weight, -1 and 0
-// where no more can be chosen (an expert whose logit is -infinity or NaN is none).
-__device__ __forceinline__ void route_token(const MoeArgs& a, int t, int lane, int& id, float& weight) {
-    constexpr int PER = kMoeExperts / 64;
+// 16 lanes (g: the lane among them): token t's choices, the j-th in lane j: its
+// expert and weight, -1 and 0 where no more can be chosen (an expert whose logit is
+// -infinity or NaN is none; tokens from a.tokens on have none).  PER: logits a lane.
+template <int PER> __device__ __forceinline__ void route_token(const MoeArgs& a, int t, int g, int& id, float& weight) {
     float v[PER];
     uint32_t key[PER];  // order of the values; 0: cannot be chosen
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int e = lane + 64 * i;
-        v[i] = e < a.experts ? load_as_float(a.logits, a.l_dtype, (int64_t)t * a.ldl + e) : -__builtin_inff();
+        const int e = g + 16 * i;
+        v[i] = e < a.experts && t < a.tokens ? load_as_float(a.logits, a.l_dtype, (int64_t)t * a.ldl + e) : -__builtin_inff();
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
         const float z = v[i] == 0.0f ? 0.0f : v[i];  // -0 is 0
         const uint32_t u = __float_as_uint(z);
         key[i] = z > -__builtin_inff() ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;  // (NaN fails the test)
@@ -103,20 +113,19 @@ __device__ __forceinline__ void route_token(const MoeArgs& a, int t, int lane, i
         uint32_t best = key[0];
 #pragma unroll
         for (int i = 1; i < PER; ++i) best = max(best, key[i]);
-        best = wave_fold(best, [](uint32_t x, uint32_t y) { return max(x, y); });
-        if (best == 0) break;
+        best = row_fold(best, [](uint32_t x, uint32_t y) { return max(x, y); });
         uint32_t who = 0xFFFFFFFFu;
 #pragma unroll
-        for (int i = PER - 1; i >= 0; --i) who = key[i] == best ? (uint32_t)(lane + 64 * i) : who;
-        who = wave_fold(who, [](uint32_t x, uint32_t y) { return min(x, y); });
+        for (int i = PER - 1; i >= 0; --i) who = key[i] == best ? (uint32_t)(g + 16 * i) : who;
+        who = row_fold(who, [](uint32_t x, uint32_t y) { return min(x, y); });
         if (j == 0) first = best;
-        if (lane == j) {
+        if (g == j && best) {
             id = (int)who;
             mine = best;
         }
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if ((uint32_t)(lane + 64 * i) == who) key[i] = 0;
+            if ((uint32_t)(g + 16 * i) == who) key[i] = 0;
     }
     auto value = [](uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); };
     const float most = value(first);
@@ -130,25 +139,29 @@ __device__ __forceinline__ void route_token(const MoeArgs& a, int t, int lane, i
         for (int i = 0; i < PER; ++i)
             if (v[i] > -__builtin_inff()) sum += part(v[i]);
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, 64);
+    sum = row_fold(sum, [](float x, float y) { return x + y; });
     weight = id >= 0 ? own / sum : 0.0f;
+}
+__device__ __forceinline__ void route_any(const MoeArgs& a, int t, int g, int& id, float& weight) {
+    if (a.experts <= 64) route_token<4>(a, t, g, id, weight);
+    else route_token<kMoeExperts / 16>(a, t, g, id, weight);
 }
 
 // One block: every token's choices, then the plan.
 __global__ __launch_bounds__(1024) void moe_route_kernel(const MoeArgs a) {
     __shared__ int ids[kMoePairs];
     __shared__ uint32_t taken[kMoeExperts][kMoeTokens / 32];  // which tokens take an expert
-    __shared__ int start[kMoeExperts], at_wave[2][4];
+    __shared__ int start[kMoeExperts], at_wave[3][4];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < kMoeExperts * (kMoeTokens / 32); i += 1024) (&taken[0][0])[i] = 0;
     __syncthreads();
-    for (int t = w; t < a.tokens; t += 16) {
+    {
+        const int t = threadIdx.x >> 4, g = threadIdx.x & 15;  // 64 tokens at once
         int e;
         float weight;
-        route_token(a, t, lane, e, weight);
-        if (lane < a.top) {
-            const int p = t * a.top + lane;
+        route_any(a, t, g, e, weight);
+        if (t < a.tokens && g < a.top) {
+            const int p = t * a.top + g;
             ids[p] = e;
             a.ids[p] = e;
             a.weights[p] = weight;
@@ -158,40 +171,41 @@ __global__ __launch_bounds__(1024) void moe_route_kernel(const MoeArgs a) {
     __syncthreads();
     // experts' pairs and units, added up in order of the experts
     const int e = threadIdx.x;
-    int n = 0, units = 0, s = 0, u = 0;
+    int n = 0, sum[3] = {0, 0, 0};  // pairs, units of W1, of W2
     if (e < kMoeExperts) {
 #pragma unroll
         for (int i = 0; i < kMoeTokens / 32; ++i) n += __builtin_popcount(taken[e][i]);
-        units = (n + 15) / 16;
-        s = n;
-        u = units;
+        sum[0] = n;
+        sum[1] = (n + a.up_size - 1) / a.up_size;
+        sum[2] = (n + a.down_size - 1) / a.down_size;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
-            const int so = __shfl_up(s, off, 64), uo = __shfl_up(u, off, 64);
-            if (lane >= off) {
-                s += so;
-                u += uo;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const int o = __shfl_up(sum[i], off, 64);
+                if (lane >= off) sum[i] += o;
             }
         }
-        if (lane == 63) {
-            at_wave[0][w] = s;
-            at_wave[1][w] = u;
-        }
+        if (lane == 63)
+            for (int i = 0; i < 3; ++i) at_wave[i][w] = sum[i];
     }
     __syncthreads();
     if (e < kMoeExperts) {
-        for (int i = 0; i < w; ++i) {
-            s += at_wave[0][i];
-            u += at_wave[1][i];
-        }
-        start[e] = s - n;
-        for (int i = 0; i < units; ++i) {
-            const int k = u - units + i;
-            a.plan->expert[k] = e;
-            a.plan->first[k] = s - n + 16 * i;
-            a.plan->count[k] = min(n - 16 * i, 16);
-        }
-        if (e == kMoeExperts - 1) a.plan->units = u;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            for (int v = 0; v < w; ++v) sum[i] += at_wave[i][v];
+        start[e] = sum[0] - n;
+        auto list = [&](MoeUnits& u, int size, int upto) {
+            const int k = upto - (n + size - 1) / size;
+            for (int i = 0; i * size < n; ++i) {
+                u.expert[k + i] = e;
+                u.first[k + i] = sum[0] - n + size * i;
+                u.count[k + i] = min(n - size * i, size);
+            }
+            if (e == kMoeExperts - 1) u.n = upto;
+        };
+        list(a.plan->up, a.up_size, sum[1]);
+        list(a.plan->down, a.down_size, sum[2]);
     }
     __syncthreads();
     for (int p = threadIdx.x; p < a.tokens * a.top; p += 1024) {
@@ -232,9 +246,13 @@ template <bool E8> __device__ __forceinline__ float scale_value(uint32_t raw) {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int64_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
 }
-template <bool E8> __device__ __forceinline__ uint32_t load_scale(__amdgpu_buffer_rsrc_t r, uint32_t at) {
-    if constexpr (E8) return __builtin_amdgcn_raw_buffer_load_b8(r, at, 0, 0);
-    else return __builtin_amdgcn_raw_buffer_load_b32(r, at == kOOB ? kOOB : at * 4, 0, 0);
+// at a lane's offset and one for all lanes (kOOB: nothing is read, whatever the other)
+template <bool E8> __device__ __forceinline__ uint32_t load_scale(__amdgpu_buffer_rsrc_t r, uint32_t at, int all) {
+    if constexpr (E8) return __builtin_amdgcn_raw_buffer_load_b8(r, at, all, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b32(r, at, all, 0);
+}
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t at, int all) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, all, 0));
 }
 
 __device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
@@ -247,20 +265,23 @@ __device__ __forceinline__ float gelu(float v) {  // 0.5 v (1 + tanh(sqrt(2/pi) 
 // lane l has weight row l%16 (or token l%16) and the 16-byte chunks l/16 and l/16 + 4
 // of a step of 128 codes; U steps are loaded ahead.  Products are tokens x weight
 // rows: lane l holds row l%16 and tokens 4*(l/16) .. +4, so a scale is one per lane.
-template <typename V, bool E8, bool GATED>
+template <typename V, bool E8, bool GATED, bool ALIGNED, int U>
 __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
-    constexpr int W = 4, U = 4, COLS = GATED ? 16 : 32;
+    constexpr int W = 4, COLS = GATED ? 16 : 32, SZ = E8 ? 1 : 4;
     __shared__ float red[W][2][16][20];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n0 = blockIdx.x * COLS, unit = blockIdx.y;
-    if (n0 >= a.N) return;
+    // the next launch counts its blocks from 0
+    if (blockIdx.y == 0)
+        for (int i = blockIdx.x * 256 + threadIdx.x; a.splits > 1 && i < (a.H + 15) / 16; i += gridDim.x * 256) a.arrived[i] = 0;
+    if (n0 >= a.ldh) return;
     const int fr = lane & 15, fq = lane >> 4;
     int e, count, pair = -1;
     float weight1 = 0.0f;
     if (a.tokens == 1) {  // the unit is a choice
         int id;
         float weight;
-        route_token(a, 0, lane, id, weight);
+        route_any(a, 0, fr, id, weight);
         if (blockIdx.x == 0 && unit == 0 && (int)threadIdx.x < a.top) {
             a.ids[threadIdx.x] = id;
             a.weights[threadIdx.x] = weight;
@@ -271,23 +292,27 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
         count = 1;
         if (fr == 0) pair = unit;
     } else {
-        if (unit >= a.plan->units) return;
-        e = a.plan->expert[unit];
-        count = a.plan->count[unit];
-        if (fr < count) pair = a.plan->sorted[a.plan->first[unit] + fr];
+        if (unit >= a.plan->up.n) return;
+        e = a.plan->up.expert[unit];
+        count = a.plan->up.count[unit];
+        if (fr < count) pair = a.plan->sorted[a.plan->up.first[unit] + fr];
     }
     const int rows1 = GATED ? 2 * a.N : a.N, blocks = (a.H + 127) >> 7;
     const __amdgpu_buffer_rsrc_t rW = buffer(a.W1 + (int64_t)e * rows1 * a.ldw1, (int64_t)rows1 * a.ldw1);
     const __amdgpu_buffer_rsrc_t rS =
-        buffer(static_cast<const uint8_t*>(a.s1) + (int64_t)e * blocks * a.lds1 * (E8 ? 1 : 4), (int64_t)blocks * a.lds1 * (E8 ? 1 : 4));
-    uint32_t row[2];
-    bool ok[2];
+        buffer(static_cast<const uint8_t*>(a.s1) + (int64_t)e * blocks * a.lds1 * SZ, (int64_t)blocks * a.lds1 * SZ);
+    const __amdgpu_buffer_rsrc_t rX = buffer(a.x, ((int64_t)(a.tokens - 1) * a.ldx + a.H) * 2);
+    // Offsets of a lane; a step adds the same to all of them.  Chunks behind the rows'
+    // end are read from what follows and cleared before use, in the last step.
+    uint32_t wo[2], so[2];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
         const int n = n0 + (GATED ? 0 : 16 * g) + fr;
-        ok[g] = n < a.N;
-        row[g] = (uint32_t)(n + (GATED ? g * a.N : 0));
+        const uint32_t row = (uint32_t)(n + (GATED ? g * a.N : 0));
+        wo[g] = n < a.N ? row * (uint32_t)a.ldw1 + 16u * fq : kOOB;
+        so[g] = n < a.N ? row * SZ : kOOB;
     }
+    const uint32_t xo = pair >= 0 ? (uint32_t)(pair / a.top) * (uint32_t)a.ldx * 2u + 32u * fq : kOOB;
     const uint16_t* const xr = static_cast<const uint16_t*>(a.x) + (int64_t)(max(pair, 0) / a.top) * a.ldx;
     const int K16 = (a.H + 15) & ~15;
 
@@ -296,31 +321,37 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
         uint32_t s[2];
     };
     auto load = [&](Step& s, int step) {
-        const int k = step * 128 + 16 * fq;
+        const bool live = step < blocks;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const bool in = k + 64 * h < K16;
 #pragma unroll
             for (int g = 0; g < 2; ++g)
-                s.w[g][h] = __builtin_bit_cast(
-                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                               rW, in && ok[g] ? row[g] * (uint32_t)a.ldw1 + (uint32_t)(k + 64 * h) : kOOB, 0, 0));
+                s.w[g][h] = load16(rW, (live ? wo[g] : kOOB) + 64u * h, step * 128);
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-                s.x[h][c] = pair >= 0 ? load_chunk<uint16_t>(xr, k / 8 + 8 * h + c, a.H) : u32x4{0, 0, 0, 0};
+            for (int c = 0; c < 2; ++c) {
+                if constexpr (ALIGNED) s.x[h][c] = load16(rX, (live ? xo : kOOB) + 128u * h + 16u * c, step * 256);
+                else s.x[h][c] = pair >= 0 && live ? load_chunk<uint16_t>(xr, step * 16 + 2 * fq + 8 * h + c, a.H) : u32x4{0, 0, 0, 0};
+            }
         }
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-            s.s[g] = load_scale<E8>(rS, ok[g] && step < blocks ? (uint32_t)step * (uint32_t)a.lds1 + row[g] : kOOB);
+        for (int g = 0; g < 2; ++g) s.s[g] = load_scale<E8>(rS, live ? so[g] : kOOB, step * a.lds1 * SZ);
     };
     v4f acc[2] = {};
     auto multiply = [&](Step& s, int step) {
-        if (step * 128 + 128 > a.H) {  // the row's end, which its last chunk was loaded up to
+        if (step * 128 + 128 > a.H) {  // the rows' end
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+                const int k = step * 128 + 16 * fq + 64 * h;
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    s.x[h][c] = place_chunk<uint16_t>(s.x[h][c], step * 16 + 2 * fq + 8 * h + c, a.H);
+                for (int c = 0; c < 2; ++c) {
+                    if constexpr (ALIGNED) {
+                        if (k + 8 * c >= a.H) s.x[h][c] = u32x4{0, 0, 0, 0};
+                    } else {  // its last chunk was loaded up to there
+                        s.x[h][c] = place_chunk<uint16_t>(s.x[h][c], k / 8 + c, a.H);
+                    }
+                }
+                if (k >= K16) s.w[0][h] = s.w[1][h] = u32x4{0, 0, 0, 0};
+            }
         }
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
@@ -356,11 +387,11 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
     for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int x = 0; x < W; ++x) v[g] += red[x][g][c][i];
-    const int p = a.tokens == 1 ? unit : a.plan->sorted[a.plan->first[unit] + i];
+    const int p = a.tokens == 1 ? unit : a.plan->sorted[a.plan->up.first[unit] + i];
     const float weight = a.tokens == 1 ? weight1 : a.weights[p];
     auto put = [&](int n, float h) {
         if (n >= a.ldh) return;
-        h = n < a.N ? h * weight : 0.0f;  // zeros up to the next multiple of 16
+        h = n < a.N ? h * weight : 0.0f;  // zeros up to a step's end
         const uint32_t hi = f32_to_bf16_rne(h);
         // (an infinity has no rest)
         const float rest = h - bf16_to_f32(hi);
@@ -375,12 +406,105 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
     }
 }
 
-// W2 and the weighted sum.  blockIdx.x: 16 columns of y.
-template <bool E8> __global__ __launch_bounds__(512) void moe_down_kernel(const MoeArgs a) {
-    constexpr int W = 8, U = 2;
+// How W2's product is laid out.  A memory instruction wants neighbouring lanes on
+// neighbouring bytes, a matrix instruction a row each in them, and both get it from the
+// parts of a row: a step is 256 codes, 16 chunks of 16, and lane l = 16 fq + 4 r + p
+// loads chunk 4 fq + p of weight row r of four (the four rows' 256 bytes whole, in one
+// load), and that part of token r of four.  As operands of the matrix instruction,
+// rows are (token, p) and columns (weight row, p'); a result counts where p = p', and
+// the four that do add up to a token and row's product.  The other twelve cost
+// nothing: with 16 rows and tokens to an instruction, as in W1's, each group of four
+// lanes reads from four rows, and where columns' blocks are few, as here, the address
+// lookups of their CUs, 64 a load, bound the kernel (48 tokens to two of 32 experts:
+// 26.4 us, XXX so; W1's blocks are many and bound by HBM either way).
+// TG token groups of four share the weights' registers: units of 4 TG tokens.
+constexpr int kStep = 256;
+
+struct Lane {
+    int fr, fq, r, p, chunk;  // chunk: this lane's first code of a step
+};
+__device__ __forceinline__ Lane lane_parts() {
+    const int l = threadIdx.x & 63, fr = l & 15;
+    return {fr, l >> 4, fr >> 2, fr & 3, 16 * (4 * (l >> 4) + (fr & 3))};
+}
+
+// A wave's load of 16 weight rows' scales of a step's two blocks, row l%16 and block
+// (l/16)%2 in lane l, and what lane l needs of it: row 4 g + r of block b
+__device__ __forceinline__ uint32_t scale_of(uint32_t raw, const Lane& l, int g, int b) {
+    return (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (16 * b + 4 * g + l.r), (int)raw);
+}
+
+// 16 weight rows (w: four rows a load) times TG * 4 tokens over one step, into acc[tg][g].
+// FOLD: scales are powers of two and V is bf16, they go into the widening; else each
+// block of 128 is multiplied by itself, the other's half of x cleared.  x: PLANES values
+// that add up to a token's.
+template <bool E8, bool FOLD, typename V, int TG, int PLANES>
+__device__ __forceinline__ void step_products(const u32x4 (&w)[4], uint32_t scales, const u32x4 (&x)[TG][PLANES][2],
+                                              v4f (&acc)[TG][4], const Lane& l) {
+    // the scales first, then four rows at a time: left to itself the compiler widens all
+    // rows at once, at twice the registers
+    uint32_t raw[4][FOLD ? 1 : 2];
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int b = 0; b < (FOLD ? 1 : 2); ++b) raw[g][b] = scale_of(scales, l, g, FOLD ? l.fq >> 1 : b);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (FOLD) {
+            const float sc = e8m0_value(raw[g][0]);
+            const V b0 = widen8_scaled<E4M3>(w[g][0], w[g][1], sc), b1 = widen8_scaled<E4M3>(w[g][2], w[g][3], sc);
+#pragma unroll
+            for (int t = 0; t < TG; ++t)
+#pragma unroll
+                for (int n = PLANES - 1; n >= 0; --n) {
+                    acc[t][g] = mfma16(__builtin_bit_cast(V, x[t][n][0]), b0, acc[t][g]);
+                    acc[t][g] = mfma16(__builtin_bit_cast(V, x[t][n][1]), b1, acc[t][g]);
+                }
+        } else {
+            const V b0 = widen_codes<V>(w[g][0], w[g][1]), b1 = widen_codes<V>(w[g][2], w[g][3]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float sc = scale_value<E8>(raw[g][b]);
+                const uint32_t keep = (l.fq >> 1) == b ? ~0u : 0u;
+#pragma unroll
+                for (int t = 0; t < TG; ++t) {
+                    v4f v = {};
+#pragma unroll
+                    for (int n = PLANES - 1; n >= 0; --n) {
+                        v = mfma16(__builtin_bit_cast(V, x[t][n][0] & keep), b0, v);
+                        v = mfma16(__builtin_bit_cast(V, x[t][n][1] & keep), b1, v);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[t][g][i] = __builtin_fmaf(v[i], sc, acc[t][g][i]);
+                }
+            }
+        }
+    }
+}
+
+// token fq of a group times weight row 4 g + r, in every lane p: the four parts' sum
+__device__ __forceinline__ float parts_sum(const v4f& a, const Lane& l) {
+    const float even = l.p & 2 ? a[2] : a[0], odd = l.p & 2 ? a[3] : a[1];
+    float v = l.p & 1 ? odd : even;
+#define DF_QUAD(CTRL) \
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true))
+    DF_QUAD(0xB1);  // quad_perm by 1, by 2
+    DF_QUAD(0x4E);
+#undef DF_QUAD
+    return v;
+}
+
+// W2 and the weighted sum.  blockIdx.x: 16 columns of y; blockIdx.y: a share of the
+// units' steps, where there are more than 16 columns' blocks could keep under way.
+// Shares leave fp32 sums in the workspace, and the last of a column's blocks to end
+// adds them in order.
+template <bool E8, int TG> __global__ __launch_bounds__(512) void moe_down_kernel(const MoeArgs a) {
+    constexpr int W = 8, U = 2, SZ = E8 ? 1 : 4;
     __shared__ int expert[kMoeUnits], first[kMoeUnits], count[kMoeUnits], sorted[kMoePairs];
     __shared__ float sums[W][kMoeTokens][17];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Lane l = lane_parts();
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h0 = blockIdx.x * 16, pairs = a.tokens * a.top;
     int units;
     if (a.tokens == 1) {
@@ -392,114 +516,187 @@ template <bool E8> __global__ __launch_bounds__(512) void moe_down_kernel(const 
             sorted[threadIdx.x] = threadIdx.x;
         }
     } else {
-        units = a.plan->units;
+        const MoeUnits& u = a.plan->down;
+        units = u.n;
         for (int i = threadIdx.x; i < units; i += 512) {
-            expert[i] = a.plan->expert[i];
-            first[i] = a.plan->first[i];
-            count[i] = a.plan->count[i];
+            expert[i] = u.expert[i];
+            first[i] = u.first[i];
+            count[i] = u.count[i];
         }
         for (int i = threadIdx.x; i < pairs; i += 512) sorted[i] = a.plan->sorted[i];
     }
-    for (int i = lane; i < a.tokens * 17; i += 64) sums[w][i / 17][i % 17] = 0.0f;
+    for (int i = threadIdx.x & 63; i < a.tokens * 17; i += 64) sums[w][i / 17][i % 17] = 0.0f;
     __syncthreads();
-    const int fr = lane & 15, fq = lane >> 4;
-    const int steps = (a.N + 127) >> 7, K16 = a.ldh;
-    const int64_t bytes2 = (int64_t)a.H * a.ldw2, sbytes2 = (int64_t)steps * a.lds2 * (E8 ? 1 : 4);
+    const int blocks = (a.N + 127) >> 7, steps = a.ldh / kStep, K16 = (a.N + 15) & ~15;
+    const int64_t bytes2 = (int64_t)a.H * a.ldw2, sbytes2 = (int64_t)blocks * a.lds2 * SZ;
     const __amdgpu_buffer_rsrc_t rHi = buffer(a.hi, (int64_t)pairs * a.ldh * 2), rLo = buffer(a.lo, (int64_t)pairs * a.ldh * 2);
-    const bool ok = h0 + fr < a.H;
-    const uint32_t row = (uint32_t)(h0 + fr);
-    const int total = units * steps, lo_f = (int)((int64_t)total * w / W), hi_f = (int)((int64_t)total * (w + 1) / W);
+    uint32_t wo[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+        wo[g] = h0 + 4 * g + l.r < a.H ? (uint32_t)(h0 + 4 * g + l.r) * (uint32_t)a.ldw2 + (uint32_t)l.chunk : kOOB;
+    const uint32_t so = h0 + l.fr < a.H ? (uint32_t)(h0 + l.fr + (l.fq & 1) * a.lds2) * SZ : kOOB;
+    const int total = units * steps, shares = W * a.splits, share = blockIdx.y * W + w;
+    const int lo_f = (int)((int64_t)total * share / shares), hi_f = (int)((int64_t)total * (share + 1) / shares);
 
     struct Step {
-        u32x4 w[2], hi[2][2], lo[2][2];
+        u32x4 w[4], x[TG][2][2];  // x: the inner values' hi and lo
         uint32_t s;
     };
-    auto load = [&](Step& s, int f) {
-        const bool live = f < hi_f;
-        const int u = live ? f / steps : 0, step = f - u * steps;
-        const int e = max(__builtin_amdgcn_readfirstlane(live ? expert[u] : 0), 0);
-        const int n = __builtin_amdgcn_readfirstlane(live ? count[u] : 0);
-        const int pair = fr < n ? sorted[first[u] + fr] : -1;
-        const __amdgpu_buffer_rsrc_t rW = buffer(a.W2 + (int64_t)e * bytes2, bytes2);
-        const __amdgpu_buffer_rsrc_t rS = buffer(static_cast<const uint8_t*>(a.s2) + (int64_t)e * sbytes2, sbytes2);
-        const int k = step * 128 + 16 * fq;
+    // where loading is: step l_f, the l_s-th of unit l_u; its expert's weights, and the
+    // rows of inner values of this lane's tokens
+    int l_f = lo_f, l_u = lo_f / steps, l_s = lo_f - l_u * steps;
+    __amdgpu_buffer_rsrc_t rW, rS;
+    uint32_t ho[TG];
+    auto enter = [&]() {
+        const int u = min(l_u, units - 1);
+        const int e = max(__builtin_amdgcn_readfirstlane(expert[u]), 0), n = __builtin_amdgcn_readfirstlane(count[u]);
+        rW = buffer(a.W2 + (int64_t)e * bytes2, n ? bytes2 : 0);
+        rS = buffer(static_cast<const uint8_t*>(a.s2) + (int64_t)e * sbytes2, n ? sbytes2 : 0);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const bool in = n > 0 && k + 64 * h < K16;
-            s.w[h] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                         rW, in && ok ? row * (uint32_t)a.ldw2 + (uint32_t)(k + 64 * h) : kOOB, 0, 0));
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const uint32_t at = in && pair >= 0 ? ((uint32_t)pair * (uint32_t)a.ldh + (uint32_t)(k + 64 * h + 8 * c)) * 2u : kOOB;
-                s.hi[h][c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rHi, at, 0, 0));
-                s.lo[h][c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rLo, at, 0, 0));
-            }
-        }
-        s.s = load_scale<E8>(rS, ok && n > 0 ? (uint32_t)step * (uint32_t)a.lds2 + row : kOOB);
-    };
-    v4f acc = {};
-    auto multiply = [&](const Step& s, int f) {
-        v4f p = {};
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const bf8 v = widen8_scaled<E4M3>(s.w[h][2 * c], s.w[h][2 * c + 1], 1.0f);
-                p = mfma16(__builtin_bit_cast(bf8, s.lo[h][c]), v, p);
-                p = mfma16(__builtin_bit_cast(bf8, s.hi[h][c]), v, p);
-            }
-        const float sc = scale_value<E8>(s.s);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(p[r], sc, acc[r]);
-        const int u = f / steps;
-        if (f + 1 == hi_f || f + 1 == (u + 1) * steps) {  // the unit's end, or this wave's
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 4 * fq + r;
-                if (i < count[u]) sums[w][sorted[first[u] + i] / a.top][fr] += acc[r];
-            }
-            acc = v4f{};
+        for (int t = 0; t < TG; ++t) {
+            const int pair = 4 * t + l.r < n ? sorted[first[u] + 4 * t + l.r] : -1;
+            ho[t] = pair >= 0 ? ((uint32_t)pair * (uint32_t)a.ldh + (uint32_t)l.chunk) * 2u : kOOB;
         }
     };
-    Step buf[U];
+    auto load = [&](Step& s) {
+        const bool live = l_f < hi_f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) load(buf[u], lo_f + u);
-    for (int f = lo_f; f < hi_f; f += U) {
+        for (int t = 0; t < TG; ++t)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (f + u < hi_f) multiply(buf[u], f + u);
-            load(buf[u], f + u + U);
+            for (int c = 0; c < 2; ++c) {
+                s.x[t][0][c] = load16(rHi, (live ? ho[t] : kOOB) + 16u * c, l_s * kStep * 2);
+                s.x[t][1][c] = load16(rLo, (live ? ho[t] : kOOB) + 16u * c, l_s * kStep * 2);
+            }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) s.w[g] = load16(rW, live ? wo[g] : kOOB, l_s * kStep);
+        s.s = load_scale<E8>(rS, live && 2 * l_s + (l.fq & 1) < blocks ? so : kOOB, 2 * l_s * a.lds2 * SZ);
+        ++l_f;
+        if (++l_s == steps) {
+            l_s = 0;
+            ++l_u;
+            enter();
+        }
+    };
+    v4f acc[TG][4] = {};
+    int m_u = l_u, m_s = l_s;  // the step that is multiplied
+    auto multiply = [&](Step& s, bool last) {
+        if (m_s == steps - 1 && m_s * kStep + l.chunk >= K16) {  // the rows' end (the inner values are 0 there)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) s.w[g] = u32x4{0, 0, 0, 0};
+        }
+        step_products<E8, E8, bf8, TG, 2>(s.w, s.s, s.x, acc, l);
+        if (++m_s == steps || last) {  // the unit's end, or this wave's
+#pragma unroll
+            for (int t = 0; t < TG; ++t) {
+                float v[4];
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    v[g] = parts_sum(acc[t][g], l);
+                    acc[t][g] = v4f{};
+                }
+                // lane p adds row 4 p + r
+                const float even = l.p & 2 ? v[2] : v[0], odd = l.p & 2 ? v[3] : v[1];
+                const int i = 4 * t + l.fq;
+                if (i < count[m_u]) sums[w][sorted[first[m_u] + i] / a.top][4 * l.p + l.r] += l.p & 1 ? odd : even;
+            }
+            m_s = 0;
+            ++m_u;
+        }
+    };
+    if (lo_f < hi_f) {
+        Step buf[U];
+        enter();
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(buf[u]);
+        for (int f = lo_f; f < hi_f; f += U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (f + u < hi_f) multiply(buf[u], f + u + 1 == hi_f);
+                load(buf[u]);
+            }
         }
     }
     __syncthreads();
+    auto store = [&](int t, int c, float v) {
+        const int64_t at = (int64_t)t * a.ldy + h0 + c;
+        if (h0 + c >= a.H) return;
+        if (a.x_dtype == DF_DTYPE_HALF) static_cast<f16_t*>(a.y)[at] = OutCvt<f16_t>::cvt(v);
+        else static_cast<uint16_t*>(a.y)[at] = OutCvt<uint16_t>::cvt(v);
+    };
+    const int H16 = (a.H + 15) & ~15;
     for (int i = threadIdx.x; i < a.tokens * 16; i += 512) {
         const int t = i >> 4, c = i & 15;
-        if (h0 + c >= a.H) continue;
         float v = 0.0f;
 #pragma unroll
         for (int x = 0; x < W; ++x) v += sums[x][t][c];
-        const int64_t at = (int64_t)t * a.ldy + h0 + c;
-        if (a.x_dtype == DF_DTYPE_HALF) static_cast<f16_t*>(a.y)[at] = OutCvt<f16_t>::cvt(v);
-        else static_cast<uint16_t*>(a.y)[at] = OutCvt<uint16_t>::cvt(v);
+        if (a.splits == 1) store(t, c, v);
+        else __hip_atomic_store(a.part + ((int64_t)blockIdx.y * a.tokens + t) * H16 + h0 + c, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (a.splits == 1) return;
+    __shared__ int last;
+    // The sums pass the caches of the XCDs (agent scope), both ways: once a wave's
+    // stores are done (vmcnt 0) they are seen by whoever sees the count that follows.  A
+    // release and an acquire would write back and drop all of an XCD's L2, the weights
+    // with it: 48 tokens 124 us so, XXX this way.
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(a.arrived + blockIdx.x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.splits - 1;
+    __syncthreads();
+    if (!last) return;
+    for (int i = threadIdx.x; i < a.tokens * 16; i += 512) {
+        const int t = i >> 4, c = i & 15;
+        float v = 0.0f;
+        for (int x = 0; x < a.splits; ++x) v += __hip_atomic_load(a.part + ((int64_t)x * a.tokens + t) * H16 + h0 + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        store(t, c, v);
     }
 }
 
-template <bool E8> void launch(const MoeArgs& a, hipStream_t st) {
-    const bool gated = a.act != DF_ACT_GELU;
-    const int cols = gated ? 16 : 32;
-    const int pairs = a.tokens * a.top;
-    const int units = a.tokens == 1 ? a.top : std::min(a.experts, pairs) + pairs / 16;
+template <typename V, bool E8> void launch_up(const MoeArgs& a, dim3 grid, hipStream_t st) {
+    // 16-byte loads of x through a buffer descriptor, where its rows allow them
+    const bool aligned = a.H % 8 == 0 && a.ldx % 8 == 0 && aligned16(a.x) &&
+                         ((int64_t)(a.tokens - 1) * a.ldx + a.H) * 2 < (1ll << 31), gated = a.act != DF_ACT_GELU;
+    if (gated && aligned && a.tokens == 1) moe_up_kernel<V, E8, true, true, 4><<<grid, 256, 0, st>>>(a);
+    else if (gated && aligned) moe_up_kernel<V, E8, true, true, 2><<<grid, 256, 0, st>>>(a);
+    else if (gated) moe_up_kernel<V, E8, true, false, 2><<<grid, 256, 0, st>>>(a);
+    else if (aligned) moe_up_kernel<V, E8, false, true, 2><<<grid, 256, 0, st>>>(a);
+    else moe_up_kernel<V, E8, false, false, 2><<<grid, 256, 0, st>>>(a);
+}
+
+// W2's units are of four tokens, or of 8 where experts get more than four on average:
+// two groups then share the weights' registers.
+bool many_tokens(int tokens, int experts, int top) { return (int64_t)tokens * top > 4 * (int64_t)experts; }
+
+// at most this many units of `size` tokens, dealt in any way
+int64_t most_units(int tokens, int experts, int top, int size) {
+    const int64_t pairs = (int64_t)tokens * top;
+    return tokens == 1 ? top : std::min<int64_t>(experts, pairs) + pairs / size;
+}
+
+// Blocks that share a column tile of W2: as many as make two of them for each of 256
+// CUs, each wave with two steps at least.
+int down_splits(int tokens, int H, int N, int experts, int top) {
+    const int64_t tiles = (H + 15) / 16, pairs = (int64_t)tokens * top;
+    const int64_t units = tokens == 1 ? top : std::min<int64_t>(experts, pairs);
+    const int64_t want = 512 / tiles, most = units * ((N + kStep - 1) / kStep) / (8 * 2);
+    return (int)std::max<int64_t>(1, std::min(want, most));
+}
+
+template <bool E8> void launch(MoeArgs a, hipStream_t st) {
+    const bool many = many_tokens(a.tokens, a.experts, a.top);
+    a.up_size = 16;
+    a.down_size = many ? 8 : 4;
     if (a.tokens > 1) moe_route_kernel<<<1, 1024, 0, st>>>(a);
-    // columns' blocks to a multiple of 8: an expert's units then share an XCD's L2
-    const dim3 grid((((a.N + cols - 1) / cols) + 7) / 8 * 8, units);
-    if (a.x_dtype == DF_DTYPE_HALF) {
-        if (gated) moe_up_kernel<h8, E8, true><<<grid, 256, 0, st>>>(a);
-        else moe_up_kernel<h8, E8, false><<<grid, 256, 0, st>>>(a);
-    } else {
-        if (gated) moe_up_kernel<bf8, E8, true><<<grid, 256, 0, st>>>(a);
-        else moe_up_kernel<bf8, E8, false><<<grid, 256, 0, st>>>(a);
-    }
-    moe_down_kernel<E8><<<(a.H + 15) / 16, 512, 0, st>>>(a);
+    // (columns up to a step's end, for its zeros; a multiple of 8 blocks: an expert's
+    // units share an XCD's L2)
+    const dim3 up(a.ldh / (a.act != DF_ACT_GELU ? 16 : 32), (unsigned)most_units(a.tokens, a.experts, a.top, a.up_size));
+    const dim3 down((a.H + 15) / 16, a.splits);
+    if (a.x_dtype == DF_DTYPE_HALF) launch_up<h8, E8>(a, up, st);
+    else launch_up<bf8, E8>(a, up, st);
+    if (many) moe_down_kernel<E8, 2><<<down, 512, 0, st>>>(a);
+    else moe_down_kernel<E8, 1><<<down, 512, 0, st>>>(a);
 }
 
 constexpr size_t kPlanBytes = (sizeof(MoePlan) + 255) / 256 * 256;
@@ -510,9 +707,14 @@ constexpr size_t kPlanBytes = (sizeof(MoePlan) + 255) / 256 * 256;
 
 using namespace dfk;
 
-extern "C" size_t df_moe_layer_workspace_bytes(int tokens, int top_k, int N) {
-    if (tokens <= 0 || tokens > kMoeTokens || top_k <= 0 || top_k > kMoeTop || N <= 0 || N > 0x7FFFFFF0) return 0;
-    return kPlanBytes + (size_t)tokens * top_k * (((size_t)N + 15) & ~(size_t)15) * 4;
+// the plan, the inner values, the shares' sums and counts
+extern "C" size_t df_moe_layer_workspace_bytes(int tokens, int H, int N, int experts, int top_k) {
+    if (tokens <= 0 || tokens > kMoeTokens || top_k <= 0 || top_k > kMoeTop || H <= 0 || H > 0x7FFFFFF0 || N <= 0 ||
+        N > 0x7FFFFF00 || experts < top_k || experts > kMoeExperts)
+        return 0;
+    const size_t H16 = ((size_t)H + 15) & ~(size_t)15, splits = down_splits(tokens, H, N, experts, top_k);
+    return kPlanBytes + (size_t)tokens * top_k * (((size_t)N + kStep - 1) & ~(size_t)(kStep - 1)) * 4 +
+           (splits > 1 ? splits * tokens * H16 * 4 + H16 / 16 * 4 : 0);
 }
 
 extern "C" int df_moe_layer(int dtype, const void* x, int ldx, int tokens, int H, int N, int experts, int top_k,
@@ -550,16 +752,20 @@ extern "C" int df_moe_layer(int dtype, const void* x, int ldx, int tokens, int H
     const int64_t limit = 1ll << 31;
     DF_CHECK(rows1 * ldw1 < limit && (int64_t)H * ldw2 < limit && (((int64_t)H + 127) / 128) * lds1 * sz < limit &&
                  (((int64_t)N + 127) / 128) * lds2 * sz < limit && 
-                 (int64_t)tokens * top_k * (((int64_t)N + 15) & ~15ll) * 2 < limit,
+                 (int64_t)tokens * top_k * (((int64_t)N + kStep - 1) & ~(int64_t)(kStep - 1)) * 2 < limit,
              DF_ERR_UNSUPPORTED, "%s: one expert's weights or scales, or the inner values of 2^31 bytes or more", fn);
-    const size_t need = df_moe_layer_workspace_bytes(tokens, top_k, N);
+    const size_t need = df_moe_layer_workspace_bytes(tokens, H, N, experts, top_k);
     DF_CHECK(ws && aligned16(ws) && ws_bytes >= need, DF_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu, or not 16-byte aligned",
              fn, ws ? ws_bytes : (size_t)0, need);
-    const int ldh = (N + 15) & ~15;
+    const int ldh = (N + kStep - 1) & ~(kStep - 1);
     uint16_t* const hi = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(ws) + kPlanBytes);
-    const MoeArgs a{x, logits, W1, s1, W2, s2, y, ids, weights, static_cast<MoePlan*>(ws), hi,
-                    hi + (int64_t)tokens * top_k * ldh, tokens, H, N, experts, top_k, ldx, ld_logits, ldy, ldw1, ldw2, lds1,
-                    lds2, ldh, act, renormalize, dtype, logits_dtype};
+    uint16_t* const lo = hi + (int64_t)tokens * top_k * ldh;
+    float* const part = reinterpret_cast<float*>(lo + (int64_t)tokens * top_k * ldh);
+    const int splits = down_splits(tokens, H, N, experts, top_k);
+    int* const arrived = reinterpret_cast<int*>(part + (int64_t)splits * tokens * ((H + 15) & ~15));
+    const MoeArgs a{x, logits, W1, s1, W2, s2, y, ids, weights, static_cast<MoePlan*>(ws), hi, lo, part,
+                    arrived, tokens, H, N, experts, top_k, ldx, ld_logits, ldy, ldw1, ldw2, lds1, lds2, ldh, act, renormalize,
+                    dtype, logits_dtype, splits, 0, 0};
     if (scale_kind == DF_SCALE_E8M0) launch<true>(a, as_stream(stream));
     else launch<false>(a, as_stream(stream));
     return launch_status(fn);

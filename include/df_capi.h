@@ -575,10 +575,10 @@ int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const uint8_t* B, i
  * Sums in fp32, the inner values kept to 16 bits of significand, y rounded once.
  * At most 64 tokens, 256 experts, top_k 16, and 2^31 bytes of codes an expert.
  * y and ids, weights [tokens * top_k] overlap no input.  ws:
- * df_moe_layer_workspace_bytes(tokens, top_k, N), 16-byte aligned (0: sizes not
+ * df_moe_layer_workspace_bytes(tokens, H, N, experts, top_k), 16-byte aligned (0: sizes not
  * taken).  Two launches for one token, three for more. */
 typedef enum { DF_ACT_SWIGLU = 0, DF_ACT_GEGLU = 1, DF_ACT_GELU = 2 } df_activation;
-size_t df_moe_layer_workspace_bytes(int tokens, int top_k, int N);
+size_t df_moe_layer_workspace_bytes(int tokens, int H, int N, int experts, int top_k);
 int df_moe_layer(int dtype, const void* x, int ldx, int tokens, int H, int N, int experts, int top_k,
                  int logits_dtype, const void* logits, int ld_logits, int renormalize, int act,
                  const uint8_t* W1, int ldw1, const uint8_t* W2, int ldw2, int scale_kind, const void* s1, int lds1,
