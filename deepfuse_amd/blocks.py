@@ -10,19 +10,18 @@ brings scales from elsewhere into that form.
 """
 from __future__ import annotations
 
-from . import (DType, Fmt, _check_gpu, _check_like, _fits, _in_dtype, _INT_MAX, _on, _plain, _ptr, _row_vector, _rows,
+from . import (Fmt, _check_gpu, _check_like, _fits, _in_dtype, _INT_MAX, _on, _plain, _ptr, _row_vector, _rows,
                _stream, _torch, call, lib, round16)
 
 BLOCK = 128  # values that share a scale
-SCALE_F32, SCALE_E8M0 = 0, 1  # df_scale_kind
 
 
 def _kind(fn: str, dtype) -> int:
     torch = _torch()
     if dtype is torch.float8_e8m0fnu:
-        return SCALE_E8M0
+        return 1  # DF_SCALE_E8M0
     if dtype is torch.float32:
-        return SCALE_F32
+        return 0
     raise TypeError(f"{fn}: scales are float8_e8m0fnu or float32, not {dtype}")
 
 
@@ -32,10 +31,12 @@ def _code_dtype(fmt):
 
 
 def _new_scales(like, blocks: int, rows: int, dtype):
-    """[blocks, rows], each block's at a multiple of 16 bytes."""
-    step = 16 if dtype.itemsize == 1 else 4
-    ld = -(-rows // step) * step
-    return like.new_empty((blocks, ld), dtype=dtype)[:, :rows], ld
+    """[blocks, rows], each block's at a multiple of 16 bytes, and the leading
+    dimension."""
+    step = 15 if dtype.itemsize == 1 else 3
+    ld = (rows + step) & ~step
+    s = like.new_empty((blocks, ld), dtype=dtype)
+    return (s if ld == rows else s.as_strided((blocks, rows), (ld, 1))), ld
 
 
 def _scales_ld(fn: str, name: str, s, blocks: int, rows: int, dtype) -> int:
@@ -43,12 +44,13 @@ def _scales_ld(fn: str, name: str, s, blocks: int, rows: int, dtype) -> int:
     them: 16 bytes at a time, the last ones of a block too."""
     if s.shape != (blocks, rows) or s.dtype is not dtype:
         raise ValueError(f"{fn}: {name} is {tuple(s.shape)} {s.dtype}, not {(blocks, rows)} {dtype}")
-    size = dtype.itemsize
-    need = -(-rows * size // 16) * 16 // size  # of one block
-    ld = s.stride(0) if blocks > 1 else need
-    end = s.storage_offset() + (blocks - 1) * ld + need
-    if (rows > 1 and s.stride(1) != 1 or ld < rows or ld * size % 16 or s.data_ptr() % 16
-            or end * size > s.untyped_storage().nbytes()):
+    step, size = (15, 1) if dtype.itemsize == 1 else (3, 4)
+    need = (rows + step) & ~step  # of one block
+    ld, one = s.stride()
+    if blocks <= 1:
+        ld = need
+    if (one != 1 and rows > 1 or ld < rows or ld & step or s.data_ptr() & 15
+            or need != rows and (s.storage_offset() + (blocks - 1) * ld + need) * size > s.untyped_storage().nbytes()):
         raise ValueError(f"{fn}: {name} with strides {s.stride()} does not lie as block_scales() leaves it")
     return ld
 
@@ -88,7 +90,8 @@ def quantize_blocks(x, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=False, square=F
     rows, cols = x.shape
     if (rows | cols) > _INT_MAX:
         _fits(fn, rows, cols)
-    _check_gpu(fn, x=x)
+    if not x.is_cuda:
+        raise ValueError(f"{fn}: x is on {x.device}, not on a GPU")
     ldx = cols if x.is_contiguous() else _rows(fn, "x", x, x.shape, x.dtype)
     dt = _in_dtype(x)
     with _on(x):
@@ -108,13 +111,15 @@ def quantize_blocks(x, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=False, square=F
     return q, s, qt, st
 
 
-def _codes(fn: str, name: str, t, red: int, formats):
-    """Format and leading dimension of an operand's codes."""
-    if t.dim() != 2 or t.dtype not in formats:
-        raise ValueError(f"{fn}: {name} {tuple(t.shape)} {t.dtype} is not a matrix of {' or '.join(map(str, formats))}")
+def _codes(fn: str, name: str, t, red: int, ok: bool):
+    """The leading dimension of an operand's codes (``ok``: their type is right)."""
+    if not ok or t.dim() != 2:
+        raise ValueError(f"{fn}: {name} {tuple(t.shape)} {t.dtype} is not a matrix of codes in its format")
     rows, width = t.shape
-    ld = t.stride(0) if rows > 1 else -(-width // 16) * 16
-    if width < red or width > 1 and t.stride(1) != 1 or ld < width or ld % 16 or t.data_ptr() % 16:
+    ld, one = t.stride()
+    if rows <= 1:
+        ld = (width + 15) & ~15
+    if width < red or one != 1 and width > 1 or ld < width or ld & 15 or t.data_ptr() & 15:
         raise ValueError(f"{fn}: {name} {tuple(t.shape)} with strides {t.stride()} has no rows of {red} codes at "
                          "multiples of 16 bytes")
     return ld
@@ -130,28 +135,35 @@ def gemm_blocks(a_q, sa, b_q, sb, K: int, bias=None, out_dtype=None, out=None):
     y = gemm_blocks(xq, sx, wq, sw, K), dx = gemm_blocks(dyq, sdy, wqt, swt, N),
     dw = gemm_blocks(dyqt, sdyt, xqt, sxt, M)."""
     fn, torch = "gemm_blocks", _torch()
-    e4, e5 = torch.float8_e4m3fn, torch.float8_e5m2
     if K < 0:
         raise ValueError(f"{fn}: K = {K}")
-    lda, ldb = _codes(fn, "a_q", a_q, K, (e4, e5)), _codes(fn, "b_q", b_q, K, (e4,))
+    ta, kinds = a_q.dtype, sa.dtype
+    e4 = ta is torch.float8_e4m3fn
+    lda = _codes(fn, "a_q", a_q, K, e4 or ta is torch.float8_e5m2)
+    ldb = _codes(fn, "b_q", b_q, K, b_q.dtype is torch.float8_e4m3fn)
     M, N, blocks = a_q.shape[0], b_q.shape[0], -(-K // BLOCK)
-    kind = _kind(fn, sa.dtype)
-    ldsa, ldsb = _scales_ld(fn, "sa", sa, blocks, M, sa.dtype), _scales_ld(fn, "sb", sb, blocks, N, sa.dtype)
-    _check_gpu(fn, a_q=a_q, sa=sa, b_q=b_q, sb=sb, bias=bias, out=out)
+    kind = _kind(fn, kinds)
+    ldsa, ldsb = _scales_ld(fn, "sa", sa, blocks, M, kinds), _scales_ld(fn, "sb", sb, blocks, N, kinds)
+    at = a_q.get_device()
+    if at < 0 or not (sa.get_device() == b_q.get_device() == sb.get_device() == at):
+        _check_gpu(fn, a_q=a_q, sa=sa, b_q=b_q, sb=sb)
     if (M | N | K | lda | ldb | ldsa | ldsb) > _INT_MAX:
         _fits(fn, M, N, K, lda, ldb, ldsa, ldsb)
-    bias_dt = DType.FLOAT32
+    bias_dt = 0
     if bias is not None:
         bias_dt = _in_dtype(bias)
-        _row_vector(fn, "bias", bias, N, bias.dtype)
+        if not _plain(bias, (N,), bias.dtype, at):
+            _check_gpu(fn, a_q=a_q, bias=bias)
+            _row_vector(fn, "bias", bias, N, bias.dtype)
     with _on(a_q):
         if out is None:
             out, ldc = a_q.new_empty((M, N), dtype=out_dtype or torch.bfloat16), N
         else:
+            _check_gpu(fn, a_q=a_q, out=out)
             ldc = _rows(fn, "out", out, (M, N), out_dtype or out.dtype)
-        call("df_fp8_gemm_blocks", int(Fmt.E4M3 if a_q.dtype is e4 else Fmt.E5M2), a_q.data_ptr(), lda, b_q.data_ptr(), ldb,
-             M, N, K, kind, sa.data_ptr(), ldsa, sb.data_ptr(), ldsb, int(bias_dt), _ptr(bias), int(_in_dtype(out)),
-             out.data_ptr(), ldc, _stream())
+        call("df_fp8_gemm_blocks", 0 if e4 else 1, a_q.data_ptr(), lda, b_q.data_ptr(), ldb, M, N, K, kind, sa.data_ptr(),
+             ldsa, sb.data_ptr(), ldsb, bias_dt, None if bias is None else bias.data_ptr(), _in_dtype(out), out.data_ptr(),
+             ldc, _stream())
     return out
 
 
@@ -187,21 +199,25 @@ def quantize_experts_blocks(w, scale_dtype=None):
 
 def _expert_weights(fn: str, n: int, w, s, rows: int, cols: int, experts: int):
     """Leading dimensions of experts' codes and scales, checked."""
-    torch = _torch()
-    if w.dim() != 3 or w.dtype is not torch.float8_e4m3fn or w.shape[0] != experts or w.shape[1] != rows or w.shape[2] < cols:
+    blocks = -(-cols // BLOCK)
+    if (w.dim() != 3 or w.dtype is not _torch().float8_e4m3fn or w.shape[0] != experts or w.shape[1] != rows
+            or w.shape[2] < cols):
         raise ValueError(f"{fn}: w{n} is {tuple(w.shape)} {w.dtype}, not e4m3 codes of {(experts, rows, cols)}")
-    ldw = w.stride(1) if rows > 1 else w.stride(0) if experts > 1 else -(-w.shape[2] // 16) * 16
-    if (w.shape[2] > 1 and w.stride(2) != 1 or ldw < w.shape[2] or ldw % 16 or w.data_ptr() % 16
-            or experts > 1 and w.stride(0) != rows * ldw):
+    width, (each, ldw, one) = w.shape[2], w.stride()
+    if rows <= 1:
+        ldw = each if experts > 1 else (width + 15) & ~15
+    if one != 1 and width > 1 or ldw < width or ldw & 15 or w.data_ptr() & 15 or experts > 1 and each != rows * ldw:
         raise ValueError(f"{fn}: w{n} with strides {w.stride()} has no rows at multiples of 16 bytes, expert behind expert")
-    blocks, size = -(-cols // BLOCK), s.dtype.itemsize
     if s.dim() != 3 or s.shape != (experts, blocks, rows):
         raise ValueError(f"{fn}: s{n} is {tuple(s.shape)}, not {(experts, blocks, rows)}")
-    need = -(-rows * size // 16) * 16 // size
-    lds = s.stride(1) if blocks > 1 else s.stride(0) if experts > 1 else need
-    end = s.storage_offset() + (experts * blocks - 1) * lds + need
-    if (rows > 1 and s.stride(2) != 1 or lds < rows or lds * size % 16 or s.data_ptr() % 16
-            or experts > 1 and s.stride(0) != blocks * lds or end * size > s.untyped_storage().nbytes()):
+    step, size = (15, 1) if s.dtype.itemsize == 1 else (3, 4)
+    need = (rows + step) & ~step
+    each, lds, one = s.stride()
+    if blocks <= 1:
+        lds = each if experts > 1 else need
+    if (one != 1 and rows > 1 or lds < rows or lds & step or s.data_ptr() & 15 or experts > 1 and each != blocks * lds
+            or need != rows
+            and (s.storage_offset() + (experts * blocks - 1) * lds + need) * size > s.untyped_storage().nbytes()):
         raise ValueError(f"{fn}: s{n} with strides {s.stride()} does not lie as quantize_experts_blocks() leaves it")
     return ldw, lds
 
@@ -226,13 +242,16 @@ def moe_layer(x, logits, w1, s1, w2, s2, top_k: int, activation: str = "swiglu",
     N = w2.shape[-1] if w2.dim() == 3 else 0
     if w1.dim() == 3:  # w2's rows may be padded, w1's are not
         N = w1.shape[1] if activation == "gelu" else w1.shape[1] // 2
-    _check_gpu(fn, x=x, logits=logits, w1=w1, s1=s1, w2=w2, s2=s2)
+    at = x.get_device()
+    if at < 0 or not (logits.get_device() == w1.get_device() == s1.get_device() == w2.get_device() == s2.get_device() == at):
+        _check_gpu(fn, x=x, logits=logits, w1=w1, s1=s1, w2=w2, s2=s2)
     kind = _kind(fn, s1.dtype)
     if s2.dtype is not s1.dtype:
         raise ValueError(f"{fn}: s1 is {s1.dtype} and s2 {s2.dtype}")
     ldw1, lds1 = _expert_weights(fn, 1, w1, s1, N if activation == "gelu" else 2 * N, H, experts)
     ldw2, lds2 = _expert_weights(fn, 2, w2, s2, H, N, experts)
-    ldx, ldl = _rows(fn, "x", x, x.shape, x.dtype), _rows(fn, "logits", logits, logits.shape, logits.dtype)
+    ldx = H if x.is_contiguous() else _rows(fn, "x", x, x.shape, x.dtype)
+    ldl = experts if logits.is_contiguous() else _rows(fn, "logits", logits, logits.shape, logits.dtype)
     dt, lt = _in_dtype(x), _in_dtype(logits)
     if max(H, 2 * N, ldw1, ldw2, lds1, lds2) > _INT_MAX:
         _fits(fn, H, 2 * N, ldw1, ldw2, lds1, lds2)

@@ -24,10 +24,11 @@ namespace {
 
 // ------------------------------------------------------------ small tiles --
 // A block owns a 16*MT x 16*NT tile; its W waves take the 128-byte steps in turn
-// and add up through LDS, in wave order.  Fragments go from memory to registers
-// as the instruction wants them: lane l has row l%16 and the 16-byte chunks l/16
-// and l/16 + 4 of a step (which K a lane holds is free as long as A and B agree
-// and share a scale).  U steps are loaded ahead.
+// and add up through LDS, in wave order.  Loads take 8 rows x 128 bytes, eight lanes
+// a row; each wave passes them to its fragments (lane l: row l%16, 32 bytes of K)
+// through a slab of LDS of its own.  Straight from memory a fragment's load has four
+// rows to every four lanes, 64 address lookups (16 x 4800 x 1600 with tiles of 16 x
+// 16: 5.7 us, 5.1 so).  U steps are loaded ahead.
 template <int FA, bool E8, bool WIDE, int MT, int NT, int W, int U>
 __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g, int c_dtype, int extent_a, int extent_b) {
     constexpr int FB = E4M3;
@@ -35,7 +36,11 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
     constexpr int RSTR = COLS + 4;  // row of a partial tile (floats)
     constexpr uint32_t kOOB = 0x80000000u;
     constexpr int SZ = E8 ? 1 : 4;
-    __shared__ __attribute__((aligned(16))) float red[W * ROWS * RSTR];
+    constexpr int NL = 2 * (MT + NT);  // loads of 8 rows x 128 bytes per step
+    constexpr int SLAB = NL * 1024;    // a wave's step: A rows, then B rows
+    constexpr int RED = ROWS * RSTR * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[W * (SLAB > RED ? SLAB : RED)];
+    float* const red = reinterpret_cast<float*>(lds);
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // tiles in order of rows within a column of tiles, an XCD's (every eighth
@@ -54,30 +59,46 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
     // (bytes behind a matrix's last row of scales read as 0, and so do its codes)
     const __amdgpu_buffer_rsrc_t rSA = rsrc(static_cast<const uint8_t*>(g.sa) + (int64_t)m0 * SZ, max(extent_a - m0 * SZ, 0));
     const __amdgpu_buffer_rsrc_t rSB = rsrc(static_cast<const uint8_t*>(g.sb) + (int64_t)n0 * SZ, max(extent_b - n0 * SZ, 0));
-    const uint32_t oa = (uint32_t)fr * (uint32_t)g.lda + 16u * fq, ob = (uint32_t)fr * (uint32_t)g.ldb + 16u * fq;
+    // loads: lane l takes 16-byte chunk l%8 of row l/8 of each 8-row group
+    const int lr = lane >> 3, lc = (lane & 7) * 16;
+    const uint32_t oa = (uint32_t)lr * (uint32_t)g.lda + (uint32_t)lc, ob = (uint32_t)lr * (uint32_t)g.ldb + (uint32_t)lc;
+    // slab: rows of 128 bytes, 16-byte chunk c of row r in slot c ^ (r/2 % 8)
+    uint8_t* const slab = lds + w * SLAB;
+    const int wr_even = lr * 128 + (((lane & 7) ^ (lr >> 1)) << 4), wr_odd = wr_even ^ 64;
+    const int fs = (fr >> 1) & 7;
+    const int rd0 = fr * 128 + (((2 * fq) ^ fs) << 4), rd1 = fr * 128 + (((2 * fq + 1) ^ fs) << 4);
+    // the lanes of a wave hand chunks to each other through the slab: LDS operations of
+    // a wave execute in order, the compiler must keep that order
+    auto lanes_meet = [] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    };
 
     struct Step {
-        u32x4 a[MT][2], b[NT][2];
+        u32x4 raw[NL];
         uint32_t sa[MT];
         typename std::conditional<E8, uint32_t, u32x4>::type sb[NT];
     };
     auto load = [&](Step& s, int step) {
-        const int k = step * 128, c = k + 16 * fq;
-        const bool in0 = c < g.K, in1 = c + 64 < g.K;
+        const int k = step * 128;
+        const bool in = k + lc < g.K;
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i)
+            s.raw[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                           rA, in ? oa + (uint32_t)(8 * i) * (uint32_t)g.lda + (uint32_t)k : kOOB, 0, 0));
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i)
+            s.raw[2 * MT + i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                    rB, in ? ob + (uint32_t)(8 * i) * (uint32_t)g.ldb + (uint32_t)k : kOOB, 0, 0));
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const uint32_t at = oa + (uint32_t)(16 * i) * (uint32_t)g.lda + (uint32_t)k;
-            s.a[i][0] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rA, in0 ? at : kOOB, 0, 0));
-            s.a[i][1] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rA, in1 ? at + 64 : kOOB, 0, 0));
             const uint32_t sc = k < g.K ? ((uint32_t)step * (uint32_t)g.ldsa + 16 * i + fr) * SZ : kOOB;
             if constexpr (E8) s.sa[i] = __builtin_amdgcn_raw_buffer_load_b8(rSA, sc, 0, 0);
             else s.sa[i] = __builtin_amdgcn_raw_buffer_load_b32(rSA, sc, 0, 0);
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const uint32_t at = ob + (uint32_t)(16 * j) * (uint32_t)g.ldb + (uint32_t)k;
-            s.b[j][0] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rB, in0 ? at : kOOB, 0, 0));
-            s.b[j][1] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rB, in1 ? at + 64 : kOOB, 0, 0));
             const uint32_t sc = (uint32_t)step * (uint32_t)g.ldsb + 16 * j;
             if constexpr (E8) s.sb[j] = __builtin_amdgcn_raw_buffer_load_b8(rSB, k < g.K ? sc + fr : kOOB, 0, 0);
             else s.sb[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
@@ -90,62 +111,50 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    auto whole = [](const u32x4* p) {
-        v8i f;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            f[x] = (int)p[0][x];
-            f[4 + x] = (int)p[1][x];
-        }
-        return f;
+    // fragment t (16 rows) of a step in registers, through its part of the slab
+    auto frag = [&](const Step& s, int t) -> v8i {
+        *reinterpret_cast<u32x4*>(slab + t * 2048 + wr_even) = s.raw[2 * t];
+        *reinterpret_cast<u32x4*>(slab + t * 2048 + 1024 + wr_odd) = s.raw[2 * t + 1];
+        lanes_meet();
+        const u32x4 x = *reinterpret_cast<const u32x4*>(slab + t * 2048 + rd0);
+        const u32x4 y = *reinterpret_cast<const u32x4*>(slab + t * 2048 + rd1);
+        return v8i{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
     };
     auto multiply = [&](const Step& s) {
-        if constexpr (WIDE) {
+        lanes_meet();  // the step before has read the slab
+        v8i fb[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) fb[j] = frag(s, MT + j);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const v8i fa = frag(s, i);
+            bf8 wa[4];
+            if constexpr (WIDE) {
+                const float sa = E8 ? __uint_as_float(s.sa[i] << 23) : 1.0f;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) wa[x] = widen8_scaled<FA>((uint32_t)fa[2 * x], (uint32_t)fa[2 * x + 1], sa);
+            }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                float sb = 1.0f;
-                if constexpr (E8) sb = __uint_as_float(s.sb[j] << 23);
-                bf8 wb[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    wb[x] = widen8_scaled<FB>(s.b[j][x >> 1][2 * (x & 1)], s.b[j][x >> 1][2 * (x & 1) + 1], sb);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const float sa = E8 ? __uint_as_float(s.sa[i] << 23) : 1.0f;
-                    v4f p = E8 ? acc[i][j] : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                v4f p = E8 ? acc[i][j] : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (WIDE) {
+                    float sb = 1.0f;
+                    if constexpr (E8) sb = __uint_as_float(s.sb[j] << 23);
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
                         p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            wb[x], widen8_scaled<FA>(s.a[i][x >> 1][2 * (x & 1)], s.a[i][x >> 1][2 * (x & 1) + 1], sa), p, 0,
-                            0, 0);
-                    if constexpr (E8) {
-                        acc[i][j] = p;
-                    } else {
-#pragma unroll
-                        for (int y = 0; y < 4; ++y)
-                            acc[i][j][y] = __builtin_fmaf(p[y] * __uint_as_float(s.sb[j][y]), __uint_as_float(s.sa[i]), acc[i][j][y]);
-                    }
+                            widen8_scaled<FB>((uint32_t)fb[j][2 * x], (uint32_t)fb[j][2 * x + 1], sb), wa[x], p, 0, 0, 0);
+                } else if constexpr (E8) {
+                    p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, p, FB, FA, 0, (int)s.sb[j], 0, (int)s.sa[i]);
+                } else {
+                    p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, p, FB, FA, 0, 0, 0, 0);
                 }
-            }
-        } else {
-            v8i fb[NT];
+                if constexpr (E8) {
+                    acc[i][j] = p;
+                } else {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) fb[j] = whole(s.b[j]);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const v8i fa = whole(s.a[i]);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    if constexpr (E8) {
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, acc[i][j], FB, FA, 0,
-                                                                                     (int)s.sb[j], 0, (int)s.sa[i]);
-                    } else {
-                        const v4f z = {0.0f, 0.0f, 0.0f, 0.0f};
-                        const v4f p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, z, FB, FA, 0, 0, 0, 0);
-#pragma unroll
-                        for (int y = 0; y < 4; ++y)
-                            acc[i][j][y] = __builtin_fmaf(p[y] * __uint_as_float(s.sb[j][y]), __uint_as_float(s.sa[i]), acc[i][j][y]);
-                    }
+                    for (int y = 0; y < 4; ++y)
+                        acc[i][j][y] = __builtin_fmaf(p[y] * __uint_as_float(s.sb[j][y]), __uint_as_float(s.sa[i]), acc[i][j][y]);
                 }
             }
         }
@@ -161,6 +170,7 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
             load(buf[u], s + (u + U) * W);
         }
     }
+    __syncthreads();  // the slabs are read before sums go over them
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -168,73 +178,116 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
             *reinterpret_cast<v4f*>(red + (w * ROWS + 16 * i + fr) * RSTR + 16 * j + 4 * fq) = acc[i][j];
     __syncthreads();
     const int mrows = min(g.M - m0, ROWS);
-    for (int x = threadIdx.x; x < ROWS * COLS / 4; x += 64 * W) {
-        const int r = x / (COLS / 4), c = (x % (COLS / 4)) * 4, col = n0 + c;
-        if (r >= mrows || col >= g.N) continue;
-        v4f t = *reinterpret_cast<const v4f*>(red + r * RSTR + c);
-#pragma unroll
-        for (int v = 1; v < W; ++v) t += *reinterpret_cast<const v4f*>(red + (v * ROWS + r) * RSTR + c);
-        float o[4] = {t[0], t[1], t[2], t[3]};
+    // the waves' sums in order, V columns of a row at a time: four, or one where rows of C
+    // start anywhere, so that lanes' stores follow each other
+    auto write = [&](auto width, auto* C) {
+        constexpr int V = decltype(width)::value;
+        using T = typename std::remove_reference<decltype(*C)>::type;
+        static_assert(64 * W % (COLS / V) == 0, "a thread's columns are the same in all its rows");
+        const int c = (threadIdx.x % (COLS / V)) * V, col = n0 + c;
+        if (col >= g.N) return;
+        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (g.bias) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
-                if (col + y < g.N) o[y] += bias_at(g.bias, g.bias_dtype, col + y);
+            for (int y = 0; y < V; ++y)
+                if (col + y < g.N) bias[y] = bias_at(g.bias, g.bias_dtype, col + y);
         }
-        auto put = [&](auto* p) {
-            using T = typename std::remove_reference<decltype(*p)>::type;
-            if (g.vec_out && col + 3 < g.N) {
+        for (int r = threadIdx.x / (COLS / V); r < mrows; r += 64 * W / (COLS / V)) {
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int v = 0; v < W; ++v) {
+                const float* t = red + (v * ROWS + r) * RSTR + c;
+#pragma unroll
+                for (int y = 0; y < V; ++y) o[y] = v == 0 ? t[y] : o[y] + t[y];
+            }
+            if (g.bias) {
+#pragma unroll
+                for (int y = 0; y < V; ++y) o[y] += bias[y];
+            }
+            T* const p = C + (int64_t)(m0 + r) * g.ldc + col;
+            if (V == 4 && col + 3 < g.N) {
                 store4(p, o);
             } else {
 #pragma unroll
-                for (int y = 0; y < 4; ++y)
+                for (int y = 0; y < V; ++y)
                     if (col + y < g.N) p[y] = OutCvt<T>::cvt(o[y]);
             }
-        };
-        const int64_t at = (int64_t)(m0 + r) * g.ldc + col;
-        if (c_dtype == DF_DTYPE_FLOAT32) put(static_cast<float*>(g.C) + at);
-        else if (c_dtype == DF_DTYPE_HALF) put(static_cast<f16_t*>(g.C) + at);
-        else put(static_cast<uint16_t*>(g.C) + at);
-    }
+        }
+    };
+    auto as = [&](auto* C) {
+        if (g.vec_out) write(std::integral_constant<int, 4>{}, C);
+        else write(std::integral_constant<int, 1>{}, C);
+    };
+    if constexpr (WIDE) as(static_cast<float*>(g.C));
+    else if (c_dtype == DF_DTYPE_HALF) as(static_cast<f16_t*>(g.C));
+    else as(static_cast<uint16_t*>(g.C));
 }
 
-template <int FA, bool E8, bool WIDE> void launch_small(const BlocksArgs& g, int c_dtype, int ea, int eb, hipStream_t st) {
-    auto tiles = [&](int r, int c) { return (int)((int64_t)((g.M + r - 1) / r) * ((g.N + c - 1) / c)); };
-    if (g.M <= 16 || g.N <= 16)
-        blocks_small_kernel<FA, E8, WIDE, 1, 1, 4, 4><<<tiles(16, 16), 256, 0, st>>>(g, c_dtype, ea, eb);
-    else
-        blocks_small_kernel<FA, E8, WIDE, 2, 2, 4, 2><<<tiles(32, 32), 256, 0, st>>>(g, c_dtype, ea, eb);
-}
-
-// Which kernel a call takes, by the time each would take, in us; a step is 128 of
-// K.  Large tiles: rounds of blocks over the CUs.
+// Which kernel a call takes, by the time each would take, in us; a step is 128 of K.
+// Measured at M, N, K (bf16 out, powers of two; graph replays, a launch being 2.5 to 3
+// of it):
+//   16 x 16 tiles, while they are no more than the CUs: 32 x 1600 x 6400 5.8 (32 x 32:
+//     7.6); up to 16 rows otherwise 16 x 32: 16 x 4800 x 1600 4.4 (16 x 16: 5.1)
+//   32 x 32: 64 x 6400 x 1600 6.9, 256 x 6400 x 1600 16, 512 x 512 x 16384 16.3 (with
+//     four waves in place of eight 7.1, 16, 19.9; 1000 x 1037 x 771, seven steps, 10.2
+//     and 9.5)
+//   64 x 64: 256 x 6400 x 1600 12.1, 1024 x 1600 x 6400 27.5
+//   128 x 128: 256 x 6400 x 1600 10.1, 1024 x 1600 x 6400 25.7, 2048 x 6400 x 1600 35
+//   256 x 256: 2048 x 6400 x 1600 25.2, 1024 x 1600 x 6400 60
+// and likewise with fp32 outputs or scales, whose steps take longer on large tiles
+// (128 x 128, 1024 x 1600 x 6400: 49 and 37.5; 64 x 64: 32 and 28.7).
+enum : int { SMALL_16 = -1, SMALL_16X32 = -2, SMALL_32 = -3, SMALL_64 = -4 };
 struct BlocksPlan {
-    int fm;  // 0: small tiles
+    int fm;  // of the large tiles, or SMALL_*
     int grid;
 };
 BlocksPlan plan(const BlocksArgs& g, bool e8, bool wide) {
     const int cus = std::max(device_cu_count(), 1);
     const double steps = (double)((g.K + 127) / 128);
     auto tiles = [&](int r, int c) { return (int64_t)((g.M + r - 1) / r) * ((g.N + c - 1) / c); };
-    double best = 4.0 + 0.12 * steps + 0.35e-3 * (double)tiles(32, 32) * (steps + 10.0);
-    BlocksPlan p{0, 0};
-    if (g.K == 0) return p;
-    auto offer = [&](int fm, int r, int c, double step, double over) {
-        const int64_t n = tiles(r, c), rounds = (n + cus - 1) / cus;
-        const double t = 5.0 + (double)rounds * (wide ? 2.05 : 1.0) * (step * steps + over);
+    if (g.K == 0) return {SMALL_32, (int)tiles(32, 32)};
+    if (tiles(16, 16) <= cus) return {SMALL_16, (int)tiles(16, 16)};
+    if (g.M <= 16) return {SMALL_16X32, (int)tiles(16, 32)};
+    // fp32 scales, fp32 outputs: 0 to 3
+    const int kind = (e8 ? 0 : 2) + (wide ? 1 : 0);
+    const double slower[4] = {1.0, 1.08, 1.1, 1.2};
+    double best = 3.2 + std::max(0.1 * steps, slower[kind] * (double)tiles(32, 32) * (0.56e-3 * steps + 1.9e-3));
+    BlocksPlan p{SMALL_32, (int)tiles(32, 32)};
+    auto offer = [&](int fm, int64_t n, double t) {
         if (t < best) {
             best = t;
-            p = {fm, (int)std::min<int64_t>(n, cus)};
+            p = {fm, (int)n};
         }
     };
-    if (e8) {
-        offer(4, 256, 256, 1.2, 3.6);
-        offer(2, 256, 128, 0.72, 2.4);
-        offer(1, 128, 128, 0.5, 1.8);
-    } else {
-        offer(2, 256, 128, 1.1, 2.4);
-        offer(1, 128, 128, 0.7, 1.8);
-    }
+    if (kind != 3)
+        offer(SMALL_64, tiles(64, 64),
+              3.5 + slower[kind] * (0.25 * steps + (double)tiles(64, 64) * (0.41e-3 * steps + 8.2e-3)));
+    // rounds of blocks over the CUs, a step's time and a tile's besides
+    auto large = [&](int fm, int r, int c, const double* step, const double* over) {
+        const int64_t n = tiles(r, c), rounds = (n + cus - 1) / cus;
+        offer(fm, std::min<int64_t>(n, cus), 3.0 + (double)rounds * (step[kind] * steps + over[kind]));
+    };
+    const double s1[4] = {0.39, 0.83, 0.62, 1.03}, o1[4] = {2.6, 3.0, 2.0, 3.0};
+    const double s2[4] = {0.75, 1.28, 1.02, 1.75}, o2[4] = {3.0, 4.5, 2.5, 4.0};
+    const double s4[2] = {1.1, 2.2}, o4[2] = {6.0, 8.0};
+    large(1, 128, 128, s1, o1);
+    large(2, 256, 128, s2, o2);
+    if (e8) large(4, 256, 256, s4, o4);
     return p;
+}
+
+template <int FA, bool E8, bool WIDE>
+void launch_small(const BlocksPlan& p, const BlocksArgs& g, int c_dtype, int ea, int eb, hipStream_t st) {
+    if (p.fm == SMALL_16)
+        blocks_small_kernel<FA, E8, WIDE, 1, 1, 8, 2><<<p.grid, 512, 0, st>>>(g, c_dtype, ea, eb);
+    else if (p.fm == SMALL_16X32)
+        blocks_small_kernel<FA, E8, WIDE, 1, 2, 8, 1><<<p.grid, 512, 0, st>>>(g, c_dtype, ea, eb);
+    else if (p.fm == SMALL_32 && g.K > 8 * 128)
+        blocks_small_kernel<FA, E8, WIDE, 2, 2, 8, 1><<<p.grid, 512, 0, st>>>(g, c_dtype, ea, eb);
+    else if (p.fm == SMALL_32)
+        blocks_small_kernel<FA, E8, WIDE, 2, 2, 4, 2><<<p.grid, 256, 0, st>>>(g, c_dtype, ea, eb);
+    else if constexpr (E8 || !WIDE)
+        blocks_small_kernel<FA, E8, WIDE, 4, 4, 4, 1><<<p.grid, 256, 0, st>>>(g, c_dtype, ea, eb);
 }
 
 }  // namespace
@@ -255,7 +308,10 @@ extern "C" int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const ui
     DF_CHECK(scale_kind_ok(scale_kind), DF_ERR_INVALID, "%s: bad scale kind %d", fn, scale_kind);
     DF_CHECK(value_dtype(c_dtype), DF_ERR_UNSUPPORTED, "%s: output dtype %d not supported", fn, c_dtype);
     DF_CHECK(!bias || value_dtype(bias_dtype), DF_ERR_UNSUPPORTED, "%s: bias dtype %d not supported", fn, bias_dtype);
-    DF_CHECK((int64_t)((M + 15) / 16) * ((N + 15) / 16) < (1ll << 31), DF_ERR_INVALID, "%s: output too large", fn);
+    // (blocks of small tiles: fewer than 2^32 threads; those of M <= 16 and of large tiles
+    // are fewer)
+    DF_CHECK((int64_t)((M + 31) / 32) * ((N + 31) / 32) < (1ll << 23), DF_ERR_UNSUPPORTED, "%s: output of %d x %d too large",
+             fn, M, N);
     if (M == 0 || N == 0) return DF_OK;
     DF_CHECK(C && ldc >= N, DF_ERR_INVALID, "%s: output NULL or leading dimension %d < %d", fn, ldc, N);
     DF_CHECK(!misaligned(C, c_dtype) && !(bias && misaligned(bias, bias_dtype)), DF_ERR_ALIGN,
@@ -279,14 +335,14 @@ extern "C" int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const ui
     const hipStream_t st = as_stream(stream);
     const bool wide = c_dtype == DF_DTYPE_FLOAT32, e8 = scale_kind == DF_SCALE_E8M0;
     const BlocksPlan p = plan(g, e8, wide);
-    if (p.fm) {
+    if (p.fm > 0) {
         g.vec_out = epi_store_mode(C, ldc_bytes);
         launch_block_tiles(fmt_a, e8, p.fm, c_dtype, g, (int)ea, (int)eb, p.grid, st);
         return launch_status(fn);
     }
     g.vec_out = ldc_bytes % 16 == 0 && aligned16(C);
     auto go = [&](auto fa, auto e, auto wd) {
-        launch_small<decltype(fa)::value, decltype(e)::value, decltype(wd)::value>(g, c_dtype, (int)ea, (int)eb, st);
+        launch_small<decltype(fa)::value, decltype(e)::value, decltype(wd)::value>(p, g, c_dtype, (int)ea, (int)eb, st);
     };
     auto as = [&](auto fa) {
         using Y = std::true_type;

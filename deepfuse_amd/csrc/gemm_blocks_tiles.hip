@@ -1,10 +1,11 @@
 // gemm_blocks_tiles.hip -- the products with a scale per 128 of the reduction
 // (gemm_blocks.hip) on large tiles: one persistent block per CU of eight waves, two
-// per SIMD, operands by LDS DMA through two stages of 128 bytes of K, as the
-// persistent kernel of gemm_fp8.hip.  A wave owns FM x 2 accumulators of 32 x 32.
+// per SIMD, operands by LDS DMA through two stages of 128 bytes of K (three of the
+// smallest tiles, whose steps are shorter than memory's latency), as the persistent
+// kernel of gemm_fp8.hip.  A wave owns FM x 2 accumulators of 32 x 32.
 // What differs:
 //  - Scales come with each step by a DMA instruction of their own (waves 0 and 1),
-//    into a ring of four slots.  A lane needs the scales of its FM rows of A and 2 of
+//    into a ring of slots.  A lane needs the scales of its FM rows of A and 2 of
 //    B, 32 accumulator rows apart; the operands' rows are laid into LDS so that these
 //    are neighbours in memory (row FM * r + i of a wave's part is row r of its
 //    accumulator i), and one LDS read gives the bytes of all, which the matrix
@@ -56,18 +57,21 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
     constexpr int NDA = BM / 64, NDB = BN / 64;   // DMA instructions per wave and step
     constexpr int ND = NDA + NDB;
     constexpr int STAGE = (BM + BN) * kPKB;
+    constexpr int NS = FM == 1 ? 3 : 2;           // stages
+    // Slots of scales: step c + 1 + NS is on its way while step c's are still folded in
+    constexpr int SLOTS = NS == 2 ? 4 : 8;
     constexpr int SZ = E8 ? 1 : 4;
     constexpr int SLOT = 2 * 256 * SZ;            // one step's scales: A's, B's
     using G = EpiGeom<(int)sizeof(OutT), FM>;
     constexpr int W_AFTER = G::NST > 63 ? 63 : G::NST;
     constexpr uint32_t kOOB = 0x80000000u;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE + 4 * SLOT + 8 * (G::SLAB + 256)];
-    uint8_t* const ring = lds + 2 * STAGE;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[NS * STAGE + SLOTS * SLOT + 8 * (G::SLAB + 256)];
+    uint8_t* const ring = lds + NS * STAGE;
 
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = w / WAVES_N, wn = w % WAVES_N;
-    uint8_t* const slab = ring + 4 * SLOT + w * (G::SLAB + 256);
+    uint8_t* const slab = ring + SLOTS * SLOT + w * (G::SLAB + 256);
     float* const wbias = reinterpret_cast<float*>(slab + G::SLAB);  // the wave's 64 columns'
     const int tiles_n = (g.N + BN - 1) / BN, tiles_m = (g.M + BM - 1) / BM;
     const int nunits = tiles_m * tiles_n;
@@ -100,14 +104,14 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
     // stage's A part (and (w*NDB+d)*8 + lane/8 of its B part), 16-byte chunk c of
     // row r in slot c ^ ((r >> 1) & 7).  Row 32*i + r of a wave's part holds the
     // operand's row FM*r + i of it (B: 2*r + j).  The cursor (unit d_unit, step d_k)
-    // runs two steps ahead of the products, across units.
+    // runs NS steps ahead of the products, across units.
     const int drow = lane >> 3;
     const int dch0 = ((lane & 7) ^ (lane >> 4)) << 4;
     const int dch1 = dch0 ^ 64;
     const int pa = w * 8 * NDA, pb = w * 8 * NDB;
     const uint32_t ra = (uint32_t)(pa - pa % WR + FM * (pa % 32 + drow) + pa % WR / 32);
     const uint32_t rb = (uint32_t)(pb - pb % 64 + FN * (pb % 32 + drow) + pb % 64 / 32);
-    int d_unit = 0, d_k = 0, d_g = 0;
+    int d_unit = 0, d_k = 0, d_g = 0, d_st = 0;  // (step d_g goes to stage d_st = d_g % NS)
     Unit du = unit_of(0);
     __amdgpu_buffer_rsrc_t rA, rB, rS;
     auto rsrc = [](const void* p, int bytes) {
@@ -130,18 +134,17 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         ob0 = in0 ? rb * (uint32_t)g.ldb + (uint32_t)k0 : kOOB;
         ob1 = in1 ? (rb + 8u * FN) * (uint32_t)g.ldb + (uint32_t)k1 : kOOB;
         // 256 rows' scales (those of rows behind the tile are not read), a step's codes
-        // ahead of the codes: into the slot of the step before the one whose products
-        // are under way
+        // ahead of the codes (step c's products done: step c + 1 + NS)
         if (w < 2) {
             const uint32_t os =
                 live ? (uint32_t)d_k * (uint32_t)(w == 0 ? g.ldsa : g.ldsb) * SZ + (uint32_t)lane * (4 * SZ) : kOOB;
-            uint8_t* const to = ring + (d_g & 3) * SLOT + w * 256 * SZ;
+            uint8_t* const to = ring + (d_g & (SLOTS - 1)) * SLOT + w * 256 * SZ;
             if constexpr (E8) __builtin_amdgcn_raw_ptr_buffer_load_lds(rS, (Lds)to, 4, os, 0, 0, 0);
             else __builtin_amdgcn_raw_ptr_buffer_load_lds(rS, (Lds)to, 16, os, 0, 0, 0);
         }
     };
     auto dissue_one = [&](int k) __attribute__((always_inline)) {
-        uint8_t* base = lds + ((uint32_t)d_g & 1u) * STAGE;
+        uint8_t* base = lds + d_st * STAGE;
         if (k < NDA)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (Lds)(base + (w * NDA + k) * 1024), 16,
                                                      ((k & 1) ? oa1 : oa0) + (uint32_t)(k >> 1) * 16u * FM * (uint32_t)g.lda,
@@ -160,6 +163,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
             }
         }
         ++d_g;
+        d_st = d_st + 1 == NS ? 0 : d_st + 1;
         dprep();
     };
 
@@ -182,7 +186,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
     };
     // E8: the bytes of this lane's rows at a step, A's FM and B's 2
     auto rd_scales = [&](int step, int& a, int& b) {
-        const uint8_t* p = ring + (step & 3) * SLOT;
+        const uint8_t* p = ring + (step & (SLOTS - 1)) * SLOT;
         if constexpr (FM == 4) a = *reinterpret_cast<const int*>(p + wm * WR + 4 * fr);
         else if constexpr (FM == 2) a = *reinterpret_cast<const uint16_t*>(p + wm * WR + 2 * fr);
         else a = p[wm * WR + fr];
@@ -190,15 +194,15 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
     };
 
     v16f acc[FM][FN];
-    int after_epi = 0, c_g = 0;  // c_g: the step whose products are under way
+    int after_epi = 0, c_g = 0, c_st = 0;  // c_g: the step whose products are under way, in stage c_st
 
     // Before the first read of step c_g + 1: this wave's part of it has landed
     // (after an epilogue its stores may still be under way: they were issued
     // later), then every wave's.  Every wave has read the last of step c_g, so the
-    // DMA of step c_g + 2 may go over it.
+    // DMA of step c_g + NS may go over it.
     auto next_step = [&]() __attribute__((always_inline)) {
-        if (after_epi == 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(W_AFTER));
-        else __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(0));
+        if (NS == 2 && after_epi == 1) __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(W_AFTER));
+        else __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((NS - 2) * ND));
         after_epi = 0;
         __builtin_amdgcn_s_barrier();
     };
@@ -210,7 +214,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
     float usb = 0.0f;
     bool same = false;  // B's scales are the same over the wave's columns
     auto fold_scales = [&](int step) __attribute__((always_inline)) {
-        const float* p = reinterpret_cast<const float*>(ring + (step & 3) * SLOT);
+        const float* p = reinterpret_cast<const float*>(ring + (step & (SLOTS - 1)) * SLOT);
 #pragma unroll
         for (int i = 0; i < FM; ++i) fsa[i] = p[wm * WR + FM * fr + i];
         const float b = p[256 + wn * 64 + lane];
@@ -225,7 +229,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(part[i][j][e], s, acc[i][j][e]);
         } else {
-            const float* p = reinterpret_cast<const float*>(ring + (step & 3) * SLOT) + 256 + wn * 64 + 8 * (lane >> 5);
+            const float* p = reinterpret_cast<const float*>(ring + (step & (SLOTS - 1)) * SLOT) + 256 + wn * 64 + 8 * (lane >> 5);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const f32x4 lo = *reinterpret_cast<const f32x4*>(p + 16 * x), hi = *reinterpret_cast<const f32x4*>(p + 16 * x + 4);
@@ -250,7 +254,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         constexpr int NM = FM * FN, RD_OVER = NM < 4 ? NM : 4;
         __builtin_amdgcn_sched_barrier(0);
         if (ODD) next_step();
-        const int stage = (ODD ? c_g + 1 : c_g) & 1;
+        const int stage = ODD ? (c_st + 1 == NS ? 0 : c_st + 1) : c_st;
         constexpr int NR = 2 * NF;
         u32x4 frag[NR];
         int nsa = sa, nsb = sb;
@@ -298,6 +302,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
             sa = nsa;
             sb = nsb;
             ++c_g;
+            c_st = stage;
             dadvance();
         }
     };
@@ -322,7 +327,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         constexpr bool FIRST = decltype(first)::value;
         __builtin_amdgcn_sched_barrier(0);
         if (Q == 3) next_step();
-        const int stage = (Q == 3 ? c_g + 1 : c_g) & 1;
+        const int stage = Q == 3 ? (c_st + 1 == NS ? 0 : c_st + 1) : c_st;
 #pragma unroll
         for (int f = 0; f < NF; ++f) nxt[f] = rd(stage, f, ((Q + 1) >> 1) & 1, (Q + 1) & 1);
         // (read anew each step: kept from the step before, they took 80 registers' copies)
@@ -355,6 +360,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         });
         if (Q == 3) {
             ++c_g;
+            c_st = stage;
             dadvance();
         }
     };
@@ -442,13 +448,13 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         return rowb + WR <= g.M && colw + 64 <= g.N;
     };
 
-    // prologue: DMA steps 0 and 1; step 0's first fragments
+    // prologue: DMA steps 0 to NS - 1; step 0's first fragments
     dprep();
-    for (int k = 0; k < ND; ++k) dissue_one(k);
-    dadvance();
-    for (int k = 0; k < ND; ++k) dissue_one(k);
-    dadvance();
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(ND));
+    for (int i = 0; i < NS; ++i) {
+        for (int k = 0; k < ND; ++k) dissue_one(k);
+        dadvance();
+    }
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0((NS - 1) * ND));
     __builtin_amdgcn_s_barrier();
 
     using Y = std::true_type;
