@@ -52,6 +52,57 @@ template <bool E8> __device__ __forceinline__ void put_scales(void* p, int64_t a
     }
 }
 
+// The absmax over finite values of 8 rows and 8 columns of values, without compares
+// (fold_*_biased); 2-byte values two columns at a time.
+template <typename T> struct Folds {  // bf16 and f16
+    static constexpr bool BF = std::is_same<T, uint16_t>::value;
+    static constexpr uint32_t bias = BF ? 0x00800080u : 0x04000400u;
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(df_short2, a), __builtin_bit_cast(df_short2, b)));
+    }
+    static __device__ __forceinline__ uint32_t value(int half) {  // a biased half as a binary32 pattern
+        const uint32_t h = (uint32_t)max(half - (BF ? 0x80 : 0x400), 0);
+        return BF ? h << 16 : __float_as_uint(f16_to_f32(h));
+    }
+    static __device__ __forceinline__ void fold(const u32x4 (&w)[8][1], uint32_t* rm, uint32_t* cm) {
+        uint32_t col[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            uint32_t row = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t u = (w[p][0][i] & 0x7FFF7FFFu) + bias;  // not finite: negative
+                row = larger(row, u);
+                col[i] = larger(col[i], u);
+            }
+            rm[p] = value(max((int)(int16_t)(row >> 16), (int)(int16_t)(row & 0xFFFFu)));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            cm[2 * i] = value((int)(int16_t)(col[i] & 0xFFFFu));
+            cm[2 * i + 1] = value((int)(int16_t)(col[i] >> 16));
+        }
+    }
+};
+template <> struct Folds<float> {
+    static __device__ __forceinline__ void fold(const u32x4 (&w)[8][2], uint32_t* rm, uint32_t* cm) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cm[e] = 0;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            rm[p] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                rm[p] = fold_f32_biased(rm[p], w[p][e >> 2][e & 3]);
+                cm[e] = fold_f32_biased(cm[e], w[p][e >> 2][e & 3]);
+            }
+            rm[p] = unbias_f32(rm[p]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) cm[e] = unbias_f32(cm[e]);
+    }
+};
+
 template <typename T, int FMT, bool E8, bool SQUARE>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(const BlockQuant a) {
     constexpr int E = El<T>::E, PITCH = 132;  // bytes of a transposed row in LDS: no bank conflicts in its writes
@@ -73,7 +124,10 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(const BlockQuant a
 #pragma unroll
     for (int p = 0; p < 8; ++p)
 #pragma unroll
-        for (int h = 0; h < 8 / E; ++h) El<T>::widen(place_chunk<T>(raw[p][h], c / E + h, a.cols), v[p] + h * E);
+        for (int h = 0; h < 8 / E; ++h) {
+            raw[p][h] = place_chunk<T>(raw[p][h], c / E + h, a.cols);
+            El<T>::widen(raw[p][h], v[p] + h * E);
+        }
 
     bool nan = false;
 #pragma unroll
@@ -81,18 +135,12 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(const BlockQuant a
 #pragma unroll
         for (int e = 0; e < 8; e += 2) nan |= __builtin_isunordered(v[p][e], v[p][e + 1]);
 
+    // absmax of the thread's rows and columns, as binary32 patterns
     uint32_t rm[8], cm[8];
+    Folds<T>::fold(raw, rm, cm);
+    if (!SQUARE) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) cm[e] = 0;
-#pragma unroll
-    for (int p = 0; p < 8; ++p) {
-        rm[p] = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            rm[p] = fold_f32(rm[p], __float_as_uint(v[p][e]));
-            cm[e] = fold_f32(cm[e], __float_as_uint(v[p][e]));
-        }
-        if (!SQUARE) rm[p] = row16_max(rm[p]);
+        for (int p = 0; p < 8; ++p) rm[p] = row16_max(rm[p]);
     }
     if constexpr (SQUARE) {
         uint32_t m = 0;

@@ -63,6 +63,11 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
     constexpr int E = El<T>::E;
     constexpr int RPB = RT == 64 ? 4 : 1;  // rows a block works on at once
     constexpr int GL = kScaleBlock / E;    // lanes that share a scale
+    // The next row's loads before this row's arithmetic, gamma in registers; with codes
+    // and a wave's four chunks a thread that took 158 registers, three waves a SIMD: no
+    // row ahead then, and gamma in LDS
+    constexpr bool AHEAD = OUT == OUT_Y || CH < 4 || RT > 64;
+    __shared__ u32x4 glds[AHEAD ? 1 : CH][AHEAD ? 1 : RT];
     __shared__ float red[2][2][1][RT / 64];
     const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
     RowSum<RT> rs{red};
@@ -85,16 +90,21 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
         return a.quads ? 4 * (unit + (int64_t)(n >> 2) * units) + (n & 3) : unit + (int64_t)n * units;
     };
     int64_t r = row_of(0);
-    if (r < a.rows) fetch((int)r);
+    if (AHEAD && r < a.rows) fetch((int)r);
     if (affine) {
 #pragma unroll
-        for (int k = 0; k < CH; ++k) gw[k] = place_chunk<T>(load_chunk<T>(a.gamma, t + RT * k, a.cols), t + RT * k, a.cols);
+        for (int k = 0; k < CH; ++k) {
+            const u32x4 w = place_chunk<T>(load_chunk<T>(a.gamma, t + RT * k, a.cols), t + RT * k, a.cols);
+            if constexpr (AHEAD) gw[k] = w;
+            else glds[k][t] = w;  // (every wave the same, its own lanes')
+        }
     }
     // no wave stores of the first row before all have its loads on their way: a
     // row's last chunk holds values of the one before it, and the sum may lie over x
     if constexpr (RT > 64) __syncthreads();
     int n = 0;
     for (; r < a.rows; r = row_of(++n)) {
+        if (!AHEAD) fetch((int)r);
         float v[CH][E];
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
@@ -110,7 +120,7 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
             }
         }
         const int64_t next = row_of(n + 1);
-        if (next < a.rows) fetch((int)next);
+        if (AHEAD && next < a.rows) fetch((int)next);
         float sq = 0.0f;
 #pragma unroll
         for (int k = 0; k < CH; ++k)
@@ -125,7 +135,8 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
             for (int e = 0; e < E; ++e) v[k][e] *= rstd;
             if (affine) {
                 float g[E];
-                El<T>::widen(gw[k], g);
+                if constexpr (AHEAD) El<T>::widen(gw[k], g);
+                else El<T>::widen(glds[k][t], g);
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[k][e] *= g[e];
             }
@@ -137,9 +148,9 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     if (c + e >= a.cols) v[k][e] = 0.0f;
-                    most = fold_f32(most, __float_as_uint(v[k][e]));
+                    most = fold_f32_biased(most, __float_as_uint(v[k][e]));
                 }
-                most = row16_max(most);
+                most = row16_max(unbias_f32(most));
                 if constexpr (GL == 32) most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
                 constexpr bool E8 = OUT == OUT_E8;
                 auto codes = [&](auto fmt) {
