@@ -34,7 +34,6 @@ template <typename T> struct RmsFwd {
     uint8_t* q; void* s;  // codes [rows, ldq], scales [blocks, ldsc]
     int rows, cols, ldx, ldr, lds, ldy, ldq, ldsc, fmt;
     float eps;
-    bool quads;  // a wave (or block) takes four rows that follow each other
 };
 
 // What is written beside y: nothing, or codes with scales of a kind
@@ -72,7 +71,6 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
     const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
     RowSum<RT> rs{red};
     u32x4 gw[CH], nx[CH], nr[CH];
-    uint32_t pack[CH];
     const bool affine = a.gamma != nullptr, add = a.res != nullptr;
     auto fetch = [&](int r) __attribute__((always_inline)) {
 #pragma unroll
@@ -84,13 +82,8 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
     };
     const int units = gridDim.x * RPB;
     const int unit = blockIdx.x * RPB + (RT == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
-    // row n of this unit; the scales of four rows that follow each other leave as
-    // one store (bytes of their own are written line by line, once a row)
-    auto row_of = [&](int n) -> int64_t {
-        return a.quads ? 4 * (unit + (int64_t)(n >> 2) * units) + (n & 3) : unit + (int64_t)n * units;
-    };
-    int64_t r = row_of(0);
-    if (AHEAD && r < a.rows) fetch((int)r);
+    int r = unit;
+    if (AHEAD && r < a.rows) fetch(r);
     if (affine) {
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
@@ -102,9 +95,8 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
     // no wave stores of the first row before all have its loads on their way: a
     // row's last chunk holds values of the one before it, and the sum may lie over x
     if constexpr (RT > 64) __syncthreads();
-    int n = 0;
-    for (; r < a.rows; r = row_of(++n)) {
-        if (!AHEAD) fetch((int)r);
+    for (; r < a.rows; r += units) {
+        if (!AHEAD) fetch(r);
         float v[CH][E];
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
@@ -116,11 +108,10 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
                 for (int e = 0; e < E; ++e) v[k][e] += p[e];
                 const u32x4 w = El<T>::narrow(v[k]);  // the norm is that of the sum as stored
                 El<T>::widen(w, v[k]);
-                if (a.sum) store_chunk<T>(a.sum + r * a.lds, t + RT * k, a.cols, w);
+                if (a.sum) store_chunk<T>(a.sum + (int64_t)r * a.lds, t + RT * k, a.cols, w);
             }
         }
-        const int64_t next = row_of(n + 1);
-        if (AHEAD && next < a.rows) fetch((int)next);
+        if (AHEAD && r + units < a.rows) fetch(r + units);
         float sq = 0.0f;
 #pragma unroll
         for (int k = 0; k < CH; ++k)
@@ -140,7 +131,7 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[k][e] *= g[e];
             }
-            if (OUT == OUT_Y || a.y) store_chunk<T>(a.y + r * a.ldy, t + RT * k, a.cols, El<T>::narrow(v[k]));
+            if (OUT == OUT_Y || a.y) store_chunk<T>(a.y + (int64_t)r * a.ldy, t + RT * k, a.cols, El<T>::narrow(v[k]));
             if constexpr (OUT != OUT_Y) {
                 // (values past the row's end are 0, unless the row's rstd or sum is
                 // not finite: then they are NaN, and left out here)
@@ -156,35 +147,15 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
                 auto codes = [&](auto fmt) {
                     constexpr int F = decltype(fmt)::value;
                     const BlockDiv b = block_div<F, E8>(most);
-                    if (c < ((a.cols + 15) & ~15)) put_codes<F, E8, E>(a.q + r * a.ldq + c, v[k], b);
+                    if (c < ((a.cols + 15) & ~15)) put_codes<F, E8, E>(a.q + (int64_t)r * a.ldq + c, v[k], b);
                     if ((t & (GL - 1)) == 0 && c < a.cols) {
                         const int64_t at = (int64_t)(c / kScaleBlock) * a.ldsc + r;
-                        if constexpr (!E8) {
-                            static_cast<float*>(a.s)[at] = b.d.s;
-                        } else if (a.quads) {
-                            const int sh = 8 * (n & 3);
-                            pack[k] = sh == 0 ? b.byte : pack[k] | b.byte << sh;
-                            if (sh == 24) *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.s) + at - 3) = pack[k];
-                        } else {
-                            static_cast<uint8_t*>(a.s)[at] = (uint8_t)b.byte;
-                        }
+                        if constexpr (E8) static_cast<uint8_t*>(a.s)[at] = (uint8_t)b.byte;
+                        else static_cast<float*>(a.s)[at] = b.d.s;
                     }
                 };
                 if (a.fmt == E4M3) codes(std::integral_constant<int, E4M3>{});
                 else codes(std::integral_constant<int, E5M2>{});
-            }
-        }
-    }
-    if constexpr (OUT == OUT_E8) {
-        if (a.quads && (n & 3)) {  // the last rows, fewer than four
-            const int64_t r0 = row_of(n & ~3);
-#pragma unroll
-            for (int k = 0; k < CH; ++k) {
-                const int c = (t + RT * k) * E;
-                if ((t & (GL - 1)) == 0 && c < a.cols)
-                    for (int i = 0; i < (n & 3); ++i)
-                        static_cast<uint8_t*>(a.s)[(int64_t)(c / kScaleBlock) * a.ldsc + r0 + i] =
-                            (uint8_t)(pack[k] >> 8 * i);
             }
         }
     }
@@ -579,16 +550,11 @@ int bwd_blocks(int rows, const RmsShape& s) {
     return std::min((rows + per - 1) / per, std::min(256 * 1024 / nt, std::max(256, rows / (4 * per))));
 }
 
-// Rows from which a wave takes four in a row: every CU then has 16 waves with
-// four rows each.
-constexpr int kQuadRows = 16384;
-
-template <typename T, int OUT> void launch_forward(RmsFwd<T> a, hipStream_t st) {
+template <typename T, int OUT> void launch_forward(const RmsFwd<T>& a, hipStream_t st) {
     const RmsShape s = fwd_shape(a.cols, (int)sizeof(T));
     // 16 waves per CU walk the rows
     const int grid = s.threads == 64 ? std::min((a.rows + 3) / 4, 1024)
                                      : std::min(a.rows, s.threads == 0 ? 512 : 256 * 1024 / s.threads);
-    a.quads = OUT == OUT_E8 && a.rows >= kQuadRows;
 #define DF_RMS(RT, CH)                                                                   \
     if (s.threads == RT && s.chunks == CH) {                                             \
         rms_forward_kernel<T, RT, CH, OUT><<<grid, RT == 64 ? 256 : RT, 0, st>>>(a);     \
@@ -730,7 +696,7 @@ extern "C" int df_rmsnorm_forward(int dtype, const void* x, int rows, int cols, 
     forward_as<OUT_Y>(dtype, [&](auto& a) {
         using T = typename std::remove_reference<decltype(*a.y)>::type;
         a = {static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<T*>(sum), static_cast<T*>(y),
-             static_cast<const T*>(gamma), rstd, nullptr, nullptr, rows, cols, ldx, ldr, lds, ldy, 0, 0, 0, eps, false};
+             static_cast<const T*>(gamma), rstd, nullptr, nullptr, rows, cols, ldx, ldr, lds, ldy, 0, 0, 0, eps};
     }, as_stream(stream));
     return launch_status(fn);
 }
@@ -755,8 +721,7 @@ extern "C" int df_rmsnorm_quantize(int dtype, const void* x, int rows, int cols,
     auto fill = [&](auto& a) {
         using T = typename std::remove_reference<decltype(*a.y)>::type;
         a = {static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<T*>(sum), static_cast<T*>(y),
-             static_cast<const T*>(gamma), rstd, q, scales, rows, cols, ldx, ldr, lds, ldy, ldq, ld_scales, fmt, eps,
-             false};
+             static_cast<const T*>(gamma), rstd, q, scales, rows, cols, ldx, ldr, lds, ldy, ldq, ld_scales, fmt, eps};
     };
     if (scale_kind == DF_SCALE_E8M0) forward_as<OUT_E8>(dtype, fill, as_stream(stream));
     else forward_as<OUT_F32>(dtype, fill, as_stream(stream));
