@@ -416,7 +416,7 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
 // nothing: with 16 rows and tokens to an instruction, as in W1's, each group of four
 // lanes reads from four rows, and where columns' blocks are few, as here, the address
 // lookups of their CUs, 64 a load, bound the kernel (48 tokens to two of 32 experts:
-// 26.4 us, XXX so; W1's blocks are many and bound by HBM either way).
+// 26.4 us, 23.5 so; W1's blocks are many and bound by HBM either way).
 // TG token groups of four share the weights' registers: units of 4 TG tokens.
 constexpr int kStep = 256;
 
@@ -637,7 +637,7 @@ template <bool E8, int TG> __global__ __launch_bounds__(512) void moe_down_kerne
     // The sums pass the caches of the XCDs (agent scope), both ways: once a wave's
     // stores are done (vmcnt 0) they are seen by whoever sees the count that follows.  A
     // release and an acquire would write back and drop all of an XCD's L2, the weights
-    // with it: 48 tokens 124 us so, XXX this way.
+    // with it: 48 tokens 124 us so, 42 this way.
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __builtin_amdgcn_s_waitcnt(0);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
