@@ -297,6 +297,13 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
         count = a.plan->up.count[unit];
         if (fr < count) pair = a.plan->sorted[a.plan->up.first[unit] + fr];
     }
+    if (n0 >= a.N) {  // only the zeros up to a step's end
+        for (int i = threadIdx.x; i < count * COLS; i += 256) {
+            const int p = a.tokens == 1 ? unit : a.plan->sorted[a.plan->up.first[unit] + i / COLS];
+            a.hi[(int64_t)p * a.ldh + n0 + i % COLS] = a.lo[(int64_t)p * a.ldh + n0 + i % COLS] = 0;
+        }
+        return;
+    }
     const int rows1 = GATED ? 2 * a.N : a.N, blocks = (a.H + 127) >> 7;
     const __amdgpu_buffer_rsrc_t rW = buffer(a.W1 + (int64_t)e * rows1 * a.ldw1, (int64_t)rows1 * a.ldw1);
     const __amdgpu_buffer_rsrc_t rS =

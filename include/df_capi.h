@@ -533,7 +533,8 @@ int df_fp8_experts_dw(const uint8_t* dYtq, int lddyt, const uint8_t* Xtq, int ld
  * whose blocks are 128 rows of a column; either pair may be NULL.  square: one
  * scale per 128 x 128 (weights: both kinds of codes then stand for the same
  * values), written for each of its rows (columns) all the same.  Codes are zero
- * up to the next multiple of 16 columns (rows).  At most 128 * 65535 rows. */
+ * up to the next multiple of 16 columns (rows).  At most 128 * 65535 rows.  No
+ * output overlaps x or another. */
 int df_quantize_blocks(int dtype, const void* x, int rows, int cols, int ldx, int fmt, int scale_kind, int square,
                        uint8_t* q, int ldq, void* scales, int ld_scales,
                        uint8_t* qt, int ldqt, void* scales_t, int ld_scales_t, void* stream);
@@ -547,7 +548,10 @@ int df_quantize_blocks(int dtype, const void* x, int rows, int cols, int ldx, in
  * as above, each below 2^31 bytes.  bias (fp32, bf16 or f16, [N]) may be NULL.  C
  * fp32, bf16 or f16, rounded once from fp32 accumulation; an fp32 one is the fp32
  * sum of exact products (bf16 matrix instructions), a 2-byte one takes the fp8
- * ones (see df_fp8_experts_fwd).  K == 0 gives the bias, or 0.
+ * ones (see df_fp8_experts_fwd).  K == 0 gives the bias, or 0.  C overlaps no
+ * operand and holds fewer than 2^23 tiles of 32 x 32.  Powers of two reach an fp32
+ * output through bf16: exact while codes times scales stay in its range (2^-133 ..
+ * 2^128).
  *   forward : Xq, sx (row codes) and Wq, sw      ; M tokens, N outputs, K inputs
  *   dX      : dYq, sdy (row codes) and Wtq, swt  ; M tokens, N inputs, K outputs
  *   dW      : dYtq, sdyt and Xtq, sxt            ; M outputs, N inputs, K tokens */

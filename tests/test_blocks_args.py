@@ -163,7 +163,8 @@ def test_python_refusals():
     w2 = torch.zeros(4, 32, 16, dtype=torch.uint8).view(torch.float8_e4m3fn)
     s = torch.zeros(4, 1, 32, dtype=torch.uint8).view(e8)
     logits = torch.zeros(2, 4)
-    for bad in (lambda: df.moe_layer(t, logits, w1, s, w2, s, 2), lambda: df.moe_layer(t, logits[0], w1, s, w2, s, 2),
+    for bad in (lambda: df.moe_layer(t, logits, w1, s, w2, s, 0), lambda: df.moe_layer(t, logits, w1, s, w2, s, 5),
+                lambda: df.moe_layer(t, logits, w1, s, w2, s, 2), lambda: df.moe_layer(t, logits[0], w1, s, w2, s, 2),
                 lambda: df.moe_layer(t, logits, w1, s, w2, s, 2, activation="relu"),
                 lambda: df.moe_layer(t, logits[:, :3], w1, s, w2, s, 2), lambda: df.moe_layer(t, logits, w1[:, :30], s, w2, s, 2),
                 lambda: df.moe_layer(t, logits, w1, s, w2, s.float(), 2)):
