@@ -310,7 +310,7 @@ extern "C" int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const ui
     DF_CHECK(!bias || value_dtype(bias_dtype), DF_ERR_UNSUPPORTED, "%s: bias dtype %d not supported", fn, bias_dtype);
     // (blocks of small tiles: fewer than 2^32 threads; those of M <= 16 and of large tiles
     // are fewer)
-    DF_CHECK((int64_t)((M + 31) / 32) * ((N + 31) / 32) < (1ll << 23), DF_ERR_UNSUPPORTED, "%s: output of %d x %d too large",
+    DF_CHECK(((M + 31ll) / 32) * ((N + 31ll) / 32) < (1ll << 23), DF_ERR_UNSUPPORTED, "%s: output of %d x %d too large",
              fn, M, N);
     if (M == 0 || N == 0) return DF_OK;
     DF_CHECK(C && ldc >= N, DF_ERR_INVALID, "%s: output NULL or leading dimension %d < %d", fn, ldc, N);

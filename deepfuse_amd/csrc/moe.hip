@@ -246,7 +246,8 @@ template <bool E8> __device__ __forceinline__ float scale_value(uint32_t raw) {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int64_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
 }
-// at a lane's offset and one for all lanes (kOOB: nothing is read, whatever the other)
+// at a lane's offset and one for all lanes; the descriptor's range counts both, and past it
+// 0 is read (kOOB: whatever the other)
 template <bool E8> __device__ __forceinline__ uint32_t load_scale(__amdgpu_buffer_rsrc_t r, uint32_t at, int all) {
     if constexpr (E8) return __builtin_amdgcn_raw_buffer_load_b8(r, at, all, 0);
     else return __builtin_amdgcn_raw_buffer_load_b32(r, at, all, 0);
@@ -758,7 +759,7 @@ extern "C" int df_moe_layer(int dtype, const void* x, int ldx, int tokens, int H
              (long long)rows1, H);
     const int64_t limit = 1ll << 31;
     DF_CHECK(rows1 * ldw1 < limit && (int64_t)H * ldw2 < limit && (((int64_t)H + 127) / 128) * lds1 * sz < limit &&
-                 (((int64_t)N + 127) / 128) * lds2 * sz < limit && 
+                 (((int64_t)N + 127) / 128) * lds2 * sz < limit &&
                  (int64_t)tokens * top_k * (((int64_t)N + kStep - 1) & ~(int64_t)(kStep - 1)) * 2 < limit,
              DF_ERR_UNSUPPORTED, "%s: one expert's weights or scales, or the inner values of 2^31 bytes or more", fn);
     const size_t need = df_moe_layer_workspace_bytes(tokens, H, N, experts, top_k);

@@ -180,3 +180,11 @@ def test_block_scales_on_the_cpu():
     assert torch.equal(got, s.t()) and got.stride(0) == 8
     got = df.block_scales(s[:2], rows=200)
     assert got.shape == (3, 200) and torch.equal(got[:, 127], s[0]) and torch.equal(got[:, 128], s[1])
+
+
+@pytest.mark.parametrize("kw", [dict(M=2**31 - 1, N=1), dict(M=1, N=2**31 - 5), dict(M=2**31 - 1, N=2**31 - 1),
+                                dict(M=2**28 + 1, N=3)])
+@pytest.mark.parametrize("K", [0, 40])
+def test_outputs_of_too_many_tiles(kw, K):
+    """Sizes next to 2^31 are not lost in the count of tiles."""
+    refused(-2, "df_fp8_gemm_blocks", gemm(K=K, ldsa=2**31 - 16, ldsb=2**31 - 16, ldc=2**31 - 1, **kw))
