@@ -22,6 +22,8 @@
 //    equal shares of the units' steps and add what a unit's end gives to their own
 //    sums in LDS, per token, which meet at the end in wave order.  No atomics on
 //    values: results do not depend on timing.
+// Measured: those 48 tokens 62 us (routing 5, W1 33 for 160 MB, W2 23 for 80 MB); one
+// token to two of 32 experts (15 MB) 11.5, launches and the chain of a block's loads.
 // Widening is exact (e4m3 to bf16 or f16), sums are fp32, scales are applied to each
 // step's 128 products in fp32.
 //

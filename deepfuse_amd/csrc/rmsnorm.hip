@@ -15,6 +15,10 @@
 // values (32 lanes' of fp32), so their absmax is a DPP row's maximum.  Sums
 // are binary32, per lane in order, then in a fixed order over lanes and waves.
 //
+// Measured (bf16, residual in and sum out): 16384 x 1600 to codes in powers of two 38
+// us (184 MB, 4.8 TB/s where a copy reaches 5.2), backward 41 (210 MB, 5.1 TB/s), of which
+// 4 for the fold of gamma's partial sums; one row of 768 3.6, a launch.
+//
 // The reference has LayerNorm only (dnn/layers/layer_norm_layer.cu:26-90).
 #include <hip/hip_runtime.h>
 
@@ -64,7 +68,7 @@ __global__ __launch_bounds__(RT == 64 ? 256 : RT) void rms_forward_kernel(const 
     constexpr int GL = kScaleBlock / E;    // lanes that share a scale
     // The next row's loads before this row's arithmetic, gamma in registers; with codes
     // and a wave's four chunks a thread that took 158 registers, three waves a SIMD: no
-    // row ahead then, and gamma in LDS
+    // row ahead then, and gamma in LDS (16384 x 1600: 43 us, 40 so)
     constexpr bool AHEAD = OUT == OUT_Y || CH < 4 || RT > 64;
     __shared__ u32x4 glds[AHEAD ? 1 : CH][AHEAD ? 1 : RT];
     __shared__ float red[2][2][1][RT / 64];
