@@ -53,9 +53,12 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 // What routing leaves for the products, at the workspace's start: the pairs t * top + j
 // by expert, then token, and lists of units, an expert's next few of them, for either
 // product.
+struct alignas(16) MoeUnit {  // (one load)
+    int expert, first, count, none;  // (first: in `sorted`)
+};
 struct MoeUnits {
+    MoeUnit unit[kMoeUnits];  // W1's are followed by units of no tokens, up to its grid's end
     int n;
-    int expert[kMoeUnits], first[kMoeUnits], count[kMoeUnits];  // (first: in `sorted`)
 };
 struct MoePlan {
     MoeUnits up, down;
@@ -69,7 +72,7 @@ struct MoeArgs {
     MoePlan* plan;
     uint16_t* hi; uint16_t* lo;  // [pairs][ldh] bf16
     float* part; int* arrived;   // W2 split: [splits][tokens][H16] sums, blocks done per column tile
-    int tokens, H, N, experts, top, ldx, ldl, ldy, ldw1, ldw2, lds1, lds2, ldh, act, renormalize, x_dtype, l_dtype, splits, up_size, down_size;
+    int tokens, H, N, experts, top, ldx, ldl, ldy, ldw1, ldw2, lds1, lds2, ldh, act, renormalize, x_dtype, l_dtype, splits, up_size, down_size, up_most;
 };
 
 // ------------------------------------------------------------------ routing --
@@ -153,7 +156,7 @@ __device__ __forceinline__ void route_any(const MoeArgs& a, int t, int g, int& i
 __global__ __launch_bounds__(1024) void moe_route_kernel(const MoeArgs a) {
     __shared__ int ids[kMoePairs];
     __shared__ uint32_t taken[kMoeExperts][kMoeTokens / 32];  // which tokens take an expert
-    __shared__ int start[kMoeExperts], at_wave[3][4];
+    __shared__ int start[kMoeExperts], at_wave[3][4], up_units;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     for (int i = threadIdx.x; i < kMoeExperts * (kMoeTokens / 32); i += 1024) (&taken[0][0])[i] = 0;
     __syncthreads();
@@ -200,16 +203,16 @@ __global__ __launch_bounds__(1024) void moe_route_kernel(const MoeArgs a) {
         auto list = [&](MoeUnits& u, int size, int upto) {
             const int k = upto - (n + size - 1) / size;
             for (int i = 0; i * size < n; ++i) {
-                u.expert[k + i] = e;
-                u.first[k + i] = sum[0] - n + size * i;
-                u.count[k + i] = min(n - size * i, size);
+                u.unit[k + i] = {e, sum[0] - n + size * i, min(n - size * i, size), 0};
             }
             if (e == kMoeExperts - 1) u.n = upto;
         };
+        if (e == kMoeExperts - 1) up_units = sum[1];
         list(a.plan->up, a.up_size, sum[1]);
         list(a.plan->down, a.down_size, sum[2]);
     }
     __syncthreads();
+    for (int i = up_units + threadIdx.x; i < a.up_most; i += 1024) a.plan->up.unit[i] = {0, 0, 0, 0};
     for (int p = threadIdx.x; p < a.tokens * a.top; p += 1024) {
         const int x = ids[p], t = p / a.top;
         if (x < 0) continue;
@@ -279,7 +282,7 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
         for (int i = blockIdx.x * 256 + threadIdx.x; a.splits > 1 && i < (a.H + 15) / 16; i += gridDim.x * 256) a.arrived[i] = 0;
     if (n0 >= a.ldh) return;
     const int fr = lane & 15, fq = lane >> 4;
-    int e, count, pair = -1;
+    int e, count, first = 0, pair = -1;
     float weight1 = 0.0f;
     if (a.tokens == 1) {  // the unit is a choice
         int id;
@@ -295,14 +298,16 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
         count = 1;
         if (fr == 0) pair = unit;
     } else {
-        if (unit >= a.plan->up.n) return;
-        e = a.plan->up.expert[unit];
-        count = a.plan->up.count[unit];
-        if (fr < count) pair = a.plan->sorted[a.plan->up.first[unit] + fr];
+        const MoeUnit u = a.plan->up.unit[unit];
+        e = u.expert;
+        count = u.count;
+        first = u.first;
+        if (count == 0) return;
+        if (fr < count) pair = a.plan->sorted[first + fr];
     }
     if (n0 >= a.N) {  // only the zeros up to a step's end
         for (int i = threadIdx.x; i < count * COLS; i += 256) {
-            const int p = a.tokens == 1 ? unit : a.plan->sorted[a.plan->up.first[unit] + i / COLS];
+            const int p = a.tokens == 1 ? unit : a.plan->sorted[first + i / COLS];
             a.hi[(int64_t)p * a.ldh + n0 + i % COLS] = a.lo[(int64_t)p * a.ldh + n0 + i % COLS] = 0;
         }
         return;
@@ -330,21 +335,24 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
         u32x4 w[2][2], x[2][2];
         uint32_t s[2];
     };
-    auto load = [&](Step& s, int step) {
+    auto load_w = [&](Step& s, int step) {
         const bool live = step < blocks;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
-                s.w[g][h] = load16(rW, (live ? wo[g] : kOOB) + 64u * h, step * 128);
+            for (int g = 0; g < 2; ++g) s.w[g][h] = load16(rW, (live ? wo[g] : kOOB) + 64u * h, step * 128);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) s.s[g] = load_scale<E8>(rS, live ? so[g] : kOOB, step * a.lds1 * SZ);
+    };
+    auto load_x = [&](Step& s, int step) {
+        const bool live = step < blocks;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 if constexpr (ALIGNED) s.x[h][c] = load16(rX, (live ? xo : kOOB) + 128u * h + 16u * c, step * 256);
                 else s.x[h][c] = pair >= 0 && live ? load_chunk<uint16_t>(xr, step * 16 + 2 * fq + 8 * h + c, a.H) : u32x4{0, 0, 0, 0};
             }
-        }
-#pragma unroll
-        for (int g = 0; g < 2; ++g) s.s[g] = load_scale<E8>(rS, live ? so[g] : kOOB, step * a.lds1 * SZ);
     };
     v4f acc[2] = {};
     auto multiply = [&](Step& s, int step) {
@@ -378,12 +386,16 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
     };
     Step buf[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load(buf[u], w + u * W);
+    for (int u = 0; u < U; ++u) load_w(buf[u], w + u * W);  // while `pair` is on its way
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_x(buf[u], w + u * W);
     for (int s = w; s < blocks; s += W * U) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (s + u * W < blocks) multiply(buf[u], s + u * W);
-            load(buf[u], s + (u + U) * W);
+            load_w(buf[u], s + (u + U) * W);
+            load_x(buf[u], s + (u + U) * W);
         }
     }
 #pragma unroll
@@ -397,7 +409,7 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
     for (int g = 0; g < 2; ++g)
 #pragma unroll
         for (int x = 0; x < W; ++x) v[g] += red[x][g][c][i];
-    const int p = a.tokens == 1 ? unit : a.plan->sorted[a.plan->up.first[unit] + i];
+    const int p = a.tokens == 1 ? unit : a.plan->sorted[first + i];
     const float weight = a.tokens == 1 ? weight1 : a.weights[p];
     auto put = [&](int n, float h) {
         if (n >= a.ldh) return;
@@ -511,7 +523,8 @@ __device__ __forceinline__ float parts_sum(const v4f& a, const Lane& l) {
 // adds them in order.
 template <bool E8, int TG> __global__ __launch_bounds__(512) void moe_down_kernel(const MoeArgs a) {
     constexpr int W = 8, U = 2, SZ = E8 ? 1 : 4;
-    __shared__ int expert[kMoeUnits], first[kMoeUnits], count[kMoeUnits], sorted[kMoePairs];
+    __shared__ MoeUnit unit[kMoeUnits];
+    __shared__ int sorted[kMoePairs];
     __shared__ float sums[W][kMoeTokens][17];
     const Lane l = lane_parts();
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -520,19 +533,15 @@ template <bool E8, int TG> __global__ __launch_bounds__(512) void moe_down_kerne
     if (a.tokens == 1) {
         units = a.top;
         if ((int)threadIdx.x < units) {
-            expert[threadIdx.x] = a.ids[threadIdx.x];
-            first[threadIdx.x] = threadIdx.x;
-            count[threadIdx.x] = a.ids[threadIdx.x] >= 0;
+            const int id = a.ids[threadIdx.x];
+            unit[threadIdx.x] = {id, (int)threadIdx.x, id >= 0, 0};
             sorted[threadIdx.x] = threadIdx.x;
         }
     } else {
         const MoeUnits& u = a.plan->down;
+        static_assert(kMoeUnits == 512, "a thread takes one");
+        unit[threadIdx.x] = u.unit[threadIdx.x];  // (of any value from u.n on: not waited for)
         units = u.n;
-        for (int i = threadIdx.x; i < units; i += 512) {
-            expert[i] = u.expert[i];
-            first[i] = u.first[i];
-            count[i] = u.count[i];
-        }
         for (int i = threadIdx.x; i < pairs; i += 512) sorted[i] = a.plan->sorted[i];
     }
     for (int i = threadIdx.x & 63; i < a.tokens * 17; i += 64) sums[w][i / 17][i % 17] = 0.0f;
@@ -559,12 +568,12 @@ template <bool E8, int TG> __global__ __launch_bounds__(512) void moe_down_kerne
     uint32_t ho[TG];
     auto enter = [&]() {
         const int u = min(l_u, units - 1);
-        const int e = max(__builtin_amdgcn_readfirstlane(expert[u]), 0), n = __builtin_amdgcn_readfirstlane(count[u]);
+        const int e = max(__builtin_amdgcn_readfirstlane(unit[u].expert), 0), n = __builtin_amdgcn_readfirstlane(unit[u].count);
         rW = buffer(a.W2 + (int64_t)e * bytes2, n ? bytes2 : 0);
         rS = buffer(static_cast<const uint8_t*>(a.s2) + (int64_t)e * sbytes2, n ? sbytes2 : 0);
 #pragma unroll
         for (int t = 0; t < TG; ++t) {
-            const int pair = 4 * t + l.r < n ? sorted[first[u] + 4 * t + l.r] : -1;
+            const int pair = 4 * t + l.r < n ? sorted[unit[u].first + 4 * t + l.r] : -1;
             ho[t] = pair >= 0 ? ((uint32_t)pair * (uint32_t)a.ldh + (uint32_t)l.chunk) * 2u : kOOB;
         }
     };
@@ -607,7 +616,7 @@ template <bool E8, int TG> __global__ __launch_bounds__(512) void moe_down_kerne
                 // lane p adds row 4 p + r
                 const float even = l.p & 2 ? v[2] : v[0], odd = l.p & 2 ? v[3] : v[1];
                 const int i = 4 * t + l.fq;
-                if (i < count[m_u]) sums[w][sorted[first[m_u] + i] / a.top][4 * l.p + l.r] += l.p & 1 ? odd : even;
+                if (i < unit[m_u].count) sums[w][sorted[unit[m_u].first + i] / a.top][4 * l.p + l.r] += l.p & 1 ? odd : even;
             }
             m_s = 0;
             ++m_u;
@@ -698,10 +707,11 @@ template <bool E8> void launch(MoeArgs a, hipStream_t st) {
     const bool many = many_tokens(a.tokens, a.experts, a.top);
     a.up_size = 16;
     a.down_size = many ? 8 : 4;
+    a.up_most = (int)most_units(a.tokens, a.experts, a.top, a.up_size);
     if (a.tokens > 1) moe_route_kernel<<<1, 1024, 0, st>>>(a);
     // (columns up to a step's end, for its zeros; a multiple of 8 blocks: an expert's
     // units share an XCD's L2)
-    const dim3 up(a.ldh / (a.act != DF_ACT_GELU ? 16 : 32), (unsigned)most_units(a.tokens, a.experts, a.top, a.up_size));
+    const dim3 up(a.ldh / (a.act != DF_ACT_GELU ? 16 : 32), (unsigned)a.up_most);
     const dim3 down((a.H + 15) / 16, a.splits);
     if (a.x_dtype == DF_DTYPE_HALF) launch_up<h8, E8>(a, up, st);
     else launch_up<bf8, E8>(a, up, st);
@@ -775,7 +785,7 @@ extern "C" int df_moe_layer(int dtype, const void* x, int ldx, int tokens, int H
     int* const arrived = reinterpret_cast<int*>(part + (int64_t)splits * tokens * ((H + 15) & ~15));
     const MoeArgs a{x, logits, W1, s1, W2, s2, y, ids, weights, static_cast<MoePlan*>(ws), hi, lo, part,
                     arrived, tokens, H, N, experts, top_k, ldx, ld_logits, ldy, ldw1, ldw2, lds1, lds2, ldh, act, renormalize,
-                    dtype, logits_dtype, splits, 0, 0};
+                    dtype, logits_dtype, splits, 0, 0, 0};
     if (scale_kind == DF_SCALE_E8M0) launch<true>(a, as_stream(stream));
     else launch<false>(a, as_stream(stream));
     return launch_status(fn);
