@@ -129,6 +129,17 @@ def test_routing(dev, T, logits_dtype, renormalize):
                 assert (out[1][k % T] == -1).all() and not out[0][k % T].any()
 
 
+@pytest.mark.parametrize("kind", [E8, torch.float32])
+@pytest.mark.parametrize("T,N", [(1, 1200), (2, 1200), (1, 4100)])
+def test_few_tokens_in_shares(dev, T, N, kind):
+    """So many steps that blocks share W2's columns, for one token (whose routing is no
+    launch of its own) too; the blocks' counts start anew in each call."""
+    t = make(dev, T, 16, 100, N, "swiglu", torch.bfloat16, kind)
+    first = df.moe_layer(*t, 16)
+    check(first, *t, 16, "swiglu")
+    assert all(torch.equal(a, b) for a, b in zip(first, df.moe_layer(*t, 16)))
+
+
 @pytest.mark.parametrize("T", [1, 16, 64])
 def test_all_tokens_to_one_expert(dev, T):
     x, logits, *w = make(dev, T, 16, 200, 150)
