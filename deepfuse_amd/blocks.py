@@ -124,17 +124,27 @@ def quantize_blocks(x, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=False, square=F
     return q, s, qt, st
 
 
+def _rows_ld(t, rows: int, ld: int, red: int) -> int:
+    """The leading dimension of ``rows`` rows of codes ``ld`` apart, which are read up to
+    the next multiple of 16 behind ``red``; -1 where the last one's do not lie in the
+    tensor's memory."""
+    width, need = t.shape[-1], (red + 15) & ~15
+    if width < need and rows:  # (the rows' own width holds them else)
+        return -1 if t.storage_offset() + (rows - 1) * ld + need > t.untyped_storage().nbytes() else ld
+    # the stride of one row is arbitrary and says nothing
+    return (width + 15) & ~15 if rows <= 1 else ld
+
+
 def _codes(fn: str, name: str, t, red: int, ok: bool):
     """The leading dimension of an operand's codes (``ok``: their type is right)."""
     if not ok or t.dim() != 2:
         raise ValueError(f"{fn}: {name} {tuple(t.shape)} {t.dtype} is not a matrix of codes in its format")
     rows, width = t.shape
     ld, one = t.stride()
-    if rows <= 1:
-        ld = (width + 15) & ~15
+    ld = _rows_ld(t, rows, ld, red)
     if width < red or one != 1 and width > 1 or ld < width or ld & 15 or t.data_ptr() & 15:
         raise ValueError(f"{fn}: {name} {tuple(t.shape)} with strides {t.stride()} has no rows of {red} codes at "
-                         "multiples of 16 bytes")
+                         "multiples of 16 bytes, readable up to the next")
     return ld
 
 
@@ -216,10 +226,12 @@ def _expert_weights(fn: str, n: int, w, s, rows: int, cols: int, experts: int):
     if len(shape) != 3 or w.dtype is not _torch().float8_e4m3fn or shape[:2] != (experts, rows) or shape[2] < cols:
         raise ValueError(f"{fn}: w{n} is {shape} {w.dtype}, not e4m3 codes of {(experts, rows, cols)}")
     width, (each, ldw, one) = shape[2], w.stride()
-    if rows <= 1:
-        ldw = each if experts > 1 else (width + 15) & ~15
+    if rows <= 1 and experts > 1:
+        ldw = each
+    ldw = _rows_ld(w, experts * rows, ldw, cols)
     if one != 1 and width > 1 or ldw < width or ldw & 15 or w.data_ptr() & 15 or experts > 1 and each != rows * ldw:
-        raise ValueError(f"{fn}: w{n} with strides {w.stride()} has no rows at multiples of 16 bytes, expert behind expert")
+        raise ValueError(f"{fn}: w{n} with strides {w.stride()} has no rows at multiples of 16 bytes, readable up to "
+                         "the next, expert behind expert")
     if s.shape != (experts, blocks, rows):
         raise ValueError(f"{fn}: s{n} is {tuple(s.shape)}, not {(experts, blocks, rows)}")
     step, size = (3, 4) if s.dtype is _torch().float32 else (15, 1)
