@@ -313,7 +313,9 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
         return;
     }
     const int rows1 = GATED ? 2 * a.N : a.N, blocks = (a.H + 127) >> 7;
-    const __amdgpu_buffer_rsrc_t rW = buffer(a.W1 + (int64_t)e * rows1 * a.ldw1, (int64_t)rows1 * a.ldw1);
+    const int K16 = (a.H + 15) & ~15;
+    // (up to the last row's codes: its leading dimension may reach past the tensor)
+    const __amdgpu_buffer_rsrc_t rW = buffer(a.W1 + (int64_t)e * rows1 * a.ldw1, (int64_t)(rows1 - 1) * a.ldw1 + K16);
     const __amdgpu_buffer_rsrc_t rS =
         buffer(static_cast<const uint8_t*>(a.s1) + (int64_t)e * blocks * a.lds1 * SZ, (int64_t)blocks * a.lds1 * SZ);
     const __amdgpu_buffer_rsrc_t rX = buffer(a.x, ((int64_t)(a.tokens - 1) * a.ldx + a.H) * 2);
@@ -329,7 +331,6 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
     }
     const uint32_t xo = pair >= 0 ? (uint32_t)(pair / a.top) * (uint32_t)a.ldx * 2u + 32u * fq : kOOB;
     const uint16_t* const xr = static_cast<const uint16_t*>(a.x) + (int64_t)(max(pair, 0) / a.top) * a.ldx;
-    const int K16 = (a.H + 15) & ~15;
 
     struct Step {
         u32x4 w[2][2], x[2][2];
@@ -549,6 +550,7 @@ template <bool E8, int TG> __global__ __launch_bounds__(512) void moe_down_kerne
     __syncthreads();
     const int blocks = (a.N + 127) >> 7, steps = a.ldh / kStep, K16 = (a.N + 15) & ~15;
     const int64_t bytes2 = (int64_t)a.H * a.ldw2, sbytes2 = (int64_t)blocks * a.lds2 * SZ;
+    const int64_t range2 = (int64_t)(a.H - 1) * a.ldw2 + K16;  // (up to the last row's codes)
     const __amdgpu_buffer_rsrc_t rHi = buffer(a.hi, (int64_t)pairs * a.ldh * 2), rLo = buffer(a.lo, (int64_t)pairs * a.ldh * 2);
     uint32_t wo[4];
 #pragma unroll
@@ -570,7 +572,7 @@ template <bool E8, int TG> __global__ __launch_bounds__(512) void moe_down_kerne
     auto enter = [&]() {
         const int u = min(l_u, units - 1);
         const int e = max(__builtin_amdgcn_readfirstlane(unit[u].expert), 0), n = __builtin_amdgcn_readfirstlane(unit[u].count);
-        rW = buffer(a.W2 + (int64_t)e * bytes2, n ? bytes2 : 0);
+        rW = buffer(a.W2 + (int64_t)e * bytes2, n ? range2 : 0);
         rS = buffer(static_cast<const uint8_t*>(a.s2) + (int64_t)e * sbytes2, n ? sbytes2 : 0);
 #pragma unroll
         for (int t = 0; t < TG; ++t) {

@@ -575,7 +575,8 @@ int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const uint8_t* B, i
  *  W1 [experts][2 N or N][ldw1], W2 [experts][H][ldw2]: e4m3 codes, zero from H (N) up
  *      to the next multiple of 16; s1 [experts][ceil(H/128)][lds1], s2 [experts]
  *      [ceil(N/128)][lds2], scales as df_quantize_blocks's row codes', each expert's
- *      behind the one before.
+ *      behind the one before.  Of the last expert's last row nothing behind those
+ *      multiples is read.
  * Sums in fp32, the inner values kept to 16 bits of significand, y rounded once.
  * At most 64 tokens, 256 experts, top_k 16, and 2^31 bytes of codes an expert.
  * y and ids, weights [tokens * top_k] overlap no input.  ws:
