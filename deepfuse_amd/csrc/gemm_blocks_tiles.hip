@@ -217,14 +217,17 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
     v16f part[E8 ? 1 : FM][FN];
     float fsa[FM];
     float usb = 0.0f;
-    bool same = false;  // B's scales are the same over the wave's columns
+    // B's scales are the same over the wave's columns: those in the output, what lies
+    // behind is of any value
+    bool same = false;
+    int cols_in = 0;  // of the wave's part, in the unit
     auto fold_scales = [&](int step) __attribute__((always_inline)) {
         const float* p = reinterpret_cast<const float*>(ring + (step & (SLOTS - 1)) * SLOT);
 #pragma unroll
         for (int i = 0; i < FM; ++i) fsa[i] = p[wm * WR + FM * fr + i];
         const float b = p[256 + wn * 64 + lane];
         usb = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, b)));
-        same = __builtin_amdgcn_ballot_w64(b != usb) == 0;
+        same = __builtin_amdgcn_ballot_w64(lane < cols_in && b != usb) == 0;
     };
     auto fold = [&](int step, int i) __attribute__((always_inline)) {
         if (same) {
@@ -481,8 +484,9 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         asm volatile("" ::: "memory");
         after_epi = store_unit(u) ? 1 : 2;
     };
-    auto start = [&]() __attribute__((always_inline)) {
+    auto start = [&](const Unit& u) __attribute__((always_inline)) {
         if constexpr (!E8) {
+            cols_in = g.N - u.n0 - wn * 64;
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -499,7 +503,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         for (int r = 0; r < my_units; ++r) {
             const Unit u = unit_of(r);
             const float b = bias_of(u);
-            start();
+            start(u);
             quarter(Y{}, Q0{}, r0, r1);
             quarter(N{}, Q1{}, r1, r0);
             quarter(N{}, Q2{}, r0, r1);
@@ -525,7 +529,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         for (int r = 0; r < my_units; ++r) {
             const Unit u = unit_of(r);
             const float b = bias_of(u);
-            start();
+            start(u);
             half(Y{}, N{}, fa0, fb0, fa1, fb1);
             half(N{}, Y{}, fa1, fb1, fa0, fb0);
             for (int k = 1; k < steps; ++k) {
