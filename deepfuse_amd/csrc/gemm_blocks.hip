@@ -33,7 +33,7 @@ namespace {
 // rows to every four lanes, 64 address lookups (16 x 4800 x 1600 with tiles of 16 x
 // 16: 5.7 us, 5.1 so).  U steps are loaded ahead.
 template <int FA, bool E8, bool WIDE, int MT, int NT, int W, int U>
-__global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g, int c_dtype, int extent_a, int extent_b) {
+__global__ __launch_bounds__(64 * W, W == 4 && U == 2 ? 3 : 1) void blocks_small_kernel(const BlocksArgs g, int c_dtype, int extent_a, int extent_b) {
     constexpr int FB = E4M3;
     constexpr int ROWS = 16 * MT, COLS = 16 * NT;
     constexpr int RSTR = COLS + 4;  // row of a partial tile (floats)
@@ -82,7 +82,9 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
         u32x4 raw[NL];
         uint32_t sa[MT];
         typename std::conditional<E8, uint32_t, u32x4>::type sb[NT];
+        uint32_t column;  // fp32: the scale of column `lane`, if there is one
     };
+    const uint32_t oc = lane < min(g.N - n0, COLS) ? (uint32_t)lane * 4 : kOOB;
     auto load = [&](Step& s, int step) {
         const int k = step * 128;
         const bool in = k + lc < g.K;
@@ -107,6 +109,9 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
             else s.sb[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
                               rSB, k < g.K ? (sc + 4 * fq) * SZ : kOOB, 0, 0));
         }
+        if constexpr (!E8)
+            s.column = __builtin_amdgcn_raw_buffer_load_b32(
+                rSB, k < g.K && oc != kOOB ? (uint32_t)step * (uint32_t)g.ldsb * SZ + oc : kOOB, 0, 0);
     };
     // accumulators are C^T: lane l holds row l%16 and columns 4*(l/16) .. +4
     v4f acc[MT][NT];
@@ -123,7 +128,9 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
         const u32x4 y = *reinterpret_cast<const u32x4*>(slab + t * 2048 + rd1);
         return v8i{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
     };
-    auto multiply = [&](const Step& s) {
+    // keep: 0 takes the step's products times 0
+    auto products = [&](const Step& s, auto is_far, uint32_t keep) {
+        constexpr bool FAR = decltype(is_far)::value;
         lanes_meet();  // the step before has read the slab
         v8i fb[NT];
 #pragma unroll
@@ -155,12 +162,28 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
                 if constexpr (E8) {
                     acc[i][j] = p;
                 } else {
+                    const float sa = __uint_as_float(s.sa[i]);
 #pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        acc[i][j][y] = __builtin_fmaf(p[y] * __uint_as_float(s.sb[j][y]), __uint_as_float(s.sa[i]), acc[i][j][y]);
+                    for (int y = 0; y < 4; ++y) {
+                        const float sb = __uint_as_float(s.sb[j][y] & keep);
+                        acc[i][j][y] = FAR ? add_scaled_far(p[y], sa, sb, acc[i][j][y]) : __builtin_fmaf(p[y] * sb, sa, acc[i][j][y]);
+                    }
                 }
             }
         }
+    };
+    // Steps at which some of B's scales are far come behind the others, in a loop of their
+    // own: in this one their code took 60 registers more.  Here they are left out, or add 0
+    // where the next step's loads are to go out between this one's products and a branch
+    // around these held them back (64 x 64 tiles: 1024 x 1600 x 6400 32.7 us with it, 27.6
+    // so; without a look at the scales 26.1).
+    bool some_far = false;
+    auto far = [&](const Step& s) { return !E8 && __builtin_amdgcn_ballot_w64(scale_far(s.column)) != 0; };
+    auto multiply = [&](const Step& s) {
+        const bool f = far(s);
+        if constexpr (!E8) some_far |= f;
+        if constexpr (U == 1) products(s, std::false_type{}, f ? 0u : ~0u);
+        else if (!f) products(s, std::false_type{}, ~0u);
     };
     const int nk = (g.K + 127) >> 7;
     Step buf[U];
@@ -171,6 +194,12 @@ __global__ __launch_bounds__(64 * W) void blocks_small_kernel(const BlocksArgs g
         for (int u = 0; u < U; ++u) {
             if (s + u * W < nk) multiply(buf[u]);
             load(buf[u], s + (u + U) * W);
+        }
+    }
+    if (some_far) {
+        for (int s = w; s < nk; s += W) {
+            load(buf[0], s);
+            if (far(buf[0])) products(buf[0], std::true_type{}, ~0u);
         }
     }
     __syncthreads();  // the slabs are read before sums go over them

@@ -41,6 +41,23 @@ template <int FMT> __device__ __forceinline__ bf8 widen8_scaled(uint32_t lo, uin
     return bf8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
 }
 
+// fp32 scales.  A step's product p of 128 codes is 0 or 2^-25 to 2^32 in size: p * sb is in
+// binary32's normal range unless B's scale is far (0 is not), and so is sa * sb if both lie
+// in the middle.  A fused multiply-add with the other factor then rounds once.  Products at
+// far scales take binary64, which holds all three factors'.
+__device__ __forceinline__ bool scale_far(uint32_t bits) {  // not 0 nor 2^-100 .. 2^95, infinities and NaN too
+    constexpr uint32_t least = 27u << 23, most = 222u << 23;
+    bits &= 0x7FFFFFFFu;
+    return bits != 0u && bits - least > most - least;
+}
+__device__ __forceinline__ bool scale_in_the_middle(uint32_t bits) {  // 2^-62 .. 2^62, positive
+    constexpr uint32_t least = 65u << 23, most = 189u << 23;
+    return bits - least <= most - least;
+}
+__device__ __forceinline__ float add_scaled_far(float p, float sa, float sb, float acc) {
+    return (float)__builtin_fma((double)p * (double)sa, (double)sb, (double)acc);
+}
+
 // bytes of `blocks` blocks' scales of a matrix of `rows` rows: what may be read
 inline int64_t scales_extent(int64_t blocks, int64_t ld, int64_t rows, int bytes) {
     const int64_t row = (rows * bytes + 15) & ~(int64_t)15;

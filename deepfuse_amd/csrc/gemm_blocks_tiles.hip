@@ -14,7 +14,8 @@
 //  - E8, fp32 outputs (WIDE): scales go into the widening to bf16.
 //  - fp32 scales: a step's products are made from zero and folded into the sums
 //    while the next step's are under way: one fma a value, if B's scales are the
-//    same over the wave's 64 columns (weights in squares), else a product more.
+//    same over the wave's 64 columns (weights in squares), else a product more; in
+//    binary64 before that, where some of B's are far (gemm_blocks.hpp).
 // Bound by the matrix units' feed, as the persistent kernel without blocks, and by the
 // last, partly filled round of tiles: 16384 x 6400 x 1600 (M, N, K), bf16 out, powers of
 // two, 170 us (1.97 PFLOP/s; one scale per tensor: 164), 16384 x 1600 x 6400 161 (156).
@@ -217,17 +218,28 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
     v16f part[E8 ? 1 : FM][FN];
     float fsa[FM];
     float usb = 0.0f;
-    // B's scales are the same over the wave's columns: those in the output, what lies
-    // behind is of any value
-    bool same = false;
-    int cols_in = 0;  // of the wave's part, in the unit
-    auto fold_scales = [&](int step) __attribute__((always_inline)) {
+    // (not by what lies behind the output's rows and columns, which is of any value)
+    bool same = false;  // B's scales are the same over the wave's columns, and all in the middle
+    bool far = false;   // (if not same) some of B's are scale_far()
+    uint64_t rows_in[FM], cols_in = 0;  // lanes whose row i, whose column is in the output
+    float bcol = 0.0f;
+    // a step's scales, read and looked at under its last products: its fold then waits for
+    // neither
+    auto read_scales = [&](int step) __attribute__((always_inline)) {
         const float* p = reinterpret_cast<const float*>(ring + (step & (SLOTS - 1)) * SLOT);
 #pragma unroll
         for (int i = 0; i < FM; ++i) fsa[i] = p[wm * WR + FM * fr + i];
-        const float b = p[256 + wn * 64 + lane];
-        usb = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, b)));
-        same = __builtin_amdgcn_ballot_w64(lane < cols_in && b != usb) == 0;
+        bcol = p[256 + wn * 64 + lane];
+    };
+    auto see_scales = [&]() __attribute__((always_inline)) {
+        const uint32_t bu = (uint32_t)__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, bcol));
+        usb = __uint_as_float(bu);
+        uint64_t odd = __builtin_amdgcn_ballot_w64(bcol != usb) & cols_in;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+            odd |= __builtin_amdgcn_ballot_w64(!scale_in_the_middle(__float_as_uint(fsa[i]))) & rows_in[i];
+        same = odd == 0 && scale_in_the_middle(bu);
+        far = !same && (__builtin_amdgcn_ballot_w64(scale_far(__float_as_uint(bcol))) & cols_in) != 0;
     };
     auto fold = [&](int step, int i) __attribute__((always_inline)) {
         if (same) {
@@ -252,6 +264,26 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         }
     };
 
+    // A step with far scales is folded here; the fold that follows adds 0
+    auto fold_far = [&](int step) __attribute__((always_inline)) {
+        if (__builtin_expect(!far, 1)) return;
+        const float* p = reinterpret_cast<const float*>(ring + (step & (SLOTS - 1)) * SLOT) + 256 + wn * 64 + 8 * (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        acc[i][j][4 * x + y] =
+                            add_scaled_far(part[i][j][4 * x + y], fsa[i], p[16 * x + 2 * y + j], acc[i][j][4 * x + y]);
+            fsa[i] = 0.0f;
+        }
+        usb = 0.0f;
+        same = true;
+    };
+
     // ---- fp8 products: half-steps of 64 bytes; the MFMAs on (fa, fb) while the
     // next half-step's fragments are read into (na, nb); the order frozen as in
     // gemm_fp8.hip (reads under the first MFMAs, the DMA of odd half-steps spread
@@ -266,7 +298,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         constexpr int NR = 2 * NF;
         u32x4 frag[NR];
         int nsa = sa, nsb = sb;
-        if constexpr (!E8 && !ODD && !FIRST) fold_scales(c_g - 1);
+        if constexpr (!E8 && ODD) read_scales(c_g);
         each<NM>([&](auto xc) __attribute__((always_inline)) {
             constexpr int x = decltype(xc)::value, i = x >> 1, j = x & 1;
             const v16f z = {};
@@ -287,6 +319,7 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
 #pragma unroll
                 for (int d = ND * x / NM; d < ND * (x + 1) / NM; ++d) dissue_one(d);
             }
+            if constexpr (!E8 && ODD && x == NM - 1) see_scales();
             __builtin_amdgcn_sched_barrier(0);
         });
 #pragma unroll
@@ -306,6 +339,8 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
                 for (int i = 0; i < FM; ++i)
 #pragma unroll
                     for (int j = 0; j < FN; ++j) hold(acc[i][j]);
+            } else {
+                fold_far(c_g);
             }
             sa = nsa;
             sb = nsb;
@@ -336,11 +371,11 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
         __builtin_amdgcn_sched_barrier(0);
         if (Q == 3) next_step();
         const int stage = Q == 3 ? (c_st + 1 == NS ? 0 : c_st + 1) : c_st;
+        if constexpr (!E8 && Q == 3) read_scales(c_g);
 #pragma unroll
         for (int f = 0; f < NF; ++f) nxt[f] = rd(stage, f, ((Q + 1) >> 1) & 1, (Q + 1) & 1);
         // (read anew each step: kept from the step before, they took 80 registers' copies)
         if constexpr (E8 && Q == 0) wide_scales(c_g);
-        if constexpr (!E8 && Q == 0 && !FIRST) fold_scales(c_g - 1);
         each<2>([&](auto sc) __attribute__((always_inline)) {
             constexpr int s = decltype(sc)::value;
             bf8 wb[FN];
@@ -366,6 +401,10 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
                 });
             });
         });
+        if constexpr (!E8 && Q == 3) {
+            see_scales();
+            fold_far(c_g);
+        }
         if (Q == 3) {
             ++c_g;
             c_st = stage;
@@ -476,7 +515,6 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
     };
     auto finish = [&](const Unit& u, float b) __attribute__((always_inline)) {
         if constexpr (!E8) {
-            fold_scales(c_g - 1);
 #pragma unroll
             for (int i = 0; i < FM; ++i) fold(c_g - 1, i);
         }
@@ -486,7 +524,9 @@ __global__ __launch_bounds__(512, 1) void blocks_tile_kernel(const BlocksArgs g,
     };
     auto start = [&](const Unit& u) __attribute__((always_inline)) {
         if constexpr (!E8) {
-            cols_in = g.N - u.n0 - wn * 64;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) rows_in[i] = __builtin_amdgcn_ballot_w64(u.m0 + wm * WR + FM * fr + i < g.M);
+            cols_in = __builtin_amdgcn_ballot_w64(u.n0 + wn * 64 + lane < g.N);
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll

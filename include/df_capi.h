@@ -551,7 +551,8 @@ int df_quantize_blocks(int dtype, const void* x, int rows, int cols, int ldx, in
  * ones (see df_fp8_experts_fwd).  K == 0 gives the bias, or 0.  C overlaps no
  * operand and holds fewer than 2^23 tiles of 32 x 32.  Powers of two reach an fp32
  * output through bf16: exact while codes times scales stay in its range (2^-133 ..
- * 2^128).
+ * 2^128).  fp32 scales are of any finite size: sa * sb * products is right where it
+ * is in fp32's range itself.
  *   forward : Xq, sx (row codes) and Wq, sw      ; M tokens, N outputs, K inputs
  *   dX      : dYq, sdy (row codes) and Wtq, swt  ; M tokens, N inputs, K outputs
  *   dW      : dYtq, sdyt and Xtq, sxt            ; M outputs, N inputs, K tokens */

@@ -1,5 +1,6 @@
-"""Products with fp32 scales per 128 whose neighbours in memory are unusual: the values
-behind the last row's and column's scales change no bit.
+"""Products with fp32 scales per 128 whose size, or whose neighbours in memory, are
+unusual: scales whose product with each other or with a step's sum leaves binary32's
+range though the result does not, zero scales, and values behind the last column.
 
 Bars as in test_gpu_blocks_gemm.py; a result below binary32's normal range adds its
 step, 2^-149, once for each of K / 128 blocks and eight waves.
@@ -43,6 +44,36 @@ def check(got, a, sa, b, sb, K):
         bar = torch.finfo(got.dtype).eps / 2 * want.abs() + 2.0 ** -10 * size + torch.finfo(got.dtype).smallest_normal
     assert want.abs().max() < 2.0 ** 126  # (no result is near the type's end)
     assert ((got.double() - want).abs() <= bar).all()
+
+
+@pytest.mark.parametrize("square", [False, True])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_far_scales(dev, out, square, M, N, K):
+    g = torch.Generator(device=dev).manual_seed(M)
+    nb = -(-K // 128)
+    # large codes: sums near 2^20; small ones: near 2^-10
+    for lo, hi, ea, eb in ((0x70, 0x7E, -120, -20), (0x70, 0x7E, -20, -120), (0x70, 0x7E, -110, 112), (0x70, 0x7E, 112, -110),
+                           (1, 4, 66, 64), (1, 16, 120, -122), (1, 16, -122, 120), (0x70, 0x7E, -140, 60), (0x70, 0x7E, 60, -140)):
+        a, b = codes(g, M, K, lo, hi, dev), codes(g, N, K, lo, hi, dev)
+        sa, sb = scales(g, nb, M, ea, dev, False), scales(g, nb, N, eb, dev, square)
+        check(df.gemm_blocks(a, sa, b, sb, K, out_dtype=out), a, sa, b, sb, K)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_far_scales_among_others(dev, out, M, N, K):
+    """Some far, some zero, most of them ordinary; blocks of zero codes at scales whose
+    product is infinite."""
+    g = torch.Generator(device=dev).manual_seed(N)
+    nb = -(-K // 128)
+    a, b = codes(g, M, K, 0x30, 0x48, dev), codes(g, N, K, 0x30, 0x48, dev)
+    sa, sb = scales(g, nb, M, 0, dev, False), scales(g, nb, N, -10, dev, False)
+    sa[0, M // 2], sa[nb - 1, M - 1], sa[1, 0] = 2.0 ** -110, 2.0 ** 70, 0.0
+    sb[0, N // 3], sb[1, N - 1], sb[nb - 1, 1] = 2.0 ** -115, 2.0 ** -149, 0.0
+    a.view(torch.uint8)[M // 2, 128:256], sa[1, M // 2] = 0, 2.0 ** 100
+    b.view(torch.uint8)[2, 128:256], sb[1, 2] = 0, 2.0 ** 100
+    check(df.gemm_blocks(a, sa, b, sb, K, out_dtype=out), a, sa, b, sb, K)
 
 
 @pytest.mark.parametrize("square", [False, True])
