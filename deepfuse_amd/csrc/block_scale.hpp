@@ -52,13 +52,24 @@ template <int FMT, bool E8> __device__ __forceinline__ BlockDiv block_div(uint32
     return b;
 }
 
-// Four values to four codes.  PLAIN: none is NaN and (fp32 scales) the division
+// Four values to four codes, a zero's being zero at any scale.  PLAIN: none is NaN and (fp32 scales) the division
 // is in its fast range; the caller asks for a whole wave at once.
 template <int FMT, bool E8, bool PLAIN>
 __device__ __forceinline__ uint32_t block_quant4(const float* v, const QDiv& q) {
     if constexpr (!E8) {
-        if constexpr (PLAIN) return quant4_nonan<FMT>(v[0], v[1], v[2], v[3], q);
-        else return encode2_hw<FMT>(qdiv(v[0], q), qdiv(v[1], q)) | (encode2_hw<FMT>(qdiv(v[2], q), qdiv(v[3], q)) << 16);
+        if constexpr (PLAIN) {
+            return quant4_nonan<FMT>(v[0], v[1], v[2], v[3], q);
+        } else {
+            // (absmax / fmax is 0 below 2^-150 fmax, and 0 / 0 NaN: the zero itself then, as a
+            // NaN is its own quotient)
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = qdiv(v[i], q);
+                x[i] = x[i] != x[i] ? v[i] : x[i];
+            }
+            return encode2_hw<FMT>(x[0], x[1]) | (encode2_hw<FMT>(x[2], x[3]) << 16);
+        }
     } else if constexpr (PLAIN) {
         constexpr float fm = Fp8<FMT>::fmax;
         float x[4];

@@ -522,6 +522,9 @@ int df_fp8_experts_dw(const uint8_t* dYtq, int lddyt, const uint8_t* Xtq, int ld
  * 16-byte aligned, and each block's scales are readable up to the next multiple of
  * 16 bytes (of any value).  Kinds (df_scale_kind):
  *   DF_SCALE_F32  : absmax / FMAX, 1 where the absmax is 0 (rule D1/D2 of a block).
+ *                   It rounds to 0 where the absmax is below FMAX * 2^-150 (3e-43
+ *                   for e4m3): such a block's codes are zero for zeros and +-max for
+ *                   the others, and stand for 0.
  *   DF_SCALE_E8M0 : the smallest power of two that keeps absmax / s <= FMAX, as
  *                   2^(byte - 127), at least 2^-127; 1 (byte 127) where the absmax
  *                   is 0.  x / s is exact.  Byte 255 is no scale.
