@@ -118,20 +118,22 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(const BlockQuant a
     const int64_t r0 = (int64_t)blockIdx.y * kScaleBlock;
     const int c0 = blockIdx.x * kScaleBlock, c = c0 + 8 * tc;
     const int64_t r = r0 + 8 * tr;
-    const T* const x = static_cast<const T*>(a.x);
+    // columns from the square before on: an offset in a row has 32 bits, its length more
+    const int cb = max(c0 - kScaleBlock, 0), cols = a.cols - cb;
+    const T* const x = static_cast<const T*>(a.x) + cb;
 
     u32x4 raw[8][8 / E];
 #pragma unroll
     for (int p = 0; p < 8; ++p)
 #pragma unroll
         for (int h = 0; h < 8 / E; ++h)
-            raw[p][h] = r + p < a.rows ? load_chunk<T>(x + (r + p) * a.ldx, c / E + h, a.cols) : u32x4{0, 0, 0, 0};
+            raw[p][h] = r + p < a.rows ? load_chunk<T>(x + (r + p) * a.ldx, (c - cb) / E + h, cols) : u32x4{0, 0, 0, 0};
     float v[8][8];
 #pragma unroll
     for (int p = 0; p < 8; ++p)
 #pragma unroll
         for (int h = 0; h < 8 / E; ++h) {
-            raw[p][h] = place_chunk<T>(raw[p][h], c / E + h, a.cols);
+            raw[p][h] = place_chunk<T>(raw[p][h], (c - cb) / E + h, cols);
             El<T>::widen(raw[p][h], v[p] + h * E);
         }
 

@@ -82,7 +82,7 @@ template <typename T> __device__ __forceinline__ u32x4 load_chunk(const T* row, 
     const int c = j * E;
     u32x4 w = {0, 0, 0, 0};
     if (cols >= E) {
-        // (a 32-bit offset on the row's address, the same for every tensor)
+        // (a 32-bit offset on the row's address, the same for every tensor: rows below 4 GiB)
         const uint32_t at = (uint32_t)min(c, cols - E) * (uint32_t)sizeof(T);
         if (c < cols) w = *reinterpret_cast<const u32x4_el*>(reinterpret_cast<const char*>(row) + at);
     } else if (j == 0) {  // a row shorter than a chunk
