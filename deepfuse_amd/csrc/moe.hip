@@ -698,15 +698,20 @@ int64_t most_units(int tokens, int experts, int top, int size) {
 }
 
 // Blocks that share a column tile of W2: as many as make two of them for each of 256
-// CUs, each wave with two steps at least; one, unless sharing spares a wave six steps:
-// a step takes 0.8 us, the blocks' meeting 4 (4 tokens to two of 32 experts, 1600 wide:
-// 9.0 us with one, 10.8 with three; 8 tokens: 14.6 with one, 12.4 with five).
+// CUs, each wave with two steps at least; one, unless sharing spares a wave six steps, or
+// more where more tokens' sums meet: a step takes 0.7 us, the blocks' meeting 4 for a few
+// tokens and 7 for 64.  us with one and shared, powers of two, 1600 wide: 4 tokens to two
+// of 32 experts (W2 alone) 9.0 and 10.8 with three, 8 tokens 14.6 and 12.4 with five; the
+// layer, 64 tokens to eight of 8 experts 113 and 90 with five, to two of 8 45.6 and 45.5
+// (fp32 scales 57.4 and 51.6), to four of 16 with N = 400 34.2 and 38.1 with four; 32
+// tokens to two of 4, 768 and N = 3000, 37.2 and 34.6 with six.
 int down_splits(int tokens, int H, int N, int experts, int top) {
-    const int64_t tiles = (H + 15) / 16, pairs = (int64_t)tokens * top;
-    const int64_t units = tokens == 1 ? top : std::min<int64_t>(experts, pairs);
-    const int64_t want = 512 / tiles, most = units * ((N + kStep - 1) / kStep) / (8 * 2);
-    const int64_t n = std::max<int64_t>(1, std::min(want, most)), steps = units * ((N + kStep - 1) / kStep);
-    return steps - steps / n < 8 * 6 ? 1 : (int)n;
+    const int64_t tiles = (H + 15) / 16, pairs = (int64_t)tokens * top, size = many_tokens(tokens, experts, top) ? 8 : 4;
+    // (dealt evenly: an expert's tokens may be several units)
+    const int64_t units = tokens == 1 ? top : std::max(std::min<int64_t>(experts, pairs), (pairs + size - 1) / size);
+    const int64_t steps = units * ((N + kStep - 1) / kStep), want = 512 / tiles, most = steps / (8 * 2);
+    const int64_t n = std::max<int64_t>(1, std::min(want, most));
+    return steps - steps / n < 8 * std::max<int64_t>(6, tokens / 6) ? 1 : (int)n;
 }
 
 template <bool E8> void launch(MoeArgs a, hipStream_t st) {
