@@ -130,6 +130,7 @@ _SIGS = {
                                     _vp, _c_int, _vp, _c_int, _vp]),
     "df_fp8_gemm_blocks": (_c_int, [_c_int, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _vp,
                                     _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp]),
+    "df_fp8_gemm_blocks_plan": (_c_int, [_c_int] * 5 + [_vp]),
     "df_moe_layer_workspace_bytes": (_c_sz, [_c_int] * 5),
     "df_moe_layer": (_c_int, [_c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _c_int,
                               _vp, _c_int, _vp, _c_int, _c_int, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp,
@@ -1178,5 +1179,5 @@ def quantize_experts(w, fmt: Fmt = Fmt.E4M3, want_q=True, want_qt=True):
 
 
 # fp8 with a scale per 128 values, the root-mean-square norm
-from .blocks import (block_scales, gemm_blocks, moe_layer, quantize_blocks, quantize_experts_blocks,  # noqa: E402,F401
-                     rmsnorm_backward, rmsnorm_forward, rmsnorm_quantize)
+from .blocks import (BlocksKernel, block_scales, gemm_blocks, gemm_blocks_plan, moe_layer, quantize_blocks,  # noqa: E402,F401
+                     quantize_experts_blocks, rmsnorm_backward, rmsnorm_forward, rmsnorm_quantize)

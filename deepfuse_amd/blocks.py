@@ -10,6 +10,8 @@ brings scales from elsewhere into that form.
 """
 from __future__ import annotations
 
+import ctypes
+import enum
 import functools
 
 from . import (Fmt, _check_gpu, _check_like, _fits, _in_dtype, _INT_MAX, _on, _plain, _ptr, _row_vector, _rows,
@@ -188,6 +190,29 @@ def gemm_blocks(a_q, sa, b_q, sb, K: int, bias=None, out_dtype=None, out=None):
              ldsa, sb.data_ptr(), ldsb, bias_dt, None if bias is None else bias.data_ptr(), _in_dtype(out), out.data_ptr(),
              ldc, _stream())
     return out
+
+
+class BlocksKernel(enum.IntEnum):
+    """DF_BLOCKS_KERNEL_* of include/df_capi.h: by tiles."""
+    T16 = 0
+    T16X32 = 1
+    T32 = 2
+    T32_LONG = 3
+    T64 = 4
+    T128 = 5
+    T256X128 = 6
+    T256 = 7
+
+
+def gemm_blocks_plan(M: int, N: int, K: int, scale_dtype=None, out_dtype=None) -> BlocksKernel:
+    """The kernel that :func:`gemm_blocks` takes for these sizes on the current GPU
+    (df_fp8_gemm_blocks_plan)."""
+    fn, torch = "gemm_blocks_plan", _torch()
+    kind = _kind(fn, scale_dtype or torch.float8_e8m0fnu)
+    out = ctypes.c_int()
+    call("df_fp8_gemm_blocks_plan", M, N, K, kind, _in_dtype(torch.empty(0, dtype=out_dtype or torch.bfloat16)),
+         ctypes.byref(out))
+    return BlocksKernel(out.value)
 
 
 # ----------------------------------------------------------------------------

@@ -268,55 +268,54 @@ __global__ __launch_bounds__(64 * W, W == 4 && U == 2 ? 3 : 1) void blocks_small
 //   256 x 256: 2048 x 6400 x 1600 25.2, 1024 x 1600 x 6400 60
 // and likewise with fp32 outputs or scales, whose steps take longer on large tiles
 // (128 x 128, 1024 x 1600 x 6400: 49 and 37.5; 64 x 64: 32 and 28.7).
-enum : int { SMALL_16 = -1, SMALL_16X32 = -2, SMALL_32 = -3, SMALL_64 = -4 };
 struct BlocksPlan {
-    int fm;  // of the large tiles, or SMALL_*
+    int kernel;  // DF_BLOCKS_KERNEL_*
     int grid;
 };
 BlocksPlan plan(const BlocksArgs& g, bool e8, bool wide) {
     const int cus = std::max(device_cu_count(), 1);
     const double steps = (double)((g.K + 127) / 128);
     auto tiles = [&](int r, int c) { return (int64_t)((g.M + r - 1) / r) * ((g.N + c - 1) / c); };
-    if (g.K == 0) return {SMALL_32, (int)tiles(32, 32)};
-    if (tiles(16, 16) <= cus) return {SMALL_16, (int)tiles(16, 16)};
-    if (g.M <= 16) return {SMALL_16X32, (int)tiles(16, 32)};
+    if (g.K == 0) return {DF_BLOCKS_KERNEL_32, (int)tiles(32, 32)};
+    if (tiles(16, 16) <= cus) return {DF_BLOCKS_KERNEL_16, (int)tiles(16, 16)};
+    if (g.M <= 16) return {DF_BLOCKS_KERNEL_16X32, (int)tiles(16, 32)};
     // fp32 scales, fp32 outputs: 0 to 3
     const int kind = (e8 ? 0 : 2) + (wide ? 1 : 0);
     const double slower[4] = {1.0, 1.08, 1.1, 1.2};
     double best = 3.2 + std::max(0.1 * steps, slower[kind] * (double)tiles(32, 32) * (0.56e-3 * steps + 1.9e-3));
-    BlocksPlan p{SMALL_32, (int)tiles(32, 32)};
-    auto offer = [&](int fm, int64_t n, double t) {
+    BlocksPlan p{g.K > 8 * 128 ? DF_BLOCKS_KERNEL_32_LONG : DF_BLOCKS_KERNEL_32, (int)tiles(32, 32)};
+    auto offer = [&](int kernel, int64_t n, double t) {
         if (t < best) {
             best = t;
-            p = {fm, (int)n};
+            p = {kernel, (int)n};
         }
     };
     if (kind != 3)
-        offer(SMALL_64, tiles(64, 64),
+        offer(DF_BLOCKS_KERNEL_64, tiles(64, 64),
               3.5 + slower[kind] * (0.25 * steps + (double)tiles(64, 64) * (0.41e-3 * steps + 8.2e-3)));
     // rounds of blocks over the CUs, a step's time and a tile's besides
-    auto large = [&](int fm, int r, int c, const double* step, const double* over) {
+    auto large = [&](int kernel, int r, int c, const double* step, const double* over) {
         const int64_t n = tiles(r, c), rounds = (n + cus - 1) / cus;
-        offer(fm, std::min<int64_t>(n, cus), 3.0 + (double)rounds * (step[kind] * steps + over[kind]));
+        offer(kernel, std::min<int64_t>(n, cus), 3.0 + (double)rounds * (step[kind] * steps + over[kind]));
     };
     const double s1[4] = {0.39, 0.83, 0.62, 1.03}, o1[4] = {2.6, 3.0, 2.0, 3.0};
     const double s2[4] = {0.75, 1.28, 1.02, 1.75}, o2[4] = {3.0, 4.5, 2.5, 4.0};
     const double s4[2] = {1.1, 2.2}, o4[2] = {6.0, 8.0};
-    large(1, 128, 128, s1, o1);
-    large(2, 256, 128, s2, o2);
-    if (e8) large(4, 256, 256, s4, o4);
+    large(DF_BLOCKS_KERNEL_128, 128, 128, s1, o1);
+    large(DF_BLOCKS_KERNEL_256X128, 256, 128, s2, o2);
+    if (e8) large(DF_BLOCKS_KERNEL_256, 256, 256, s4, o4);
     return p;
 }
 
 template <int FA, bool E8, bool WIDE>
 void launch_small(const BlocksPlan& p, const BlocksArgs& g, int c_dtype, int ea, int eb, hipStream_t st) {
-    if (p.fm == SMALL_16)
+    if (p.kernel == DF_BLOCKS_KERNEL_16)
         blocks_small_kernel<FA, E8, WIDE, 1, 1, 8, 2><<<p.grid, 512, 0, st>>>(g, c_dtype, ea, eb);
-    else if (p.fm == SMALL_16X32)
+    else if (p.kernel == DF_BLOCKS_KERNEL_16X32)
         blocks_small_kernel<FA, E8, WIDE, 1, 2, 8, 1><<<p.grid, 512, 0, st>>>(g, c_dtype, ea, eb);
-    else if (p.fm == SMALL_32 && g.K > 8 * 128)
+    else if (p.kernel == DF_BLOCKS_KERNEL_32_LONG)
         blocks_small_kernel<FA, E8, WIDE, 2, 2, 8, 1><<<p.grid, 512, 0, st>>>(g, c_dtype, ea, eb);
-    else if (p.fm == SMALL_32)
+    else if (p.kernel == DF_BLOCKS_KERNEL_32)
         blocks_small_kernel<FA, E8, WIDE, 2, 2, 4, 2><<<p.grid, 256, 0, st>>>(g, c_dtype, ea, eb);
     else if constexpr (E8 || !WIDE)
         blocks_small_kernel<FA, E8, WIDE, 4, 4, 4, 1><<<p.grid, 256, 0, st>>>(g, c_dtype, ea, eb);
@@ -327,6 +326,27 @@ void launch_small(const BlocksPlan& p, const BlocksArgs& g, int c_dtype, int ea,
 }  // namespace dfk
 
 using namespace dfk;
+
+// (blocks of small tiles: fewer than 2^32 threads; those of M <= 16 and of large tiles
+// are fewer)
+static bool tiles_fit(int M, int N) { return ((M + 31ll) / 32) * ((N + 31ll) / 32) < (1ll << 23); }
+
+extern "C" int df_fp8_gemm_blocks_plan(int M, int N, int K, int scale_kind, int c_dtype, int* kernel) {
+    clear_error();
+    const char* fn = "df_fp8_gemm_blocks_plan";
+    DF_CHECK(kernel, DF_ERR_INVALID, "%s: NULL output", fn);
+    DF_CHECK(M > 0 && N > 0 && K >= 0, DF_ERR_INVALID, "%s: bad sizes (M=%d, N=%d, K=%d)", fn, M, N, K);
+    DF_CHECK(scale_kind_ok(scale_kind), DF_ERR_INVALID, "%s: bad scale kind %d", fn, scale_kind);
+    DF_CHECK(c_dtype == DF_DTYPE_FLOAT32 || c_dtype == DF_DTYPE_BFLOAT16 || c_dtype == DF_DTYPE_HALF, DF_ERR_UNSUPPORTED,
+             "%s: output dtype %d not supported", fn, c_dtype);
+    DF_CHECK(tiles_fit(M, N), DF_ERR_UNSUPPORTED, "%s: output of %d x %d too large", fn, M, N);
+    BlocksArgs g{};
+    g.M = M;
+    g.N = N;
+    g.K = (int)std::min(((int64_t)K + 15) & ~(int64_t)15, (int64_t)0x7FFFFFF0);
+    *kernel = plan(g, scale_kind == DF_SCALE_E8M0, c_dtype == DF_DTYPE_FLOAT32).kernel;
+    return DF_OK;
+}
 
 extern "C" int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const uint8_t* B, int ldb, int M, int N, int K,
                                   int scale_kind, const void* sa, int ldsa, const void* sb, int ldsb, int bias_dtype,
@@ -340,9 +360,7 @@ extern "C" int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const ui
     DF_CHECK(scale_kind_ok(scale_kind), DF_ERR_INVALID, "%s: bad scale kind %d", fn, scale_kind);
     DF_CHECK(value_dtype(c_dtype), DF_ERR_UNSUPPORTED, "%s: output dtype %d not supported", fn, c_dtype);
     DF_CHECK(!bias || value_dtype(bias_dtype), DF_ERR_UNSUPPORTED, "%s: bias dtype %d not supported", fn, bias_dtype);
-    // (blocks of small tiles: fewer than 2^32 threads; those of M <= 16 and of large tiles
-    // are fewer)
-    DF_CHECK(((M + 31ll) / 32) * ((N + 31ll) / 32) < (1ll << 23), DF_ERR_UNSUPPORTED, "%s: output of %d x %d too large",
+    DF_CHECK(tiles_fit(M, N), DF_ERR_UNSUPPORTED, "%s: output of %d x %d too large",
              fn, M, N);
     if (M == 0 || N == 0) return DF_OK;
     DF_CHECK(C && ldc >= N, DF_ERR_INVALID, "%s: output NULL or leading dimension %d < %d", fn, ldc, N);
@@ -367,9 +385,10 @@ extern "C" int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const ui
     const hipStream_t st = as_stream(stream);
     const bool wide = c_dtype == DF_DTYPE_FLOAT32, e8 = scale_kind == DF_SCALE_E8M0;
     const BlocksPlan p = plan(g, e8, wide);
-    if (p.fm > 0) {
+    if (p.kernel >= DF_BLOCKS_KERNEL_128) {
+        const int fm = p.kernel == DF_BLOCKS_KERNEL_128 ? 1 : p.kernel == DF_BLOCKS_KERNEL_256X128 ? 2 : 4;
         g.vec_out = epi_store_mode(C, ldc_bytes);
-        launch_block_tiles(fmt_a, e8, p.fm, c_dtype, g, (int)ea, (int)eb, p.grid, st);
+        launch_block_tiles(fmt_a, e8, fm, c_dtype, g, (int)ea, (int)eb, p.grid, st);
         return launch_status(fn);
     }
     g.vec_out = ldc_bytes % 16 == 0 && aligned16(C);

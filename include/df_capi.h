@@ -562,6 +562,19 @@ int df_quantize_blocks(int dtype, const void* x, int rows, int cols, int ldx, in
 int df_fp8_gemm_blocks(int fmt_a, const uint8_t* A, int lda, const uint8_t* B, int ldb, int M, int N, int K,
                        int scale_kind, const void* sa, int ldsa, const void* sb, int ldsb, int bias_dtype,
                        const void* bias, int c_dtype, void* C, int ldc, void* stream);
+/* The kernel that df_fp8_gemm_blocks takes on the current device, by its tiles: *kernel =
+ * DF_BLOCKS_KERNEL_*.  32 x 32 tiles have four waves, or eight where K is long (LONG). */
+enum {
+    DF_BLOCKS_KERNEL_16 = 0,
+    DF_BLOCKS_KERNEL_16X32 = 1,
+    DF_BLOCKS_KERNEL_32 = 2,
+    DF_BLOCKS_KERNEL_32_LONG = 3,
+    DF_BLOCKS_KERNEL_64 = 4,
+    DF_BLOCKS_KERNEL_128 = 5,
+    DF_BLOCKS_KERNEL_256X128 = 6,
+    DF_BLOCKS_KERNEL_256 = 7
+};
+int df_fp8_gemm_blocks_plan(int M, int N, int K, int scale_kind, int c_dtype, int* kernel);
 
 /* ---- a mixture-of-experts layer for a few tokens (new: the reference has no
  * mixture of experts) ----
