@@ -290,6 +290,8 @@ def moe_layer(x, logits, w1, s1, w2, s2, top_k: int, activation: str = "swiglu",
     (tokens, H), experts = x.shape, logits.shape[1]
     if not 1 <= top_k <= experts:
         raise ValueError(f"{fn}: top_k = {top_k} of {experts} experts")
+    if H == 0 and tokens:
+        raise ValueError(f"{fn}: x has no columns")
     N = w2.shape[-1] if w2.dim() == 3 else 0
     if w1.dim() == 3:  # w2's rows may be padded, w1's are not
         N = w1.shape[1] if activation == "gelu" else w1.shape[1] // 2

@@ -596,7 +596,8 @@ int df_fp8_gemm_blocks_plan(int M, int N, int K, int scale_kind, int c_dtype, in
  *      multiples is read.
  * Sums in fp32, the inner values kept to 16 bits of significand, y rounded once.
  * At most 64 tokens, 256 experts, top_k 16, and 2^31 bytes of codes an expert.
- * y and ids, weights [tokens * top_k] overlap no input.  ws:
+ * y and ids, weights [tokens * top_k] overlap no input.  tokens == 0 or H == 0 writes
+ * nothing, not the ids and weights either.  ws:
  * df_moe_layer_workspace_bytes(tokens, H, N, experts, top_k), 16-byte aligned (0: sizes not
  * taken).  Two launches for one token, three for more. */
 typedef enum { DF_ACT_SWIGLU = 0, DF_ACT_GEGLU = 1, DF_ACT_GELU = 2 } df_activation;

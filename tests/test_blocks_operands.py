@@ -77,3 +77,11 @@ def test_weights_that_end_inside_the_last_sixteen():
     assert layer_takes(w1, codes(1, 1, 48)[:, :, :N], 1) == [True, True]
     assert layer_takes(w1, codes(1, 1, N), 1) == [True, False]
     assert layer_takes(w1, codes(6, N)[None, 2:3], 1) == [True, False]
+
+
+def test_no_columns():
+    """The library writes nothing for H = 0, ids and weights neither."""
+    x, logits = torch.zeros(2, 0, dtype=torch.bfloat16), torch.zeros(2, 4)
+    w = codes(4, 32, 16), torch.zeros(4, 0, 32).to(E8), codes(4, 0, 16), torch.zeros(4, 1, 0).to(E8)
+    with pytest.raises(ValueError, match="no columns"):
+        df.moe_layer(x, logits, w[0], w[1], w[2], w[3], 2)
