@@ -6,8 +6,9 @@
 // act: silu(gate) * up or gelu(gate) * up, W1 holding gate's rows, then up's; or
 // gelu.
 //
-// Bound by reading the chosen experts' weights, each once: at 48 tokens to two of
-// 32 experts of 3 x 1600 x 1600 that is 240 MB.  So activations stay in 16 bits (no
+// Bound by reading the chosen experts' weights: at 48 tokens to two of 32 experts of
+// 3 x 1600 x 1600 that is 240 MB.  A unit of an expert's tokens reads them, once from HBM
+// and, where an expert has several, from L2 again.  So activations stay in 16 bits (no
 // pass to quantize them), weights are widened in registers, 16 weight rows and 16
 // tokens to a matrix instruction, and the launches are few: routing (for one token
 // part of the next), W1 with the activation, W2 with the weighted sum.
@@ -25,7 +26,8 @@
 // Measured: those 48 tokens 62 us (routing 5, W1 33 for 160 MB, W2 23 for 80 MB); one
 // token to two of 32 experts (15 MB) 11.5, launches and the chain of a block's loads.
 // Widening is exact (e4m3 to bf16 or f16), sums are fp32, scales are applied to each
-// step's 128 products in fp32.
+// block's 128 products in fp32; W2's powers of two go into the widening to bf16, exact
+// while codes times scales are multiples of 2^-133 below 2^128.
 //
 // The reference has no mixture of experts.
 #include <hip/hip_runtime.h>
@@ -280,7 +282,6 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
     // the next launch counts its blocks from 0
     if (blockIdx.y == 0)
         for (int i = blockIdx.x * 256 + threadIdx.x; a.splits > 1 && i < (a.H + 15) / 16; i += gridDim.x * 256) a.arrived[i] = 0;
-    if (n0 >= a.ldh) return;
     const int fr = lane & 15, fq = lane >> 4;
     int e, count, first = 0, pair = -1;
     float weight1 = 0.0f;
@@ -413,7 +414,6 @@ __global__ __launch_bounds__(256) void moe_up_kernel(const MoeArgs a) {
     const int p = a.tokens == 1 ? unit : a.plan->sorted[first + i];
     const float weight = a.tokens == 1 ? weight1 : a.weights[p];
     auto put = [&](int n, float h) {
-        if (n >= a.ldh) return;
         h = n < a.N ? h * weight : 0.0f;  // zeros up to a step's end
         const uint32_t hi = f32_to_bf16_rne(h);
         // (an infinity has no rest)

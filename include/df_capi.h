@@ -553,8 +553,8 @@ int df_quantize_blocks(int dtype, const void* x, int rows, int cols, int ldx, in
  * sum of exact products (bf16 matrix instructions), a 2-byte one takes the fp8
  * ones (see df_fp8_experts_fwd).  K == 0 gives the bias, or 0.  C overlaps no
  * operand and holds fewer than 2^23 tiles of 32 x 32.  Powers of two reach an fp32
- * output through bf16: exact while codes times scales stay in its range (2^-133 ..
- * 2^128).  fp32 scales are of any finite size: sa * sb * products is right where it
+ * output through bf16: exact while codes times scales are multiples of 2^-133 below
+ * 2^128.  fp32 scales are of any finite size: sa * sb * products is right where it
  * is in fp32's range itself.
  *   forward : Xq, sx (row codes) and Wq, sw      ; M tokens, N outputs, K inputs
  *   dX      : dYq, sdy (row codes) and Wtq, swt  ; M tokens, N inputs, K outputs
@@ -594,7 +594,9 @@ int df_fp8_gemm_blocks_plan(int M, int N, int K, int scale_kind, int c_dtype, in
  *      [ceil(N/128)][lds2], scales as df_quantize_blocks's row codes', each expert's
  *      behind the one before.  Of the last expert's last row nothing behind those
  *      multiples is read.
- * Sums in fp32, the inner values kept to 16 bits of significand, y rounded once.
+ * Sums in fp32, the inner values kept to 16 bits of significand, y rounded once.  With
+ * powers of two W2's codes times scales pass through bf16: exact while they are
+ * multiples of 2^-133 below 2^128.
  * At most 64 tokens, 256 experts, top_k 16, and 2^31 bytes of codes an expert.
  * y and ids, weights [tokens * top_k] overlap no input.  tokens == 0 or H == 0 writes
  * nothing, not the ids and weights either.  ws:
