@@ -519,6 +519,31 @@ __device__ __forceinline__ float parts_sum(const v4f& a, const Lane& l) {
     return v;
 }
 
+// Blocks that meet: each puts its values (meeting_put), then arrives, and the last to
+// arrive gets all (meeting_get).  Order rests on the hardware, not on the language's
+// memory model: puts and gets are agent-scope atomics, which pass the caches of the XCDs,
+// both ways, so a put that is done (vmcnt 0 in every wave, then the block's barrier) is
+// seen by whoever sees the count that follows it.  What the model asks for, a release and
+// an acquire, would write back and drop all of an XCD's L2, the weights with it: 48 tokens
+// 124 us so, 42 this way.
+__device__ __forceinline__ void meeting_put(float* p, float v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float meeting_get(const float* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// (the whole block; count is 0 before the first arrives)
+__device__ __forceinline__ bool last_to_arrive(int* count, int blocks) {
+    __shared__ int last;
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == blocks - 1;
+    __syncthreads();
+    return last;
+}
+
 // W2 and the weighted sum.  blockIdx.x: 16 columns of y; blockIdx.y: a share of the
 // units' steps, where there are more than 16 columns' blocks could keep under way.
 // Shares leave fp32 sums in the workspace, and the last of a column's blocks to end
@@ -652,26 +677,13 @@ template <bool E8, int TG> __global__ __launch_bounds__(512) void moe_down_kerne
 #pragma unroll
         for (int x = 0; x < W; ++x) v += sums[x][t][c];
         if (a.splits == 1) store(t, c, v);
-        else __hip_atomic_store(a.part + ((int64_t)blockIdx.y * a.tokens + t) * H16 + h0 + c, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        else meeting_put(a.part + ((int64_t)blockIdx.y * a.tokens + t) * H16 + h0 + c, v);
     }
-    if (a.splits == 1) return;
-    __shared__ int last;
-    // The sums pass the caches of the XCDs (agent scope), both ways: once a wave's
-    // stores are done (vmcnt 0) they are seen by whoever sees the count that follows.  A
-    // release and an acquire would write back and drop all of an XCD's L2, the weights
-    // with it: 48 tokens 124 us so, 42 this way.
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0);
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __syncthreads();
-    if (threadIdx.x == 0)
-        last = __hip_atomic_fetch_add(a.arrived + blockIdx.x, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.splits - 1;
-    __syncthreads();
-    if (!last) return;
+    if (a.splits == 1 || !last_to_arrive(a.arrived + blockIdx.x, a.splits)) return;
     for (int i = threadIdx.x; i < a.tokens * 16; i += 512) {
         const int t = i >> 4, c = i & 15;
         float v = 0.0f;
-        for (int x = 0; x < a.splits; ++x) v += __hip_atomic_load(a.part + ((int64_t)x * a.tokens + t) * H16 + h0 + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int x = 0; x < a.splits; ++x) v += meeting_get(a.part + ((int64_t)x * a.tokens + t) * H16 + h0 + c);
         store(t, c, v);
     }
 }
