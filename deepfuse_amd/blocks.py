@@ -57,7 +57,7 @@ def _scales_ld(fn: str, name: str, s, blocks: int, rows: int, dtype) -> int:
     step, size = (15, 1) if dtype.itemsize == 1 else (3, 4)
     need = (rows + step) & ~step  # of one block
     ld, one = s.stride()
-    if blocks <= 1:
+    if blocks <= 1 or rows == 0:
         ld = need
     if (one != 1 and rows > 1 or ld < rows or ld & step or s.data_ptr() & 15
             or need != rows and (s.storage_offset() + (blocks - 1) * ld + need) * size > s.untyped_storage().nbytes()):
@@ -133,8 +133,8 @@ def _rows_ld(t, rows: int, ld: int, red: int) -> int:
     width, need = t.shape[-1], (red + 15) & ~15
     if width < need and rows:  # (the rows' own width holds them else)
         return -1 if t.storage_offset() + (rows - 1) * ld + need > t.untyped_storage().nbytes() else ld
-    # the stride of one row is arbitrary and says nothing
-    return (width + 15) & ~15 if rows <= 1 else ld
+    # the stride of one row, or of rows without codes, is arbitrary and says nothing
+    return (width + 15) & ~15 if rows <= 1 or width == 0 else ld
 
 
 def _codes(fn: str, name: str, t, red: int, ok: bool):
@@ -143,7 +143,8 @@ def _codes(fn: str, name: str, t, red: int, ok: bool):
         raise ValueError(f"{fn}: {name} {tuple(t.shape)} {t.dtype} is not a matrix of codes in its format")
     rows, width = t.shape
     ld, one = t.stride()
-    ld = _rows_ld(t, rows, ld, red)
+    if rows <= 1 or not width or width < (red + 15) & ~15:  # (the usual codes are asked no more)
+        ld = _rows_ld(t, rows, ld, red)
     if width < red or one != 1 and width > 1 or ld < width or ld & 15 or t.data_ptr() & 15:
         raise ValueError(f"{fn}: {name} {tuple(t.shape)} with strides {t.stride()} has no rows of {red} codes at "
                          "multiples of 16 bytes, readable up to the next")

@@ -85,3 +85,12 @@ def test_no_columns():
     w = codes(4, 32, 16), torch.zeros(4, 0, 32).to(E8), codes(4, 0, 16), torch.zeros(4, 1, 0).to(E8)
     with pytest.raises(ValueError, match="no columns"):
         df.moe_layer(x, logits, w[0], w[1], w[2], w[3], 2)
+
+
+def test_operands_of_no_rows_and_no_codes():
+    """As quantize_blocks and rmsnorm_quantize leave them for a batch of no tokens."""
+    assert products_take(codes(0, 784)[:, :771])
+    assert blocks._codes("f", "a_q", torch.empty(5, 0, dtype=torch.float8_e4m3fn), 0, True) == 0
+    for nb in (0, 1, 3):
+        for s in (torch.empty(nb, 0).to(E8), torch.empty(nb, 0), torch.empty(max(nb, 1), 0).as_strided((nb, 0), (0, 1))):
+            assert blocks._scales_ld("f", "sa", s, nb, 0, s.dtype) == 0

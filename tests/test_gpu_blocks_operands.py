@@ -52,3 +52,24 @@ def test_products_of_one_row(dev, kind, K):
         assert same(df.gemm_blocks(a[r:r + 1, :K], s, b, sb, K), want[r:r + 1])
         one = a[r:r + 1].clone()
         assert same(df.gemm_blocks(one, s, b, sb, K), want[r:r + 1])
+
+
+@pytest.mark.parametrize("kind", [E8, torch.float32])
+def test_a_batch_of_no_tokens(dev, kind):
+    """A training step's calls: outputs without rows, gradients of the weights zero."""
+    K, N = 300, 200
+    g = torch.Generator(device=dev).manual_seed(0)
+    x, w, dy = torch.empty(0, K, device=dev), torch.randn(N, K, generator=g, device=dev), torch.empty(0, N, device=dev)
+    gamma = torch.ones(K, device=dev)
+    xq, sx, s, rstd, y = df.rmsnorm_quantize(x, gamma, want_y=True, scale_dtype=kind)
+    wq, sw, wt, swt = df.quantize_blocks(w, want_qt=True, square=True, scale_dtype=kind)
+    assert df.gemm_blocks(xq, sx, wq, sw, K).shape == (0, N)
+    xq, sx, xt, sxt = df.quantize_blocks(y, want_qt=True, scale_dtype=kind)
+    dyq, sdy, dyt, sdyt = df.quantize_blocks(dy, df.Fmt.E5M2, want_qt=True, scale_dtype=kind)
+    assert df.gemm_blocks(xq, sx, wq, sw, K).shape == (0, N)
+    dx = df.gemm_blocks(dyq, sdy, wt, swt, N, out_dtype=torch.float32)
+    assert dx.shape == (0, K)
+    dw = df.gemm_blocks(dyt, sdyt, xt, sxt, 0, out_dtype=torch.float32)
+    assert dw.shape == (N, K) and not dw.any()
+    dx, dg = df.rmsnorm_backward(dx, s, gamma, rstd)
+    assert dx.shape == (0, K) and not dg.any()
