@@ -55,3 +55,25 @@ def test_layer(dev, T):
     out = df.moe_layer(x, logits, w1, s1, w2, s2, 2, activation="gelu")
     assert out[0].abs().max() > 2.0 ** -40
     check_layer(out, x, logits, w1, s1, w2, s2, 2, "gelu")
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_bytes_behind_the_scales_change_nothing(dev, out, M, N, K):
+    """Scales' rows are padded with whatever the memory held, NaN's byte too."""
+    g = torch.Generator(device=dev).manual_seed(K)
+    nb = -(-K // 128)
+    a, b = codes(g, M, K, 0x20, 0x47, E4, dev), codes(g, N, K, 0x20, 0x47, E4, dev)
+    sa, sb = scales(g, nb, M, 110, 130, dev), scales(g, nb, N, 110, 130, dev)
+
+    def padded(s, fill):
+        wide = torch.full((nb, -(-s.shape[1] // 16) * 16 + 256), fill, dtype=torch.uint8, device=dev)
+        wide[:, :s.shape[1]] = s.view(torch.uint8)
+        return wide.view(E8)[:, :s.shape[1]]
+
+    raw = torch.int32 if out == torch.float32 else torch.int16
+    first = df.gemm_blocks(a, padded(sa, 127), b, padded(sb, 127), K, out_dtype=out)
+    check(first, a, sa, b, sb, K)
+    for fill in (0, 254, 255):
+        got = df.gemm_blocks(a, padded(sa, fill), b, padded(sb, fill), K, out_dtype=out)
+        assert torch.equal(got.view(raw), first.view(raw))
