@@ -10,7 +10,8 @@
 // with an fp32 output they go into the codes' widening to bf16 instead
 // (v_cvt_scalef32_pk_bf16_*), whose products the bf16 instructions add exactly,
 // for the reason given in gemm_experts.hip.  fp32 scales cannot: a step's product
-// is made from zero and added to the sum by the VALU, times sa * sb.
+// is made from zero and added to the sum by the VALU, times sa * sb (in binary64
+// where B's are far, gemm_blocks.hpp).
 //
 // Few rows are bound by latency and by reading B once (16 x 4800 x 1600 with 7.7 MB of
 // weights: 4.4 us, 3 of them a launch), many by the matrix units (gemm_blocks_tiles.hip).
@@ -31,9 +32,11 @@ namespace {
 // a row; each wave passes them to its fragments (lane l: row l%16, 32 bytes of K)
 // through a slab of LDS of its own.  Straight from memory a fragment's load has four
 // rows to every four lanes, 64 address lookups (16 x 4800 x 1600 with tiles of 16 x
-// 16: 5.7 us, 5.1 so).  U steps are loaded ahead.
+// 16: 5.7 us, 5.1 so).  U steps are loaded ahead; with two of them registers are kept to
+// three waves a SIMD (1000 x 1037 x 771, fp32 scales and outputs: 11.7 us with two, 9.8).
 template <int FA, bool E8, bool WIDE, int MT, int NT, int W, int U>
-__global__ __launch_bounds__(64 * W, W == 4 && U == 2 ? 3 : 1) void blocks_small_kernel(const BlocksArgs g, int c_dtype, int extent_a, int extent_b) {
+__global__ __launch_bounds__(64 * W, W == 4 && U == 2 ? 3 : 1)
+void blocks_small_kernel(const BlocksArgs g, int c_dtype, int extent_a, int extent_b) {
     constexpr int FB = E4M3;
     constexpr int ROWS = 16 * MT, COLS = 16 * NT;
     constexpr int RSTR = COLS + 4;  // row of a partial tile (floats)
@@ -85,8 +88,17 @@ __global__ __launch_bounds__(64 * W, W == 4 && U == 2 ? 3 : 1) void blocks_small
         uint32_t column;  // fp32: the scale of column `lane`, if there is one
     };
     const uint32_t oc = lane < min(g.N - n0, COLS) ? (uint32_t)lane * 4 : kOOB;
+    auto load_column = [&](Step& s, int step) {
+        if constexpr (!E8)
+            s.column = __builtin_amdgcn_raw_buffer_load_b32(
+                rSB, step * 128 < g.K && oc != kOOB ? (uint32_t)step * (uint32_t)g.ldsb * SZ + oc : kOOB, 0, 0);
+    };
+    // (the first of 24 loads, or the last of a few: 1024 x 1600 x 6400 26.2 us and 27.4, but 16 x
+    // 4800 x 1600 4.28 and 4.19)
+    constexpr bool COL_FIRST = MT == 4;
     auto load = [&](Step& s, int step) {
         const int k = step * 128;
+        if constexpr (COL_FIRST) load_column(s, step);
         const bool in = k + lc < g.K;
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i)
@@ -109,9 +121,7 @@ __global__ __launch_bounds__(64 * W, W == 4 && U == 2 ? 3 : 1) void blocks_small
             else s.sb[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
                               rSB, k < g.K ? (sc + 4 * fq) * SZ : kOOB, 0, 0));
         }
-        if constexpr (!E8)
-            s.column = __builtin_amdgcn_raw_buffer_load_b32(
-                rSB, k < g.K && oc != kOOB ? (uint32_t)step * (uint32_t)g.ldsb * SZ + oc : kOOB, 0, 0);
+        if constexpr (!COL_FIRST) load_column(s, step);
     };
     // accumulators are C^T: lane l holds row l%16 and columns 4*(l/16) .. +4
     v4f acc[MT][NT];
@@ -128,8 +138,7 @@ __global__ __launch_bounds__(64 * W, W == 4 && U == 2 ? 3 : 1) void blocks_small
         const u32x4 y = *reinterpret_cast<const u32x4*>(slab + t * 2048 + rd1);
         return v8i{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
     };
-    // keep: 0 takes the step's products times 0
-    auto products = [&](const Step& s, auto is_far, uint32_t keep) {
+    auto multiply = [&](const Step& s, auto is_far) {
         constexpr bool FAR = decltype(is_far)::value;
         lanes_meet();  // the step before has read the slab
         v8i fb[NT];
@@ -165,41 +174,41 @@ __global__ __launch_bounds__(64 * W, W == 4 && U == 2 ? 3 : 1) void blocks_small
                     const float sa = __uint_as_float(s.sa[i]);
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        const float sb = __uint_as_float(s.sb[j][y] & keep);
+                        const float sb = __uint_as_float(s.sb[j][y]);
                         acc[i][j][y] = FAR ? add_scaled_far(p[y], sa, sb, acc[i][j][y]) : __builtin_fmaf(p[y] * sb, sa, acc[i][j][y]);
                     }
                 }
             }
         }
     };
-    // Steps at which some of B's scales are far come behind the others, in a loop of their
-    // own: in this one their code took 60 registers more.  Here they are left out, or add 0
-    // where the next step's loads are to go out between this one's products and a branch
-    // around these held them back (64 x 64 tiles: 1024 x 1600 x 6400 32.7 us with it, 27.6
-    // so; without a look at the scales 26.1).
-    bool some_far = false;
-    auto far = [&](const Step& s) { return !E8 && __builtin_amdgcn_ballot_w64(scale_far(s.column)) != 0; };
-    auto multiply = [&](const Step& s) {
-        const bool f = far(s);
-        if constexpr (!E8) some_far |= f;
-        if constexpr (U == 1) products(s, std::false_type{}, f ? 0u : ~0u);
-        else if (!f) products(s, std::false_type{}, ~0u);
-    };
     const int nk = (g.K + 127) >> 7;
+    bool odd = false;  // fp32: a scale of this lane's column was far
     Step buf[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) load(buf[u], w + u * W);
     for (int s = w; s < nk; s += W * U) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (s + u * W < nk) multiply(buf[u]);
+            if (s + u * W < nk) {
+                if constexpr (!E8) odd |= scale_far(buf[u].column);
+                multiply(buf[u], std::false_type{});
+            }
             load(buf[u], s + (u + U) * W);
         }
     }
-    if (some_far) {
-        for (int s = w; s < nk; s += W) {
-            load(buf[0], s);
-            if (far(buf[0])) products(buf[0], std::true_type{}, ~0u);
+    // Once more, all steps, where some of B's scales were far.  (Told apart step by step in
+    // the loop, their code took it 60 registers more, and a branch held the next step's
+    // loads back, 1024 x 1600 x 6400 32.7 us; 26.2 so, 25.7 without a look.)
+    if constexpr (!E8) {
+        if (__builtin_amdgcn_ballot_w64(odd) != 0) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int s = w; s < nk; s += W) {
+                load(buf[0], s);
+                multiply(buf[0], std::true_type{});
+            }
         }
     }
     __syncthreads();  // the slabs are read before sums go over them
